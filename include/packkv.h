@@ -228,6 +228,29 @@ typedef struct pkv_cut_args {
 } pkv_cut_args;
 int pkv_window_cut(const pkv_cut_args *args, pkv_stream_t s);
 
+/* ---- head norms and rotary embedding --------------------------------------------------
+ * pkv_norm_rotary: queries [B, Hq, n, 128] and keys [B, Hkv, n, 128] (element strides of batch, head and token; channels
+ * contiguous) get the RMS norm of each head's row (`q_norm` / `k_norm` [128] of the data type; NULL: none) and the rotary
+ * embedding in one pass: y = x * rsqrt(mean(x^2) + eps) * w, then out_i = y_i cos t_i - y_{i+64} sin t_i and
+ * out_{i+64} = y_{i+64} cos t_i + y_i sin t_i, t_i = position[axis[i]] * inv_freq[i].  fp32 with the angle in fp64, one
+ * rounding at the end.  `positions`: 32- or 64-bit integers (pos_bytes 4 or 8) at strides of axis, batch and token (0: shared);
+ * n_axes 1..4, axis[i] the axis of frequency i.  An output may be its own input, row for row.  With v / v_out the values' rows
+ * are copied: with the outputs inside a cache's window (pkv_window_append) this is a decode step's whole write.  In place of
+ * the norms of models/qwen3.py:175-198 and apply_rotary_pos_emb_single (utils/compute.py:35-43), which round to 16 bits in
+ * between. */
+typedef struct pkv_rotary_args {
+    const void *q, *k, *v;
+    void *q_out, *k_out, *v_out;
+    int64_t q_stride[3], k_stride[3], v_stride[3], q_out_stride[3], k_out_stride[3], v_out_stride[3];
+    const void *q_norm, *k_norm, *positions;
+    const float *inv_freq;
+    int64_t pos_stride[3];
+    int pos_bytes, dtype, B, Hq, Hkv, n, n_axes;
+    float eps;
+    uint8_t axis[64];
+} pkv_rotary_args;
+int pkv_norm_rotary(const pkv_rotary_args *args, pkv_stream_t s);
+
 /* ---- token repacking and the analytic pack-size model ---------------------------------
  * On the uint8 code matrix [ctx_len, hidden_dim] (channel = (b * H + h) * 128 + d).
  * pkv_bit_pack_size (utils/compute.py:272-297, `bit_pack`, one of its two halves): packs are

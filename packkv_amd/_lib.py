@@ -54,6 +54,13 @@ class CutArgs(ctypes.Structure):
                 [("k_rel", _f), ("v_rel", _f)])
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "q_out", "k_out", "v_out")] +
+                [(n, _i64 * 3) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride", "k_out_stride", "v_out_stride")] +
+                [(n, _vp) for n in ("q_norm", "k_norm", "positions", "inv_freq")] + [("pos_stride", _i64 * 3)] +
+                [(n, _i) for n in ("pos_bytes", "dtype", "B", "Hq", "Hkv", "n", "n_axes")] + [("eps", _f), ("axis", ctypes.c_uint8 * 64)])
+
+
 # name -> (restype, argtypes); every symbol include/packkv.h declares
 SIGNATURES = {
     "pkv_abi_version": (_i, []),
@@ -86,6 +93,7 @@ SIGNATURES = {
     "pkv_window_cut": (_i, [ctypes.POINTER(CutArgs), _vp]),
     "pkv_window_append": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64,
                                ctypes.c_int64, _vp, _vp, _i, _i, _vp]),
+    "pkv_norm_rotary": (_i, [ctypes.POINTER(RotaryArgs), _vp]),
     "pkv_bit_pack_size": (_i, [_vp, _i, _i, _i, _u64p, ctypes.POINTER(ctypes.c_uint32), _fp, _vp]),
     "pkv_bit_pack_size_pair": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _u64p, ctypes.POINTER(ctypes.c_uint32), _vp]),
     "pkv_median_repack": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _fp, _vp]),

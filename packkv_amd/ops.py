@@ -22,6 +22,7 @@ __all__ = [
     "k_encode", "v_encode", "k_decode", "v_decode",
     "quant_params", "quantize", "dequantize", "k_quant_encode", "v_quant_encode",
     "attn_decode", "AttnPlan", "block_bound", "bits_for_rel", "repack_quant_encode", "encode_status",
+    "norm_rotary", "window_append_rotary",
 ]
 
 
@@ -624,6 +625,107 @@ def window_append(k_new, v_new, cos, sin, k_win, v_win, win_pos):
                                            sin.data_ptr() if cos is not None else None, _dtype_code(k_new), B, H, n, ks[0], ks[1],
                                            ks[2], rot_sb, k_win.data_ptr(), v_win.data_ptr(), int(win_pos), win[2], _stream(dev))
     _lib.check(rc)
+
+
+def _frequency_axes(sections, interleaved):
+    """The position axis of each of the 64 frequencies, 64 bytes.  sections = None: one axis.  Otherwise sections[a] of them belong
+    to axis a: in order, or interleaved -- axis a >= 1 of A has the frequencies a, a + A, a + 2 A .., axis 0 the rest."""
+    if sections is None:
+        return bytes(64)
+    sec = tuple(int(w) for w in sections)
+    _require(1 <= len(sec) <= 4 and min(sec) >= 0 and sum(sec) == 64, "sections must be one to four counts that make 64 frequencies")
+    if not interleaved:
+        return bytes(a for a, w in enumerate(sec) for _ in range(w))
+    axes, A = bytearray(64), len(sec)
+    for a in range(1, A):
+        _require(sec[a] == 0 or a + A * (sec[a] - 1) < 64, "interleaved sections run past the 64 frequencies")
+        for j in range(sec[a]):
+            axes[a + A * j] = a
+    return bytes(axes)
+
+
+def _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved):
+    """The checked arguments of pkv_norm_rotary without its outputs, and the tensors that the addresses in it need alive."""
+    _require(q.dim() == 4 and k.dim() == 4 and q.size(3) == 128 and k.size(3) == 128 and q.size(0) == k.size(0) and q.size(2) == k.size(2)
+             and q.is_cuda, "q and k must be device tensors [B, heads, n, 128] of one batch and length")
+    B, Hq, n, _ = q.shape
+    at, dtype = q.get_device(), q.dtype
+    code = _dtype_code(q)
+    _require(k.dtype == dtype, "q and k must have one dtype")
+    axes = _frequency_axes(sections, interleaved)
+    A = 1 if sections is None else len(tuple(sections))
+    for w in (q_norm, k_norm):
+        _require(w is None or (w.shape == (128,) and w.dtype == dtype), "norm weights must be [128] of the tokens' dtype")
+    _require(inv_freq.shape == (64,) and inv_freq.dtype == torch.float32, "inv_freq must be [64] float32")
+    _require(positions.dtype in (torch.int32, torch.int64), "positions must be int32 or int64")
+    shape = (B, n) if sections is None else (A, B, n)
+    _require(positions.dim() <= len(shape) and all(p in (1, w) for p, w in zip(reversed(positions.shape), reversed(shape))),
+             "positions must be [B, n] (several axes: [axes, B, n]) or broadcast to it")
+    for t in (k, positions, inv_freq, q_norm, k_norm):
+        _require(t is None or t.get_device() == at, _ONE_DEVICE)
+    q, k = (t if t.stride(3) == 1 else t.contiguous() for t in (q, k))
+    inv_freq = inv_freq.contiguous()
+    q_norm, k_norm = (w if w is None else w.contiguous() for w in (q_norm, k_norm))
+    positions = positions.expand(shape)
+    a = _lib.RotaryArgs()
+    a.q, a.k, a.positions, a.inv_freq = q.data_ptr(), k.data_ptr(), positions.data_ptr(), inv_freq.data_ptr()
+    a.q_norm = q_norm.data_ptr() if q_norm is not None else None
+    a.k_norm = k_norm.data_ptr() if k_norm is not None else None
+    a.q_stride[:], a.k_stride[:] = _strides(q)[:3], _strides(k)[:3]
+    ps = _strides(positions)
+    a.pos_stride[:] = ps if sections is not None else (0,) + tuple(ps)
+    a.pos_bytes, a.dtype, a.B, a.Hq, a.Hkv, a.n, a.n_axes, a.eps = positions.element_size(), code, B, Hq, k.size(1), n, A, float(eps)
+    ctypes.memmove(a.axis, axes, 64)
+    return a, (q, k, positions, inv_freq, q_norm, k_norm)
+
+
+def _launch_rotary(a, dev):
+    if a.B and a.Hq and a.Hkv and a.n:
+        with _on(dev):
+            rc = _lib.load().pkv_norm_rotary(ctypes.byref(a), _stream(dev))
+        _lib.check(rc)
+
+
+def norm_rotary(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, sections=None, interleaved=False):
+    """(q, k) [B, Hq, n, 128] and [B, Hkv, n, 128] with the RMS norm of every head's row (weights q_norm / k_norm [128]; None: no
+    norm) and the rotary embedding applied in one launch, in fp32 and rounded once.  positions: integers [B, n], or anything that
+    broadcasts to it; with `sections` (counts of the 64 frequencies for each position axis, e.g. (16, 24, 24) for time, height and
+    width) [axes, B, n], frequencies assigned in order or, with interleaved=True, in turn.  inv_freq [64] float32; angles are formed
+    in 64 bits, so positions may be far.  Strided views (slices of a projection's output) are read in place; the results are
+    contiguous."""
+    a, keep = _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    a.q_out, a.k_out = q_out.data_ptr(), k_out.data_ptr()
+    a.q_out_stride[:], a.k_out_stride[:] = q_out.stride()[:3], k_out.stride()[:3]
+    _launch_rotary(a, q.device)
+    return q_out, k_out
+
+
+def window_append_rotary(q, k, v, positions, inv_freq, k_win, v_win, win_pos, q_norm=None, k_norm=None, eps=1e-6, sections=None,
+                         interleaved=False):
+    """norm_rotary for a step's new tokens with the keys written into rows win_pos.. of the 16-bit window k_win [B, Hkv, cap, 128]
+    and the values v [B, Hkv, n, 128] into those of v_win, in one launch; returns the queries.  window_append for a model whose
+    projections come raw."""
+    a, keep = _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
+    B, H, n, _ = k.shape
+    at, win_pos = q.get_device(), int(win_pos)
+    _require(v.shape == k.shape and v.dtype == q.dtype, "K and V must be device tensors [B, H, n, 128] of one dtype")
+    _require(k_win.is_contiguous() and v_win.is_contiguous() and k_win.dim() == 4 and v_win.shape == k_win.shape and k_win.dtype == q.dtype
+             and v_win.dtype == q.dtype and k_win.shape[:2] == (B, H) and k_win.size(3) == 128,
+             "windows must be contiguous [B, H, cap, 128] of the tokens' dtype")
+    _require(v.get_device() == at and k_win.get_device() == at and v_win.get_device() == at, _ONE_DEVICE)
+    cap = k_win.size(2)
+    _require(0 <= win_pos and win_pos + n <= cap, "the new rows do not fit the window (%d + %d > %d)" % (win_pos, n, cap))
+    v = v if v.stride(3) == 1 else v.contiguous()
+    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    a.v, a.q_out = v.data_ptr(), q_out.data_ptr()
+    a.v_stride[:], a.q_out_stride[:] = _strides(v)[:3], q_out.stride()[:3]
+    es = 256 * win_pos
+    a.k_out, a.v_out = k_win.data_ptr() + es, v_win.data_ptr() + es
+    a.k_out_stride[:] = a.v_out_stride[:] = (H * cap * 128, cap * 128, 128)
+    _launch_rotary(a, q.device)
+    return q_out
 
 
 def _strides(t):
