@@ -410,6 +410,35 @@ int pkv_attn_decode_noalloc(const pkv_attn_args *args, pkv_stream_t s);
  * `update` (models/cache/packkv_quant.py:84-85).  k_bits and v_bits 2..8; outputs and windows 16-byte aligned. */
 int pkv_dense_view(const pkv_attn_args *args, void *k_out, void *v_out, pkv_stream_t s);
 
+/* ---- attention of several new tokens ---------------------------------------------------
+ * pkv_attn_chunk: pkv_attn_decode for n queries a sequence, which are the cache's last n tokens (their keys and values are in the
+ * streams and the window already): query i attends to tokens starts[b] .. T_c + T_w - n + i; with causal = 0 to all from
+ * starts[b] on.  `starts` [B] int32 (NULL: zeroes) is for batches padded on the left; a query that sees no token gets zeroes, and
+ * what lies in front of starts[b] may be anything.  (A NaN or an infinity among the new tokens' window rows may reach queries
+ * before it.)  q and out [B, Hq, n, 128] at element strides of batch, head and token, rows 16-byte aligned; Hq any multiple of Hkv;
+ * widths 2..8; streams and windows 16-byte aligned; the rest as in pkv_attn_args.  fp32 accumulation, weights in fp16.  `workspace`:
+ * 16-byte aligned device memory of pkv_attn_chunk_workspace(args) bytes (may be 0), used until the call's kernels are done: calls
+ * that overlap need one each.  Launches kernels only.  Stands in for cache.update's dense tensors + eager attention
+ * (models/llama.py:189-212) where a prompt continues a cache. */
+typedef struct pkv_chunk_args {
+    const uint8_t *k_stream;
+    const uint32_t *k_info;
+    const uint8_t *v_stream;
+    const uint32_t *v_info;
+    uint64_t k_bytes, v_bytes;
+    const void *k_scale, *k_zero, *v_scale, *v_zero;
+    const void *q;
+    void *out;
+    const void *k_win, *v_win;
+    const int32_t *starts;
+    int64_t q_stride[3], out_stride[3];
+    int B, Hq, Hkv, n, T_c, T_w;
+    int k_bits, v_bits, dtype, par_stride, win_stride, causal;
+    float sm_scale;
+} pkv_chunk_args;
+uint64_t pkv_attn_chunk_workspace(const pkv_chunk_args *args);
+int pkv_attn_chunk(const pkv_chunk_args *args, void *workspace, uint64_t workspace_bytes, pkv_stream_t s);
+
 /* pkv_stream_release: gives back the device memory the library keeps for stream `s` of the current device -- its
  * scratch buffers (attention partials, the encoders' look-back state), its tile counters and every buffer it has
  * outgrown (kept until now because a captured HIP graph might still hold its address).  It has no counterpart in the

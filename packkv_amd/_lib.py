@@ -61,6 +61,14 @@ class RotaryArgs(ctypes.Structure):
                 [(n, _i) for n in ("pos_bytes", "dtype", "B", "Hq", "Hkv", "n", "n_axes")] + [("eps", _f), ("axis", ctypes.c_uint8 * 64)])
 
 
+class ChunkArgs(ctypes.Structure):
+    _fields_ = ([("k_stream", _vp), ("k_info", _vp), ("v_stream", _vp), ("v_info", _vp), ("k_bytes", _u64), ("v_bytes", _u64)] +
+                [(n, _vp) for n in ("k_scale", "k_zero", "v_scale", "v_zero", "q", "out", "k_win", "v_win", "starts")] +
+                [("q_stride", _i64 * 3), ("out_stride", _i64 * 3)] +
+                [(n, _i) for n in ("B", "Hq", "Hkv", "n", "T_c", "T_w", "k_bits", "v_bits", "dtype", "par_stride", "win_stride", "causal")] +
+                [("sm_scale", _f)])
+
+
 # name -> (restype, argtypes); every symbol include/packkv.h declares
 SIGNATURES = {
     "pkv_abi_version": (_i, []),
@@ -105,6 +113,8 @@ SIGNATURES = {
     "pkv_attn_decode": (_i, [ctypes.POINTER(AttnArgs), _fp, _vp]),
     "pkv_attn_decode_noalloc": (_i, [ctypes.POINTER(AttnArgs), _vp]),
     "pkv_dense_view": (_i, [ctypes.POINTER(AttnArgs), _vp, _vp, _vp]),
+    "pkv_attn_chunk_workspace": (_u64, [ctypes.POINTER(ChunkArgs)]),
+    "pkv_attn_chunk": (_i, [ctypes.POINTER(ChunkArgs), _vp, _u64, _vp]),
     "pkv_stream_release": (_i, [_vp]),
 }
 

@@ -1,0 +1,676 @@
+// Attention of several new tokens over a compressed cache: query i of n sits at position T - n + i of the T tokens (streams, then
+// the 16-bit window) and attends to those from the sequence's first token up to itself.
+//
+// Rows are the (token, query head) pairs of one KV head, row = token * G + head of the group: a workgroup takes 32 NB of them and a
+// run of 128-token tiles; each of its four wavefronts takes 32 tokens of every tile for ALL of these rows and keeps a softmax state
+// and an accumulator of its own, so nothing of the softmax crosses wavefronts until the run ends.
+//
+// Both products are formed transposed, on 32x32x16 fp16 matrix instructions (a product's columns are the lanes, here the rows):
+//   S^T [token x row]   = K codes x q      a lane holds 16 tokens' scores of one row: maxima and sums are the lane's own but for
+//                                          one exchange with lane ^ 32, and exp2's results are the next product's operand as they lie
+//   O^T [channel x row] = V codes x p      the factor of a new maximum is a number of the lane
+// Codes enter as whole numbers in fp16: 0x6400 | code is 1024 + code, and one packed subtraction takes the 1024 away.  (The integer
+// itself, read as a half, is the code times 2^-24 and needs no subtraction, but the matrix cores add up products of subnormals
+// without normalising them, to about 18 bits.)  Scale and zero of a token are applied to what the products need of them, in fp32:  score = scale (q . code + zero sum(q)),
+// out = sum p scale code + sum p scale zero.  The weight p * scale is rounded to fp16 (2^-11), scaled by a power of two that follows
+// the largest scale met; the zero's sum takes the rounded weight, so that the error is 2^-11 of p |v|, not of p * scale * code.
+// q in bf16 becomes fp16 times one power of two for the workgroup's rows, which loses bits only 2^-39 below their largest.
+//
+// K turns through LDS (a pack holds 16 tokens of one channel, the product wants channels of one token): codes as bytes in rows of
+// 136 bytes, private to the wavefront.  V needs no turn: lane = channel, and the order of the tokens in the contraction is free as
+// long as both operands agree, so a lane unpacks ONE pack per 32 channels straight into its operand -- tokens (k, k + 8) side by
+// side, since both halves of a pack's word take the same shifts.  Which pack is where comes from a table that the half-wavefronts
+// fill, one unit each (offset, width, minimum of its 128 packs).
+#include "pkv_block.hpp"
+#include "pkv_runtime.hpp"
+
+namespace pkv {
+
+typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+typedef float f16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+
+constexpr int kChunkTile = 128;
+constexpr int kKRow = 136;                     // bytes of a token's K codes in LDS: 34 dwords, 32 rows start at 32 different banks
+constexpr int kQRow = 272;                     // bytes of a row of q: 68 dwords
+constexpr int kVRow = 264;                     // bytes of a window token's V
+constexpr int kPart = 132;                     // floats of a partial: maximum, sum, 2 unused, 128 channels
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLowest = -3.0e38f;            // a maximum before any score; a masked score is -inf, so its weight is 0 against it
+
+struct ChunkParams {
+    const uint8_t *k_stream, *v_stream;
+    const uint32_t *k_info, *v_info;
+    const uint16_t *k_scale, *k_zero, *v_scale, *v_zero, *k_win, *v_win, *q;
+    uint16_t *out;
+    float *part;                               // NULL: one run, the result is written
+    const int32_t *starts;
+    int64_t q_b, q_h, q_t, o_b, o_h, o_t;
+    uint64_t k_bytes, v_bytes;
+    int Hq, Hkv, BH, G, n, rows, T_c, T_w, par_stride, win_stride, k_bits, v_bits, causal;
+    int tiles_c, tiles, run, nsplit, row_tiles;
+    uint32_t slot, ring;                       // LDS bytes of a staged block and of everything staged
+    float sm_log2;
+};
+
+__device__ __forceinline__ float chunk_f32(uint32_t bits16, bool bf) {
+    return bf ? __uint_as_float(bits16 << 16) : __half2float(__ushort_as_half((unsigned short)bits16));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
+    return __builtin_bit_cast(uint32_t, (h2v){(_Float16)a, (_Float16)b});
+}
+__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2){a, b}, b2));
+}
+template <bool BF> __device__ __forceinline__ f16v product(u4 a, u4 b, f16v c) {
+    if (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+// Two of four codes (one a byte) as halves.
+__device__ __forceinline__ uint32_t codes_f16(uint32_t c4, uint32_t which) {
+    return __builtin_bit_cast(uint32_t, (h2v)(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, c4, which)) - (h2v){(_Float16)1024.f, (_Float16)1024.f}));
+}
+
+// The eight operand registers of one V pack (table entry e: LDS address | width << 16 | minimum << 20): tokens (j, j + 8) side by
+// side, j = 0..7.  The field, 1024 + (code - minimum), and minimum - 1024 add up exactly.
+__device__ __forceinline__ uint32_t field_code(uint32_t shifted, uint32_t mask, h2v low) {
+    return __builtin_bit_cast(uint32_t, (h2v)(__builtin_bit_cast(h2v, (shifted & mask) | 0x64006400u) + low));
+}
+template <bool WIDE> __device__ __forceinline__ void pack_operand(const uint8_t *ring, uint32_t e, uint32_t out[8]) {
+    typedef unsigned short u16pair __attribute__((ext_vector_type(2)));
+    const uint32_t at = e & 0xFFFFu, len = (e >> 16) & 15u;
+    const uint32_t mask = ((1u << len) - 1u) * 0x00010001u;
+    const h2v low = __builtin_bit_cast(h2v, 0x64006400u | ((e >> 20) * 0x00010001u)) - (h2v){(_Float16)2048.f, (_Float16)2048.f};
+    if (WIDE) {                                // words of up to 128 bits: two tokens at a time, bits (14 - j) * len of the word on
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) {
+            uint32_t win[2];
+#pragma unroll
+            for (int half = 0; half < 2; half++) {
+                const uint32_t bit = (uint32_t)(14 - 8 * half - j) * len, byte = at + (bit >> 3);
+                const uint32_t *d = reinterpret_cast<const uint32_t *>(ring + (byte & ~3u));
+                win[half] = __builtin_amdgcn_alignbyte(d[1], d[0], byte & 3u) >> (bit & 7u);
+            }
+            const u16pair w = __builtin_bit_cast(u16pair, __builtin_amdgcn_perm(win[1], win[0], 0x05040100u));
+            out[j] = field_code(__builtin_bit_cast(uint32_t, (u16pair)(w >> __builtin_bit_cast(u16pair, len * 0x00010001u))), mask, low);
+            out[j + 1] = field_code(__builtin_bit_cast(uint32_t, w), mask, low);
+        }
+        return;
+    }
+    const uint64_t word = lds_load64(ring, at);
+    const uint32_t hi = (uint32_t)(word >> (8u * len)), lo = (uint32_t)word;       // tokens 0..7 | 8..15
+    const u16pair w[2] = {__builtin_bit_cast(u16pair, __builtin_amdgcn_perm(lo >> (4u * len), hi >> (4u * len), 0x05040100u)),
+                          __builtin_bit_cast(u16pair, __builtin_amdgcn_perm(lo, hi, 0x05040100u))};
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const u16pair sh = __builtin_bit_cast(u16pair, len * (uint32_t)(3 - (j & 3)) * 0x00010001u);
+        out[j] = field_code(__builtin_bit_cast(uint32_t, (u16pair)(w[j >> 2] >> sh)), mask, low);
+    }
+}
+
+// One 32-row block's softmax step for 16 scores of the lane's row: the new maximum, the factor for what was summed before, and the
+// weights in place of the scores.
+__device__ __forceinline__ float softmax_step(f16v &y, float &m) {
+    float top = y[0];
+#pragma unroll
+    for (int r = 1; r < 16; r++) top = fmaxf(top, y[r]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64));
+    const float was = m;
+    m = fmaxf(m, top);
+#pragma unroll
+    for (int r = 0; r < 16; r++) y[r] = __builtin_amdgcn_exp2f(y[r] - m);
+    return __builtin_amdgcn_exp2f(was - m);
+}
+
+template <bool BF, int NB, bool WIDE>
+__global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const ChunkParams p) {
+    constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
+    extern __shared__ __align__(16) uint8_t lds[];
+    uint8_t *ring = lds;                                   // two tiles of four staged blocks; window: V rows; end: sums
+    uint8_t *kt_all = lds + p.ring;                        // [4 wavefronts][32 tokens][kKRow]
+    uint32_t *tab = reinterpret_cast<uint32_t *>(kt_all + 4 * 32 * kKRow);         // [8 units][4 slots][32 lanes]
+    float4 *par_all = reinterpret_cast<float4 *>(tab + 1024);                      // [4][32] (scale, zero * scale, V scale, V zero)
+    float *st = reinterpret_cast<float *>(par_all + 128);                          // [2][4][32 NB] maxima, sums at the end
+    uint8_t *qt = reinterpret_cast<uint8_t *>(st + 8 * 32 * NB);                   // [32 NB][kQRow]
+
+    // Row tiles of one (KV head, run) follow each other on one XCD (workgroups go round the eight of them), so that they find its
+    // blocks in that L2.
+    const uint32_t groups = (uint32_t)p.BH * (uint32_t)p.nsplit, seq = blockIdx.x >> 3;
+    const uint32_t group = (seq / (uint32_t)p.row_tiles) * 8u + (blockIdx.x & 7u);
+    if (group >= groups) return;
+    const int rt = (int)(seq % (uint32_t)p.row_tiles), bh = (int)(group % (uint32_t)p.BH), split = (int)(group / (uint32_t)p.BH);
+    const int b = bh / p.Hkv, hkv = bh % p.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, t = lane & 31, hw = tid >> 5;
+    const int T = p.T_c + p.T_w;
+    const int row0 = rt * 32 * NB, row_last = min(row0 + 32 * NB, p.rows) - 1;
+    const int start = p.starts ? min(max(p.starts[b], 0), T) : 0;
+    const int pos_first = p.causal ? T - p.n + row0 / p.G : T - 1, pos_last = p.causal ? T - p.n + row_last / p.G : T - 1;
+
+    int row[NB], pos[NB];                                  // the lane's rows, and the last token that each sees
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        row[nb] = min(row0 + 32 * nb + t, p.rows - 1);
+        pos[nb] = p.causal ? T - p.n + row[nb] / p.G : T - 1;
+    }
+    auto q_row = [&](int r) -> const uint16_t * {
+        return p.q + (int64_t)b * p.q_b + (int64_t)(hkv * p.G + r % p.G) * p.q_h + (int64_t)(r / p.G) * p.q_t;
+    };
+
+    // ---- this run's tiles: compressed ones [c0, c1), then window ones [w0, w1) ----
+    const int first = split * p.run, last = min(first + p.run, p.tiles);
+    const int seen_c = min(p.T_c, pos_last + 1);           // (tokens behind the last row's own are nobody's)
+    const int c0 = max(first, start / kChunkTile), c1 = min(last, (seen_c + kChunkTile - 1) / kChunkTile);
+    const int w0 = max(first - p.tiles_c, max(start - p.T_c, 0) / kChunkTile), w1 = min(last - p.tiles_c, (pos_last - p.T_c) / kChunkTile + 1);
+
+    // ---- staging of a tile's four blocks (wavefront = block) and this wavefront's parameters, one tile ahead in registers ----
+    const uint32_t cap = wave < 2 ? (uint32_t)k_block_bound(64, p.k_bits) : (uint32_t)v_block_bound(64, p.v_bits);
+    const uint64_t bytes = wave < 2 ? p.k_bytes : p.v_bytes;
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wave < 2 ? p.k_stream : p.v_stream), 0,
+                                                                          (int)(uint32_t)((bytes + 3u) & ~3ull), 0x00020000);
+    u4 raw[NQ];
+    uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
+    auto fetch = [&](int tile) {
+        const uint32_t blk = wave < 2 ? (2u * (uint32_t)tile + (uint32_t)wave) * (uint32_t)p.BH + (uint32_t)bh
+                                      : 2u * ((uint32_t)tile * (uint32_t)p.BH + (uint32_t)bh) + (uint32_t)(wave - 2);
+        uint32_t off, size;
+        block_span(wave < 2 ? p.k_info : p.v_info, blk, cap, bytes, off, size);
+        raw_phase = off & 15u;
+        const uint32_t n16 = (raw_phase + size + 15u) >> 4, src = off - raw_phase;
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+            const uint32_t c = (uint32_t)(lane + 64 * i);
+            raw[i] = c < n16 ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, src + 16u * c, 0, 0)) : (u4){0, 0, 0, 0};
+        }
+        const size_t at = (size_t)b * p.par_stride + (size_t)tile * kChunkTile + 32 * wave + t;
+        par_k = p.k_scale[at]; par_kz = p.k_zero[at]; par_v = p.v_scale[at]; par_vz = p.v_zero[at];
+    };
+    __shared__ uint32_t phase_s[2][4];
+    auto put = [&](int buf) {
+        uint8_t *dst = ring + (uint32_t)(4 * buf + wave) * p.slot;
+#pragma unroll
+        for (int i = 0; i < NQ; i++)
+            if ((uint32_t)(lane + 64 * i) * 16u < p.slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
+        if (lane == 0) phase_s[buf][wave] = raw_phase;
+    };
+    if (c0 < c1) fetch(c0);
+
+    // ---- q: rows into LDS as fp16 (bf16: times 2^up), their sums ----
+    int up = 0;
+    if (BF) {
+        uint32_t top = 0;
+        for (int r = wave; r <= row_last - row0; r += 4) {
+            const uint32_t w = reinterpret_cast<const uint32_t *>(q_row(row0 + r))[lane];
+            top = max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
+        if (lane == 0) tab[wave] = top;
+        __syncthreads();
+        top = max(max(tab[0], tab[1]), max(tab[2], tab[3]));
+        up = top ? min(max(141 - (int)(top >> 7), -120), 120) : 0;        // the largest comes to 2^14 .. 2^15
+    }
+    const float up_f = __uint_as_float((uint32_t)(127 + up) << 23);
+    for (int i = tid; i < 32 * NB * 16; i += 256) {
+        const int r = i >> 4, c = i & 15;
+        u4 w = *reinterpret_cast<const u4 *>(q_row(min(row0 + r, p.rows - 1)) + 8 * c);
+        if (BF) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) w[k] = pack_f16(__uint_as_float(w[k] << 16) * up_f, __uint_as_float(w[k] & 0xFFFF0000u) * up_f);
+        }
+        *reinterpret_cast<u4 *>(qt + r * kQRow + 16 * c) = w;
+    }
+    if (c0 < c1) put(0);
+    __syncthreads();
+    float qsum[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {                      // half the channels each
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < 8; c++) {
+            const h8 v = *reinterpret_cast<const h8 *>(qt + (32 * nb + t) * kQRow + 32 * c + 16 * h);
+#pragma unroll
+            for (int k = 0; k < 8; k++) s += (float)v[k];
+        }
+        qsum[nb] = s + __shfl_xor(s, 32, 64);
+    }
+
+    f16v acc[NB][4];
+    float m[NB], l[NB], z[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        m[nb] = kLowest; l[nb] = 0.f; z[nb] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[nb][c][r] = 0.f;
+    }
+    const float to_score = p.sm_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
+    uint8_t *kt = kt_all + wave * 32 * kKRow;
+    float4 *par = par_all + wave * 32;
+    uint32_t emax = 0;                                     // exponent field of the largest V scale met, at least 14; 0: none yet
+    float unit = 1.f;                                      // result = (acc + z) * unit
+    const UnitGeom gk = unit_geom(p.k_bits), gv = unit_geom(p.v_bits);
+    const int tau = (t & 3) + 4 * (t >> 3) + 16 * ((t >> 2) & 1);          // the token (of 32) in row t of S^T: lane half = pack
+
+    // ---- compressed tiles ----
+    for (int tile = c0; tile < c1; tile++) {
+        const int buf = (tile - c0) & 1;
+        if (tile != c0) __syncthreads();                   // the tile is staged, and the table's readers are done
+        const int tok0 = tile * kChunkTile + 32 * wave;    // this wavefront's first token
+        float grow = 1.f;
+        {   // parameters of the 32 tokens; those in front of the sequence count as nothing
+            const bool real = tok0 + t >= start;
+            const float ks = real ? chunk_f32(par_k, BF) * to_score : 0.f, kz = real ? chunk_f32(par_kz, BF) : 0.f;
+            const float vs = real ? chunk_f32(par_v, BF) : 0.f, vz = real ? chunk_f32(par_vz, BF) : 0.f;
+            uint32_t e = (__float_as_uint(vs) >> 23) & 255u;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) e = max(e, (uint32_t)__shfl_xor((int)e, d, 64));
+            e = __builtin_amdgcn_readfirstlane(max(e, 14u));
+            if (e > emax) {
+                if (emax) grow = __builtin_amdgcn_exp2f((float)(int)(emax - e));
+                emax = e;
+                unit = __uint_as_float((e - 13u) << 23);   // 1 / (the weights' power of two, 2^(140 - e))
+            }
+            const float vw = vs * __uint_as_float(min(267u - emax, 254u) << 23);
+            if (h == 0) par[t] = make_float4(ks, kz * ks, vw, vz);
+        }
+        if (tile + 1 < c1) fetch(tile + 1);
+        const uint8_t *blk_k = ring + (uint32_t)(4 * buf + (hw >> 2)) * p.slot, *blk_v = ring + (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot;
+        const int u = hw & 3;
+        {   // V unit of this half-wavefront: where its packs are
+            const uint32_t phase = phase_s[buf][2 + (hw >> 2)];
+            const uint32_t at = min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk_v + phase)[u - 1] : 0u), p.slot - 16u);
+            const uint32_t minsw = lds_meta_word(blk_v + at, t, gv.W), lensw = lds_meta_word(blk_v + at + gv.mins_bytes, t, gv.LB);
+            uint32_t len[4], off[4], payload;
+#pragma unroll
+            for (int i = 0; i < 4; i++) len[i] = min((lensw >> (i * gv.LB)) & ((1u << gv.LB) - 1u), (uint32_t)gv.W);
+            pack_offsets(len, off, payload);
+            const uint32_t base = (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot + at + (uint32_t)(gv.mins_bytes + gv.lens_bytes);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                tab[(hw * 4 + i) * 32 + t] = min(base + off[i], p.ring - 32u) | (len[i] << 16) | (((minsw >> (i * gv.W)) & ((1u << gv.W) - 1u)) << 20);
+        }
+        {   // K unit: 16 tokens x 128 channels, the wavefront's two make its 32 tokens
+            const uint32_t phase = phase_s[buf][hw >> 2];
+            const uint32_t at = min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk_k + phase)[u - 1] : 0u), p.slot - 16u);
+            uint8_t *dst = kt + 16 * h * kKRow + 4 * t;
+            unit_codes(blk_k, at, t, gk, [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
+        }
+        wave_lds_order();
+        f16v y[NB];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) y[nb][r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 8; s++) {
+            const uint2 c8 = *reinterpret_cast<const uint2 *>(kt + tau * kKRow + 16 * s + 8 * h);
+            const u4 a = {codes_f16(c8.x, 0x04010400u), codes_f16(c8.x, 0x04030402u), codes_f16(c8.y, 0x04010400u), codes_f16(c8.y, 0x04030402u)};
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+                y[nb] = product<false>(a, *reinterpret_cast<const u4 *>(qt + (32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
+        }
+        const bool masked = tok0 + 31 > pos_first || tok0 < start;             // (uniform)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const float4 q4 = par[16 * h + r];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) y[nb][r] = y[nb][r] * q4.x + q4.y * qsum[nb];
+        }
+        if (masked) {
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int tok = tok0 + 16 * h + r;
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+                    if (tok > pos[nb] || tok < start) y[nb][r] = -INFINITY;
+            }
+        }
+        u4 w[NB][2];
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) {
+            const float alpha = softmax_step(y[nb], m[nb]), both = alpha * grow;
+            l[nb] *= alpha;
+            z[nb] *= both;
+            if (__any(both != 1.f)) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[nb][c][r] *= both;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const float4 pa = par[16 * h + j], pb = par[16 * h + j + 8];
+                l[nb] += y[nb][j] + y[nb][j + 8];
+                uint32_t f = pack_f16(y[nb][j] * pa.z, y[nb][j + 8] * pb.z);
+                asm("" : "+v"(f));                         // (the sum takes these very halves: formed again they round once less)
+                const h2v f2 = __builtin_bit_cast(h2v, f);
+                z[nb] += (float)f2[0] * pa.w + (float)f2[1] * pb.w;
+                w[nb][j >> 2][j & 3] = f;
+            }
+        }
+        __syncthreads();                                   // the table is there
+#pragma unroll
+        for (int c = 0; c < 4; c++) {                      // 32 channels: block c / 2, column of units c % 2
+            const uint32_t e = tab[((((c >> 1) * 4 + (c & 1) * 2 + (wave >> 1)) * 4) + 2 * (wave & 1) + h) * 32 + t];
+            uint32_t v[8];
+            pack_operand<WIDE>(ring, e, v);
+            const u4 v0 = {v[0], v[1], v[2], v[3]}, v1 = {v[4], v[5], v[6], v[7]};
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                acc[nb][c] = product<false>(v0, w[nb][0], acc[nb][c]);
+                acc[nb][c] = product<false>(v1, w[nb][1], acc[nb][c]);
+            }
+        }
+        if (tile + 1 < c1) put(buf ^ 1);
+    }
+
+    // ---- window tiles: the same products on the 16-bit rows ----
+    if (w0 < w1) {
+        __syncthreads();                                   // the staged blocks are dead
+        constexpr float kUp = BF ? 1.f : 16384.f;          // fp16 weights: 2^14 p, so that small ones keep their bits
+        if (emax) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                z[nb] = z[nb] * unit * kUp;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[nb][c][r] = acc[nb][c][r] * unit * kUp;
+            }
+        }
+        unit = 1.f / kUp;
+        uint8_t *vt = ring + wave * 32 * kVRow;
+        for (int wt = w0; wt < w1; wt++) {
+            const int r0 = wt * kChunkTile + 32 * wave, tok0 = p.T_c + r0;     // window row and position of the wavefront's first token
+            if (r0 >= p.T_w || tok0 > pos_last || tok0 + 31 < start) continue; // (uniform, and no barrier in here)
+            const uint16_t *kr = p.k_win + ((size_t)bh * p.win_stride + min(r0 + tau, p.T_w - 1)) * kHeadDim + 8 * h;
+            const uint16_t *vr = p.v_win + ((size_t)bh * p.win_stride) * kHeadDim;
+            wave_lds_order();
+#pragma unroll
+            for (int i = 0; i < 8; i++) {                  // four rows of V a step, 16 lanes each; rows that nobody sees as zeroes
+                const int k = 4 * i + (lane >> 4), c = lane & 15;
+                const bool real = r0 + k < p.T_w && tok0 + k >= start && tok0 + k <= pos_last;
+                const uint2 *src = reinterpret_cast<const uint2 *>(vr + (size_t)min(r0 + k, p.T_w - 1) * kHeadDim + 8 * c);
+                const uint2 a = src[0], d = src[1];
+                uint2 *dst = reinterpret_cast<uint2 *>(vt + k * kVRow + 16 * c);
+                dst[0] = real ? a : make_uint2(0u, 0u);
+                dst[1] = real ? d : make_uint2(0u, 0u);
+            }
+            f16v y[NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                for (int r = 0; r < 16; r++) y[nb][r] = 0.f;
+#pragma unroll
+            for (int s = 0; s < 8; s++) {
+                const u4 a = *reinterpret_cast<const u4 *>(kr + 16 * s);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+                    y[nb] = product<BF>(a, BF ? *reinterpret_cast<const u4 *>(q_row(row[nb]) + 16 * s + 8 * h)
+                                              : *reinterpret_cast<const u4 *>(qt + (32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const int tok = tok0 + 16 * h + r;
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++) y[nb][r] = tok > pos[nb] || tok < start ? -INFINITY : y[nb][r] * p.sm_log2;
+            }
+            wave_lds_order();
+            u4 w[NB][2], wl[NB][2];                        // bf16: what the rounding leaves goes through the matrix cores as well
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                const float alpha = softmax_step(y[nb], m[nb]);
+                l[nb] *= alpha;
+                z[nb] *= alpha;
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[nb][c][r] *= alpha;
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float a = y[nb][j], d = y[nb][j + 8];
+                    l[nb] += a + d;
+                    if (BF) {
+                        const uint32_t hi = pack_bf16(a, d);
+                        w[nb][j >> 2][j & 3] = hi;
+                        wl[nb][j >> 2][j & 3] = pack_bf16(a - __uint_as_float(hi << 16), d - __uint_as_float(hi & 0xFFFF0000u));
+                    } else {
+                        w[nb][j >> 2][j & 3] = pack_f16(a * kUp, d * kUp);
+                    }
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const uint16_t *col = reinterpret_cast<const uint16_t *>(vt + 16 * h * kVRow) + 32 * c + t;
+                u4 v[2];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j >> 2][j & 3] = (uint32_t)col[j * (kVRow / 2)] | ((uint32_t)col[(j + 8) * (kVRow / 2)] << 16);
+#pragma unroll
+                for (int nb = 0; nb < NB; nb++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        acc[nb][c] = product<BF>(v[e], w[nb][e], acc[nb][c]);
+                        if (BF) acc[nb][c] = product<BF>(v[e], wl[nb][e], acc[nb][c]);
+                    }
+            }
+        }
+    }
+
+    // ---- the four wavefronts' states become one ----
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        l[nb] += __shfl_xor(l[nb], 32, 64);
+        z[nb] += __shfl_xor(z[nb], 32, 64);
+        if (h == 0) st[wave * 32 * NB + 32 * nb + t] = m[nb];
+    }
+    __syncthreads();
+    float *sums = st + 4 * 32 * NB;
+    float top[NB];
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        const float *at = st + 32 * nb + t;
+        top[nb] = fmaxf(fmaxf(at[0], at[32 * NB]), fmaxf(at[64 * NB], at[96 * NB]));
+        const float f = __builtin_amdgcn_exp2f(m[nb] - top[nb]);
+        if (h == 0) sums[wave * 32 * NB + 32 * nb + t] = l[nb] * f;
+        const float fu = f * unit;
+#pragma unroll
+        for (int c = 0; c < 4; c++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) acc[nb][c][r] = (acc[nb][c][r] + z[nb]) * fu;
+    }
+    float *buf0 = reinterpret_cast<float *>(ring);         // [2][32 rows][129]: wavefronts 0 + 2 and 1 + 3
+    constexpr int kSumRow = 129;
+#pragma unroll
+    for (int nb = 0; nb < NB; nb++) {
+        float *mine = buf0 + (wave & 1) * 32 * kSumRow + t * kSumRow + 4 * h;
+#pragma unroll
+        for (int step = 0; step < 2; step++) {
+            if ((wave >> 1) == step) {
+#pragma unroll
+                for (int c = 0; c < 4; c++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) {
+                        float *at = mine + 32 * c + 8 * (r >> 2) + (r & 3);
+                        *at = step ? *at + acc[nb][c][r] : acc[nb][c][r];
+                    }
+            }
+            __syncthreads();
+        }
+        const int i = tid >> 3, ch = 16 * (tid & 7), r = row0 + 32 * nb + i;                  // a row's 16 channels each
+        if (r < p.rows) {
+            const float *s0 = buf0 + i * kSumRow + ch, *s1 = s0 + 32 * kSumRow;
+            const float *sl = sums + 32 * nb + i;
+            const float total = (sl[0] + sl[32 * NB]) + (sl[64 * NB] + sl[96 * NB]);
+            const int64_t head = hkv * p.G + r % p.G, token = r / p.G;
+            if (p.part) {
+                float *dst = p.part + ((((int64_t)b * p.Hq + head) * p.n + token) * p.nsplit + split) * kPart;
+                if (ch == 0) {
+                    const float *sm = st + 32 * nb + i;
+                    dst[0] = fmaxf(fmaxf(sm[0], sm[32 * NB]), fmaxf(sm[64 * NB], sm[96 * NB]));
+                    dst[1] = total;
+                }
+#pragma unroll
+                for (int k = 0; k < 16; k++) dst[4 + ch + k] = s0[k] + s1[k];
+            } else {
+                const float inv = total == 0.f ? 0.f : 1.f / total;         // (a row that sees no token: zeroes)
+                uint32_t o[8];
+#pragma unroll
+                for (int k = 0; k < 8; k++) {
+                    const float a = (s0[2 * k] + s1[2 * k]) * inv, d = (s0[2 * k + 1] + s1[2 * k + 1]) * inv;
+                    o[k] = BF ? pack_bf16(a, d) : pack_f16(a, d);
+                }
+                u4 *dst = reinterpret_cast<u4 *>(p.out + (int64_t)b * p.o_b + head * p.o_h + token * p.o_t + ch);
+                dst[0] = (u4){o[0], o[1], o[2], o[3]};
+                dst[1] = (u4){o[4], o[5], o[6], o[7]};
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The runs' partials of a row become its result: eight rows a workgroup, four channels a lane.
+template <bool BF>
+__global__ void __launch_bounds__(256) chunk_merge_kernel(const float *__restrict__ part, uint16_t *__restrict__ out, int64_t rows, int Hq, int n,
+                                                          int nsplit, int64_t o_b, int64_t o_h, int64_t o_t) {
+    const int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (r >= rows) return;
+    const int c = threadIdx.x & 31;
+    const float *src = part + r * nsplit * kPart;
+    float m = kLowest;
+    for (int s = c; s < nsplit; s += 32) m = fmaxf(m, src[(int64_t)s * kPart]);
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, 32));
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < nsplit; s++) {
+        const float *at = src + (int64_t)s * kPart;
+        const float f = __builtin_amdgcn_exp2f(at[0] - m);
+        const float4 v = *reinterpret_cast<const float4 *>(at + 4 + 4 * c);
+        l += f * at[1];
+        o.x += f * v.x; o.y += f * v.y; o.z += f * v.z; o.w += f * v.w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int64_t token = r % n, head = r / n % Hq, b = r / n / Hq;
+    uint2 *dst = reinterpret_cast<uint2 *>(out + b * o_b + head * o_h + token * o_t + 4 * c);
+    *dst = BF ? make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv))
+              : make_uint2(pack_f16(o.x * inv, o.y * inv), pack_f16(o.z * inv, o.w * inv));
+}
+
+// How a call is cut: rows a workgroup, runs of tiles.  Workgroups are wanted for two a CU (512); a run of one tile is the least.
+static void chunk_cut(const pkv_chunk_args *a, int &nb, int &row_tiles, int &tiles, int &run, int &nsplit) {
+    const int64_t rows = (int64_t)a->n * (a->Hq / a->Hkv);
+    nb = rows <= 32 ? 1 : 2;
+    row_tiles = (int)((rows + 32 * nb - 1) / (32 * nb));
+    tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
+    const int64_t groups = (int64_t)a->B * a->Hkv * row_tiles;
+    int64_t want = (512 + groups - 1) / groups;
+    if (want > tiles) want = tiles;
+    run = (int)((tiles + want - 1) / want);
+    nsplit = (tiles + run - 1) / run;
+}
+
+static int chunk_check(const pkv_chunk_args *a) {
+    PKV_REQUIRE(a != nullptr, PKV_ERR_INVALID, "null pointer argument");
+    PKV_REQUIRE(a->dtype == PKV_F16 || a->dtype == PKV_BF16, PKV_ERR_UNSUPPORTED, "Unsupported data type");
+    PKV_REQUIRE(a->B > 0 && a->Hkv > 0 && a->n > 0 && a->Hq > 0 && a->Hq % a->Hkv == 0, PKV_ERR_INVALID, "Hq must be a multiple of Hkv, all sizes positive");
+    PKV_REQUIRE(a->T_c >= 0 && a->T_w >= 0 && (int64_t)a->T_c + a->T_w > 0 && (int64_t)a->T_c + a->T_w < (1ll << 30), PKV_ERR_INVALID, "empty cache");
+    PKV_REQUIRE(a->T_c % kChunkTile == 0, PKV_ERR_INVALID, "compressed length must be a multiple of 128 tokens");
+    PKV_REQUIRE(!a->causal || a->n <= a->T_c + a->T_w, PKV_ERR_INVALID, "more queries than tokens");
+    PKV_REQUIRE((int64_t)a->n * (a->Hq / a->Hkv) < (1ll << 30) && (int64_t)a->B * a->Hkv < (1ll << 24), PKV_ERR_UNSUPPORTED, "batch x queries too large");
+    return PKV_OK;
+}
+
+}  // namespace pkv
+
+extern "C" {
+
+uint64_t pkv_attn_chunk_workspace(const pkv_chunk_args *a) {
+    using namespace pkv;
+    if (chunk_check(a)) return 0;
+    int nb, row_tiles, tiles, run, nsplit;
+    chunk_cut(a, nb, row_tiles, tiles, run, nsplit);
+    return nsplit > 1 ? (uint64_t)a->B * a->Hq * a->n * nsplit * kPart * sizeof(float) : 0;
+}
+
+int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_bytes, pkv_stream_t s_) {
+    using namespace pkv;
+    hipStream_t s = (hipStream_t)s_;
+    const int bad = chunk_check(a);
+    if (bad) return bad;
+    PKV_REQUIRE(a->q && a->out, PKV_ERR_INVALID, "null pointer argument");
+    uint64_t off = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->out);
+    for (int i = 0; i < 3; i++) off |= 2u * (uint64_t)(a->q_stride[i] | a->out_stride[i]);
+    PKV_REQUIRE((off & 15u) == 0, PKV_ERR_INVALID, "rows of q and out must start on 16-byte boundaries");
+    ChunkParams p;
+    p.par_stride = a->par_stride ? a->par_stride : a->T_c;
+    p.win_stride = a->win_stride ? a->win_stride : a->T_w;
+    PKV_REQUIRE(p.par_stride >= a->T_c && p.win_stride >= a->T_w, PKV_ERR_INVALID, "row stride shorter than the row");
+    if (a->T_c > 0) {
+        PKV_REQUIRE(a->k_stream && a->k_info && a->v_stream && a->v_info && a->k_scale && a->k_zero && a->v_scale && a->v_zero, PKV_ERR_INVALID,
+                    "null pointer argument");
+        PKV_REQUIRE(a->k_bits >= 2 && a->k_bits <= kMaxBits && a->v_bits >= 2 && a->v_bits <= kMaxBits, PKV_ERR_UNSUPPORTED,
+                    "not supported: bits_len outside 2..8");
+        PKV_REQUIRE(a->k_bytes > 0 && a->v_bytes > 0 && a->k_bytes < (1ull << 32) - 4 && a->v_bytes < (1ull << 32) - 4, PKV_ERR_INVALID,
+                    "stream sizes must be in 1 .. 4 GiB - 5");
+        PKV_REQUIRE(((reinterpret_cast<uintptr_t>(a->k_stream) | reinterpret_cast<uintptr_t>(a->v_stream)) & 15u) == 0, PKV_ERR_INVALID,
+                    "streams must be 16-byte aligned");
+        PKV_REQUIRE((uint64_t)(a->T_c / 64) * (uint64_t)a->B * a->Hkv < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x tokens too large");
+    }
+    if (a->T_w > 0)
+        PKV_REQUIRE(a->k_win && a->v_win && ((reinterpret_cast<uintptr_t>(a->k_win) | reinterpret_cast<uintptr_t>(a->v_win)) & 15u) == 0, PKV_ERR_INVALID,
+                    "window tensors must be present and 16-byte aligned");
+    int nb;
+    chunk_cut(a, nb, p.row_tiles, p.tiles, p.run, p.nsplit);
+    const uint64_t need = p.nsplit > 1 ? (uint64_t)a->B * a->Hq * a->n * p.nsplit * kPart * sizeof(float) : 0;
+    PKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0), PKV_ERR_CAPACITY,
+                "the call needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
+    p.k_stream = a->k_stream; p.v_stream = a->v_stream; p.k_info = a->k_info; p.v_info = a->v_info;
+    p.k_scale = (const uint16_t *)a->k_scale; p.k_zero = (const uint16_t *)a->k_zero;
+    p.v_scale = (const uint16_t *)a->v_scale; p.v_zero = (const uint16_t *)a->v_zero;
+    p.k_win = (const uint16_t *)a->k_win; p.v_win = (const uint16_t *)a->v_win;
+    p.q = (const uint16_t *)a->q; p.out = (uint16_t *)a->out;
+    p.part = need ? (float *)workspace : nullptr;
+    p.starts = a->starts;
+    p.q_b = a->q_stride[0]; p.q_h = a->q_stride[1]; p.q_t = a->q_stride[2];
+    p.o_b = a->out_stride[0]; p.o_h = a->out_stride[1]; p.o_t = a->out_stride[2];
+    p.k_bytes = a->k_bytes; p.v_bytes = a->v_bytes;
+    p.Hq = a->Hq; p.Hkv = a->Hkv; p.BH = a->B * a->Hkv; p.G = a->Hq / a->Hkv; p.n = a->n; p.rows = a->n * p.G;
+    p.T_c = a->T_c; p.T_w = a->T_w; p.causal = a->causal != 0;
+    p.k_bits = a->T_c ? a->k_bits : 2; p.v_bits = a->T_c ? a->v_bits : 2;
+    p.tiles_c = a->T_c / kChunkTile;
+    p.sm_log2 = a->sm_scale * kLog2e;
+    const uint32_t k_cap = (uint32_t)k_block_bound(64, p.k_bits), v_cap = (uint32_t)v_block_bound(64, p.v_bits);
+    p.slot = (((k_cap > v_cap ? k_cap : v_cap) + 15u) & ~15u) + 32u;       // a block at any phase, and a last word's reach
+    p.ring = 8u * p.slot;
+    if (p.ring < 4u * 32u * kVRow) p.ring = 4u * 32u * kVRow;               // (the end's sums take less: 2 x 32 x 129 floats)
+    const bool wide = p.k_bits > 4 || p.v_bits > 4, bf = a->dtype == PKV_BF16;
+    const uint32_t lds = p.ring + 4u * 32u * kKRow + 4096u + 2048u + 8u * 32u * nb * 4u + 32u * nb * kQRow;
+    const uint64_t groups = ((uint64_t)p.BH * p.nsplit + 7) / 8, wgs = groups * 8 * (uint64_t)p.row_tiles;
+    PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x queries too large");
+    const void *kernels[2][2][2] = {
+        {{(const void *)attn_chunk_kernel<false, 1, false>, (const void *)attn_chunk_kernel<false, 1, true>},
+         {(const void *)attn_chunk_kernel<false, 2, false>, (const void *)attn_chunk_kernel<false, 2, true>}},
+        {{(const void *)attn_chunk_kernel<true, 1, false>, (const void *)attn_chunk_kernel<true, 1, true>},
+         {(const void *)attn_chunk_kernel<true, 2, false>, (const void *)attn_chunk_kernel<true, 2, true>}}};
+    const void *kernel = kernels[bf][nb - 1][wide];
+    PKV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    void *params[] = {&p};
+    PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256), params, lds, s));
+    if (need) {
+        const int64_t rows = (int64_t)a->B * a->Hq * a->n;
+        const dim3 grid((unsigned)((rows + 7) / 8));
+        if (bf) chunk_merge_kernel<true><<<grid, 256, 0, s>>>(p.part, p.out, rows, a->Hq, a->n, p.nsplit, p.o_b, p.o_h, p.o_t);
+        else chunk_merge_kernel<false><<<grid, 256, 0, s>>>(p.part, p.out, rows, a->Hq, a->n, p.nsplit, p.o_b, p.o_h, p.o_t);
+        PKV_HIP_CHECK(hipGetLastError());
+    }
+    return PKV_OK;
+}
+
+}  // extern "C"

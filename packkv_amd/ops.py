@@ -22,7 +22,7 @@ __all__ = [
     "k_encode", "v_encode", "k_decode", "v_decode",
     "quant_params", "quantize", "dequantize", "k_quant_encode", "v_quant_encode",
     "attn_decode", "AttnPlan", "block_bound", "bits_for_rel", "repack_quant_encode", "encode_status",
-    "norm_rotary", "window_append_rotary",
+    "norm_rotary", "window_append_rotary", "attn_chunk",
 ]
 
 
@@ -1277,6 +1277,84 @@ def dense_view(k, v, k_win=None, v_win=None, win_len=None):
         rc = _lib.load().pkv_dense_view(ctypes.byref(a), _ptr(k_out), _ptr(v_out), _stream(dev))
     _lib.check(rc)
     return k_out, v_out
+
+
+def _chunk_rows(x):
+    """x [B, H, n, 128] as the chunk kernel reads its rows: in place where they start on 16-byte boundaries."""
+    return x if _rows16(x, _strides(x)) else _copy(x)
+
+
+def attn_chunk(q, k, v, k_win=None, v_win=None, sm_scale=None, out=None, win_len=None, starts=None, causal=True):
+    """attn_decode for several new tokens: q [B, Hq, n, 128] are the queries of the cache's last n tokens, whose keys and values k, v
+    (dicts as attn_decode takes them, or None) and the windows hold already.  Query i attends to tokens starts[b] .. T - n + i of the T
+    tokens, with causal=False to all of them from starts[b] on; starts, an int32 tensor [B], is for batches padded on the left (what
+    lies in the padding may be anything).  A query that sees no token gets zeroes.  Strided queries (a transposed projection output)
+    are read in place; the result has their layout unless `out` is given.  Widths 2..8, any number of query heads to a KV head."""
+    _require(q.is_cuda and q.dim() == 4 and q.size(3) == 128, "q must be a device tensor [B, Hq, n, 128]")
+    B, Hq, n, _ = q.shape
+    at, dtype = q.get_device(), q.dtype
+    a = _lib.ChunkArgs()
+    a.dtype = _dtype_code(q)
+    T_c, Hkv, keep = 0, None, []
+    _require((k is None) == (v is None) and (k_win is None) == (v_win is None), "K and V go together")
+    if k is not None:
+        T_c = int(k.get("tokens", k["scale"].size(1)))
+        _require(int(v.get("tokens", v["scale"].size(1))) == T_c, "K and V hold different token counts")
+        _require(T_c > 0 and T_c % 128 == 0, "compressed length must be a multiple of 128 tokens")
+        for d in (k, v):
+            _require(all(d[f].get_device() == at and d[f].is_contiguous() for f in ("stream", "info", "scale", "zero")),
+                     "stream, info, scale and zero must be contiguous and on q's device")
+            _require(d["scale"].dtype == dtype and d["zero"].dtype == dtype and d["scale"].shape == k["scale"].shape == d["zero"].shape
+                     and d["scale"].size(0) == B and T_c <= d["scale"].size(1) and d["stream"].dtype == torch.uint8 and d["info"].dtype == torch.uint32,
+                     "scale / zero must be [B, >= tokens] of q's dtype, streams uint8, block_info uint32")
+        Hkv = int(k["heads"]) if "heads" in k else k["info"].numel() // 2 // (T_c // 64) // max(B, 1)
+        _require(Hkv > 0 and all(d["info"].numel() // 2 >= (T_c // 64) * B * Hkv for d in (k, v)), "block_info_buffer block num mismatch")
+        ks, vs = (d["stream"] if d["stream"].data_ptr() % 16 == 0 else _copy(d["stream"]) for d in (k, v))
+        keep += [ks, vs]
+        a.k_stream, a.v_stream, a.k_bytes, a.v_bytes = ks.data_ptr(), vs.data_ptr(), ks.numel(), vs.numel()
+        a.k_info, a.k_scale, a.k_zero = (k[f].data_ptr() for f in ("info", "scale", "zero"))
+        a.v_info, a.v_scale, a.v_zero = (v[f].data_ptr() for f in ("info", "scale", "zero"))
+        a.k_bits, a.v_bits, a.par_stride = int(k["bits"]), int(v["bits"]), k["scale"].size(1)
+    T_w = 0
+    if k_win is not None:
+        T_w = k_win.size(2) if win_len is None else int(win_len)
+        _require(k_win.get_device() == at and v_win.get_device() == at and k_win.is_contiguous() and v_win.is_contiguous() and k_win.dim() == 4
+                 and v_win.shape == k_win.shape and k_win.size(0) == B and k_win.size(3) == 128 and k_win.dtype == dtype and v_win.dtype == dtype,
+                 "window tensors must be contiguous [B, Hkv, cap, 128] of q's dtype on its device")
+        _require(0 <= T_w <= k_win.size(2), "win_len outside the window tensors")
+        _require(Hkv is None or Hkv == k_win.size(1), "window head count mismatch")
+        Hkv = k_win.size(1)
+        if T_w and (k_win.data_ptr() | v_win.data_ptr()) % 16:
+            k_win, v_win = _copy(k_win), _copy(v_win)
+            keep += [k_win, v_win]
+        a.k_win, a.v_win, a.win_stride = k_win.data_ptr(), v_win.data_ptr(), k_win.size(2)
+    _require(Hkv is not None and T_c + T_w > 0, "empty cache")
+    _require(Hq % Hkv == 0, "Hq must be a multiple of Hkv")
+    _require(not causal or n <= T_c + T_w, "more queries than tokens")
+    if starts is not None:
+        _require(starts.shape == (B,) and starts.dtype == torch.int32 and starts.get_device() == at, "starts must be int32 [B] on q's device")
+        starts = starts.contiguous()
+        a.starts = starts.data_ptr()
+    if out is None:
+        out = torch.empty_like(q)
+    else:
+        _require(out.shape == q.shape and out.dtype == dtype and out.get_device() == at, "out must match q's shape, dtype and device")
+        _require(0 not in (st for st, w in zip(out.stride(), out.shape) if w > 1), "out must not share elements")
+    if q.numel() == 0:
+        return out
+    q = _chunk_rows(q)
+    res = out if _rows16(out, _strides(out)) else torch.empty(q.shape, dtype=dtype, device=q.device)
+    a.q, a.out = q.data_ptr(), res.data_ptr()
+    a.q_stride[:], a.out_stride[:] = _strides(q)[:3], _strides(res)[:3]
+    a.B, a.Hq, a.Hkv, a.n, a.T_c, a.T_w, a.causal = B, Hq, Hkv, n, T_c, T_w, int(bool(causal))
+    a.sm_scale = float(sm_scale if sm_scale is not None else 128 ** -0.5)
+    lib, ref = _lib.load(), ctypes.byref(a)
+    with _on(q.device):
+        need = lib.pkv_attn_chunk_workspace(ref)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        rc = lib.pkv_attn_chunk(ref, ws.data_ptr() if need else None, need, _stream(q.device))
+    _lib.check(rc)
+    return out if res is out else out.copy_(res)
 
 
 class AttnPlan:
