@@ -439,6 +439,31 @@ typedef struct pkv_chunk_args {
 uint64_t pkv_attn_chunk_workspace(const pkv_chunk_args *args);
 int pkv_attn_chunk(const pkv_chunk_args *args, void *workspace, uint64_t workspace_bytes, pkv_stream_t s);
 
+/* ---- sampling --------------------------------------------------------------------------
+ * pkv_sample: a token for each row of logits [rows, vocab] (`dtype` PKV_F16, PKV_BF16 or PKV_F32; row_stride elements from row to
+ * row) from the row's uniform number u in [0, 1).  The row's order is logit descending, equal logits (-0 equals 0) by index; -inf
+ * and NaN are never chosen; weights are exp((logit - max) / temperature).  In this order: the first top_k tokens are kept (0 or
+ * less: all); of them those with less than top_p times their mass in front of them (1 or more, or NaN: all; the first always); of
+ * them those whose weight is at least min_p times the first's (0 or less, or NaN: all).  The token is the first of the order
+ * whose mass with all in front of it exceeds u times the mass kept.  Temperature 0 (or less, or NaN): the first of the order.  A
+ * row in which nothing can be chosen gives token -1.  temperature, top_k, top_p, min_p: device arrays [rows], or NULL and the _all
+ * numbers for every row.  token [rows] int64; logprob [rows] fp32 (NULL: none): log of the token's share of the mass kept (-inf
+ * with token -1).  Weights in fp64, sums as whole numbers: the same token whatever the launch.  vocab at most 2^20.  `workspace` as
+ * in pkv_attn_chunk.  No counterpart in the reference. */
+#define PKV_F32 2
+typedef struct pkv_sample_args {
+    const void *logits;
+    const float *u, *temperature, *top_p, *min_p;
+    const int32_t *top_k;
+    int64_t *token;
+    float *logprob;
+    int64_t row_stride;
+    int dtype, rows, vocab, top_k_all;
+    float temperature_all, top_p_all, min_p_all;
+} pkv_sample_args;
+uint64_t pkv_sample_workspace(const pkv_sample_args *args);
+int pkv_sample(const pkv_sample_args *args, void *workspace, uint64_t workspace_bytes, pkv_stream_t s);
+
 /* pkv_stream_release: gives back the device memory the library keeps for stream `s` of the current device -- its
  * scratch buffers (attention partials, the encoders' look-back state), its tile counters and every buffer it has
  * outgrown (kept until now because a captured HIP graph might still hold its address).  It has no counterpart in the

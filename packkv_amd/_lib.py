@@ -14,7 +14,7 @@ LIB_PATH = os.environ.get("PACKKV_HIP_LIB") or os.path.join(_HERE, "libpackkv_hi
 HOST_SYMBOLS = ("pkv_attn_decode", "pkv_window_append", "pkv_dense_view", "pkv_kq_mat_vec_mul", "pkv_wv_mat_vec_mul", "pkv_fused_kq",
                 "pkv_fused_wv")
 
-F16, BF16 = 0, 1
+F16, BF16, F32 = 0, 1, 2
 OK, ERR_UNSUPPORTED, ERR_INVALID, ERR_HIP, ERR_CAPACITY, ERR_INTERNAL = range(6)
 ATTN_REF_ROUNDING, ATTN_OUT_F32 = 1, 2
 
@@ -69,6 +69,11 @@ class ChunkArgs(ctypes.Structure):
                 [("sm_scale", _f)])
 
 
+class SampleArgs(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("logits", "u", "temperature", "top_p", "min_p", "top_k", "token", "logprob")] + [("row_stride", _i64)] +
+                [(n, _i) for n in ("dtype", "rows", "vocab", "top_k_all")] + [(n, _f) for n in ("temperature_all", "top_p_all", "min_p_all")])
+
+
 # name -> (restype, argtypes); every symbol include/packkv.h declares
 SIGNATURES = {
     "pkv_abi_version": (_i, []),
@@ -115,6 +120,8 @@ SIGNATURES = {
     "pkv_dense_view": (_i, [ctypes.POINTER(AttnArgs), _vp, _vp, _vp]),
     "pkv_attn_chunk_workspace": (_u64, [ctypes.POINTER(ChunkArgs)]),
     "pkv_attn_chunk": (_i, [ctypes.POINTER(ChunkArgs), _vp, _u64, _vp]),
+    "pkv_sample_workspace": (_u64, [ctypes.POINTER(SampleArgs)]),
+    "pkv_sample": (_i, [ctypes.POINTER(SampleArgs), _vp, _u64, _vp]),
     "pkv_stream_release": (_i, [_vp]),
 }
 

@@ -22,7 +22,7 @@ __all__ = [
     "k_encode", "v_encode", "k_decode", "v_decode",
     "quant_params", "quantize", "dequantize", "k_quant_encode", "v_quant_encode",
     "attn_decode", "AttnPlan", "block_bound", "bits_for_rel", "repack_quant_encode", "encode_status",
-    "norm_rotary", "window_append_rotary", "attn_chunk",
+    "norm_rotary", "window_append_rotary", "attn_chunk", "sample",
 ]
 
 
@@ -1234,6 +1234,63 @@ def fused_wv(our_wv, w, v_quant_zero, v_quant_scale, term1):
     del w_c, z_c, s_c, t_c
     _lib.check(rc)
     return float(ms.value)
+
+
+# ------------------------------------------------------------------ sampling ---------
+
+def _row_setting(a, name, x, rows, dtype, at, keep):
+    """A sampling setting into the arguments: a number for all rows, or a device tensor [rows]."""
+    if not torch.is_tensor(x):
+        setattr(a, name + "_all", x)
+        return
+    _require(x.shape == (rows,) and x.dtype == dtype and x.get_device() == at, "%s must be a number or a %s tensor [rows] on the logits' device"
+             % (name, str(dtype).split(".")[-1]))
+    x = x.contiguous()
+    keep.append(x)
+    setattr(a, name, x.data_ptr())
+
+
+def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, want_logprob=False):
+    """A token, int64 [rows], for each row of logits [rows, vocab] (fp16, bf16 or fp32; at most 2^20 tokens) from uniform numbers u [rows]
+    float32 in [0, 1).  In this order: the top_k largest logits are kept (0: all), of them the smallest set that holds top_p of their
+    mass (1: all), of them those at least min_p times as likely as the first (0: all); the draw goes through what is left, most likely
+    first.  Equal logits are ordered by index.  temperature 0 takes the first.  Every setting is a number or a device tensor [rows]
+    (float32; top_k int32; numbers are rounded to float32).  -inf and NaN are never chosen; a row with nothing else gives -1.  With
+    want_logprob returns (tokens, log-probabilities float32 [rows]) under the filtered distribution.  The same numbers give the same
+    token on every call and for every batch size."""
+    _require(logits.is_cuda and logits.dim() == 2 and logits.size(1) > 0, "logits must be a device tensor [rows, vocab]")
+    R, V = logits.shape
+    at, dev, keep = logits.get_device(), logits.device, []
+    a = _lib.SampleArgs()
+    if logits.dtype == torch.float32:
+        a.dtype = _lib.F32
+    else:
+        a.dtype = _dtype_code(logits)
+    _require(V <= 1 << 20, "not supported: %d tokens (at most 2^20)" % V)
+    _require(u.shape == (R,) and u.dtype == torch.float32 and u.get_device() == at, "u must be a float32 tensor [rows] on the logits' device")
+    for name, x, ok in (("temperature", temperature, lambda x: x >= 0), ("top_k", top_k, lambda x: x >= 0 and x == int(x) and x < 1 << 31),
+                        ("top_p", top_p, lambda x: 0 <= x <= 1), ("min_p", min_p, lambda x: 0 <= x <= 1)):
+        _require(torch.is_tensor(x) or ok(x), "%s is out of range" % name)
+        _row_setting(a, name, int(x) if name == "top_k" and not torch.is_tensor(x) else x, R, torch.int32 if name == "top_k" else torch.float32, at, keep)
+    if out is None:
+        out = torch.empty(R, dtype=torch.int64, device=dev)
+    else:
+        _require(out.shape == (R,) and out.dtype == torch.int64 and out.get_device() == at and out.is_contiguous(),
+                 "out must be a contiguous int64 tensor [rows] on the logits' device")
+    logprob = torch.empty(R, dtype=torch.float32, device=dev) if want_logprob else None
+    if R:
+        if logits.stride(1) != 1 and V > 1:
+            logits = logits.contiguous()
+        u = u.contiguous()
+        a.logits, a.u, a.token, a.logprob = logits.data_ptr(), u.data_ptr(), out.data_ptr(), logprob.data_ptr() if want_logprob else None
+        a.row_stride, a.rows, a.vocab = logits.stride(0) if R > 1 else 0, R, V
+        lib, ref = _lib.load(), ctypes.byref(a)
+        with _on(dev):
+            need = lib.pkv_sample_workspace(ref)
+            ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+            rc = lib.pkv_sample(ref, ws.data_ptr() if need else None, need, _stream(dev))
+        _lib.check(rc)
+    return (out, logprob) if want_logprob else out
 
 
 # ------------------------------------------------- fused decompress-attention --------
