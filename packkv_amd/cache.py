@@ -128,6 +128,12 @@ class PackKVCompressedCache:
                                     self.device)
         return self.layers[i]
 
+    def _cut(self, L, n):
+        """(tokens in the buffer with n new ones, how many of them leave it) for a layer."""
+        cfg = self.config
+        total = L.win_len - L.pend + n
+        return total, max((total + cfg.block_size - total % cfg.block_size - cfg.buffer_size) // cfg.block_size, 0) * cfg.block_size
+
     # -- reference contract --------------------------------------------------------------------------
     def update(self, key_states, value_states, layer_idx, cache_kwargs=None, return_dense=True):
         """Append key_states / value_states [B, H, n, 128].  Returns the dense (K, V) [B, H, T, 128] the reference's
@@ -138,10 +144,7 @@ class PackKVCompressedCache:
         cfg = self.config
         rotary = bool(cache_kwargs) and cache_kwargs.get("cos") is not None
         n = key_states.size(2)
-        buf_len = L.win_len - L.pend
-        total = buf_len + n
-        n_blk = max((total + cfg.block_size - total % cfg.block_size - cfg.buffer_size) // cfg.block_size, 0)
-        n_cut = n_blk * cfg.block_size
+        total, n_cut = self._cut(L, n)
         if n_cut == 0 and L.win_len + n <= L.cap:                 # the common decode step: rotary + the new rows, one launch
             ops.window_append(key_states, value_states, cache_kwargs["cos"] if rotary else None,
                               cache_kwargs["sin"] if rotary else None, L.k_win, L.v_win, L.win_len)
@@ -182,23 +185,47 @@ class PackKVCompressedCache:
             return self.materialize(layer_idx)
         return None
 
+    def update_rotary(self, query_states, key_states, value_states, layer_idx, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6,
+                      sections=None, interleaved=False):
+        """``update`` for raw projections: the head norms and the rotary embedding of ops.norm_rotary (its arguments) on
+        query_states [B, Hq, n, 128] and key_states, which go into the cache with value_states.  Returns the queries, for
+        ``attend``.  A step that cuts nothing is one launch (ops.window_append_rotary)."""
+        L, n = self._layer(layer_idx), key_states.size(2)
+        if self._cut(L, n)[1] == 0 and L.win_len + n <= L.cap:
+            q = ops.window_append_rotary(query_states, key_states, value_states, positions, inv_freq, L.k_win, L.v_win, L.win_len, q_norm, k_norm,
+                                         eps, sections, interleaved)
+            L.win_len += n
+            return q
+        q, k = ops.norm_rotary(query_states, key_states, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
+        self.update(k, value_states, layer_idx, return_dense=False)
+        return q
+
     def get_seq_length(self, layer_idx=0):
         L = self.layers[layer_idx or 0]
         return 0 if L is None else L.k.tokens + L.win_len
 
     # -- hot path ------------------------------------------------------------------------------------
-    def attend(self, query_states, layer_idx, sm_scale=None, out=None, variant=0, ref_rounding=False, out_f32=False):
+    def attend(self, query_states, layer_idx, sm_scale=None, out=None, variant=0, ref_rounding=False, out_f32=False, starts=None):
         """One decode step: query_states [B, Hq, 128] (or [B, Hq, 1, 128]) against everything cached in the
         layer; returns [B, Hq, 128] (same rank as given).  variant / ref_rounding / out_f32 select the checking
-        kernels of ops.attn_decode (not cached as a plan)."""
+        kernels of ops.attn_decode (not cached as a plan).  [B, Hq, n, 128] with n > 1: the queries of the last n cached
+        tokens, each against the tokens up to its own (ops.attn_chunk); `starts` (int32 [B]): every sequence's first token,
+        of a batch padded on the left."""
         L = self.layers[layer_idx] or self._layer(layer_idx)
         q = query_states
         plan, rows = L.plan, L.win_len
-        if plan is not None and plan.sm_scale_arg == sm_scale and rows and out is None and not (variant or ref_rounding or out_f32):
+        if plan is not None and plan.sm_scale_arg == sm_scale and rows and out is None and starts is None and not (variant or ref_rounding or out_f32):
             res = plan.step(q, rows)
             if res is not None:
                 return res
         squeeze = q.dim() == 4
+        if starts is not None or (squeeze and q.size(2) != 1):
+            if variant or ref_rounding or out_f32:
+                raise RuntimeError("not supported: the checking kernels take one unpadded token a sequence")
+            k, v = (side.as_dict() if side.tokens else None for side in (L.k, L.v))
+            q4, o4 = (q, out) if squeeze else (q.unsqueeze(2), out.unsqueeze(2) if out is not None else None)
+            res = ops.attn_chunk(q4, k, v, L.k_win if L.win_len else None, L.v_win if L.win_len else None, sm_scale, o4, L.win_len or None, starts)
+            return res if squeeze else res.squeeze(2)
         if squeeze:
             q = q[:, :, 0]
         q = q.contiguous()

@@ -11,13 +11,16 @@ meets its cache (models/llama.py:242-294, and models/qwen3.py:175-198 for the pe
 At decode time (one new token) ``attention="fused"`` replaces the last two lines by ``cache.update(...,
 return_dense=False)`` and ``cache.attend(q, layer)``, the fused decompress-attention kernel;
 ``attention="dense"`` keeps the reference's decompress-then-attend through ``cache.materialize``.  Prefill always
-attends to the dense tensors the cache returns, as the reference does.
+attends to the dense tensors the cache returns, as the reference does.  A later prompt, several tokens on a cache that holds
+some, attends through the fused kernel too.  ``rotary="fused"`` replaces the head norms and the rotary embedding of both
+sides by ``cache.update_rotary``, one pass that rounds once; ``generate`` decodes that way and samples.
 """
 import math
 
 import torch
 import torch.nn.functional as F
 
+from . import ops
 from .cache import PackKVCompressedCache, PackKVCacheConfig, rotate_half
 
 
@@ -25,9 +28,10 @@ class DecoderShape:
     """Qwen3-8B by default: 36 layers, hidden 4096, 32 query / 8 KV heads of 128, MLP 12288, vocabulary 151936."""
 
     def __init__(self, layers=36, hidden=4096, q_heads=32, kv_heads=8, head_dim=128, mlp=12288, vocab=151936,
-                 rope_theta=1.0e6, rms_eps=1.0e-6, head_norm=True):
+                 rope_theta=1.0e6, rms_eps=1.0e-6, head_norm=True, rope_sections=None, rope_interleaved=False):
         self.layers, self.hidden, self.q_heads, self.kv_heads, self.head_dim = layers, hidden, q_heads, kv_heads, head_dim
         self.mlp, self.vocab, self.rope_theta, self.rms_eps, self.head_norm = mlp, vocab, rope_theta, rms_eps, head_norm
+        self.rope_sections, self.rope_interleaved = rope_sections, rope_interleaved      # position axes (ops.norm_rotary)
 
 
 def _rms(x, w, eps):
@@ -92,7 +96,8 @@ class ShapedDecoder:
     def _dense_attention(self, q, k, v, scaling):
         """Decode step (one query token): the reference's eager attention (models/llama.py:189-212: fp32 softmax
         cast back to the storage dtype), with the query heads of a group stacked instead of K / V repeated.
-        Prompt pass: the library's causal attention, a few sequences at a time."""
+        Prompt pass: the library's causal attention, a few sequences at a time (behind cached tokens with a mask of its
+        own: the library's would count both from the first token)."""
         B, Hq, n, D = q.shape
         Hkv = k.size(1)
         if n == 1:
@@ -101,31 +106,52 @@ class ShapedDecoder:
             w = F.softmax(w, dim=-1, dtype=torch.float32).to(q.dtype)
             return torch.matmul(w, v).reshape(B, Hq, 1, D)
         out = torch.empty_like(q)
+        T = k.size(2)
+        mask = None if T == n else torch.ones(n, T, dtype=torch.bool, device=q.device).tril(T - n)
         for b in range(0, B, 4):
-            out[b:b + 4] = F.scaled_dot_product_attention(q[b:b + 4], k[b:b + 4], v[b:b + 4], is_causal=True,
+            out[b:b + 4] = F.scaled_dot_product_attention(q[b:b + 4], k[b:b + 4], v[b:b + 4], attn_mask=mask, is_causal=mask is None,
                                                           scale=scaling, enable_gqa=True)
         return out
 
     @torch.no_grad()
-    def forward(self, ids, cache, attention="fused", taps=None):
+    def forward(self, ids, cache, attention="fused", taps=None, rotary="chain", positions=None):
         """ids [B, n] continue the sequences held in `cache`; returns the logits of the last position [B, vocab]
         (fp32).  `taps`, a list, receives every layer's (rotated query, attention output), both [B, Hq, n, 128],
-        when given."""
+        when given.  rotary="fused": norms and rotary embedding through ops.norm_rotary, at `positions` (default: counted
+        on from the cache's tokens), several axes with shape.rope_sections; "chain": library operators, one axis."""
         s = self.shape
         B, n = ids.shape
         pos0 = cache.get_seq_length(0)
+        one_pass = rotary == "fused"
+        if one_pass:
+            if positions is None:
+                positions = torch.arange(pos0, pos0 + n, device=self.device)
+        elif positions is not None or s.rope_sections is not None:
+            raise RuntimeError("not supported: positions of their own need rotary=\"fused\"")
         cos, sin = self._rotary(pos0, n, B)
-        fused = attention == "fused" and n == 1
+        fused = attention == "fused" and (n == 1 or pos0 > 0)
         scaling = 1.0 / math.sqrt(s.head_dim)
         half = s.head_dim // 2
         sin_signed = torch.cat((-sin[..., :half], sin[..., half:]), dim=-1)
-        nq = s.q_heads * s.head_dim
         kw = {"cos": cos, "sin": sin}
         h = self.embed[ids].view(B * n, s.hidden)
         for li, blk in enumerate(self.blocks):
             x = _rms(h, blk["in_norm"], s.rms_eps)
             qkv = F.linear(x, blk["qkv"]).view(B, n, s.q_heads + 2 * s.kv_heads, s.head_dim)
             q, k, v = qkv[:, :, :s.q_heads], qkv[:, :, s.q_heads:s.q_heads + s.kv_heads], qkv[:, :, s.q_heads + s.kv_heads:]
+            if one_pass:
+                q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+                how = (positions, self.inv_freq, blk["q_norm"] if s.head_norm else None, blk["k_norm"] if s.head_norm else None, s.rms_eps,
+                       s.rope_sections, s.rope_interleaved)
+                if fused:
+                    q = cache.update_rotary(q, k, v, li, *how)
+                    a = cache.attend(q, li, sm_scale=scaling)
+                else:
+                    q, k = ops.norm_rotary(q, k, *how)
+                    kd, vd = cache.update(k, v, li, None, return_dense=True)
+                    a = self._dense_attention(q, kd, vd, scaling)
+                h = self._rest(blk, h, a, taps, q)
+                continue
             if s.head_norm:
                 q, k = _rms(q, blk["q_norm"], s.rms_eps), _rms(k, blk["k_norm"], s.rms_eps)
                 v = v.contiguous()                        # the cache reads K and V with one set of strides
@@ -137,15 +163,20 @@ class ShapedDecoder:
             else:
                 kd, vd = cache.update(k, v, li, kw, return_dense=True)
                 a = self._dense_attention(q, kd, vd, scaling)
-            if taps is not None:
-                taps.append((q, a))
-            h = torch.addmm(h, a.transpose(1, 2).reshape(B * n, nq), blk["o"].t())
-            x = _rms(h, blk["post_norm"], s.rms_eps)
-            gu = F.linear(x, blk["gate_up"])
-            h = torch.addmm(h, F.silu(gu[:, :s.mlp]) * gu[:, s.mlp:], blk["down"].t())
+            h = self._rest(blk, h, a, taps, q)
         h = h.view(B, n, s.hidden)
         h = _rms(h[:, -1], self.final_norm, s.rms_eps)
         return F.linear(h, self.lm_head).float()
+
+    def _rest(self, blk, h, a, taps, q):
+        """A layer behind its attention output a [B, Hq, n, 128]."""
+        s = self.shape
+        if taps is not None:
+            taps.append((q, a))
+        h = torch.addmm(h, a.transpose(1, 2).reshape(h.size(0), s.q_heads * s.head_dim), blk["o"].t())
+        x = _rms(h, blk["post_norm"], s.rms_eps)
+        gu = F.linear(x, blk["gate_up"])
+        return torch.addmm(h, F.silu(gu[:, :s.mlp]) * gu[:, s.mlp:], blk["down"].t())
 
     @torch.no_grad()
     def prefill(self, ids, cache):
@@ -161,4 +192,16 @@ class ShapedDecoder:
             nxt = logits.argmax(dim=-1, keepdim=True)
             out.append(nxt)
             logits = self.forward(nxt, cache, attention=attention)
+        return torch.cat(out, dim=1)
+
+    @torch.no_grad()
+    def generate(self, ids, cache, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """`ids` [B, n] (a first prompt, or a later one on a cache that holds tokens), then a sampled token for each row of u
+        [steps, B], uniform numbers in [0, 1); the settings as ops.sample takes them.  Returns the generated ids [B, steps]."""
+        logits = self.forward(ids, cache, attention="fused" if cache.get_seq_length(0) else "dense", rotary="fused")
+        out = []
+        for row in u:
+            nxt = ops.sample(logits, row, temperature, top_k, top_p, min_p).unsqueeze(1)
+            out.append(nxt)
+            logits = self.forward(nxt, cache, rotary="fused")
         return torch.cat(out, dim=1)
