@@ -1,10 +1,10 @@
 // A token for each row of logits from a given uniform number: temperature, top-k, top-p, min-p, and the draw.
 //
-// Order of a row: logit descending, equal logits by index.  Weight of a token: e = 2^a, a = (logit - max) log2(e) / T.  Each filter
-// keeps a prefix of the order -- the first k; the tokens with less than p of the k's mass before them; those with e >= min_p -- and
-// the draw takes the first token whose inclusive mass exceeds u times the mass kept.  So nothing is sorted as a whole: a histogram
-// of the row over 2048 bins of a (1/48 each, counts and masses) says in which bins a filter can end and in which the draw can fall;
-// only those bins' tokens are gathered, ordered and looked at one by one.
+// Order of a row: logit descending, equal logits by index.  Weight of a token: e = 2^-(y / 64), y = (max - logit) 64 log2(e) / T, its
+// place.  Each filter keeps a prefix of the order -- the first k; the tokens with less than p of the k's mass before them; those with
+// e >= min_p -- and the draw takes the first token whose inclusive mass exceeds u times the mass kept.  So nothing is sorted as a
+// whole: a histogram over the whole parts of y (2816 bins, counts and masses) says in which bins a filter can end and in which the
+// draw can fall; only those bins' tokens are gathered, ordered and looked at one by one.
 //
 // Exact whatever the order of the additions: weights are formed in fp64 and held as integers of 2^-43, their sums are whole numbers
 // (below 2^63 for 2^20 tokens), so a row gives the same token from any number of workgroups.  Two tokens of a row of 150000 are told
@@ -14,8 +14,11 @@
 
 namespace pkv {
 
-constexpr int kSampThreads = 1024, kBins = 2048, kCand = 2048, kFracBits = 43;
-constexpr double kBinsPerUnit = 48.0;
+constexpr int kSampThreads = 1024, kFracBits = 43;
+constexpr double kPerUnit = 64.0;                          // bins for each halving of the weight
+// Behind 44 halvings weights are below half of 2^-43: such tokens have no mass, so they are never drawn, and where a filter ends among
+// them makes no difference.  The bins go a little further, to three a thread.
+constexpr int kNoMass = 44 * 64, kBins = 3072, kCand = 3072, kMine = kBins / kSampThreads;           // (kCand: tokens looked at one by one)
 constexpr int kF32 = 2;                                    // (beside PKV_F16 and PKV_BF16)
 
 struct SampleParams {
@@ -31,46 +34,41 @@ struct SampleParams {
 
 // A row's filters.
 struct RowRule {
-    double per_unit, top_p, min_a, u;                      // a = (x - max) * per_unit; tokens need a >= min_a
+    double per_logit, top_p, last, u;                      // place y = (max - logit) * per_logit; min-p keeps y <= last
     uint32_t top_k;                                        // 0: off
     bool by_p, by_min;
 };
-__device__ __forceinline__ RowRule row_rule(const SampleParams &p, int row) {
+__device__ __forceinline__ RowRule row_rule(const SampleParams &p, int row, float largest) {
     RowRule r;
     float t = p.temperature ? p.temperature[row] : p.temperature_all;
     const float top = p.top_p ? p.top_p[row] : p.top_p_all, least = p.min_p ? p.min_p[row] : p.min_p_all;
     const int k = p.top_k ? p.top_k[row] : p.top_k_all;
     r.top_k = k > 0 ? (uint32_t)k : 0u;
     if (!(t > 0.f)) { t = 1.f; r.top_k = 1; }              // temperature 0: the first of the order
-    r.per_unit = 1.4426950408889634074 / (double)t;
+    r.per_logit = largest == INFINITY ? kPerUnit : kPerUnit * 1.4426950408889634074 / (double)t;   // (behind +inf at any temperature)
     r.by_p = top < 1.f;
     r.top_p = fmax((double)top, 0.0);
     r.by_min = least > 0.f;
-    r.min_a = r.by_min ? fmin(log2((double)least), 0.0) : 0.0;
+    r.last = r.by_min ? fmax(-kPerUnit * log2((double)least), 0.0) : 0.0;
     r.u = fmin(fmax((double)p.u[row], 0.0), 1.0 - 0x1p-30);
     return r;
 }
-__device__ __forceinline__ double exponent_of(float x, float top, const RowRule &r) {
-    return x == top ? 0.0 : fmax(((double)x - (double)top) * r.per_unit, -1.0e9);
+__device__ __forceinline__ double place_of(float x, float top, const RowRule &r) {
+    return fmax(((double)top - (double)x) * r.per_logit, 0.0);             // (inf - inf: 0)
 }
-__device__ __forceinline__ int bin_of(double a) { return (int)fmin(a * -kBinsPerUnit, (double)(kBins - 1)); }
-// 2^a as a whole number of 2^-43, a <= 0: the series of 2^f around 0, |f| <= 1/2, to f^11 / 11! (the rest is below 2^-47).
-__device__ __forceinline__ uint64_t weight_of(double a) {
-    a = fmax(a, -100.0);
-    const double k = rint(a), f = a - k;
-    double s = 4.4455382718708114976e-10;
-    s = fma(s, f, 7.0549116208011233299e-09);
-    s = fma(s, f, 1.0178086009239699728e-07);
-    s = fma(s, f, 1.3215486790144309488e-06);
-    s = fma(s, f, 1.5252733804059840280e-05);
-    s = fma(s, f, 1.5403530393381609954e-04);
-    s = fma(s, f, 1.3333558146428443423e-03);
-    s = fma(s, f, 9.6181291076284771619e-03);
-    s = fma(s, f, 5.5504108664821579953e-02);
-    s = fma(s, f, 2.4022650695910071233e-01);
-    s = fma(s, f, 6.9314718055994530942e-01);
-    s = fma(s, f, 1.0);
-    const double fixed = ldexp(s, (int)k + kFracBits) + 0x1p52;              // (the low bits of the sum are the rounded number)
+__device__ __forceinline__ int bin_of(double y) { return (int)fmin(y, (double)(kBins - 1)); }
+// 2^-(y / 64) as a whole number of 2^-43: halves[j] = 2^(43 - (j + 1/2) / 64) for the place in the middle of bin j (of 64), the series
+// of 2^-(g / 64) around it, |g| <= 1/2, to the fifth power (the rest is below 2^-54), and as many halvings as there are 64s in the bin.
+__device__ __forceinline__ uint64_t weight_of(const double *halves, double y, int bin) {
+    const double g = y - ((double)bin + 0.5);
+    constexpr double c = 0.69314718055994530942 / kPerUnit;
+    double e = -c * c * c * c * c / 120.0;
+    e = fma(e, g, c * c * c * c / 24.0);
+    e = fma(e, g, -c * c * c / 6.0);
+    e = fma(e, g, c * c / 2.0);
+    e = fma(e, g, -c);
+    e = fma(e, g, 1.0);
+    const double fixed = ldexp(e * halves[bin & 63], -(bin >> 6)) + 0x1p52;         // (the low bits of the sum are the rounded number)
     return (uint64_t)__double_as_longlong(fixed) & ((1ull << 52) - 1ull);
 }
 // Ascending order of (logit descending, index ascending); x is finite or +inf and not -0.
@@ -83,8 +81,8 @@ __device__ __forceinline__ float key_logit(uint64_t key) {
     return __uint_as_float(b ^ ((b >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// f(index, logit) for the row's tokens that can be chosen in 16-byte pieces from .. to - 1 (piece 0 holds the row's first logit): the
-// pieces are aligned, so the first and the last may hold others' bytes as well, which are not looked at.  -inf and NaN are left out.
+// A row in 16-byte pieces (piece 0 holds its first logit): the pieces are aligned, so the first and the last may hold others' bytes as
+// well, which count as -inf.
 template <int DT> __device__ __forceinline__ int row_pieces(const SampleParams &p, int row, const uint4 *&base, int &phase) {
     constexpr int ES = DT == kF32 ? 4 : 2;
     const uintptr_t at = reinterpret_cast<uintptr_t>(p.logits) + (uintptr_t)((int64_t)row * p.row_stride) * ES;
@@ -92,33 +90,90 @@ template <int DT> __device__ __forceinline__ int row_pieces(const SampleParams &
     phase = (int)(at & 15) / ES;
     return (phase + p.vocab + 16 / ES - 1) / (16 / ES);
 }
+// f(index of the first, logits, the largest) for pieces from .. to - 1, called by whole wavefronts but for lanes that ran out.
 template <int DT, class F>
-__device__ __forceinline__ void for_tokens(const SampleParams &p, const uint4 *base, int phase, int from, int to, F f) {
-    constexpr int N = DT == kF32 ? 4 : 8;
-    for (int c = from + (int)threadIdx.x; c < to; c += kSampThreads) {
-        const uint4 v = base[c];
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+__device__ __forceinline__ void for_pieces(const SampleParams &p, const uint4 *base, int phase, int from, int to, F f) {
+    constexpr int N = DT == kF32 ? 4 : 8, U = 4;           // four pieces in flight a thread
+    for (int c0 = from + (int)threadIdx.x; c0 < to; c0 += U * kSampThreads) {
+        uint4 v[U];
 #pragma unroll
-        for (int e = 0; e < N; e++) {
-            float x;
-            if (DT == kF32) x = __uint_as_float(w[e]);
-            else {
-                const uint32_t half = (w[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-                x = DT == PKV_F16 ? __half2float(__ushort_as_half((unsigned short)half)) : __uint_as_float(half << 16);
+        for (int i = 0; i < U; i++) v[i] = base[min(c0 + i * kSampThreads, to - 1)];
+#pragma unroll
+        for (int i = 0; i < U; i++) {
+            const int c = c0 + i * kSampThreads;
+            if (c >= to) break;
+            const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+            float x[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                if (DT == kF32) x[e] = __uint_as_float(w[e]);
+                else if (DT == PKV_F16) x[e] = __half2float(__ushort_as_half((unsigned short)(w[e >> 1] >> (16 * (e & 1)))));
+                else x[e] = __uint_as_float(e & 1 ? w[e >> 1] & 0xFFFF0000u : w[e >> 1] << 16);
             }
-            const int idx = c * N + e - phase;
-            if ((uint32_t)idx < (uint32_t)p.vocab && x > -INFINITY) f((uint32_t)idx, x + 0.f);       // (+ 0: -0 equals 0)
+            const int idx = c * N - phase;
+            if (idx < 0 || idx + N > p.vocab) {
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    if ((uint32_t)(idx + e) >= (uint32_t)p.vocab) x[e] = -INFINITY;
+            }
+            float top = x[0];
+#pragma unroll
+            for (int e = 1; e < N; e++) top = fmaxf(top, x[e]);            // (NaN: the other one)
+            f(idx, x, top);
         }
     }
 }
+template <int DT>
+__device__ __forceinline__ float largest(const SampleParams &p, const uint4 *base, int phase, int from, int to) {
+    float top = -INFINITY;
+    for_pieces<DT>(p, base, phase, from, to, [&](int, const float *, float x) { top = fmaxf(top, x); });
+    return top + 0.f;                                      // (-0 equals 0)
+}
+// f(index, logit) for the tokens with a logit of `least` (a finite number) or more; NaN has none.
+template <int DT, class F>
+__device__ __forceinline__ void for_tokens(const SampleParams &p, const uint4 *base, int phase, int from, int to, float least, F f) {
+    constexpr int N = DT == kF32 ? 4 : 8;
+    for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float top) {
+        if (!__any(top >= least)) return;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (x[e] >= least) f((uint32_t)(idx + e), x[e] + 0.f);
+    });
+}
+// A finite logit below which every place is at `bin` or behind it, whatever the roundings: one fp32 comparison instead of the place.
+__device__ __forceinline__ float surely_behind(float top, int bin, const RowRule &r) {
+    const double x = (double)top - ((double)bin + 1.0) / r.per_logit;
+    return fabs((double)top) < 3.0e38 && x > -3.0e38 ? (float)(x - fabs(x) * 0x1p-22) : -3.402823466e38f;
+}
 
+// A logit above which every place is in front of `bin`.
+__device__ __forceinline__ float surely_before(float top, int bin, const RowRule &r) {
+    const double x = (double)top - ((double)bin - 1.0) / r.per_logit;
+    return bin > 1 && fabs((double)top) < 3.0e38 && x > -3.0e38 ? (float)(x + fabs(x) * 0x1p-22) : INFINITY;
+}
+
+// A run of bins whose tokens are looked at one by one: what lies in front of it and in it.
+struct Span {
+    int from, to;                                          // (from > to: none)
+    uint32_t count, size;
+    uint64_t mass, total;
+};
+// What the histogram says about a row.
+struct RowPlan {
+    float top;
+    uint32_t gathered;                                     // tokens in the spans
+    uint64_t k_mass, low_mass;                             // mass of the k tokens unless the k-th is in a span; of what is kept for certain
+    int k_inside, k_limits;                                // top-k ends inside a bin; anywhere
+    Span span[3];
+};
 // What the launches of a split call hand on, in the workspace: one of these a row.
-constexpr int kMaxSlices = 64;
+constexpr int kMaxSlices = 64;                             // (a lane each where they are put together)
 struct RowState {
     uint64_t mass[kBins], cand[kCand];
-    uint32_t count[kBins], need[kBins / 32];
+    uint32_t count[kBins];
     float slice_top[kMaxSlices];
-    uint32_t n_need, n_cand, arrived[2];
+    RowPlan plan;
+    uint32_t n_cand, arrived[3];
 };
 template <class T> __device__ __forceinline__ T far_load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class T> __device__ __forceinline__ void far_store(T *p, T x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -127,16 +182,16 @@ struct Prefix { uint64_t mass; uint32_t count; };
 
 // What a row's resolution keeps in LDS.
 struct SampleLds {
-    uint64_t mass[kBins];                                  // of the bin; after scan(): up to and with the bin
+    uint64_t mass[kBins];                                  // of the bin; after scan_bins: up to and with it; then the candidates' weights
+    uint64_t cand[kCand];                                  // keys; of a row resolved by digits the digits' masses and counts
     uint32_t count[kBins];
-    uint64_t cand[kCand];
     uint64_t wave_mass[16];
     uint32_t wave_count[16];
-    uint32_t need[kBins / 32];
+    double halves[64];
     float top;
     uint32_t n_cand;
-    uint64_t best, sums[3];
-    int at[4];
+    uint64_t best, sums[2];
+    int at[8];
 };
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
@@ -157,180 +212,218 @@ __device__ __forceinline__ Prefix block_scan(SampleLds &s, Prefix v) {
     for (int w = 0; w < wave; w++) { v.mass += s.wave_mass[w]; v.count += s.wave_count[w]; }
     return v;
 }
-// The histogram becomes inclusive sums.
+// The histogram becomes inclusive sums, and at[] is made ready for the searches.
 __device__ __forceinline__ void scan_bins(SampleLds &s) {
-    const int b = 2 * threadIdx.x;
-    const uint64_t m0 = s.mass[b], m1 = s.mass[b + 1];
-    const uint32_t c0 = s.count[b], c1 = s.count[b + 1];
-    const Prefix v = block_scan(s, Prefix{m0 + m1, c0 + c1});
-    s.mass[b] = v.mass - m1; s.mass[b + 1] = v.mass;
-    s.count[b] = v.count - c1; s.count[b + 1] = v.count;
+    const int b = kMine * threadIdx.x;
+    uint64_t m[kMine];
+    uint32_t c[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; i++) {
+        m[i] = s.mass[b + i] + (i ? m[i - 1] : 0ull);
+        c[i] = s.count[b + i] + (i ? c[i - 1] : 0u);
+    }
+    const Prefix v = block_scan(s, Prefix{m[kMine - 1], c[kMine - 1]});
+    const uint64_t m0 = v.mass - m[kMine - 1];
+    const uint32_t c0 = v.count - c[kMine - 1];
+#pragma unroll
+    for (int i = 0; i < kMine; i++) { s.mass[b + i] = m0 + m[i]; s.count[b + i] = c0 + c[i]; }
+    if (threadIdx.x < 8) s.at[threadIdx.x] = kBins;
     __syncthreads();
 }
-// The first bin whose inclusive sum satisfies the condition (kBins: none).  Every thread of the workgroup calls it.
+// at[slot] = the first bin whose inclusive sum satisfies the condition (kBins: none); there behind the next barrier.
+template <class F> __device__ __forceinline__ void search_bin(SampleLds &s, int slot, F holds) {
+    const int b = kMine * threadIdx.x;
+    if (!holds(b + kMine - 1) || (b && holds(b - 1))) return;
+#pragma unroll
+    for (int i = kMine - 1; i >= 0; i--)
+        if (holds(b + i)) s.at[slot] = b + i;
+}
 template <class F> __device__ __forceinline__ int first_bin(SampleLds &s, F holds) {
     __syncthreads();
-    if (threadIdx.x == 0) s.at[0] = kBins;
+    if (threadIdx.x == 0) s.at[7] = kBins;
     __syncthreads();
-    const int b = 2 * threadIdx.x;
-    const bool h0 = holds(b), h1 = holds(b + 1);
-    if (h0 && (b == 0 || !holds(b - 1))) s.at[0] = b;
-    else if (h1 && !h0) s.at[0] = b + 1;
+    search_bin(s, 7, holds);
     __syncthreads();
-    return s.at[0];
+    return s.at[7];
 }
 __device__ __forceinline__ uint64_t mass_before(const SampleLds &s, int bin) { return bin ? s.mass[bin - 1] : 0ull; }
 __device__ __forceinline__ uint32_t count_before(const SampleLds &s, int bin) { return bin ? s.count[bin - 1] : 0u; }
 
-// Where the filters can end, from the scanned histogram.
-struct Cuts {
-    uint32_t n;                                            // tokens that can be chosen
-    int k_bin;                                             // top-k: ends inside this bin (k_inside) or before it; kBins: nowhere
-    bool k_inside;
-    int low, high;                                         // the bins that the last kept token can be in (kBins: every token is kept)
-};
-__device__ __forceinline__ Cuts find_cuts(SampleLds &s, const RowRule &r) {
-    Cuts c;
-    c.n = s.count[kBins - 1];
-    c.k_bin = kBins;
-    c.k_inside = false;
-    uint64_t k_low = s.mass[kBins - 1], k_high = k_low;    // mass of the k tokens, between these
-    if (r.top_k && r.top_k < c.n) {
-        const int b = first_bin(s, [&](int i) { return s.count[i] >= r.top_k; });
-        c.k_inside = s.count[b] != r.top_k;
-        c.k_bin = c.k_inside ? b : b + 1;
-        k_low = c.k_inside ? mass_before(s, b) : s.mass[b];
+__device__ __forceinline__ void order_spans(Span &a, Span &b) {            // the earlier one first; overlapping ones become one
+    if (b.from > b.to) return;
+    if (a.from > a.to || b.from < a.from) { const Span t = a; a = b; b = t; }
+    if (b.from > b.to || b.from > a.to + 1) return;
+    a.to = max(a.to, b.to);
+    b.from = 1; b.to = 0;
+}
+// Which bins the answer depends on one by one, from the scanned histogram: the one that the k-th token is in, those in which the last
+// kept token can be, those in which the draw can fall.  The same in every thread.
+__device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, float top) {
+    RowPlan p;
+    p.top = top;
+    const uint64_t all = s.mass[kBins - 1];
+    int k_bin = kBins;                                     // top-k ends inside this bin, or in front of it
+    p.k_inside = 0;
+    p.k_limits = r.top_k && r.top_k < s.count[kBins - 1];  // (of the tokens that have mass)
+    uint64_t k_low = all, k_high = all;                    // mass of the k tokens, between these
+    if (p.k_limits) {
+        search_bin(s, 0, [&](int i) { return s.count[i] >= r.top_k; });
+        __syncthreads();
+        const int b = s.at[0];
+        p.k_inside = s.count[b] != r.top_k;
+        k_bin = p.k_inside ? b : b + 1;
+        k_low = p.k_inside ? mass_before(s, b) : s.mass[b];
         k_high = s.mass[b];
     }
-    c.low = c.high = c.k_bin;
+    p.k_mass = k_low;
+    int low = k_bin, high = k_bin;                         // the bins in which the last kept token can be (kBins: all are kept)
     if (r.by_p) {
-        const double low = r.top_p * (double)k_low, high = r.top_p * (double)k_high;
-        c.low = min(c.low, first_bin(s, [&](int i) { return s.count[i] && (double)s.mass[i] >= low; }));
-        c.high = min(c.high, first_bin(s, [&](int i) { return s.count[i] && (double)s.mass[i] >= high; }));
+        const double from = r.top_p * (double)k_low, to = r.top_p * (double)k_high;
+        search_bin(s, 1, [&](int i) { return s.count[i] && (double)s.mass[i] >= from; });
+        search_bin(s, 2, [&](int i) { return s.count[i] && (double)s.mass[i] >= to; });
+        __syncthreads();
+        low = min(low, s.at[1]);
+        high = min(high, s.at[2]);
     }
-    if (r.by_min) {
-        const int b = bin_of(r.min_a);
-        c.low = min(c.low, b);
-        c.high = min(c.high, b);
+    const bool by_min = r.by_min && bin_of(r.last) < kNoMass;
+    if (by_min) {
+        low = min(low, bin_of(r.last));
+        high = min(high, bin_of(r.last));
     }
-    return c;
-}
-__device__ __forceinline__ void need_bins(SampleLds &s, int from, int to) {              // one thread
-    for (int b = from; b <= min(to, kBins - 1); b++) s.need[b >> 5] |= 1u << (b & 31);
-}
-// Marks the bins whose tokens the answer depends on one by one.
-__device__ __forceinline__ void mark_bins(SampleLds &s, const RowRule &r, const Cuts &c) {
-    const uint64_t low = c.low < kBins ? max(mass_before(s, c.low), 1ull << kFracBits) : s.mass[kBins - 1];
-    const uint64_t high = c.high >= kBins ? s.mass[kBins - 1] : c.high == c.k_bin && !c.k_inside ? mass_before(s, c.high) : s.mass[c.high];
-    const double from = r.u * (double)low, to = r.u * (double)max(low, high);
-    const int d0 = first_bin(s, [&](int i) { return (double)s.mass[i] > from; }), d1 = first_bin(s, [&](int i) { return (double)s.mass[i] > to; });
-    if (threadIdx.x < kBins / 32) s.need[threadIdx.x] = 0u;
+    p.low_mass = low < kBins ? mass_before(s, low) : all;
+    const bool whole = high >= kBins || (high == k_bin && !p.k_inside);    // the last bin that can hold a kept token is kept as a whole
+    const uint64_t high_mass = high >= kBins ? all : whole ? mass_before(s, high) : s.mass[high];
+    const double from = r.u * (double)max(p.low_mass, (1ull << kFracBits) - 1ull), to = r.u * (double)max(high_mass, 1ull << kFracBits);
+    search_bin(s, 3, [&](int i) { return (double)s.mass[i] > from; });
+    search_bin(s, 4, [&](int i) { return (double)s.mass[i] > to; });
     __syncthreads();
-    if (threadIdx.x == 0) {
-        if (c.k_inside) need_bins(s, c.k_bin, c.k_bin);
-        if (r.by_p || r.by_min) need_bins(s, c.low, c.high == c.k_bin && !c.k_inside ? c.high - 1 : c.high);
-        need_bins(s, d0, d1);
+    p.span[0].from = k_bin; p.span[0].to = p.k_inside ? k_bin : -1;
+    p.span[1].from = low; p.span[1].to = r.by_p || by_min ? min(whole ? high - 1 : high, kBins - 1) : -1;
+    p.span[2].from = s.at[3]; p.span[2].to = min(s.at[4], kBins - 1);
+    order_spans(p.span[0], p.span[1]);
+    order_spans(p.span[1], p.span[2]);
+    order_spans(p.span[0], p.span[1]);
+    order_spans(p.span[1], p.span[2]);
+    p.gathered = 0;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        Span &v = p.span[i];
+        const bool is = v.from <= v.to;
+        v.count = is ? count_before(s, v.from) : 0u;
+        v.mass = is ? mass_before(s, v.from) : 0ull;
+        v.size = is ? s.count[v.to] - v.count : 0u;
+        v.total = is ? s.mass[v.to] - v.mass : 0ull;
+        p.gathered += v.size;
     }
-    __syncthreads();
+    return p;
 }
-__device__ __forceinline__ bool needed(const SampleLds &s, int bin) { return (s.need[bin >> 5] >> (bin & 31)) & 1u; }
 
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
+    return ((uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
+}
+// The keys s.cand[0 .. n) into s.mass in ascending order.  A wavefront sorts 64 in registers; a key's place is its own in its 64 plus
+// how many are smaller in each of the others, a search of six steps: two barriers, where a sort across the workgroup has one a step
+// (512 keys: 45 of them, some 25 us).
 __device__ __forceinline__ void sort_candidates(SampleLds &s, uint32_t n) {
-    uint32_t size = 64;
-    while (size < n) size <<= 1;
-    for (uint32_t i = n + threadIdx.x; i < size; i += kSampThreads) s.cand[i] = ~0ull;
-    for (uint32_t k = 2; k <= size; k <<= 1)
-        for (uint32_t j = k >> 1; j; j >>= 1) {
-            __syncthreads();
-            for (uint32_t t = threadIdx.x; t < size / 2; t += kSampThreads) {
-                const uint32_t i = ((t & ~(j - 1)) << 1) | (t & (j - 1));
-                const uint64_t a = s.cand[i], b = s.cand[i + j];
-                if ((a > b) == ((i & k) == 0)) { s.cand[i] = b; s.cand[i + j] = a; }
+    const int lane = threadIdx.x & 63;
+    const uint32_t chunks = (n + 63) / 64;
+    for (uint32_t c = threadIdx.x >> 6; c < chunks; c += kSampThreads / 64) {
+        uint64_t key = 64 * c + lane < n ? s.cand[64 * c + lane] : ~0ull;
+#pragma unroll
+        for (int k = 2; k <= 64; k <<= 1)
+#pragma unroll
+            for (int j = k >> 1; j; j >>= 1) {
+                const uint64_t other = shfl_xor64(key, j);
+                const bool low = ((lane & j) == 0) == ((lane & k) == 0);
+                key = (other < key) == low ? other : key;
             }
+        s.cand[64 * c + lane] = key;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < 64 * chunks; i += kSampThreads) {
+        const uint64_t key = s.cand[i];
+        if (key == ~0ull) continue;
+        uint32_t place = i & 63;
+        for (uint32_t c = 0; c < chunks; c++) {
+            if (c == i >> 6) continue;
+            const uint64_t *at = s.cand + 64 * c;
+            uint32_t less = 0;                             // 0 .. 64
+#pragma unroll
+            for (uint32_t step = 32; step; step >>= 1)
+                if (at[less + step - 1] < key) less += step;
+            place += less + (at[less] < key ? 1u : 0u);
         }
+        s.mass[place] = key;
+    }
     __syncthreads();
 }
 
 __device__ __forceinline__ void answer(const SampleParams &p, int row, uint64_t key, float top, const RowRule &r, uint64_t kept) {
     p.token[row] = (int64_t)(uint32_t)key;
-    if (p.logprob) p.logprob[row] = (float)((exponent_of(key_logit(key), top, r) - (log2((double)kept) - kFracBits)) * 0.69314718055994530942);
+    if (p.logprob) p.logprob[row] = (float)((-place_of(key_logit(key), top, r) / kPerUnit - (log2((double)kept) - kFracBits)) * 0.69314718055994530942);
 }
 
-// The answer from at most kCand gathered tokens.  A candidate's rank and the mass in front of it are its bin's plus those of the
-// candidates of its bin in front of it.
-__device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const Cuts &c, uint32_t n) {
+// The answer from at most kCand gathered tokens (s.cand, behind a barrier; s.mass is not looked at any more).  All tokens of a span are there, so a candidate's rank and
+// the mass in front of it are its span's plus those of the candidates of its span in front of it.
+__device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const RowPlan &plan) {
+    const uint32_t n = plan.gathered;
+    uint64_t key[kMine], w[kMine], front[kMine];
+    int bin[kMine];
+    double y[kMine];
     sort_candidates(s, n);
-    uint64_t key[2] = {~0ull, ~0ull}, w[2] = {0, 0}, before[2] = {0, 0};
-    uint32_t rank[2] = {0, 0};
-    double a[2] = {0, 0};
-    int bin[2] = {0, 0};
-    const uint32_t i0 = 2 * threadIdx.x;
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (i0 + e < n) {
-            key[e] = s.cand[i0 + e];
-            a[e] = exponent_of(key_logit(key[e]), s.top, r);
-            w[e] = weight_of(a[e]);
-            bin[e] = bin_of(a[e]);
+    for (int e = 0; e < kMine; e++) {
+        const uint32_t i = kMine * threadIdx.x + e;
+        key[e] = ~0ull; w[e] = 0; y[e] = 0; bin[e] = 0;
+        if (i < n) {
+            key[e] = s.mass[i];
+            y[e] = place_of(key_logit(key[e]), plan.top, r);
+            bin[e] = bin_of(y[e]);
+            w[e] = weight_of(s.halves, y[e], bin[e]);
         }
-    const Prefix v = block_scan(s, Prefix{w[0] + w[1], 0u});
-    const uint64_t sum[2] = {v.mass - w[1] - w[0], v.mass - w[1]};         // of the candidates in front
-    // where the bin's first candidate stands: a chain of candidates of one bin covers the bin, so its start is found by its count
-    __syncthreads();
-    uint64_t *sums = s.cand;                                              // (the keys are in registers)
+    }
+    if (threadIdx.x == 0) { s.sums[0] = plan.k_mass; s.sums[1] = plan.low_mass; s.best = ~0ull; }
+    uint64_t sum = 0;
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (i0 + e < n) sums[i0 + e] = sum[e];
-    __syncthreads();
+    for (int e = 0; e < kMine; e++) { front[e] = sum; sum += w[e]; }
+    const uint64_t ahead = block_scan(s, Prefix{sum, 0u}).mass - sum;
+    uint32_t rank[kMine];
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (i0 + e < n) {
-            uint32_t lo = 0;                                               // candidates of needed bins in front of this bin
-            for (int q = 0; q < (bin[e] >> 5); q++) {
-                uint32_t bits = s.need[q];
-                while (bits) { const int b = 32 * q + __ffs((int)bits) - 1; lo += s.count[b] - count_before(s, b); bits &= bits - 1; }
-            }
-            uint32_t bits = s.need[bin[e] >> 5] & ((1u << (bin[e] & 31)) - 1u);
-            while (bits) { const int b = 32 * (bin[e] >> 5) + __ffs((int)bits) - 1; lo += s.count[b] - count_before(s, b); bits &= bits - 1; }
-            rank[e] = count_before(s, bin[e]) + (i0 + e - lo);
-            before[e] = mass_before(s, bin[e]) + (sum[e] - sums[lo]);
-        }
-    // mass of the k tokens
-    if (threadIdx.x == 0) {
-        s.sums[0] = c.k_bin >= kBins ? s.mass[kBins - 1] : mass_before(s, c.k_bin);
-        s.sums[1] = c.low < kBins ? mass_before(s, c.low) : s.mass[kBins - 1];
-        s.best = ~0ull;
-        s.sums[2] = 0;
+    for (int e = 0; e < kMine; e++) {
+        const Span &a = plan.span[0], &b = plan.span[1], &c = plan.span[2];
+        const bool in_a = a.from <= a.to && bin[e] <= a.to, in_b = !in_a && b.from <= b.to && bin[e] <= b.to;
+        rank[e] = kMine * threadIdx.x + e + (in_a ? a.count : in_b ? b.count - a.size : c.count - a.size - b.size);
+        front[e] += ahead + (in_a ? a.mass : in_b ? b.mass - a.total : c.mass - a.total - b.total);
+        if (kMine * threadIdx.x + e < n && plan.k_inside && rank[e] + 1 == r.top_k) s.sums[0] = front[e] + w[e];
     }
     __syncthreads();
-#pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (i0 + e < n && c.k_inside && rank[e] + 1 == r.top_k) s.sums[0] = before[e] + w[e];
-    __syncthreads();
     const double limit = r.by_p ? r.top_p * (double)s.sums[0] : 0.0;
-    bool kept[2];
+    bool kept[kMine];
 #pragma unroll
-    for (int e = 0; e < 2; e++) {
-        kept[e] = i0 + e < n && (c.k_bin >= kBins || rank[e] < r.top_k) && (!r.by_p || rank[e] == 0 || (double)before[e] < limit) &&
-                  (!r.by_min || a[e] >= r.min_a);
-        if (kept[e]) atomicMax((unsigned long long *)&s.sums[1], (unsigned long long)(before[e] + w[e]));
+    for (int e = 0; e < kMine; e++) {
+        kept[e] = kMine * threadIdx.x + e < n && (!plan.k_limits || rank[e] < r.top_k) && (!r.by_p || rank[e] == 0 || (double)front[e] < limit) &&
+                  (!r.by_min || y[e] <= r.last);
+        if (kept[e]) atomicMax((unsigned long long *)&s.sums[1], (unsigned long long)(front[e] + w[e]));
     }
     __syncthreads();
     const uint64_t total = s.sums[1];
     const double target = r.u * (double)total;
 #pragma unroll
-    for (int e = 0; e < 2; e++)
-        if (kept[e] && (double)(before[e] + w[e]) > target) atomicMin((unsigned long long *)&s.best, (unsigned long long)key[e]);
+    for (int e = 0; e < kMine; e++)
+        if (kept[e] && (double)(front[e] + w[e]) > target) atomicMin((unsigned long long *)&s.best, (unsigned long long)key[e]);
     __syncthreads();
-    if (threadIdx.x == 0) answer(p, row, s.best, s.top, r, total);
+    if (threadIdx.x == 0) answer(p, row, s.best, plan.top, r, total);
 }
 
 // ---- the answer when the bins in question hold more tokens than that (long runs of equal logits): by digits of the order ----
 // The token at which a sum of the order first reaches what is asked for, among those of one bin: five passes over the row, each a
 // histogram of the next digit (11 + 11 + 10 bits of the logit, 10 + 10 of the index) of the tokens that share the digits so far.
 template <int DT, class F>
-__device__ __forceinline__ uint64_t descend(SampleLds &s, uint64_t *hist_mass, uint32_t *hist_count, const SampleParams &p, int row, const RowRule &r,
-                                            int bin, Prefix &before, F reached) {
+__device__ __forceinline__ uint64_t descend(SampleLds &s, const SampleParams &p, int row, const RowRule &r, int bin, Prefix &before, F reached) {
+    constexpr int kDigits = 2048;
+    uint64_t *hist_mass = s.cand;
+    uint32_t *hist_count = reinterpret_cast<uint32_t *>(s.cand + kDigits);
+    static_assert(kDigits * 12 <= sizeof(s.cand) && kDigits == 2 * kSampThreads, "two digits a thread, in the candidates' place");
     const uint4 *base;
     int phase;
     const int pieces = row_pieces<DT>(p, row, base, phase);
@@ -340,19 +433,18 @@ __device__ __forceinline__ uint64_t descend(SampleLds &s, uint64_t *hist_mass, u
     for (int level = 0; level < 5; level++) {
         const int shift = kShift[level], above = shift + kWidth[level];
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kSampThreads) { hist_mass[i] = 0; hist_count[i] = 0; }
+        for (int i = threadIdx.x; i < kDigits; i += kSampThreads) { hist_mass[i] = 0; hist_count[i] = 0; }
+        if (threadIdx.x == 0) { s.at[1] = 0; s.at[2] = 0; }
         __syncthreads();
-        for_tokens<DT>(p, base, phase, 0, pieces, [&](uint32_t idx, float x) {
-            const double a = exponent_of(x, s.top, r);
-            if (bin_of(a) != bin) return;
-            uint64_t key = order_key(x, idx);
+        for_tokens<DT>(p, base, phase, 0, pieces, surely_behind(s.top, bin + 1, r), [&](uint32_t idx, float x) {
+            const double y = place_of(x, s.top, r);
+            if (bin_of(y) != bin) return;
+            const uint64_t key = order_key(x, idx);
             if (above < 64 && (key >> above) != (prefix >> above)) return;
             const int digit = (int)((key >> shift) & ((1u << kWidth[level]) - 1u));
-            atomicAdd((unsigned long long *)&hist_mass[digit], (unsigned long long)weight_of(a));
+            atomicAdd((unsigned long long *)&hist_mass[digit], (unsigned long long)weight_of(s.halves, y, bin));
             atomicAdd(&hist_count[digit], 1u);
         });
-        __syncthreads();
-        if (threadIdx.x == 0) { s.at[1] = 0; s.at[2] = 0; }
         __syncthreads();
         const int d = 2 * threadIdx.x;
         const uint64_t m0 = hist_mass[d], m1 = hist_mass[d + 1];
@@ -361,62 +453,61 @@ __device__ __forceinline__ uint64_t descend(SampleLds &s, uint64_t *hist_mass, u
         const Prefix in[2] = {{before.mass + v.mass - m1, before.count + v.count - c1}, {before.mass + v.mass, before.count + v.count}};
         const Prefix out[2] = {{in[0].mass - m0, in[0].count - c0}, {in[1].mass - m1, in[1].count - c1}};
         const uint32_t have[2] = {c0, c1};
-        __syncthreads();
         // the digit in which it is reached; where rounding leaves none, the last one that holds a token
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             if (!have[e]) continue;
             atomicMax(&s.at[2], d + e + 1);
-            if (reached(in[e])) atomicMax(&s.at[1], kBins - (d + e));
+            if (reached(in[e])) atomicMax(&s.at[1], kDigits - (d + e));
         }
         __syncthreads();
-        const int digit = s.at[1] ? kBins - s.at[1] : s.at[2] - 1;
+        const int digit = s.at[1] ? kDigits - s.at[1] : s.at[2] - 1;
 #pragma unroll
         for (int e = 0; e < 2; e++)
             if (d + e == digit) { s.sums[0] = out[e].mass; s.at[3] = (int)out[e].count; }
         __syncthreads();
         before = Prefix{s.sums[0], (uint32_t)s.at[3]};
         prefix |= (uint64_t)digit << shift;
-        __syncthreads();
     }
+    __syncthreads();
     return prefix;
 }
 
+// (s.mass and s.count hold the sums.)
 template <int DT>
-__device__ __forceinline__ void resolve_many(SampleLds &s, uint64_t *hist_mass, uint32_t *hist_count, const SampleParams &p, int row, const RowRule &r,
-                                             const Cuts &c) {
-    auto weight = [&](uint64_t key) { return weight_of(exponent_of(key_logit(key), s.top, r)); };
+__device__ __forceinline__ void resolve_many(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const RowPlan &plan) {
+    auto weight = [&](uint64_t key) {
+        const double y = place_of(key_logit(key), s.top, r);
+        return weight_of(s.halves, y, bin_of(y));
+    };
     // sums up to and with a token, in order: what the k tokens hold, then where the kept ones end
-    uint64_t all = s.mass[kBins - 1];
-    uint32_t count = c.n;
+    uint64_t all = plan.k_mass;
+    uint32_t count = plan.k_limits ? r.top_k : s.count[kBins - 1];
     Prefix before;
-    if (c.k_bin < kBins) {
-        count = r.top_k;
-        all = mass_before(s, c.k_bin);
-        if (c.k_inside) {
-            const uint64_t key = descend<DT>(s, hist_mass, hist_count, p, row, r, c.k_bin, before, [&](Prefix v) { return v.count >= r.top_k; });
-            all = before.mass + weight(key);
-        }
+    if (plan.k_inside) {
+        const int b = first_bin(s, [&](int i) { return s.count[i] >= r.top_k; });
+        const uint64_t key = descend<DT>(s, p, row, r, b, before, [&](Prefix v) { return v.count >= r.top_k; });
+        all = before.mass + weight(key);
     }
     if (r.by_p) {                                          // the last token with less than the limit before it is the first to reach it
         const double limit = r.top_p * (double)all;
         const int b = first_bin(s, [&](int i) { return s.count[i] && (double)s.mass[i] >= limit; });
-        const uint64_t key = descend<DT>(s, hist_mass, hist_count, p, row, r, b, before, [&](Prefix v) { return (double)v.mass >= limit; });
+        const uint64_t key = descend<DT>(s, p, row, r, b, before, [&](Prefix v) { return (double)v.mass >= limit; });
         if (before.count + 1 < count) { count = before.count + 1; all = before.mass + weight(key); }
     }
     if (r.by_min) {                                        // by value: its bin's tokens are added up in one pass
-        const int b = bin_of(r.min_a);
-        if (count_before(s, b) < count) {
+        const int b = bin_of(r.last);
+        if (b < kNoMass && count_before(s, b) < count) {
             __syncthreads();
             if (threadIdx.x == 0) { s.sums[1] = mass_before(s, b); s.n_cand = count_before(s, b); }
             __syncthreads();
             const uint4 *base;
             int phase;
             const int pieces = row_pieces<DT>(p, row, base, phase);
-            for_tokens<DT>(p, base, phase, 0, pieces, [&](uint32_t, float x) {
-                const double a = exponent_of(x, s.top, r);
-                if (bin_of(a) != b || a < r.min_a) return;
-                atomicAdd((unsigned long long *)&s.sums[1], (unsigned long long)weight_of(a));
+            for_tokens<DT>(p, base, phase, 0, pieces, surely_behind(s.top, b + 1, r), [&](uint32_t, float x) {
+                const double y = place_of(x, s.top, r);
+                if (bin_of(y) != b || y > r.last) return;
+                atomicAdd((unsigned long long *)&s.sums[1], (unsigned long long)weight_of(s.halves, y, b));
                 atomicAdd(&s.n_cand, 1u);
             });
             __syncthreads();
@@ -426,7 +517,7 @@ __device__ __forceinline__ void resolve_many(SampleLds &s, uint64_t *hist_mass, 
     }
     const double target = r.u * (double)all;
     const int b = first_bin(s, [&](int i) { return (double)s.mass[i] > target; });
-    const uint64_t key = descend<DT>(s, hist_mass, hist_count, p, row, r, b, before, [&](Prefix v) { return (double)v.mass > target; });
+    const uint64_t key = descend<DT>(s, p, row, r, b, before, [&](Prefix v) { return (double)v.mass > target; });
     if (threadIdx.x == 0) answer(p, row, key, s.top, r, all);
 }
 
@@ -442,23 +533,70 @@ __device__ __forceinline__ float block_max(SampleLds &s, float top) {
     return top;
 }
 
-__device__ __forceinline__ uint32_t needed_tokens(const SampleLds &s) {
-    uint32_t n = 0;
-    for (int q = 0; q < kBins / 32; q++)
-        for (uint32_t bits = s.need[q]; bits; bits &= bits - 1) {
-            const int b = 32 * q + __ffs((int)bits) - 1;
-            n += s.count[b] - count_before(s, b);
-        }
-    return n;
-}
+// Counts and masses by bin, of the tokens that have mass, into s.mass and s.count.
 template <int DT>
 __device__ __forceinline__ void histogram(SampleLds &s, const SampleParams &p, const RowRule &r, const uint4 *base, int phase, int from, int to, float top) {
-    for_tokens<DT>(p, base, phase, from, to, [&](uint32_t, float x) {
-        const double a = exponent_of(x, top, r);
-        const int b = bin_of(a);
-        atomicAdd((unsigned long long *)&s.mass[b], (unsigned long long)weight_of(a));
-        atomicAdd(&s.count[b], 1u);
+    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = 0; s.count[i] = 0; }
+    __syncthreads();
+    const float least = surely_behind(top, kNoMass, r);
+    for_pieces<DT>(p, base, phase, from, to, [&](int, const float *x, float most) {
+        if (!__any(most >= least)) return;
+        // four at a time without a branch: one token's steps wait for each other, four tokens' do not
+#pragma unroll
+        for (int e0 = 0; e0 < (DT == kF32 ? 4 : 8); e0 += 4) {
+            uint64_t w[4];
+            int b[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const double y = place_of(x[e0 + e], top, r);
+                b[e] = bin_of(y);
+                w[e] = weight_of(s.halves, y, b[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (x[e0 + e] >= least && b[e] < kNoMass) {
+                    atomicAdd((unsigned long long *)&s.mass[b[e]], (unsigned long long)w[e]);
+                    atomicAdd(&s.count[b[e]], 1u);
+                }
+        }
     });
+    __syncthreads();
+}
+// Tokens of the spans, each to put(index, logit).  Two fp32 comparisons a span leave few that need their place; a span that is not there
+// lets none through.
+template <int DT, class F>
+__device__ __forceinline__ void gather(const SampleParams &p, const RowRule &r, const RowPlan &plan, const uint4 *base, int phase, int from, int to, F put) {
+    float low[3], high[3], least = INFINITY;
+#pragma unroll
+    for (int i = 0; i < 3; i++) {
+        const bool is = plan.span[i].from <= plan.span[i].to;
+        low[i] = is ? surely_behind(plan.top, plan.span[i].to + 1, r) : INFINITY;
+        high[i] = is ? surely_before(plan.top, plan.span[i].from, r) : -INFINITY;
+        least = fminf(least, low[i]);
+    }
+    for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float most) {
+        if (!__any(most >= least)) return;
+        uint32_t maybe = 0;                                // a bit a token; few lanes have one
+#pragma unroll
+        for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) {
+            const bool in = (x[e] >= low[0] && x[e] <= high[0]) | (x[e] >= low[1] && x[e] <= high[1]) | (x[e] >= low[2] && x[e] <= high[2]);
+            maybe |= in ? 1u << e : 0u;
+        }
+        for (; maybe; maybe &= maybe - 1) {
+            const int e = __ffs((int)maybe) - 1;
+            float v = x[0];
+#pragma unroll
+            for (int k = 1; k < (DT == kF32 ? 4 : 8); k++) v = e == k ? x[k] : v;
+            const int b = bin_of(place_of(v, plan.top, r));
+            bool in = false;
+#pragma unroll
+            for (int i = 0; i < 3; i++) in |= b >= plan.span[i].from && b <= plan.span[i].to;
+            if (in) put((uint32_t)(idx + e), v + 0.f);
+        }
+    });
+}
+__device__ __forceinline__ void fill_halves(SampleLds &s) {
+    if (threadIdx.x < 64) s.halves[threadIdx.x] = exp2((double)kFracBits - ((double)threadIdx.x + 0.5) / kPerUnit);
 }
 __device__ __forceinline__ void no_token(const SampleParams &p, int row) {
     p.token[row] = -1;
@@ -487,13 +625,12 @@ __global__ void __launch_bounds__(kSampThreads) slice_top_kernel(const SamplePar
     const uint4 *base;
     int phase, from, to;
     row_slice<DT>(p, base, phase, from, to);
-    float top = -INFINITY;
-    for_tokens<DT>(p, base, phase, from, to, [&](uint32_t, float x) { top = fmaxf(top, x); });
+    float top = largest<DT>(p, base, phase, from, to);
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     for (int i = (int)(blockIdx.x * kSampThreads + threadIdx.x); i < kBins; i += (int)gridDim.x * kSampThreads) { st.mass[i] = 0; st.count[i] = 0; }
-    if (blockIdx.x == 0 && threadIdx.x < 4) (&st.n_need)[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x < 4) (&st.n_cand)[threadIdx.x] = 0;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; w++) top = fmaxf(top, tops[w]);
@@ -501,9 +638,11 @@ __global__ void __launch_bounds__(kSampThreads) slice_top_kernel(const SamplePar
     }
 }
 __device__ __forceinline__ float slices_top(const RowState &st) {
-    float top = -INFINITY;
-    for (int i = 0; i < (int)gridDim.x; i++) top = fmaxf(top, st.slice_top[i]);
-    return top;
+    const int lane = threadIdx.x & 63;
+    float top = lane < (int)gridDim.x ? st.slice_top[lane] : -INFINITY;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(top)));
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const SampleParams p, RowState *state) {
@@ -516,14 +655,12 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
         if (blockIdx.x == 0 && threadIdx.x == 0) no_token(p, row);
         return;
     }
-    const RowRule r = row_rule(p, row);
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = 0; s.count[i] = 0; }
-    __syncthreads();
+    const RowRule r = row_rule(p, row, top);
+    fill_halves(s);
     const uint4 *base;
     int phase, from, to;
     row_slice<DT>(p, base, phase, from, to);
     histogram<DT>(s, p, r, base, phase, from, to, top);
-    __syncthreads();
     for (int i = threadIdx.x; i < kBins; i += kSampThreads)
         if (s.count[i]) {
             atomicAdd((unsigned long long *)&st.mass[i], (unsigned long long)s.mass[i]);
@@ -533,43 +670,41 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
     for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = far_load(&st.mass[i]); s.count[i] = far_load(&st.count[i]); }
     __syncthreads();
     scan_bins(s);
-    mark_bins(s, r, find_cuts(s, r));
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { st.mass[i] = s.mass[i]; st.count[i] = s.count[i]; }      // (sums from here on)
-    if (threadIdx.x < kBins / 32) st.need[threadIdx.x] = s.need[threadIdx.x];
-    if (threadIdx.x == 0) st.n_need = needed_tokens(s);
+    const RowPlan plan = make_plan(s, r, top);
+    if (threadIdx.x == 0) st.plan = plan;
+    if (plan.gathered > kCand)                             // (sums from here on)
+        for (int i = threadIdx.x; i < kBins; i += kSampThreads) { st.mass[i] = s.mass[i]; st.count[i] = s.count[i]; }
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const SampleParams p, RowState *state) {
     extern __shared__ __align__(16) uint8_t lds[];
     SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
-    uint64_t *hist_mass = reinterpret_cast<uint64_t *>(lds + sizeof(SampleLds));
     const int row = blockIdx.y;
     RowState &st = state[row];
     const float top = slices_top(st);
     if (top == -INFINITY) return;
-    const RowRule r = row_rule(p, row);
-    const uint32_t n = st.n_need;
-    if (threadIdx.x < kBins / 32) s.need[threadIdx.x] = st.need[threadIdx.x];
-    if (threadIdx.x == 0) s.top = top;
-    __syncthreads();
-    if (n <= kCand) {
-        const uint4 *base;
-        int phase, from, to;
-        row_slice<DT>(p, base, phase, from, to);
-        for_tokens<DT>(p, base, phase, from, to, [&](uint32_t idx, float x) {
-            if (needed(s, bin_of(exponent_of(x, top, r)))) far_store(&st.cand[min(atomicAdd(&st.n_cand, 1u), (uint32_t)kCand - 1u)], order_key(x, idx));
-        });
-        if (!last_to_arrive(s, &st.arrived[1])) return;
-    } else if (blockIdx.x) {
+    const RowRule r = row_rule(p, row, top);
+    const RowPlan plan = st.plan;
+    const uint32_t n = plan.gathered;
+    fill_halves(s);
+    if (n > kCand) {
+        if (blockIdx.x) return;
+        for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = st.mass[i]; s.count[i] = st.count[i]; }
+        if (threadIdx.x == 0) s.top = plan.top;
+        __syncthreads();
+        resolve_many<DT>(s, p, row, r, plan);
         return;
     }
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = st.mass[i]; s.count[i] = st.count[i]; }
-    if (n <= kCand)
-        for (uint32_t i = threadIdx.x; i < n; i += kSampThreads) s.cand[i] = far_load(&st.cand[i]);
+    const uint4 *base;
+    int phase, from, to;
+    row_slice<DT>(p, base, phase, from, to);
+    gather<DT>(p, r, plan, base, phase, from, to, [&](uint32_t idx, float x) {
+        far_store(&st.cand[min(atomicAdd(&st.n_cand, 1u), (uint32_t)kCand - 1u)], order_key(x, idx));
+    });
+    if (!last_to_arrive(s, &st.arrived[1])) return;
+    for (uint32_t i = threadIdx.x; i < n; i += kSampThreads) s.cand[i] = far_load(&st.cand[i]);
     __syncthreads();
-    const Cuts c = find_cuts(s, r);
-    if (n <= kCand) resolve_few(s, p, row, r, c, n);
-    else resolve_many<DT>(s, hist_mass, reinterpret_cast<uint32_t *>(hist_mass + kBins), p, row, r, c);
+    resolve_few(s, p, row, r, plan);
 }
 
 // One workgroup a row.
@@ -577,38 +712,28 @@ template <int DT>
 __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleParams p) {
     extern __shared__ __align__(16) uint8_t lds[];
     SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
-    uint64_t *hist_mass = reinterpret_cast<uint64_t *>(lds + sizeof(SampleLds));
-    uint32_t *hist_count = reinterpret_cast<uint32_t *>(hist_mass + kBins);
     const int row = blockIdx.x;
-    const RowRule r = row_rule(p, row);
     const uint4 *base;
     int phase;
     const int pieces = row_pieces<DT>(p, row, base, phase);
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = 0; s.count[i] = 0; }
-    float top = -INFINITY;
-    for_tokens<DT>(p, base, phase, 0, pieces, [&](uint32_t, float x) { top = fmaxf(top, x); });
-    top = block_max(s, top);
+    const float top = block_max(s, largest<DT>(p, base, phase, 0, pieces));
     if (top == -INFINITY) {                                // nothing can be chosen
         if (threadIdx.x == 0) no_token(p, row);
         return;
     }
+    const RowRule r = row_rule(p, row, top);
     if (threadIdx.x == 0) { s.top = top; s.n_cand = 0; }
-    __syncthreads();
+    fill_halves(s);
     histogram<DT>(s, p, r, base, phase, 0, pieces, top);
-    __syncthreads();
     scan_bins(s);
-    const Cuts c = find_cuts(s, r);
-    mark_bins(s, r, c);
-    const uint32_t n = needed_tokens(s);
-    if (n > kCand) {
-        resolve_many<DT>(s, hist_mass, hist_count, p, row, r, c);
+    const RowPlan plan = make_plan(s, r, top);
+    if (plan.gathered > kCand) {
+        resolve_many<DT>(s, p, row, r, plan);
         return;
     }
-    for_tokens<DT>(p, base, phase, 0, pieces, [&](uint32_t idx, float x) {
-        if (needed(s, bin_of(exponent_of(x, top, r)))) s.cand[atomicAdd(&s.n_cand, 1u)] = order_key(x, idx);
-    });
+    gather<DT>(p, r, plan, base, phase, 0, pieces, [&](uint32_t idx, float x) { s.cand[atomicAdd(&s.n_cand, 1u)] = order_key(x, idx); });
     __syncthreads();
-    resolve_few(s, p, row, r, c, n);
+    resolve_few(s, p, row, r, plan);
 }
 
 // Slices a row: as many as make 256 workgroups, of 4096 logits or more; one where that leaves a single one.
@@ -627,16 +752,17 @@ static int sample_check(const pkv_sample_args *a) {
 }
 
 template <int DT> static int sample_launch(const SampleParams &p, int slices, void *workspace, hipStream_t s) {
-    const size_t lds = sizeof(SampleLds) + kBins * 12;
+    const size_t lds = sizeof(SampleLds);
     if (slices == 1) {
         PKV_HIP_CHECK(hipFuncSetAttribute((const void *)sample_rows_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         sample_rows_kernel<DT><<<dim3((unsigned)p.rows), kSampThreads, lds, s>>>(p);
     } else {
         RowState *state = (RowState *)workspace;
         const dim3 grid((unsigned)slices, (unsigned)p.rows);
+        PKV_HIP_CHECK(hipFuncSetAttribute((const void *)slice_histogram_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         PKV_HIP_CHECK(hipFuncSetAttribute((const void *)slice_resolve_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         slice_top_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
-        slice_histogram_kernel<DT><<<grid, kSampThreads, sizeof(SampleLds), s>>>(p, state);
+        slice_histogram_kernel<DT><<<grid, kSampThreads, lds, s>>>(p, state);
         slice_resolve_kernel<DT><<<grid, kSampThreads, lds, s>>>(p, state);
     }
     PKV_HIP_CHECK(hipGetLastError());

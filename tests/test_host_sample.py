@@ -34,7 +34,7 @@ def test_workspace_is_for_rows_that_are_cut():
     size = lambda **kw: _lib.load().pkv_sample_workspace(ctypes.byref(_args(**kw)))
     assert size() == 0 and size(rows=256, vocab=151936) == 0 and size(vocab=(1 << 20) + 1) == 0
     one = size(rows=1, vocab=151936)
-    assert one % 16 == 0 and 0 < one < 1 << 17 and size(rows=3, vocab=151936) == 3 * one
+    assert one % 16 == 0 and 0 < one < 1 << 18 and size(rows=3, vocab=151936) == 3 * one
 
 
 def test_host_tensors_are_refused():
