@@ -14,6 +14,8 @@
 // without normalising them, to about 18 bits.)  Scale and zero of a token are applied to what the products need of them, in fp32:  score = scale (q . code + zero sum(q)),
 // out = sum p scale code + sum p scale zero.  The weight p * scale is rounded to fp16 (2^-11), scaled by a power of two that follows
 // the largest scale met; the zero's sum takes the rounded weight, so that the error is 2^-11 of p |v|, not of p * scale * code.
+// p is taken against a maximum that is raised only once a score exceeds it by 2^8 (weights stay below 2^15): the factor on the
+// accumulators, and the exchange of maxima between lanes, are rare, and the reference goes into the scores' own multiply-add.
 // q in bf16 becomes fp16 times one power of two for the workgroup's rows, which loses bits only 2^-39 below their largest.
 //
 // K turns through LDS (a pack holds 16 tokens of one channel, the product wants channels of one token): codes as bytes in rows of
@@ -113,6 +115,26 @@ template <bool WIDE> __device__ __forceinline__ void pack_operand(const uint8_t 
     }
 }
 
+// Blocks of widths up to 4 travel from memory to LDS without registers, 16 bytes a lane: lane l's land at lds_addr + 16 l, lanes behind
+// the buffer's end get zeroes, lanes that are off write nothing.  lds_addr and rsrc are wave-uniform.  The compiler does not see the
+// copies: s_waitcnt vmcnt(0) stands in front of the barrier that hands them on, and the barrier between waits for LDS only.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy_to_lds(u4 rsrc, uint32_t lds_addr, uint32_t voff) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds_addr), "v"(voff), "s"(rsrc) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// The largest of the wavefront's values, in every lane (the upper half of the lanes repeats the lower).
+__device__ __forceinline__ uint32_t half_max(uint32_t x) {
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x111, 0xF, 0xF, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x112, 0xF, 0xF, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x114, 0xF, 0xF, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x118, 0xF, 0xF, true));
+    x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x142, 0xA, 0xF, true));
+    return (uint32_t)__builtin_amdgcn_readlane((int)x, 31);
+}
+
 // One 32-row block's softmax step for 16 scores of the lane's row: the new maximum, the factor for what was summed before, and the
 // weights in place of the scores.
 __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
@@ -128,14 +150,14 @@ __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
 }
 
 template <bool BF, int NB, bool WIDE>
-__global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p) {
     constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
     extern __shared__ __align__(16) uint8_t lds[];
     uint8_t *ring = lds;                                   // two tiles of four staged blocks; window: V rows; end: sums
     uint8_t *kt_all = lds + p.ring;                        // [4 wavefronts][32 tokens][kKRow]
     uint32_t *tab = reinterpret_cast<uint32_t *>(kt_all + 4 * 32 * kKRow);         // [8 units][4 slots][32 lanes]
-    float4 *par_all = reinterpret_cast<float4 *>(tab + 1024);                      // [4][32] (scale, zero * scale, V scale, V zero)
-    float *st = reinterpret_cast<float *>(par_all + 128);                          // [2][4][32 NB] maxima, sums at the end
+    float2 *par_all = reinterpret_cast<float2 *>(tab + 1024);                      // [4][32] (scale, zero * scale) and [4][32] (V scale, V zero)
+    float *st = reinterpret_cast<float *>(par_all + 256);                          // [2][4][32 NB] maxima, sums at the end
     uint8_t *qt = reinterpret_cast<uint8_t *>(st + 8 * 32 * NB);                   // [32 NB][kQRow]
 
     // Row tiles of one (KV head, run) follow each other on one XCD (workgroups go round the eight of them), so that they find its
@@ -167,37 +189,64 @@ __global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const 
     const int c0 = max(first, start / kChunkTile), c1 = min(last, (seen_c + kChunkTile - 1) / kChunkTile);
     const int w0 = max(first - p.tiles_c, max(start - p.T_c, 0) / kChunkTile), w1 = min(last - p.tiles_c, (pos_last - p.T_c) / kChunkTile + 1);
 
-    // ---- staging of a tile's four blocks (wavefront = block) and this wavefront's parameters, one tile ahead in registers ----
+    // ---- staging of a tile's four blocks (wavefront = block), one tile ahead; block_info a tile further, through scalar loads ----
+    typedef const __attribute__((address_space(4))) uint32_t *const_u32_ptr;
     const uint32_t cap = wave < 2 ? (uint32_t)k_block_bound(64, p.k_bits) : (uint32_t)v_block_bound(64, p.v_bits);
     const uint64_t bytes = wave < 2 ? p.k_bytes : p.v_bytes;
-    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(wave < 2 ? p.k_stream : p.v_stream), 0,
-                                                                          (int)(uint32_t)((bytes + 3u) & ~3ull), 0x00020000);
-    u4 raw[NQ];
+    const const_u32_ptr info = reinterpret_cast<const_u32_ptr>(reinterpret_cast<uintptr_t>(wave < 2 ? p.k_info : p.v_info));
+    const uint32_t blk0 = wave < 2 ? (uint32_t)wave * (uint32_t)p.BH + (uint32_t)bh : 2u * (uint32_t)bh + (uint32_t)(wave - 2);
+    uint32_t next_off = 0, next_size = 0;
+    auto look_up = [&](int tile) {
+        const size_t at = 2 * ((size_t)blk0 + 2 * (size_t)min(tile, p.tiles_c - 1) * (size_t)p.BH);
+        next_off = info[at];
+        next_size = info[at + 1];
+    };
+    const uint32_t bytes4 = (uint32_t)((bytes + 3u) & ~3ull);
+    const uintptr_t stream = reinterpret_cast<uintptr_t>(wave < 2 ? p.k_stream : p.v_stream);
+    const u4 copy_rsrc = {(uint32_t)stream, (uint32_t)(stream >> 32) & 0xFFFFu, bytes4, 0x00020000u};
+    const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(stream), 0, (int)bytes4, 0x00020000);
+    u4 raw[WIDE ? NQ : 1];
     uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
-    auto fetch = [&](int tile) {
-        const uint32_t blk = wave < 2 ? (2u * (uint32_t)tile + (uint32_t)wave) * (uint32_t)p.BH + (uint32_t)bh
-                                      : 2u * ((uint32_t)tile * (uint32_t)p.BH + (uint32_t)bh) + (uint32_t)(wave - 2);
-        uint32_t off, size;
-        block_span(wave < 2 ? p.k_info : p.v_info, blk, cap, bytes, off, size);
+    __shared__ uint32_t phase_s[2][4];
+    // starts the copies of `tile`, whose entry look_up has fetched (widths above 4: into registers, for put)
+    auto fetch = [&](int tile, int buf) {
+        uint32_t off = next_off, size = min(next_size, cap);               // (never outside the stream, whatever block_info says)
+        if ((uint64_t)off > bytes) off = (uint32_t)bytes;
+        size = (uint32_t)min((uint64_t)size, bytes - (uint64_t)off);
         raw_phase = off & 15u;
         const uint32_t n16 = (raw_phase + size + 15u) >> 4, src = off - raw_phase;
+        if (WIDE) {
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-            const uint32_t c = (uint32_t)(lane + 64 * i);
-            raw[i] = c < n16 ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, src + 16u * c, 0, 0)) : (u4){0, 0, 0, 0};
+            for (int i = 0; i < (WIDE ? NQ : 1); i++) {
+                const uint32_t c = (uint32_t)(lane + 64 * i);
+                raw[i] = c < n16 ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, src + 16u * c, 0, 0)) : (u4){0, 0, 0, 0};
+            }
+        } else {
+            const uint32_t dst = (uint32_t)reinterpret_cast<uintptr_t>(ring) + (uint32_t)(4 * buf + wave) * p.slot;
+#pragma unroll
+            for (int i = 0; i < NQ; i++)
+                if ((uint32_t)(lane + 64 * i) < n16) copy_to_lds(copy_rsrc, __builtin_amdgcn_readfirstlane(dst + 1024u * i), src + 16u * (uint32_t)(lane + 64 * i));
+            if (lane == 0) phase_s[buf][wave] = raw_phase;
         }
+        look_up(tile + 1);
         const size_t at = (size_t)b * p.par_stride + (size_t)tile * kChunkTile + 32 * wave + t;
         par_k = p.k_scale[at]; par_kz = p.k_zero[at]; par_v = p.v_scale[at]; par_vz = p.v_zero[at];
     };
-    __shared__ uint32_t phase_s[2][4];
-    auto put = [&](int buf) {
-        uint8_t *dst = ring + (uint32_t)(4 * buf + wave) * p.slot;
+    auto put = [&](int buf) {                              // what fetch has started is in LDS behind the next barrier
+        if (WIDE) {
+            uint8_t *dst = ring + (uint32_t)(4 * buf + wave) * p.slot;
 #pragma unroll
-        for (int i = 0; i < NQ; i++)
-            if ((uint32_t)(lane + 64 * i) * 16u < p.slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
-        if (lane == 0) phase_s[buf][wave] = raw_phase;
+            for (int i = 0; i < (WIDE ? NQ : 1); i++)
+                if ((uint32_t)(lane + 64 * i) * 16u < p.slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
+            if (lane == 0) phase_s[buf][wave] = raw_phase;
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
     };
-    if (c0 < c1) fetch(c0);
+    if (c0 < c1) {
+        look_up(c0);
+        fetch(c0, 0);
+    }
 
     // ---- q: rows into LDS as fp16 (bf16: times 2^up), their sums ----
     int up = 0;
@@ -251,7 +300,7 @@ __global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const 
     }
     const float to_score = p.sm_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
     uint8_t *kt = kt_all + wave * 32 * kKRow;
-    float4 *par = par_all + wave * 32;
+    float2 *par_s = par_all + wave * 32, *par_w = par_s + 128;
     uint32_t emax = 0;                                     // exponent field of the largest V scale met, at least 14; 0: none yet
     float unit = 1.f;                                      // result = (acc + z) * unit
     const UnitGeom gk = unit_geom(p.k_bits), gv = unit_geom(p.v_bits);
@@ -267,19 +316,19 @@ __global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const 
             const bool real = tok0 + t >= start;
             const float ks = real ? chunk_f32(par_k, BF) * to_score : 0.f, kz = real ? chunk_f32(par_kz, BF) : 0.f;
             const float vs = real ? chunk_f32(par_v, BF) : 0.f, vz = real ? chunk_f32(par_vz, BF) : 0.f;
-            uint32_t e = (__float_as_uint(vs) >> 23) & 255u;
-#pragma unroll
-            for (int d = 16; d; d >>= 1) e = max(e, (uint32_t)__shfl_xor((int)e, d, 64));
-            e = __builtin_amdgcn_readfirstlane(max(e, 14u));
+            const uint32_t e = max(half_max((__float_as_uint(vs) >> 23) & 255u), 14u);
             if (e > emax) {
                 if (emax) grow = __builtin_amdgcn_exp2f((float)(int)(emax - e));
                 emax = e;
-                unit = __uint_as_float((e - 13u) << 23);   // 1 / (the weights' power of two, 2^(140 - e))
+                unit = __uint_as_float((e - 6u) << 23);    // 1 / (the weights' power of two, 2^(133 - e): V scales come to 2^7 at most)
             }
-            const float vw = vs * __uint_as_float(min(267u - emax, 254u) << 23);
-            if (h == 0) par[t] = make_float4(ks, kz * ks, vw, vz);
+            const float vw = vs * __uint_as_float((260u - emax) << 23);
+            if (h == 0) {
+                par_s[t] = make_float2(ks, kz * ks);
+                par_w[t] = make_float2(vw, vz);
+            }
         }
-        if (tile + 1 < c1) fetch(tile + 1);
+        if (tile + 1 < c1) fetch(tile + 1, buf ^ 1);
         const uint8_t *blk_k = ring + (uint32_t)(4 * buf + (hw >> 2)) * p.slot, *blk_v = ring + (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot;
         const int u = hw & 3;
         {   // V unit of this half-wavefront: where its packs are
@@ -316,11 +365,14 @@ __global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const 
                 y[nb] = product<false>(a, *reinterpret_cast<const u4 *>(qt + (32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
         }
         const bool masked = tok0 + 31 > pos_first || tok0 < start;             // (uniform)
+        float ref[NB];                                     // what the scores are taken against
+#pragma unroll
+        for (int nb = 0; nb < NB; nb++) ref[nb] = m[nb] == kLowest ? 0.f : m[nb];
 #pragma unroll
         for (int r = 0; r < 16; r++) {
-            const float4 q4 = par[16 * h + r];
+            const float2 q2 = par_s[16 * h + r];
 #pragma unroll
-            for (int nb = 0; nb < NB; nb++) y[nb][r] = y[nb][r] * q4.x + q4.y * qsum[nb];
+            for (int nb = 0; nb < NB; nb++) y[nb][r] = fmaf(y[nb][r], q2.x, fmaf(q2.y, qsum[nb], -ref[nb]));
         }
         if (masked) {
 #pragma unroll
@@ -334,27 +386,40 @@ __global__ void __launch_bounds__(256, NB == 1 ? 2 : 1) attn_chunk_kernel(const 
         u4 w[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
-            const float alpha = softmax_step(y[nb], m[nb]), both = alpha * grow;
-            l[nb] *= alpha;
-            z[nb] *= both;
-            if (__any(both != 1.f)) {
+            float over = y[nb][0];
+#pragma unroll
+            for (int r = 1; r < 16; r++) over = fmaxf(over, y[nb][r]);
+            if (__any(over > 8.f || m[nb] == kLowest) || grow != 1.f) {
+                over = fmaxf(over, __shfl_xor(over, 32, 64));
+                const bool first = m[nb] == kLowest;
+                const float raise = over > 8.f || (first && over > -INFINITY) ? over : 0.f;
+                if (raise != 0.f || (first && over == 0.f)) m[nb] = ref[nb] + raise;
+                const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(-raise);           // (nothing is summed before the first)
+#pragma unroll
+                for (int r = 0; r < 16; r++) y[nb][r] -= raise;
+                l[nb] *= alpha;
+                z[nb] *= alpha * grow;
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
-                    for (int r = 0; r < 16; r++) acc[nb][c][r] *= both;
+                    for (int r = 0; r < 16; r++) acc[nb][c][r] *= alpha * grow;
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float4 pa = par[16 * h + j], pb = par[16 * h + j + 8];
-                l[nb] += y[nb][j] + y[nb][j + 8];
-                uint32_t f = pack_f16(y[nb][j] * pa.z, y[nb][j + 8] * pb.z);
+                const float2 pa = par_w[16 * h + j], pb = par_w[16 * h + j + 8];
+                const float a = __builtin_amdgcn_exp2f(y[nb][j]), d = __builtin_amdgcn_exp2f(y[nb][j + 8]);
+                l[nb] += a;
+                l[nb] += d;
+                uint32_t f = pack_f16(a * pa.x, d * pb.x);
                 asm("" : "+v"(f));                         // (the sum takes these very halves: formed again they round once less)
                 const h2v f2 = __builtin_bit_cast(h2v, f);
-                z[nb] += (float)f2[0] * pa.w + (float)f2[1] * pb.w;
+                z[nb] = fmaf((float)f2[0], pa.y, z[nb]);
+                z[nb] = fmaf((float)f2[1], pb.y, z[nb]);
                 w[nb][j >> 2][j & 3] = f;
             }
         }
-        __syncthreads();                                   // the table is there
+        if (WIDE) __syncthreads();
+        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the table is there; copies go on
 #pragma unroll
         for (int c = 0; c < 4; c++) {                      // 32 channels: block c / 2, column of units c % 2
             const uint32_t e = tab[((((c >> 1) * 4 + (c & 1) * 2 + (wave >> 1)) * 4) + 2 * (wave & 1) + h) * 32 + t];
@@ -563,10 +628,12 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const float *__restric
               : make_uint2(pack_f16(o.x * inv, o.y * inv), pack_f16(o.z * inv, o.w * inv));
 }
 
+static bool chunk_wide(const pkv_chunk_args *a) { return a->T_c && (a->k_bits > 4 || a->v_bits > 4); }
+
 // How a call is cut: rows a workgroup, runs of tiles.  Workgroups are wanted for two a CU (512); a run of one tile is the least.
 static void chunk_cut(const pkv_chunk_args *a, int &nb, int &row_tiles, int &tiles, int &run, int &nsplit) {
     const int64_t rows = (int64_t)a->n * (a->Hq / a->Hkv);
-    nb = rows <= 32 ? 1 : 2;
+    nb = rows <= 32 || chunk_wide(a) ? 1 : 2;
     row_tiles = (int)((rows + 32 * nb - 1) / (32 * nb));
     tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
     const int64_t groups = (int64_t)a->B * a->Hkv * row_tiles;
@@ -650,16 +717,14 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     p.slot = (((k_cap > v_cap ? k_cap : v_cap) + 15u) & ~15u) + 32u;       // a block at any phase, and a last word's reach
     p.ring = 8u * p.slot;
     if (p.ring < 4u * 32u * kVRow) p.ring = 4u * 32u * kVRow;               // (the end's sums take less: 2 x 32 x 129 floats)
-    const bool wide = p.k_bits > 4 || p.v_bits > 4, bf = a->dtype == PKV_BF16;
+    const bool wide = chunk_wide(a), bf = a->dtype == PKV_BF16;
     const uint32_t lds = p.ring + 4u * 32u * kKRow + 4096u + 2048u + 8u * 32u * nb * 4u + 32u * nb * kQRow;
     const uint64_t groups = ((uint64_t)p.BH * p.nsplit + 7) / 8, wgs = groups * 8 * (uint64_t)p.row_tiles;
     PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x queries too large");
-    const void *kernels[2][2][2] = {
-        {{(const void *)attn_chunk_kernel<false, 1, false>, (const void *)attn_chunk_kernel<false, 1, true>},
-         {(const void *)attn_chunk_kernel<false, 2, false>, (const void *)attn_chunk_kernel<false, 2, true>}},
-        {{(const void *)attn_chunk_kernel<true, 1, false>, (const void *)attn_chunk_kernel<true, 1, true>},
-         {(const void *)attn_chunk_kernel<true, 2, false>, (const void *)attn_chunk_kernel<true, 2, true>}}};
-    const void *kernel = kernels[bf][nb - 1][wide];
+    const void *kernels[2][3] = {
+        {(const void *)attn_chunk_kernel<false, 1, false>, (const void *)attn_chunk_kernel<false, 2, false>, (const void *)attn_chunk_kernel<false, 1, true>},
+        {(const void *)attn_chunk_kernel<true, 1, false>, (const void *)attn_chunk_kernel<true, 2, false>, (const void *)attn_chunk_kernel<true, 1, true>}};
+    const void *kernel = kernels[bf][wide ? 2 : nb - 1];
     PKV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *params[] = {&p};
     PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256), params, lds, s));
