@@ -149,16 +149,19 @@ __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
     return __builtin_amdgcn_exp2f(was - m);
 }
 
-template <bool BF, int NB, bool WIDE>
-__global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p) {
+template <bool BF, int NB, int RG, bool WIDE>
+__global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(const ChunkParams p) {
+    static_assert(RG == 1 || !WIDE, "wide codes: one group of rows");
     constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
+    constexpr int M = 32 * NB * RG, kBufs = RG + 1, kSets = RG;
     extern __shared__ __align__(16) uint8_t lds[];
-    uint8_t *ring = lds;                                   // two tiles of four staged blocks; window: V rows; end: sums
-    uint8_t *kt_all = lds + p.ring;                        // [4 wavefronts][32 tokens][kKRow]
-    uint32_t *tab = reinterpret_cast<uint32_t *>(kt_all + 4 * 32 * kKRow);         // [8 units][4 slots][32 lanes]
-    float2 *par_all = reinterpret_cast<float2 *>(tab + 1024);                      // [4][32] (scale, zero * scale) and [4][32] (V scale, V zero)
-    float *st = reinterpret_cast<float *>(par_all + 256);                          // [2][4][32 NB] maxima, sums at the end
-    uint8_t *qt = reinterpret_cast<uint8_t *>(st + 8 * 32 * NB);                   // [32 NB][kQRow]
+    uint8_t *ring = lds;                                   // kBufs tiles of four staged blocks; window and end: V rows, sums (kt as well)
+    uint8_t *kt_all = lds + p.ring;                        // [kSets][4 quarters][32 tokens][kKRow]
+    uint32_t *tab_all = reinterpret_cast<uint32_t *>(kt_all + kSets * 4 * 32 * kKRow);        // [kSets][8 units][4 slots][32 lanes]
+    float2 *par_all = reinterpret_cast<float2 *>(tab_all + kSets * 1024);          // [kSets][2][4][32]: (scale, zero * scale), (V scale, V zero)
+    float *st = reinterpret_cast<float *>(par_all + kSets * 256);                  // [2][4][M] maxima, sums at the end
+    uint8_t *qt = reinterpret_cast<uint8_t *>(st + 8 * M);                         // [M][kQRow]
+    __shared__ uint32_t phase_s[kBufs][4], top_s[kSets][4];
 
     // Row tiles of one (KV head, run) follow each other on one XCD (workgroups go round the eight of them), so that they find its
     // blocks in that L2.
@@ -167,16 +170,17 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
     if (group >= groups) return;
     const int rt = (int)(seq % (uint32_t)p.row_tiles), bh = (int)(group % (uint32_t)p.BH), split = (int)(group / (uint32_t)p.BH);
     const int b = bh / p.Hkv, hkv = bh % p.Hkv;
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, t = lane & 31, hw = tid >> 5;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, t = lane & 31;
+    const int rg = wave >> 2, quarter = wave & 3;          // rows, and tokens, of this wavefront
     const int T = p.T_c + p.T_w;
-    const int row0 = rt * 32 * NB, row_last = min(row0 + 32 * NB, p.rows) - 1;
+    const int row0 = rt * M, row_last = min(row0 + M, p.rows) - 1, mine0 = 32 * NB * rg;
     const int start = p.starts ? min(max(p.starts[b], 0), T) : 0;
-    const int pos_first = p.causal ? T - p.n + row0 / p.G : T - 1, pos_last = p.causal ? T - p.n + row_last / p.G : T - 1;
+    const int pos_first = p.causal ? T - p.n + min(row0 + mine0, p.rows - 1) / p.G : T - 1, pos_last = p.causal ? T - p.n + row_last / p.G : T - 1;
 
     int row[NB], pos[NB];                                  // the lane's rows, and the last token that each sees
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        row[nb] = min(row0 + 32 * nb + t, p.rows - 1);
+        row[nb] = min(row0 + mine0 + 32 * nb + t, p.rows - 1);
         pos[nb] = p.causal ? T - p.n + row[nb] / p.G : T - 1;
     }
     auto q_row = [&](int r) -> const uint16_t * {
@@ -189,12 +193,12 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
     const int c0 = max(first, start / kChunkTile), c1 = min(last, (seen_c + kChunkTile - 1) / kChunkTile);
     const int w0 = max(first - p.tiles_c, max(start - p.T_c, 0) / kChunkTile), w1 = min(last - p.tiles_c, (pos_last - p.T_c) / kChunkTile + 1);
 
-    // ---- staging of a tile's four blocks (wavefront = block), one tile ahead; block_info a tile further, through scalar loads ----
+    // ---- staging of a tile's four blocks (quarter = block), ahead of their use; block_info a tile further, through scalar loads ----
     typedef const __attribute__((address_space(4))) uint32_t *const_u32_ptr;
-    const uint32_t cap = wave < 2 ? (uint32_t)k_block_bound(64, p.k_bits) : (uint32_t)v_block_bound(64, p.v_bits);
-    const uint64_t bytes = wave < 2 ? p.k_bytes : p.v_bytes;
-    const const_u32_ptr info = reinterpret_cast<const_u32_ptr>(reinterpret_cast<uintptr_t>(wave < 2 ? p.k_info : p.v_info));
-    const uint32_t blk0 = wave < 2 ? (uint32_t)wave * (uint32_t)p.BH + (uint32_t)bh : 2u * (uint32_t)bh + (uint32_t)(wave - 2);
+    const uint32_t cap = quarter < 2 ? (uint32_t)k_block_bound(64, p.k_bits) : (uint32_t)v_block_bound(64, p.v_bits);
+    const uint64_t bytes = quarter < 2 ? p.k_bytes : p.v_bytes;
+    const const_u32_ptr info = reinterpret_cast<const_u32_ptr>(reinterpret_cast<uintptr_t>(quarter < 2 ? p.k_info : p.v_info));
+    const uint32_t blk0 = quarter < 2 ? (uint32_t)quarter * (uint32_t)p.BH + (uint32_t)bh : 2u * (uint32_t)bh + (uint32_t)(quarter - 2);
     uint32_t next_off = 0, next_size = 0;
     auto look_up = [&](int tile) {
         const size_t at = 2 * ((size_t)blk0 + 2 * (size_t)min(tile, p.tiles_c - 1) * (size_t)p.BH);
@@ -202,12 +206,11 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
         next_size = info[at + 1];
     };
     const uint32_t bytes4 = (uint32_t)((bytes + 3u) & ~3ull);
-    const uintptr_t stream = reinterpret_cast<uintptr_t>(wave < 2 ? p.k_stream : p.v_stream);
+    const uintptr_t stream = reinterpret_cast<uintptr_t>(quarter < 2 ? p.k_stream : p.v_stream);
     const u4 copy_rsrc = {(uint32_t)stream, (uint32_t)(stream >> 32) & 0xFFFFu, bytes4, 0x00020000u};
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(stream), 0, (int)bytes4, 0x00020000);
     u4 raw[WIDE ? NQ : 1];
     uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
-    __shared__ uint32_t phase_s[2][4];
     // starts the copies of `tile`, whose entry look_up has fetched (widths above 4: into registers, for put)
     auto fetch = [&](int tile, int buf) {
         uint32_t off = next_off, size = min(next_size, cap);               // (never outside the stream, whatever block_info says)
@@ -222,23 +225,27 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
                 raw[i] = c < n16 ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, src + 16u * c, 0, 0)) : (u4){0, 0, 0, 0};
             }
         } else {
-            const uint32_t dst = (uint32_t)reinterpret_cast<uintptr_t>(ring) + (uint32_t)(4 * buf + wave) * p.slot;
+            const uint32_t dst = (uint32_t)reinterpret_cast<uintptr_t>(ring) + (uint32_t)(4 * buf + quarter) * p.slot;
 #pragma unroll
-            for (int i = 0; i < NQ; i++)
-                if ((uint32_t)(lane + 64 * i) < n16) copy_to_lds(copy_rsrc, __builtin_amdgcn_readfirstlane(dst + 1024u * i), src + 16u * (uint32_t)(lane + 64 * i));
-            if (lane == 0) phase_s[buf][wave] = raw_phase;
+            for (int i = 0; i < (NQ + RG - 1) / RG; i++) {                 // (two groups of rows: every other step each)
+                const uint32_t step = (uint32_t)(RG * i + rg);
+                if ((uint32_t)lane + 64u * step < n16) copy_to_lds(copy_rsrc, __builtin_amdgcn_readfirstlane(dst + 1024u * step), src + 16u * ((uint32_t)lane + 64u * step));
+            }
+            if (lane == 0 && rg == 0) phase_s[buf][quarter] = raw_phase;
         }
         look_up(tile + 1);
-        const size_t at = (size_t)b * p.par_stride + (size_t)tile * kChunkTile + 32 * wave + t;
+    };
+    auto fetch_par = [&](int tile) {                       // the parameters of this wavefront's 32 tokens
+        const size_t at = (size_t)b * p.par_stride + (size_t)tile * kChunkTile + 32 * quarter + t;
         par_k = p.k_scale[at]; par_kz = p.k_zero[at]; par_v = p.v_scale[at]; par_vz = p.v_zero[at];
     };
     auto put = [&](int buf) {                              // what fetch has started is in LDS behind the next barrier
         if (WIDE) {
-            uint8_t *dst = ring + (uint32_t)(4 * buf + wave) * p.slot;
+            uint8_t *dst = ring + (uint32_t)(4 * buf + quarter) * p.slot;
 #pragma unroll
             for (int i = 0; i < (WIDE ? NQ : 1); i++)
                 if ((uint32_t)(lane + 64 * i) * 16u < p.slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
-            if (lane == 0) phase_s[buf][wave] = raw_phase;
+            if (lane == 0) phase_s[buf][quarter] = raw_phase;
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
@@ -246,25 +253,29 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
     if (c0 < c1) {
         look_up(c0);
         fetch(c0, 0);
+        if (RG == 2 && c0 + 1 < c1) fetch(c0 + 1, 1);
+        fetch_par(c0);
     }
 
     // ---- q: rows into LDS as fp16 (bf16: times 2^up), their sums ----
     int up = 0;
     if (BF) {
         uint32_t top = 0;
-        for (int r = wave; r <= row_last - row0; r += 4) {
+        for (int r = wave; r <= row_last - row0; r += 4 * RG) {
             const uint32_t w = reinterpret_cast<const uint32_t *>(q_row(row0 + r))[lane];
             top = max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-        if (lane == 0) tab[wave] = top;
+        if (lane == 0) tab_all[wave] = top;
         __syncthreads();
-        top = max(max(tab[0], tab[1]), max(tab[2], tab[3]));
+        top = tab_all[0];
+#pragma unroll
+        for (int i = 1; i < 4 * RG; i++) top = max(top, tab_all[i]);
         up = top ? min(max(141 - (int)(top >> 7), -120), 120) : 0;        // the largest comes to 2^14 .. 2^15
     }
     const float up_f = __uint_as_float((uint32_t)(127 + up) << 23);
-    for (int i = tid; i < 32 * NB * 16; i += 256) {
+    for (int i = tid; i < M * 16; i += 256 * RG) {
         const int r = i >> 4, c = i & 15;
         u4 w = *reinterpret_cast<const u4 *>(q_row(min(row0 + r, p.rows - 1)) + 8 * c);
         if (BF) {
@@ -281,7 +292,7 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
         float s = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; c++) {
-            const h8 v = *reinterpret_cast<const h8 *>(qt + (32 * nb + t) * kQRow + 32 * c + 16 * h);
+            const h8 v = *reinterpret_cast<const h8 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * c + 16 * h);
 #pragma unroll
             for (int k = 0; k < 8; k++) s += (float)v[k];
         }
@@ -299,58 +310,70 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
             for (int r = 0; r < 16; r++) acc[nb][c][r] = 0.f;
     }
     const float to_score = p.sm_log2 * __uint_as_float((uint32_t)(127 - up) << 23);
-    uint8_t *kt = kt_all + wave * 32 * kKRow;
-    float2 *par_s = par_all + wave * 32, *par_w = par_s + 128;
     uint32_t emax = 0;                                     // exponent field of the largest V scale met, at least 14; 0: none yet
     float unit = 1.f;                                      // result = (acc + z) * unit
     const UnitGeom gk = unit_geom(p.k_bits), gv = unit_geom(p.v_bits);
+    if (!WIDE) { __builtin_assume(gk.W <= 4); __builtin_assume(gv.W <= 4); }
     const int tau = (t & 3) + 4 * (t >> 3) + 16 * ((t >> 2) & 1);          // the token (of 32) in row t of S^T: lane half = pack
 
-    // ---- compressed tiles ----
-    for (int tile = c0; tile < c1; tile++) {
-        const int buf = (tile - c0) & 1;
-        if (tile != c0) __syncthreads();                   // the tile is staged, and the table's readers are done
-        const int tok0 = tile * kChunkTile + 32 * wave;    // this wavefront's first token
+    // A half-wavefront's unit of a staged tile: where it starts in its block.
+    const int hw = 2 * quarter + h, u = hw & 3;
+    auto unit_start = [&](int buf, int side) -> uint32_t {
+        const uint32_t phase = phase_s[buf][2 * side + (hw >> 2)];
+        const uint8_t *blk = ring + (uint32_t)(4 * buf + 2 * side + (hw >> 2)) * p.slot;
+        return min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk + phase)[u - 1] : 0u), p.slot - 16u);
+    };
+    auto unpack_k = [&](int buf, uint8_t *kt) {            // 16 tokens x 128 channels; the quarter's two units make its 32 tokens
+        uint8_t *dst = kt + quarter * 32 * kKRow + 16 * h * kKRow + 4 * t;
+        unit_codes(ring + (uint32_t)(4 * buf + (hw >> 2)) * p.slot, unit_start(buf, 0), t, gk,
+                   [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
+    };
+    auto parse_v = [&](int buf, uint32_t *tab) {           // where the unit's packs are
+        const uint32_t slot_at = (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot, at = unit_start(buf, 1);
+        const uint8_t *blk = ring + slot_at;
+        const uint32_t minsw = lds_meta_word(blk + at, t, gv.W), lensw = lds_meta_word(blk + at + gv.mins_bytes, t, gv.LB);
+        uint32_t len[4], off[4], payload;
+#pragma unroll
+        for (int i = 0; i < 4; i++) len[i] = min((lensw >> (i * gv.LB)) & ((1u << gv.LB) - 1u), (uint32_t)gv.W);
+        pack_offsets(len, off, payload);
+        const uint32_t base = slot_at + at + (uint32_t)(gv.mins_bytes + gv.lens_bytes);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            tab[(hw * 4 + i) * 32 + t] = min(base + off[i], p.ring - 32u) | (len[i] << 16) | (((minsw >> (i * gv.W)) & ((1u << gv.W) - 1u)) << 20);
+    };
+    // Parameters of the quarter's 32 tokens into LDS; those in front of the sequence count as nothing.  Returns what the accumulators
+    // are to be multiplied with where a larger V scale than before came up.  (Two groups of rows: the group that writes and the one
+    // that reads follow the same scales.)
+    auto raise_scale = [&](uint32_t e) -> float {
         float grow = 1.f;
-        {   // parameters of the 32 tokens; those in front of the sequence count as nothing
-            const bool real = tok0 + t >= start;
-            const float ks = real ? chunk_f32(par_k, BF) * to_score : 0.f, kz = real ? chunk_f32(par_kz, BF) : 0.f;
-            const float vs = real ? chunk_f32(par_v, BF) : 0.f, vz = real ? chunk_f32(par_vz, BF) : 0.f;
-            const uint32_t e = max(half_max((__float_as_uint(vs) >> 23) & 255u), 14u);
-            if (e > emax) {
-                if (emax) grow = __builtin_amdgcn_exp2f((float)(int)(emax - e));
-                emax = e;
-                unit = __uint_as_float((e - 6u) << 23);    // 1 / (the weights' power of two, 2^(133 - e): V scales come to 2^7 at most)
-            }
-            const float vw = vs * __uint_as_float((260u - emax) << 23);
-            if (h == 0) {
-                par_s[t] = make_float2(ks, kz * ks);
-                par_w[t] = make_float2(vw, vz);
-            }
+        if (e > emax) {
+            if (emax) grow = __builtin_amdgcn_exp2f((float)(int)(emax - e));
+            emax = e;
+            unit = __uint_as_float((e - 6u) << 23);        // 1 / (the weights' power of two, 2^(133 - e): V scales come to 2^7 at most)
         }
-        if (tile + 1 < c1) fetch(tile + 1, buf ^ 1);
-        const uint8_t *blk_k = ring + (uint32_t)(4 * buf + (hw >> 2)) * p.slot, *blk_v = ring + (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot;
-        const int u = hw & 3;
-        {   // V unit of this half-wavefront: where its packs are
-            const uint32_t phase = phase_s[buf][2 + (hw >> 2)];
-            const uint32_t at = min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk_v + phase)[u - 1] : 0u), p.slot - 16u);
-            const uint32_t minsw = lds_meta_word(blk_v + at, t, gv.W), lensw = lds_meta_word(blk_v + at + gv.mins_bytes, t, gv.LB);
-            uint32_t len[4], off[4], payload;
-#pragma unroll
-            for (int i = 0; i < 4; i++) len[i] = min((lensw >> (i * gv.LB)) & ((1u << gv.LB) - 1u), (uint32_t)gv.W);
-            pack_offsets(len, off, payload);
-            const uint32_t base = (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot + at + (uint32_t)(gv.mins_bytes + gv.lens_bytes);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-                tab[(hw * 4 + i) * 32 + t] = min(base + off[i], p.ring - 32u) | (len[i] << 16) | (((minsw >> (i * gv.W)) & ((1u << gv.W) - 1u)) << 20);
+        return grow;
+    };
+    uint32_t writer_top = 0;                               // the largest V scale that the parameters in LDS have met
+    auto write_par = [&](int tile, int set) -> uint32_t {
+        const bool real = tile * kChunkTile + 32 * quarter + t >= start;
+        const float ks = real ? chunk_f32(par_k, BF) * to_score : 0.f, kz = real ? chunk_f32(par_kz, BF) : 0.f;
+        const float vs = real ? chunk_f32(par_v, BF) : 0.f, vz = real ? chunk_f32(par_vz, BF) : 0.f;
+        const uint32_t e = max(half_max((__float_as_uint(vs) >> 23) & 255u), 14u);
+        writer_top = max(writer_top, e);
+        const float vw = vs * __uint_as_float((260u - writer_top) << 23);
+        float2 *dst = par_all + set * 256 + quarter * 32 + t;
+        if (h == 0) {
+            dst[0] = make_float2(ks, kz * ks);
+            dst[128] = make_float2(vw, vz);
         }
-        {   // K unit: 16 tokens x 128 channels, the wavefront's two make its 32 tokens
-            const uint32_t phase = phase_s[buf][hw >> 2];
-            const uint32_t at = min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk_k + phase)[u - 1] : 0u), p.slot - 16u);
-            uint8_t *dst = kt + 16 * h * kKRow + 4 * t;
-            unit_codes(blk_k, at, t, gk, [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
-        }
-        wave_lds_order();
+        return e;
+    };
+
+    // Scores of a tile's 32 tokens against the lane's rows, the softmax step, and the weights as operands.
+    auto weights_of = [&](int tile, const uint8_t *kt, const float2 *par, float grow, u4 (&w)[NB][2]) {
+        const int tok0 = tile * kChunkTile + 32 * quarter;                     // this wavefront's first token
+        kt += quarter * 32 * kKRow;
+        const float2 *par_s = par + quarter * 32, *par_w = par_s + 128;
         f16v y[NB];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++)
@@ -362,9 +385,8 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
             const u4 a = {codes_f16(c8.x, 0x04010400u), codes_f16(c8.x, 0x04030402u), codes_f16(c8.y, 0x04010400u), codes_f16(c8.y, 0x04030402u)};
 #pragma unroll
             for (int nb = 0; nb < NB; nb++)
-                y[nb] = product<false>(a, *reinterpret_cast<const u4 *>(qt + (32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
+                y[nb] = product<false>(a, *reinterpret_cast<const u4 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
         }
-        const bool masked = tok0 + 31 > pos_first || tok0 < start;             // (uniform)
         float ref[NB];                                     // what the scores are taken against
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) ref[nb] = m[nb] == kLowest ? 0.f : m[nb];
@@ -374,7 +396,7 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
 #pragma unroll
             for (int nb = 0; nb < NB; nb++) y[nb][r] = fmaf(y[nb][r], q2.x, fmaf(q2.y, qsum[nb], -ref[nb]));
         }
-        if (masked) {
+        if (tok0 + 31 > pos_first || tok0 < start) {       // (uniform: some row does not see every token)
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int tok = tok0 + 16 * h + r;
@@ -383,7 +405,6 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
                     if (tok > pos[nb] || tok < start) y[nb][r] = -INFINITY;
             }
         }
-        u4 w[NB][2];
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) {
             float over = y[nb][0];
@@ -391,10 +412,10 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
             for (int r = 1; r < 16; r++) over = fmaxf(over, y[nb][r]);
             if (__any(over > 8.f || m[nb] == kLowest) || grow != 1.f) {
                 over = fmaxf(over, __shfl_xor(over, 32, 64));
-                const bool first = m[nb] == kLowest;
-                const float raise = over > 8.f || (first && over > -INFINITY) ? over : 0.f;
-                if (raise != 0.f || (first && over == 0.f)) m[nb] = ref[nb] + raise;
-                const float alpha = first ? 1.f : __builtin_amdgcn_exp2f(-raise);           // (nothing is summed before the first)
+                const bool none = m[nb] == kLowest;
+                const float raise = over > 8.f || (none && over > -INFINITY) ? over : 0.f;
+                if (raise != 0.f || (none && over == 0.f)) m[nb] = ref[nb] + raise;
+                const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(-raise);           // (nothing is summed before the first)
 #pragma unroll
                 for (int r = 0; r < 16; r++) y[nb][r] -= raise;
                 l[nb] *= alpha;
@@ -418,11 +439,11 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
                 w[nb][j >> 2][j & 3] = f;
             }
         }
-        if (WIDE) __syncthreads();
-        else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the table is there; copies go on
+    };
+    auto add_values = [&](const uint32_t *tab, const u4 (&w)[NB][2]) {
 #pragma unroll
         for (int c = 0; c < 4; c++) {                      // 32 channels: block c / 2, column of units c % 2
-            const uint32_t e = tab[((((c >> 1) * 4 + (c & 1) * 2 + (wave >> 1)) * 4) + 2 * (wave & 1) + h) * 32 + t];
+            const uint32_t e = tab[((((c >> 1) * 4 + (c & 1) * 2 + (quarter >> 1)) * 4) + 2 * (quarter & 1) + h) * 32 + t];
             uint32_t v[8];
             pack_operand<WIDE>(ring, e, v);
             const u4 v0 = {v[0], v[1], v[2], v[3]}, v1 = {v[4], v[5], v[6], v[7]};
@@ -432,7 +453,60 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
                 acc[nb][c] = product<false>(v1, w[nb][1], acc[nb][c]);
             }
         }
-        if (tile + 1 < c1) put(buf ^ 1);
+    };
+
+    // ---- compressed tiles ----
+    if (RG == 1) {
+        // Few rows: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
+        for (int tile = c0; tile < c1; tile++) {
+            const int buf = (tile - c0) & 1;
+            if (tile != c0) __syncthreads();               // the tile is staged, and the table's readers are done
+            const float grow = raise_scale(write_par(tile, 0));
+            if (tile + 1 < c1) {
+                fetch(tile + 1, buf ^ 1);
+                fetch_par(tile + 1);
+            }
+            parse_v(buf, tab_all);
+            unpack_k(buf, kt_all);
+            wave_lds_order();
+            u4 w[NB][2];
+            weights_of(tile, kt_all, par_all, grow, w);
+            if (WIDE) __syncthreads();
+            else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the table is there; copies go on
+            add_values(tab_all, w);
+            if (tile + 1 < c1) put(buf ^ 1);
+        }
+    } else if (c0 < c1) {
+        // Many rows: the two groups of rows share what is unpacked -- the first group's wavefronts unpack K, the second's find V's
+        // packs and write the parameters, a tile ahead, while the others are at their products.  One barrier a tile.
+        auto prepare = [&](int tile, int set, int buf) {
+            if (rg == 0) {
+                unpack_k(buf, kt_all + set * 4 * 32 * kKRow);
+            } else {
+                parse_v(buf, tab_all + set * 1024);
+                const uint32_t e = write_par(tile, set);
+                if (lane == 0) top_s[set][quarter] = e;
+            }
+        };
+        prepare(c0, 0, 0);
+        if (rg == 1 && c0 + 1 < c1) fetch_par(c0 + 1);
+        __syncthreads();
+        int buf = 0;
+        for (int tile = c0; tile < c1; tile++) {
+            const int set = (tile - c0) & 1, buf1 = buf == 2 ? 0 : buf + 1, buf2 = buf1 == 2 ? 0 : buf1 + 1;
+            if (tile + 2 < c1) fetch(tile + 2, buf2);
+            if (tile + 1 < c1) {
+                prepare(tile + 1, set ^ 1, buf1);
+                if (rg == 1 && tile + 2 < c1) fetch_par(tile + 2);
+            }
+            const float grow = raise_scale(__builtin_amdgcn_readfirstlane(top_s[set][quarter]));
+            u4 w[NB][2];
+            weights_of(tile, kt_all + set * 4 * 32 * kKRow, par_all + set * 256, grow, w);
+            add_values(tab_all + set * 1024, w);
+            put(buf2);
+            __syncthreads();
+            buf = buf1;
+        }
     }
 
     // ---- window tiles: the same products on the 16-bit rows ----
@@ -450,9 +524,9 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
             }
         }
         unit = 1.f / kUp;
-        uint8_t *vt = ring + wave * 32 * kVRow;
+        uint8_t *vt = ring + wave * 32 * kVRow;            // (into the K codes' place, where two groups of rows need it)
         for (int wt = w0; wt < w1; wt++) {
-            const int r0 = wt * kChunkTile + 32 * wave, tok0 = p.T_c + r0;     // window row and position of the wavefront's first token
+            const int r0 = wt * kChunkTile + 32 * quarter, tok0 = p.T_c + r0;     // window row and position of the wavefront's first token
             if (r0 >= p.T_w || tok0 > pos_last || tok0 + 31 < start) continue; // (uniform, and no barrier in here)
             const uint16_t *kr = p.k_win + ((size_t)bh * p.win_stride + min(r0 + tau, p.T_w - 1)) * kHeadDim + 8 * h;
             const uint16_t *vr = p.v_win + ((size_t)bh * p.win_stride) * kHeadDim;
@@ -478,7 +552,7 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
                     y[nb] = product<BF>(a, BF ? *reinterpret_cast<const u4 *>(q_row(row[nb]) + 16 * s + 8 * h)
-                                              : *reinterpret_cast<const u4 *>(qt + (32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
+                                              : *reinterpret_cast<const u4 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
@@ -527,36 +601,36 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
         }
     }
 
-    // ---- the four wavefronts' states become one ----
+    // ---- the states of a row's four wavefronts become one ----
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
         l[nb] += __shfl_xor(l[nb], 32, 64);
         z[nb] += __shfl_xor(z[nb], 32, 64);
-        if (h == 0) st[wave * 32 * NB + 32 * nb + t] = m[nb];
+        if (h == 0) st[quarter * M + mine0 + 32 * nb + t] = m[nb];
     }
     __syncthreads();
-    float *sums = st + 4 * 32 * NB;
+    float *sums = st + 4 * M;
     float top[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        const float *at = st + 32 * nb + t;
-        top[nb] = fmaxf(fmaxf(at[0], at[32 * NB]), fmaxf(at[64 * NB], at[96 * NB]));
+        const float *at = st + mine0 + 32 * nb + t;
+        top[nb] = fmaxf(fmaxf(at[0], at[M]), fmaxf(at[2 * M], at[3 * M]));
         const float f = __builtin_amdgcn_exp2f(m[nb] - top[nb]);
-        if (h == 0) sums[wave * 32 * NB + 32 * nb + t] = l[nb] * f;
+        if (h == 0) sums[quarter * M + mine0 + 32 * nb + t] = l[nb] * f;
         const float fu = f * unit;
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
             for (int r = 0; r < 16; r++) acc[nb][c][r] = (acc[nb][c][r] + z[nb]) * fu;
     }
-    float *buf0 = reinterpret_cast<float *>(ring);         // [2][32 rows][129]: wavefronts 0 + 2 and 1 + 3
     constexpr int kSumRow = 129;
+    float *buf0 = reinterpret_cast<float *>(ring) + rg * 2 * 32 * kSumRow;           // [2][32 rows][129]: quarters 0 + 2 and 1 + 3
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        float *mine = buf0 + (wave & 1) * 32 * kSumRow + t * kSumRow + 4 * h;
+        float *mine = buf0 + (quarter & 1) * 32 * kSumRow + t * kSumRow + 4 * h;
 #pragma unroll
         for (int step = 0; step < 2; step++) {
-            if ((wave >> 1) == step) {
+            if ((quarter >> 1) == step) {
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -567,17 +641,15 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
             }
             __syncthreads();
         }
-        const int i = tid >> 3, ch = 16 * (tid & 7), r = row0 + 32 * nb + i;                  // a row's 16 channels each
+        const int i = (tid & 255) >> 3, ch = 16 * (tid & 7), at = mine0 + 32 * nb + i, r = row0 + at;      // a row's 16 channels each
         if (r < p.rows) {
             const float *s0 = buf0 + i * kSumRow + ch, *s1 = s0 + 32 * kSumRow;
-            const float *sl = sums + 32 * nb + i;
-            const float total = (sl[0] + sl[32 * NB]) + (sl[64 * NB] + sl[96 * NB]);
+            const float total = (sums[at] + sums[M + at]) + (sums[2 * M + at] + sums[3 * M + at]);
             const int64_t head = hkv * p.G + r % p.G, token = r / p.G;
             if (p.part) {
                 float *dst = p.part + ((((int64_t)b * p.Hq + head) * p.n + token) * p.nsplit + split) * kPart;
                 if (ch == 0) {
-                    const float *sm = st + 32 * nb + i;
-                    dst[0] = fmaxf(fmaxf(sm[0], sm[32 * NB]), fmaxf(sm[64 * NB], sm[96 * NB]));
+                    dst[0] = fmaxf(fmaxf(st[at], st[M + at]), fmaxf(st[2 * M + at], st[3 * M + at]));
                     dst[1] = total;
                 }
 #pragma unroll
@@ -587,8 +659,8 @@ __global__ void __launch_bounds__(256, 2) attn_chunk_kernel(const ChunkParams p)
                 uint32_t o[8];
 #pragma unroll
                 for (int k = 0; k < 8; k++) {
-                    const float a = (s0[2 * k] + s1[2 * k]) * inv, d = (s0[2 * k + 1] + s1[2 * k + 1]) * inv;
-                    o[k] = BF ? pack_bf16(a, d) : pack_f16(a, d);
+                    const float x = (s0[2 * k] + s1[2 * k]) * inv, y = (s0[2 * k + 1] + s1[2 * k + 1]) * inv;
+                    o[k] = BF ? pack_bf16(x, y) : pack_f16(x, y);
                 }
                 u4 *dst = reinterpret_cast<u4 *>(p.out + (int64_t)b * p.o_b + head * p.o_h + token * p.o_t + ch);
                 dst[0] = (u4){o[0], o[1], o[2], o[3]};
@@ -630,17 +702,25 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const float *__restric
 
 static bool chunk_wide(const pkv_chunk_args *a) { return a->T_c && (a->k_bits > 4 || a->v_bits > 4); }
 
-// How a call is cut: rows a workgroup, runs of tiles.  Workgroups are wanted for two a CU (512); a run of one tile is the least.
-static void chunk_cut(const pkv_chunk_args *a, int &nb, int &row_tiles, int &tiles, int &run, int &nsplit) {
+// How a call is cut: rows a workgroup (32 NB RG), runs of tiles.  Two workgroups a CU are wanted of the small kind (512), one of the large
+// (256); a run of one tile is the least.
+struct ChunkCut {
+    int nb, rg, row_tiles, tiles, run, nsplit;
+};
+static ChunkCut chunk_cut(const pkv_chunk_args *a) {
+    ChunkCut c;
     const int64_t rows = (int64_t)a->n * (a->Hq / a->Hkv);
-    nb = rows <= 32 || chunk_wide(a) ? 1 : 2;
-    row_tiles = (int)((rows + 32 * nb - 1) / (32 * nb));
-    tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
-    const int64_t groups = (int64_t)a->B * a->Hkv * row_tiles;
-    int64_t want = (512 + groups - 1) / groups;
-    if (want > tiles) want = tiles;
-    run = (int)((tiles + want - 1) / want);
-    nsplit = (tiles + run - 1) / run;
+    c.rg = rows <= 32 || chunk_wide(a) ? 1 : 2;
+    c.nb = c.rg == 1 || rows <= 64 ? 1 : 2;
+    const int64_t m = 32 * c.nb * c.rg;
+    c.row_tiles = (int)((rows + m - 1) / m);
+    c.tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
+    const int64_t groups = (int64_t)a->B * a->Hkv * c.row_tiles, aim = c.rg == 1 ? 512 : 256;
+    int64_t want = (aim + groups - 1) / groups;
+    if (want > c.tiles) want = c.tiles;
+    c.run = (int)((c.tiles + want - 1) / want);
+    c.nsplit = (c.tiles + c.run - 1) / c.run;
+    return c;
 }
 
 static int chunk_check(const pkv_chunk_args *a) {
@@ -661,8 +741,7 @@ extern "C" {
 uint64_t pkv_attn_chunk_workspace(const pkv_chunk_args *a) {
     using namespace pkv;
     if (chunk_check(a)) return 0;
-    int nb, row_tiles, tiles, run, nsplit;
-    chunk_cut(a, nb, row_tiles, tiles, run, nsplit);
+    const int nsplit = chunk_cut(a).nsplit;
     return nsplit > 1 ? (uint64_t)a->B * a->Hq * a->n * nsplit * kPart * sizeof(float) : 0;
 }
 
@@ -693,8 +772,8 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     if (a->T_w > 0)
         PKV_REQUIRE(a->k_win && a->v_win && ((reinterpret_cast<uintptr_t>(a->k_win) | reinterpret_cast<uintptr_t>(a->v_win)) & 15u) == 0, PKV_ERR_INVALID,
                     "window tensors must be present and 16-byte aligned");
-    int nb;
-    chunk_cut(a, nb, p.row_tiles, p.tiles, p.run, p.nsplit);
+    const ChunkCut cut = chunk_cut(a);
+    p.row_tiles = cut.row_tiles; p.tiles = cut.tiles; p.run = cut.run; p.nsplit = cut.nsplit;
     const uint64_t need = p.nsplit > 1 ? (uint64_t)a->B * a->Hq * a->n * p.nsplit * kPart * sizeof(float) : 0;
     PKV_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0), PKV_ERR_CAPACITY,
                 "the call needs a 16-byte aligned workspace of %llu bytes", (unsigned long long)need);
@@ -715,19 +794,22 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     p.sm_log2 = a->sm_scale * kLog2e;
     const uint32_t k_cap = (uint32_t)k_block_bound(64, p.k_bits), v_cap = (uint32_t)v_block_bound(64, p.v_bits);
     p.slot = (((k_cap > v_cap ? k_cap : v_cap) + 15u) & ~15u) + 32u;       // a block at any phase, and a last word's reach
-    p.ring = 8u * p.slot;
-    if (p.ring < 4u * 32u * kVRow) p.ring = 4u * 32u * kVRow;               // (the end's sums take less: 2 x 32 x 129 floats)
+    const uint32_t rg = (uint32_t)cut.rg, m = 32u * (uint32_t)cut.nb * rg, kt = rg * 4u * 32u * kKRow;
+    p.ring = (rg + 1u) * 4u * p.slot;
+    if (p.ring + kt < 4u * rg * 32u * kVRow) p.ring = 4u * rg * 32u * kVRow - kt;      // (the end's sums take less: rg * 2 x 32 x 129 floats)
     const bool wide = chunk_wide(a), bf = a->dtype == PKV_BF16;
-    const uint32_t lds = p.ring + 4u * 32u * kKRow + 4096u + 2048u + 8u * 32u * nb * 4u + 32u * nb * kQRow;
+    const uint32_t lds = p.ring + kt + rg * (4096u + 2048u) + 8u * m * 4u + m * kQRow;
     const uint64_t groups = ((uint64_t)p.BH * p.nsplit + 7) / 8, wgs = groups * 8 * (uint64_t)p.row_tiles;
     PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x queries too large");
-    const void *kernels[2][3] = {
-        {(const void *)attn_chunk_kernel<false, 1, false>, (const void *)attn_chunk_kernel<false, 2, false>, (const void *)attn_chunk_kernel<false, 1, true>},
-        {(const void *)attn_chunk_kernel<true, 1, false>, (const void *)attn_chunk_kernel<true, 2, false>, (const void *)attn_chunk_kernel<true, 1, true>}};
-    const void *kernel = kernels[bf][wide ? 2 : nb - 1];
+    const void *kernels[2][4] = {
+        {(const void *)attn_chunk_kernel<false, 1, 1, false>, (const void *)attn_chunk_kernel<false, 1, 1, true>,
+         (const void *)attn_chunk_kernel<false, 1, 2, false>, (const void *)attn_chunk_kernel<false, 2, 2, false>},
+        {(const void *)attn_chunk_kernel<true, 1, 1, false>, (const void *)attn_chunk_kernel<true, 1, 1, true>,
+         (const void *)attn_chunk_kernel<true, 1, 2, false>, (const void *)attn_chunk_kernel<true, 2, 2, false>}};
+    const void *kernel = kernels[bf][cut.rg == 2 ? 1 + cut.nb : wide];
     PKV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *params[] = {&p};
-    PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256), params, lds, s));
+    PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256u * rg), params, lds, s));
     if (need) {
         const int64_t rows = (int64_t)a->B * a->Hq * a->n;
         const dim3 grid((unsigned)((rows + 7) / 8));
