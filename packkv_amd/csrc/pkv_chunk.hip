@@ -398,11 +398,11 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         }
         if (tok0 + 31 > pos_first || tok0 < start) {       // (uniform: some row does not see every token)
 #pragma unroll
-            for (int r = 0; r < 16; r++) {
-                const int tok = tok0 + 16 * h + r;
+            for (int nb = 0; nb < NB; nb++) {
+                int up_to = pos[nb] - (tok0 + 16 * h), from = start - (tok0 + 16 * h);
+                asm volatile("" : "+v"(up_to), "+v"(from));                    // (a branch, not a hundred selects that every tile pays for)
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++)
-                    if (tok > pos[nb] || tok < start) y[nb][r] = -INFINITY;
+                for (int r = 0; r < 16; r++) y[nb][r] = r > up_to || r < from ? -INFINITY : y[nb][r];
             }
         }
 #pragma unroll
@@ -509,6 +509,11 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         }
     }
 
+    // What the rest needs of the arguments is read again here: held in scalar registers across the loop above it made that loop spill.
+    typedef const __attribute__((address_space(4))) ChunkParams *late_ptr;
+    late_ptr late = reinterpret_cast<late_ptr>(reinterpret_cast<uintptr_t>(__builtin_amdgcn_kernarg_segment_ptr()));
+    asm volatile("" : "+s"(late));
+
     // ---- window tiles: the same products on the 16-bit rows ----
     if (w0 < w1) {
         __syncthreads();                                   // the staged blocks are dead
@@ -526,16 +531,16 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         unit = 1.f / kUp;
         uint8_t *vt = ring + wave * 32 * kVRow;            // (into the K codes' place, where two groups of rows need it)
         for (int wt = w0; wt < w1; wt++) {
-            const int r0 = wt * kChunkTile + 32 * quarter, tok0 = p.T_c + r0;     // window row and position of the wavefront's first token
-            if (r0 >= p.T_w || tok0 > pos_last || tok0 + 31 < start) continue; // (uniform, and no barrier in here)
-            const uint16_t *kr = p.k_win + ((size_t)bh * p.win_stride + min(r0 + tau, p.T_w - 1)) * kHeadDim + 8 * h;
-            const uint16_t *vr = p.v_win + ((size_t)bh * p.win_stride) * kHeadDim;
+            const int r0 = wt * kChunkTile + 32 * quarter, tok0 = late->T_c + r0;     // window row and position of the wavefront's first token
+            if (r0 >= late->T_w || tok0 > pos_last || tok0 + 31 < start) continue; // (uniform, and no barrier in here)
+            const uint16_t *kr = late->k_win + ((size_t)bh * late->win_stride + min(r0 + tau, late->T_w - 1)) * kHeadDim + 8 * h;
+            const uint16_t *vr = late->v_win + ((size_t)bh * late->win_stride) * kHeadDim;
             wave_lds_order();
 #pragma unroll
             for (int i = 0; i < 8; i++) {                  // four rows of V a step, 16 lanes each; rows that nobody sees as zeroes
                 const int k = 4 * i + (lane >> 4), c = lane & 15;
-                const bool real = r0 + k < p.T_w && tok0 + k >= start && tok0 + k <= pos_last;
-                const uint2 *src = reinterpret_cast<const uint2 *>(vr + (size_t)min(r0 + k, p.T_w - 1) * kHeadDim + 8 * c);
+                const bool real = r0 + k < late->T_w && tok0 + k >= start && tok0 + k <= pos_last;
+                const uint2 *src = reinterpret_cast<const uint2 *>(vr + (size_t)min(r0 + k, late->T_w - 1) * kHeadDim + 8 * c);
                 const uint2 a = src[0], d = src[1];
                 uint2 *dst = reinterpret_cast<uint2 *>(vt + k * kVRow + 16 * c);
                 dst[0] = real ? a : make_uint2(0u, 0u);
@@ -551,14 +556,14 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
                 const u4 a = *reinterpret_cast<const u4 *>(kr + 16 * s);
 #pragma unroll
                 for (int nb = 0; nb < NB; nb++)
-                    y[nb] = product<BF>(a, BF ? *reinterpret_cast<const u4 *>(q_row(row[nb]) + 16 * s + 8 * h)
+                    y[nb] = product<BF>(a, BF ? *reinterpret_cast<const u4 *>((late->q + (int64_t)b * late->q_b + (int64_t)(hkv * late->G + row[nb] % late->G) * late->q_h + (int64_t)(row[nb] / late->G) * late->q_t) + 16 * s + 8 * h)
                                               : *reinterpret_cast<const u4 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
             }
 #pragma unroll
             for (int r = 0; r < 16; r++) {
                 const int tok = tok0 + 16 * h + r;
 #pragma unroll
-                for (int nb = 0; nb < NB; nb++) y[nb][r] = tok > pos[nb] || tok < start ? -INFINITY : y[nb][r] * p.sm_log2;
+                for (int nb = 0; nb < NB; nb++) y[nb][r] = tok > pos[nb] || tok < start ? -INFINITY : y[nb][r] * late->sm_log2;
             }
             wave_lds_order();
             u4 w[NB][2], wl[NB][2];                        // bf16: what the rounding leaves goes through the matrix cores as well
@@ -642,12 +647,12 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
             __syncthreads();
         }
         const int i = (tid & 255) >> 3, ch = 16 * (tid & 7), at = mine0 + 32 * nb + i, r = row0 + at;      // a row's 16 channels each
-        if (r < p.rows) {
+        if (r < late->rows) {
             const float *s0 = buf0 + i * kSumRow + ch, *s1 = s0 + 32 * kSumRow;
             const float total = (sums[at] + sums[M + at]) + (sums[2 * M + at] + sums[3 * M + at]);
-            const int64_t head = hkv * p.G + r % p.G, token = r / p.G;
-            if (p.part) {
-                float *dst = p.part + ((((int64_t)b * p.Hq + head) * p.n + token) * p.nsplit + split) * kPart;
+            const int64_t head = hkv * late->G + r % late->G, token = r / late->G;
+            if (late->part) {
+                float *dst = late->part + ((((int64_t)b * late->Hq + head) * late->n + token) * late->nsplit + split) * kPart;
                 if (ch == 0) {
                     dst[0] = fmaxf(fmaxf(st[at], st[M + at]), fmaxf(st[2 * M + at], st[3 * M + at]));
                     dst[1] = total;
@@ -662,7 +667,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
                     const float x = (s0[2 * k] + s1[2 * k]) * inv, y = (s0[2 * k + 1] + s1[2 * k + 1]) * inv;
                     o[k] = BF ? pack_bf16(x, y) : pack_f16(x, y);
                 }
-                u4 *dst = reinterpret_cast<u4 *>(p.out + (int64_t)b * p.o_b + head * p.o_h + token * p.o_t + ch);
+                u4 *dst = reinterpret_cast<u4 *>(late->out + (int64_t)b * late->o_b + head * late->o_h + token * late->o_t + ch);
                 dst[0] = (u4){o[0], o[1], o[2], o[3]};
                 dst[1] = (u4){o[4], o[5], o[6], o[7]};
             }
