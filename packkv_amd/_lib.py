@@ -12,7 +12,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # PACKKV_HIP_LIB names another build of the same library (kernel development: A/B runs of two builds)
 LIB_PATH = os.environ.get("PACKKV_HIP_LIB") or os.path.join(_HERE, "libpackkv_hip.so")
 HOST_SYMBOLS = ("pkv_attn_decode", "pkv_window_append", "pkv_dense_view", "pkv_kq_mat_vec_mul", "pkv_wv_mat_vec_mul", "pkv_fused_kq",
-                "pkv_fused_wv")
+                "pkv_fused_wv", "pkv_norm_rotary", "pkv_attn_chunk_workspace", "pkv_attn_chunk", "pkv_sample_workspace", "pkv_sample")
 
 F16, BF16, F32 = 0, 1, 2
 OK, ERR_UNSUPPORTED, ERR_INVALID, ERR_HIP, ERR_CAPACITY, ERR_INTERNAL = range(6)

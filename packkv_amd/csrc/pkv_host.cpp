@@ -1,5 +1,6 @@
 // The host side of the calls that a decode loop repeats, in native code: the checks, the argument block and the result
-// tensors of ops.attn_decode, AttnPlan's step, ops.window_append, ops.dense_view and the four matrix-vector ops.
+// tensors of ops.attn_decode, AttnPlan's step, ops.window_append, ops.dense_view, the four matrix-vector ops, and ops.norm_rotary,
+// window_append_rotary, attn_chunk and sample.
 //
 // A decode step is two such calls around 12 us of GPU time, and in Python their checks and ctypes' conversions take 6 to
 // 12 us each besides the launch.  Every function here serves the usual call and gives up on any other before it has done
@@ -29,6 +30,11 @@ struct Library {                   // libpackkv_hip.so, as _lib.py has loaded it
     decltype(&pkv_wv_mat_vec_mul) wv = nullptr;
     decltype(&pkv_fused_kq) fused_kq = nullptr;
     decltype(&pkv_fused_wv) fused_wv = nullptr;
+    decltype(&pkv_norm_rotary) norm_rotary = nullptr;
+    decltype(&pkv_attn_chunk_workspace) chunk_workspace = nullptr;
+    decltype(&pkv_attn_chunk) attn_chunk = nullptr;
+    decltype(&pkv_sample_workspace) sample_workspace = nullptr;
+    decltype(&pkv_sample) sample = nullptr;
 } lib;
 
 // A plain torch.Tensor (a subclass, or a mode that wants to see the calls, gets the general code).
@@ -309,14 +315,253 @@ PyObject *fused(PyObject *, PyObject *const *o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of attn_decode, window_append, dense_view, kq, wv, fused_kq, fused_wv)
+// Element strides of batch, head and token of x [B, H, n, 128]; dimensions of one element have none.
+void row_strides(const at::Tensor &x, int64_t out[3]) {
+    for (int i = 0; i < 3; i++) out[i] = x.size(i) > 1 ? x.stride(i) : 0;
+}
+bool whole_rows(const at::Tensor &x, int dev) { return there(x, dev) && x.dim() == 4 && x.size(3) == 128 && x.stride(3) == 1; }
+bool real(PyObject *o, float *out) {
+    if (!o || !PyFloat_CheckExact(o)) return false;
+    *out = (float)PyFloat_AS_DOUBLE(o);
+    return true;
+}
+// The position axis of each frequency (ops._frequency_axes) from sections, a tuple or None.
+bool frequency_axes(PyObject *sections, PyObject *interleaved, pkv_rotary_args &a) {
+    a.n_axes = 1;
+    if (sections == Py_None) return true;                  // (all zeroes)
+    if (!PyTuple_CheckExact(sections) || (interleaved != Py_True && interleaved != Py_False)) return false;
+    const int A = (int)PyTuple_GET_SIZE(sections);
+    int width[4], sum = 0;
+    if (A < 1 || A > 4) return false;
+    for (int i = 0; i < A; i++) {
+        if (!integer(PyTuple_GET_ITEM(sections, i), &width[i]) || width[i] < 0 || width[i] > 64) return false;
+        sum += width[i];
+    }
+    if (sum != 64) return false;
+    a.n_axes = A;
+    if (interleaved == Py_True) {
+        for (int i = 1; i < A; i++)
+            for (int j = 0; j < width[i]; j++) {
+                if (i + A * j >= 64) return false;
+                a.axis[i + A * j] = (uint8_t)i;
+            }
+        return true;
+    }
+    for (int i = 0, at = 0; i < A; i++)
+        for (int j = 0; j < width[i]; j++) a.axis[at++] = (uint8_t)i;
+    return true;
+}
+// What ops.norm_rotary and ops.window_append_rotary share: o = q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved.
+bool rotary_args(PyObject *const *o, const at::Tensor *&q, const at::Tensor *&k, int &dev, pkv_rotary_args &a) {
+    q = tensor(o[0]);
+    k = tensor(o[1]);
+    const at::Tensor *pos = tensor(o[2]), *freq = tensor(o[3]), *w[2] = {tensor(o[4]), tensor(o[5])};
+    dev = here(q);
+    if (dev < 0 || !k || !pos || !freq || !whole_rows(*q, dev) || !whole_rows(*k, dev) || !half(*q) || k->scalar_type() != q->scalar_type()) return false;
+    const int64_t B = q->size(0), n = q->size(2);
+    if (B < 1 || n < 1 || B > INT_MAX || n > INT_MAX || q->size(1) < 1 || k->size(1) < 1 || q->size(1) > INT_MAX || k->size(1) > INT_MAX ||
+        k->size(0) != B || k->size(2) != n) return false;
+    if (!dense(*freq, dev) || freq->scalar_type() != at::kFloat || freq->dim() != 1 || freq->size(0) != 64) return false;
+    for (int i = 0; i < 2; i++)
+        if (o[4 + i] != Py_None && (!w[i] || !dense(*w[i], dev) || w[i]->dim() != 1 || w[i]->size(0) != 128 || w[i]->scalar_type() != q->scalar_type())) return false;
+    if (!real(o[6], &a.eps) || !frequency_axes(o[7], o[8], a)) return false;
+    if (!there(*pos, dev) || (pos->scalar_type() != at::kLong && pos->scalar_type() != at::kInt)) return false;
+    const int64_t shape[3] = {o[7] == Py_None ? 1 : a.n_axes, B, n}, d = pos->dim();
+    if (d > (o[7] == Py_None ? 2 : 3)) return false;
+    for (int64_t i = 0; i < d; i++) {                      // broadcast from the right
+        const int64_t size = pos->size(d - 1 - i);
+        if (size != shape[2 - i] && size != 1) return false;
+        a.pos_stride[2 - i] = size > 1 ? pos->stride(d - 1 - i) : 0;
+    }
+    a.pos_bytes = pos->scalar_type() == at::kLong ? 8 : 4;
+    a.q = at_ptr<void>(*q);
+    a.k = at_ptr<void>(*k);
+    a.positions = at_ptr<void>(*pos);
+    a.inv_freq = at_ptr<float>(*freq);
+    a.q_norm = w[0] ? at_ptr<void>(*w[0]) : nullptr;
+    a.k_norm = w[1] ? at_ptr<void>(*w[1]) : nullptr;
+    row_strides(*q, a.q_stride);
+    row_strides(*k, a.k_stride);
+    a.dtype = code(*q);
+    a.B = (int)B; a.Hq = (int)q->size(1); a.Hkv = (int)k->size(1); a.n = (int)n;
+    return true;
+}
+
+// norm_rotary(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved) -> (q, k), a status that is not zero, or None
+PyObject *norm_rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *q, *k;
+    int dev;
+    pkv_rotary_args a{};
+    if (n != 9 || modes() || !rotary_args(o, q, k, dev, a)) Py_RETURN_NONE;
+    at::Tensor q_out = at::empty(q->sizes(), q->options()), k_out = at::empty(k->sizes(), k->options());
+    a.q_out = at_ptr<void>(q_out);
+    a.k_out = at_ptr<void>(k_out);
+    row_strides(q_out, a.q_out_stride);
+    row_strides(k_out, a.k_out_stride);
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.norm_rotary(&a, s); });
+    if (rc) return status(rc);
+    PyObject *both = PyTuple_New(2);
+    if (!both) return nullptr;
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(q_out)));
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(k_out)));
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// window_append_rotary(... as norm_rotary, v, k_win, v_win, win_pos) -> q, a status that is not zero, or None
+PyObject *window_append_rotary(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *q, *k;
+    int dev, pos;
+    pkv_rotary_args a{};
+    if (n != 13 || modes() || !rotary_args(o, q, k, dev, a) || !integer(o[12], &pos)) Py_RETURN_NONE;
+    const at::Tensor *v = tensor(o[9]), *kw = tensor(o[10]), *vw = tensor(o[11]);
+    const auto type = q->scalar_type();
+    if (!v || !kw || !vw || !whole_rows(*v, dev) || v->sizes() != k->sizes() || v->scalar_type() != type || !dense(*kw, dev) || !dense(*vw, dev) || kw->dim() != 4 ||
+        vw->sizes() != kw->sizes() || kw->size(0) != a.B || kw->size(1) != a.Hkv || kw->size(3) != 128 || kw->scalar_type() != type || vw->scalar_type() != type ||
+        pos < 0 || (int64_t)pos + a.n > kw->size(2)) Py_RETURN_NONE;
+    at::Tensor q_out = at::empty(q->sizes(), q->options());
+    a.q_out = at_ptr<void>(q_out);
+    row_strides(q_out, a.q_out_stride);
+    a.v = at_ptr<void>(*v);
+    row_strides(*v, a.v_stride);
+    a.k_out = at_ptr<uint16_t>(*kw) + 128 * (int64_t)pos;
+    a.v_out = at_ptr<uint16_t>(*vw) + 128 * (int64_t)pos;
+    for (int i = 0; i < 3; i++) a.k_out_stride[i] = a.v_out_stride[i] = kw->stride(i);
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.norm_rotary(&a, s); });
+    return rc ? status(rc) : THPVariable_Wrap(std::move(q_out));
+    END_HANDLE_TH_ERRORS
+}
+
+// attn_chunk(q, k, v, k_win, v_win, sm_scale, win_len, starts, causal) -> the result, a status that is not zero, or None
+PyObject *attn_chunk(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *q = n == 9 && !modes() ? tensor(o[0]) : nullptr;
+    const int dev = here(q);
+    if (dev < 0 || !whole_rows(*q, dev) || !half(*q) || q->numel() == 0 || q->size(0) > INT_MAX || q->size(1) > INT_MAX || q->size(2) > INT_MAX ||
+        (o[8] != Py_True && o[8] != Py_False)) Py_RETURN_NONE;
+    pkv_attn_args in{};
+    Cache c;
+    c.batch = (int)q->size(0);
+    if (o[1] != Py_None) {
+        if (!cache_args(o[1], o[2], dev, c.batch, in, c) || c.like->scalar_type() != q->scalar_type() || c.tokens % 128 ||
+            (reinterpret_cast<uintptr_t>(in.k_stream) | reinterpret_cast<uintptr_t>(in.v_stream)) % 16) Py_RETURN_NONE;
+    } else if (o[2] != Py_None) {
+        Py_RETURN_NONE;
+    }
+    if (o[3] != Py_None) {
+        const at::Tensor *kw = tensor(o[3]);
+        if (o[1] == Py_None && kw && kw->dim() == 4) c.heads = (int)kw->size(1);
+        if (!window_args(kw, tensor(o[4]), o[6], dev, c, q->scalar_type(), in) ||
+            (reinterpret_cast<uintptr_t>(in.k_win) | reinterpret_cast<uintptr_t>(in.v_win)) % 16) Py_RETURN_NONE;
+    } else if (o[1] == Py_None || o[4] != Py_None) {
+        Py_RETURN_NONE;
+    }
+    pkv_chunk_args a{};
+    a.sm_scale = 0.08838834764831845f;                     // 128 ** -0.5
+    if (o[5] != Py_None && !real(o[5], &a.sm_scale)) Py_RETURN_NONE;
+    if (o[7] != Py_None) {
+        const at::Tensor *starts = tensor(o[7]);
+        if (!starts || !dense(*starts, dev) || starts->scalar_type() != at::kInt || starts->dim() != 1 || starts->size(0) != c.batch) Py_RETURN_NONE;
+        a.starts = at_ptr<int32_t>(*starts);
+    }
+    a.causal = o[8] == Py_True;
+    if (c.heads < 1 || q->size(1) % c.heads || (a.causal && q->size(2) > (int64_t)c.tokens + in.T_w)) Py_RETURN_NONE;
+    at::Tensor out = at::empty_like(*q);
+    row_strides(*q, a.q_stride);
+    row_strides(out, a.out_stride);
+    a.q = at_ptr<void>(*q);
+    a.out = at_ptr<void>(out);
+    uint64_t off = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.out);
+    for (int i = 0; i < 3; i++) off |= 2u * (uint64_t)(a.q_stride[i] | a.out_stride[i]);
+    if (off % 16 || out.stride(3) != 1) Py_RETURN_NONE;
+    a.k_stream = in.k_stream; a.k_info = in.k_info; a.v_stream = in.v_stream; a.v_info = in.v_info;
+    a.k_bytes = in.k_bytes; a.v_bytes = in.v_bytes;
+    a.k_scale = in.k_scale; a.k_zero = in.k_zero; a.v_scale = in.v_scale; a.v_zero = in.v_zero;
+    a.k_win = in.k_win; a.v_win = in.v_win;
+    a.B = c.batch; a.Hq = (int)q->size(1); a.Hkv = c.heads; a.n = (int)q->size(2);
+    a.T_c = c.tokens; a.T_w = in.T_w;
+    a.k_bits = in.k_bits; a.v_bits = in.v_bits; a.dtype = code(*q); a.par_stride = in.par_stride; a.win_stride = in.win_stride;
+    const uint64_t need = lib.chunk_workspace(&a);
+    at::Tensor space;
+    if (need) space = at::empty({(int64_t)need}, q->options().dtype(at::kByte));
+    void *const space_p = need ? at_ptr<void>(space) : nullptr;
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.attn_chunk(&a, space_p, need, s); });
+    return rc ? status(rc) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// sample(logits, u, temperature, top_k, top_p, min_p, want_logprob) -> tokens, or (tokens, log-probabilities); a status that is not
+// zero; or None
+PyObject *sample(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 7 && !modes() ? tensor(o[0]) : nullptr, *u = x ? tensor(o[1]) : nullptr;
+    const int dev = here(x);
+    if (dev < 0 || !u || !there(*x, dev) || x->dim() != 2 || x->size(0) < 1 || x->size(0) > INT_MAX || x->size(1) < 1 || x->size(1) > 1 << 20 || x->stride(1) != 1 ||
+        (!half(*x) && x->scalar_type() != at::kFloat) || (o[6] != Py_True && o[6] != Py_False)) Py_RETURN_NONE;
+    const int64_t rows = x->size(0);
+    const auto row_tensor = [&](const at::Tensor *t, at::ScalarType type) {
+        return t && dense(*t, dev) && t->scalar_type() == type && t->dim() == 1 && t->size(0) == rows;
+    };
+    if (!row_tensor(u, at::kFloat)) Py_RETURN_NONE;
+    pkv_sample_args a{};
+    const float **const at_[3] = {&a.temperature, &a.top_p, &a.min_p};
+    float *const all[3] = {&a.temperature_all, &a.top_p_all, &a.min_p_all};
+    PyObject *const given[3] = {o[2], o[4], o[5]};
+    for (int i = 0; i < 3; i++) {
+        const at::Tensor *t = tensor(given[i]);
+        if (t) {
+            if (!row_tensor(t, at::kFloat)) Py_RETURN_NONE;
+            *at_[i] = at_ptr<float>(*t);
+        } else if (!real(given[i], all[i]) || !(*all[i] >= 0.f) || (i && *all[i] > 1.f)) {
+            Py_RETURN_NONE;
+        }
+    }
+    const at::Tensor *k = tensor(o[3]);
+    if (k) {
+        if (!row_tensor(k, at::kInt)) Py_RETURN_NONE;
+        a.top_k = at_ptr<int32_t>(*k);
+    } else if (!integer(o[3], &a.top_k_all) || a.top_k_all < 0) {
+        Py_RETURN_NONE;
+    }
+    at::Tensor token = at::empty({rows}, x->options().dtype(at::kLong)), logprob;
+    if (o[6] == Py_True) logprob = at::empty({rows}, x->options().dtype(at::kFloat));
+    a.logits = at_ptr<void>(*x);
+    a.u = at_ptr<float>(*u);
+    a.token = at_ptr<int64_t>(token);
+    a.logprob = o[6] == Py_True ? at_ptr<float>(logprob) : nullptr;
+    a.row_stride = rows > 1 ? x->stride(0) : 0;
+    a.dtype = half(*x) ? code(*x) : PKV_F32;
+    a.rows = (int)rows; a.vocab = (int)x->size(1);
+    const uint64_t need = lib.sample_workspace(&a);
+    at::Tensor space;
+    if (need) space = at::empty({(int64_t)need}, x->options().dtype(at::kByte));
+    void *const space_p = need ? at_ptr<void>(space) : nullptr;
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.sample(&a, space_p, need, s); });
+    if (rc) return status(rc);
+    if (o[6] != Py_True) return THPVariable_Wrap(std::move(token));
+    PyObject *both = PyTuple_New(2);
+    if (!both) return nullptr;
+    PyTuple_SET_ITEM(both, 0, THPVariable_Wrap(std::move(token)));
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(logprob)));
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of attn_decode, window_append, dense_view, kq, wv, fused_kq, fused_wv, norm_rotary, attn_chunk_workspace, attn_chunk,
+// sample_workspace, sample)
 PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
-    void *p[7];
-    if (n != 7) {
-        PyErr_SetString(PyExc_TypeError, "seven addresses");
+    void *p[12];
+    if (n != 12) {
+        PyErr_SetString(PyExc_TypeError, "twelve addresses");
         return nullptr;
     }
-    for (int i = 0; i < 7; i++) {
+    for (int i = 0; i < 12; i++) {
         p[i] = PyLong_AsVoidPtr(o[i]);
         if (PyErr_Occurred()) return nullptr;
     }
@@ -327,6 +572,11 @@ PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
     lib.wv = (decltype(lib.wv))p[4];
     lib.fused_kq = (decltype(lib.fused_kq))p[5];
     lib.fused_wv = (decltype(lib.fused_wv))p[6];
+    lib.norm_rotary = (decltype(lib.norm_rotary))p[7];
+    lib.chunk_workspace = (decltype(lib.chunk_workspace))p[8];
+    lib.attn_chunk = (decltype(lib.attn_chunk))p[9];
+    lib.sample_workspace = (decltype(lib.sample_workspace))p[10];
+    lib.sample = (decltype(lib.sample))p[11];
     Py_RETURN_NONE;
 }
 
@@ -338,6 +588,10 @@ PyMethodDef methods[] = {
     {"dense_view", (PyCFunction)(void (*)(void))dense_view, METH_FASTCALL, nullptr},
     {"mat_vec", (PyCFunction)(void (*)(void))mat_vec, METH_FASTCALL, nullptr},
     {"fused", (PyCFunction)(void (*)(void))fused, METH_FASTCALL, nullptr},
+    {"norm_rotary", (PyCFunction)(void (*)(void))norm_rotary, METH_FASTCALL, nullptr},
+    {"window_append_rotary", (PyCFunction)(void (*)(void))window_append_rotary, METH_FASTCALL, nullptr},
+    {"attn_chunk", (PyCFunction)(void (*)(void))attn_chunk, METH_FASTCALL, nullptr},
+    {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -693,6 +693,9 @@ def norm_rotary(q, k, positions, inv_freq, q_norm=None, k_norm=None, eps=1e-6, s
     width) [axes, B, n], frequencies assigned in order or, with interleaved=True, in turn.  inv_freq [64] float32; angles are formed
     in 64 bits, so positions may be far.  Strided views (slices of a projection's output) are read in place; the results are
     contiguous."""
+    served = _host().norm_rotary(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
+    if served is not None:
+        return served if type(served) is tuple else _lib.check(served)
     a, keep = _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -707,6 +710,9 @@ def window_append_rotary(q, k, v, positions, inv_freq, k_win, v_win, win_pos, q_
     """norm_rotary for a step's new tokens with the keys written into rows win_pos.. of the 16-bit window k_win [B, Hkv, cap, 128]
     and the values v [B, Hkv, n, 128] into those of v_win, in one launch; returns the queries.  window_append for a model whose
     projections come raw."""
+    served = _host().window_append_rotary(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved, v, k_win, v_win, win_pos)
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
     a, keep = _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, interleaved)
     B, H, n, _ = k.shape
     at, win_pos = q.get_device(), int(win_pos)
@@ -1258,6 +1264,9 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     (float32; top_k int32; numbers are rounded to float32).  -inf and NaN are never chosen; a row with nothing else gives -1.  With
     want_logprob returns (tokens, log-probabilities float32 [rows]) under the filtered distribution.  The same numbers give the same
     token on every call and for every batch size."""
+    served = _host().sample(logits, u, temperature, top_k, top_p, min_p, want_logprob) if out is None else None
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
     _require(logits.is_cuda and logits.dim() == 2 and logits.size(1) > 0, "logits must be a device tensor [rows, vocab]")
     R, V = logits.shape
     at, dev, keep = logits.get_device(), logits.device, []
@@ -1347,6 +1356,9 @@ def attn_chunk(q, k, v, k_win=None, v_win=None, sm_scale=None, out=None, win_len
     tokens, with causal=False to all of them from starts[b] on; starts, an int32 tensor [B], is for batches padded on the left (what
     lies in the padding may be anything).  A query that sees no token gets zeroes.  Strided queries (a transposed projection output)
     are read in place; the result has their layout unless `out` is given.  Widths 2..8, any number of query heads to a KV head."""
+    served = _host().attn_chunk(q, k, v, k_win, v_win, sm_scale, win_len, starts, causal) if out is None else None
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
     _require(q.is_cuda and q.dim() == 4 and q.size(3) == 128, "q must be a device tensor [B, Hq, n, 128]")
     B, Hq, n, _ = q.shape
     at, dtype = q.get_device(), q.dtype
