@@ -53,7 +53,7 @@ struct ChunkParams {
     uint64_t k_bytes, v_bytes;
     int Hq, Hkv, BH, G, n, rows, T_c, T_w, par_stride, win_stride, k_bits, v_bits, causal;
     int tiles_c, tiles, run, nsplit, row_tiles;
-    uint32_t slot, ring;                       // LDS bytes of a staged block and of everything staged
+    uint32_t slot_k, slot_v, ring;             // LDS bytes of a staged block of either side and of everything staged
     float sm_log2;
 };
 
@@ -78,16 +78,16 @@ __device__ __forceinline__ uint32_t codes_f16(uint32_t c4, uint32_t which) {
     return __builtin_bit_cast(uint32_t, (h2v)(__builtin_bit_cast(h2v, __builtin_amdgcn_perm(0x64646464u, c4, which)) - (h2v){(_Float16)1024.f, (_Float16)1024.f}));
 }
 
-// The eight operand registers of one V pack (table entry e: LDS address | width << 16 | minimum << 20): tokens (j, j + 8) side by
+// The eight operand registers of one V pack (table entry e: LDS address | width << 17 | minimum << 21): tokens (j, j + 8) side by
 // side, j = 0..7.  The field, 1024 + (code - minimum), and minimum - 1024 add up exactly.
 __device__ __forceinline__ uint32_t field_code(uint32_t shifted, uint32_t mask, h2v low) {
     return __builtin_bit_cast(uint32_t, (h2v)(__builtin_bit_cast(h2v, (shifted & mask) | 0x64006400u) + low));
 }
 template <bool WIDE> __device__ __forceinline__ void pack_operand(const uint8_t *ring, uint32_t e, uint32_t out[8]) {
     typedef unsigned short u16pair __attribute__((ext_vector_type(2)));
-    const uint32_t at = e & 0xFFFFu, len = (e >> 16) & 15u;
+    const uint32_t at = e & 0x1FFFFu, len = (e >> 17) & 15u;
     const uint32_t mask = ((1u << len) - 1u) * 0x00010001u;
-    const h2v low = __builtin_bit_cast(h2v, 0x64006400u | ((e >> 20) * 0x00010001u)) - (h2v){(_Float16)2048.f, (_Float16)2048.f};
+    const h2v low = __builtin_bit_cast(h2v, 0x64006400u | ((e >> 21) * 0x00010001u)) - (h2v){(_Float16)2048.f, (_Float16)2048.f};
     if (WIDE) {                                // words of up to 128 bits: two tokens at a time, bits (14 - j) * len of the word on
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -151,11 +151,11 @@ __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
 
 template <bool BF, int NB, int RG, bool WIDE>
 __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(const ChunkParams p) {
-    static_assert(RG == 1 || !WIDE, "wide codes: one group of rows");
     constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
     constexpr int M = 32 * NB * RG, kBufs = RG + 1, kSets = RG;
+    constexpr bool COPY = !WIDE || RG == 2;                // blocks go to LDS without registers (what is staged lies below 64 KiB)
     extern __shared__ __align__(16) uint8_t lds[];
-    uint8_t *ring = lds;                                   // kBufs tiles of four staged blocks; window and end: V rows, sums (kt as well)
+    uint8_t *ring = lds;                                   // staged: two tiles' K blocks, kBufs tiles' V blocks; window and end: V rows, sums (kt as well)
     uint8_t *kt_all = lds + p.ring;                        // [kSets][4 quarters][32 tokens][kKRow]
     uint32_t *tab_all = reinterpret_cast<uint32_t *>(kt_all + kSets * 4 * 32 * kKRow);        // [kSets][8 units][4 slots][32 lanes]
     float2 *par_all = reinterpret_cast<float2 *>(tab_all + kSets * 1024);          // [kSets][2][4][32]: (scale, zero * scale), (V scale, V zero)
@@ -209,29 +209,33 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     const uintptr_t stream = reinterpret_cast<uintptr_t>(quarter < 2 ? p.k_stream : p.v_stream);
     const u4 copy_rsrc = {(uint32_t)stream, (uint32_t)(stream >> 32) & 0xFFFFu, bytes4, 0x00020000u};
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(stream), 0, (int)bytes4, 0x00020000);
-    u4 raw[WIDE ? NQ : 1];
+    const uint32_t slot = quarter < 2 ? p.slot_k : p.slot_v;
+    auto block_at = [&](int side, int j, int tile_nr) -> uint32_t {            // tile_nr: counted from the run's first
+        return side ? 4u * p.slot_k + (uint32_t)(2 * (tile_nr % kBufs) + j) * p.slot_v : (uint32_t)(2 * (tile_nr & 1) + j) * p.slot_k;
+    };
+    u4 raw[COPY ? 1 : NQ];
     uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
     // starts the copies of `tile`, whose entry look_up has fetched (widths above 4: into registers, for put)
-    auto fetch = [&](int tile, int buf) {
+    auto fetch = [&](int tile) {
         uint32_t off = next_off, size = min(next_size, cap);               // (never outside the stream, whatever block_info says)
         if ((uint64_t)off > bytes) off = (uint32_t)bytes;
         size = (uint32_t)min((uint64_t)size, bytes - (uint64_t)off);
         raw_phase = off & 15u;
         const uint32_t n16 = (raw_phase + size + 15u) >> 4, src = off - raw_phase;
-        if (WIDE) {
+        if (!COPY) {
 #pragma unroll
-            for (int i = 0; i < (WIDE ? NQ : 1); i++) {
+            for (int i = 0; i < (COPY ? 1 : NQ); i++) {
                 const uint32_t c = (uint32_t)(lane + 64 * i);
                 raw[i] = c < n16 ? __builtin_bit_cast(u4, __builtin_amdgcn_raw_buffer_load_b128(rsrc, src + 16u * c, 0, 0)) : (u4){0, 0, 0, 0};
             }
         } else {
-            const uint32_t dst = (uint32_t)reinterpret_cast<uintptr_t>(ring) + (uint32_t)(4 * buf + quarter) * p.slot;
+            const uint32_t dst = (uint32_t)reinterpret_cast<uintptr_t>(ring) + block_at(quarter >> 1, quarter & 1, tile - c0);
 #pragma unroll
             for (int i = 0; i < (NQ + RG - 1) / RG; i++) {                 // (two groups of rows: every other step each)
                 const uint32_t step = (uint32_t)(RG * i + rg);
                 if ((uint32_t)lane + 64u * step < n16) copy_to_lds(copy_rsrc, __builtin_amdgcn_readfirstlane(dst + 1024u * step), src + 16u * ((uint32_t)lane + 64u * step));
             }
-            if (lane == 0 && rg == 0) phase_s[buf][quarter] = raw_phase;
+            if (lane == 0 && rg == 0) phase_s[(tile - c0) % kBufs][quarter] = raw_phase;
         }
         look_up(tile + 1);
     };
@@ -239,21 +243,21 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         const size_t at = (size_t)b * p.par_stride + (size_t)tile * kChunkTile + 32 * quarter + t;
         par_k = p.k_scale[at]; par_kz = p.k_zero[at]; par_v = p.v_scale[at]; par_vz = p.v_zero[at];
     };
-    auto put = [&](int buf) {                              // what fetch has started is in LDS behind the next barrier
-        if (WIDE) {
-            uint8_t *dst = ring + (uint32_t)(4 * buf + quarter) * p.slot;
+    auto put = [&](int tile) {                             // what fetch has started is in LDS behind the next barrier
+        if (!COPY) {
+            uint8_t *dst = ring + block_at(quarter >> 1, quarter & 1, tile - c0);
 #pragma unroll
-            for (int i = 0; i < (WIDE ? NQ : 1); i++)
-                if ((uint32_t)(lane + 64 * i) * 16u < p.slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
-            if (lane == 0) phase_s[buf][quarter] = raw_phase;
+            for (int i = 0; i < (COPY ? 1 : NQ); i++)
+                if ((uint32_t)(lane + 64 * i) * 16u < slot) *reinterpret_cast<u4 *>(dst + 16 * (lane + 64 * i)) = raw[i];
+            if (lane == 0) phase_s[(tile - c0) % kBufs][quarter] = raw_phase;
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
     };
     if (c0 < c1) {
         look_up(c0);
-        fetch(c0, 0);
-        if (RG == 2 && c0 + 1 < c1) fetch(c0 + 1, 1);
+        fetch(c0);
+        if (RG == 2 && c0 + 1 < c1) fetch(c0 + 1);
         fetch_par(c0);
     }
 
@@ -284,7 +288,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         }
         *reinterpret_cast<u4 *>(qt + r * kQRow + 16 * c) = w;
     }
-    if (c0 < c1) put(0);
+    if (c0 < c1) put(c0);
     __syncthreads();
     float qsum[NB];
 #pragma unroll
@@ -318,28 +322,28 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
 
     // A half-wavefront's unit of a staged tile: where it starts in its block.
     const int hw = 2 * quarter + h, u = hw & 3;
-    auto unit_start = [&](int buf, int side) -> uint32_t {
-        const uint32_t phase = phase_s[buf][2 * side + (hw >> 2)];
-        const uint8_t *blk = ring + (uint32_t)(4 * buf + 2 * side + (hw >> 2)) * p.slot;
-        return min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk + phase)[u - 1] : 0u), p.slot - 16u);
+    auto unit_start = [&](int tile, int side, uint32_t blk_at) -> uint32_t {
+        const uint32_t phase = phase_s[(tile - c0) % kBufs][2 * side + (hw >> 2)];
+        const uint8_t *blk = ring + blk_at;
+        return min(phase + 8u + (u ? (uint32_t)reinterpret_cast<const uint16_t *>(blk + phase)[u - 1] : 0u), (side ? p.slot_v : p.slot_k) - 16u);
     };
-    auto unpack_k = [&](int buf, uint8_t *kt) {            // 16 tokens x 128 channels; the quarter's two units make its 32 tokens
+    auto unpack_k = [&](int tile, uint8_t *kt) {           // 16 tokens x 128 channels; the quarter's two units make its 32 tokens
         uint8_t *dst = kt + quarter * 32 * kKRow + 16 * h * kKRow + 4 * t;
-        unit_codes(ring + (uint32_t)(4 * buf + (hw >> 2)) * p.slot, unit_start(buf, 0), t, gk,
-                   [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
+        const uint32_t blk_at = block_at(0, hw >> 2, tile - c0);
+        unit_codes(ring + blk_at, unit_start(tile, 0, blk_at), t, gk, [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
     };
-    auto parse_v = [&](int buf, uint32_t *tab) {           // where the unit's packs are
-        const uint32_t slot_at = (uint32_t)(4 * buf + 2 + (hw >> 2)) * p.slot, at = unit_start(buf, 1);
-        const uint8_t *blk = ring + slot_at;
+    auto parse_v = [&](int tile, uint32_t *tab) {          // where the unit's packs are
+        const uint32_t blk_at = block_at(1, hw >> 2, tile - c0), at = unit_start(tile, 1, blk_at);
+        const uint8_t *blk = ring + blk_at;
         const uint32_t minsw = lds_meta_word(blk + at, t, gv.W), lensw = lds_meta_word(blk + at + gv.mins_bytes, t, gv.LB);
         uint32_t len[4], off[4], payload;
 #pragma unroll
         for (int i = 0; i < 4; i++) len[i] = min((lensw >> (i * gv.LB)) & ((1u << gv.LB) - 1u), (uint32_t)gv.W);
         pack_offsets(len, off, payload);
-        const uint32_t base = slot_at + at + (uint32_t)(gv.mins_bytes + gv.lens_bytes);
+        const uint32_t base = blk_at + at + (uint32_t)(gv.mins_bytes + gv.lens_bytes);
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            tab[(hw * 4 + i) * 32 + t] = min(base + off[i], p.ring - 32u) | (len[i] << 16) | (((minsw >> (i * gv.W)) & ((1u << gv.W) - 1u)) << 20);
+            tab[(hw * 4 + i) * 32 + t] = min(base + off[i], p.ring - 32u) | (len[i] << 17) | (((minsw >> (i * gv.W)) & ((1u << gv.W) - 1u)) << 21);
     };
     // Parameters of the quarter's 32 tokens into LDS; those in front of the sequence count as nothing.  Returns what the accumulators
     // are to be multiplied with where a larger V scale than before came up.  (Two groups of rows: the group that writes and the one
@@ -459,53 +463,50 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     if (RG == 1) {
         // Few rows: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
         for (int tile = c0; tile < c1; tile++) {
-            const int buf = (tile - c0) & 1;
             if (tile != c0) __syncthreads();               // the tile is staged, and the table's readers are done
             const float grow = raise_scale(write_par(tile, 0));
             if (tile + 1 < c1) {
-                fetch(tile + 1, buf ^ 1);
+                fetch(tile + 1);
                 fetch_par(tile + 1);
             }
-            parse_v(buf, tab_all);
-            unpack_k(buf, kt_all);
+            parse_v(tile, tab_all);
+            unpack_k(tile, kt_all);
             wave_lds_order();
             u4 w[NB][2];
             weights_of(tile, kt_all, par_all, grow, w);
-            if (WIDE) __syncthreads();
+            if (!COPY) __syncthreads();
             else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the table is there; copies go on
             add_values(tab_all, w);
-            if (tile + 1 < c1) put(buf ^ 1);
+            if (tile + 1 < c1) put(tile + 1);
         }
     } else if (c0 < c1) {
         // Many rows: the two groups of rows share what is unpacked -- the first group's wavefronts unpack K, the second's find V's
         // packs and write the parameters, a tile ahead, while the others are at their products.  One barrier a tile.
-        auto prepare = [&](int tile, int set, int buf) {
+        auto prepare = [&](int tile, int set) {
             if (rg == 0) {
-                unpack_k(buf, kt_all + set * 4 * 32 * kKRow);
+                unpack_k(tile, kt_all + set * 4 * 32 * kKRow);
             } else {
-                parse_v(buf, tab_all + set * 1024);
+                parse_v(tile, tab_all + set * 1024);
                 const uint32_t e = write_par(tile, set);
                 if (lane == 0) top_s[set][quarter] = e;
             }
         };
-        prepare(c0, 0, 0);
+        prepare(c0, 0);
         if (rg == 1 && c0 + 1 < c1) fetch_par(c0 + 1);
         __syncthreads();
-        int buf = 0;
         for (int tile = c0; tile < c1; tile++) {
-            const int set = (tile - c0) & 1, buf1 = buf == 2 ? 0 : buf + 1, buf2 = buf1 == 2 ? 0 : buf1 + 1;
-            if (tile + 2 < c1) fetch(tile + 2, buf2);
+            const int set = (tile - c0) & 1;
+            if (tile + 2 < c1) fetch(tile + 2);
             if (tile + 1 < c1) {
-                prepare(tile + 1, set ^ 1, buf1);
+                prepare(tile + 1, set ^ 1);
                 if (rg == 1 && tile + 2 < c1) fetch_par(tile + 2);
             }
             const float grow = raise_scale(__builtin_amdgcn_readfirstlane(top_s[set][quarter]));
             u4 w[NB][2];
             weights_of(tile, kt_all + set * 4 * 32 * kKRow, par_all + set * 256, grow, w);
             add_values(tab_all + set * 1024, w);
-            put(buf2);
+            put(tile + 2);
             __syncthreads();
-            buf = buf1;
         }
     }
 
@@ -707,24 +708,36 @@ __global__ void __launch_bounds__(256) chunk_merge_kernel(const float *__restric
 
 static bool chunk_wide(const pkv_chunk_args *a) { return a->T_c && (a->k_bits > 4 || a->v_bits > 4); }
 
-// How a call is cut: rows a workgroup (32 NB RG), runs of tiles.  Two workgroups a CU are wanted of the small kind (512), one of the large
-// (256); a run of one tile is the least.
+// LDS bytes of what is staged, and of a block of either side: a block at any phase, and a last word's reach.
+static uint32_t chunk_ring(const pkv_chunk_args *a, int rg, uint32_t &slot_k, uint32_t &slot_v) {
+    slot_k = (((uint32_t)k_block_bound(64, a->T_c ? a->k_bits : 2) + 15u) & ~15u) + 32u;
+    slot_v = (((uint32_t)v_block_bound(64, a->T_c ? a->v_bits : 2) + 15u) & ~15u) + 32u;
+    return 4u * slot_k + 2u * (uint32_t)(rg + 1) * slot_v;
+}
+
+// How a call is cut: rows a workgroup (32 NB RG), and runs of tiles, so that the rounds of workgroups the device takes -- two a CU of the
+// small kind, one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
+// partials as one.
 struct ChunkCut {
     int nb, rg, row_tiles, tiles, run, nsplit;
 };
 static ChunkCut chunk_cut(const pkv_chunk_args *a) {
     ChunkCut c;
     const int64_t rows = (int64_t)a->n * (a->Hq / a->Hkv);
-    c.rg = rows <= 32 || chunk_wide(a) ? 1 : 2;
+    uint32_t slot_k, slot_v;
+    c.rg = rows <= 32 || chunk_ring(a, 2, slot_k, slot_v) > 63u * 1024u ? 1 : 2;     // (copies reach 64 KiB: not widths of 6 and more on both sides)
     c.nb = c.rg == 1 || rows <= 64 ? 1 : 2;
     const int64_t m = 32 * c.nb * c.rg;
     c.row_tiles = (int)((rows + m - 1) / m);
     c.tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
-    const int64_t groups = (int64_t)a->B * a->Hkv * c.row_tiles, aim = c.rg == 1 ? 512 : 256;
-    int64_t want = (aim + groups - 1) / groups;
-    if (want > c.tiles) want = c.tiles;
-    c.run = (int)((c.tiles + want - 1) / want);
-    c.nsplit = (c.tiles + c.run - 1) / c.run;
+    const int64_t groups = (int64_t)a->B * a->Hkv * c.row_tiles, slots = c.rg == 1 ? 512 : 256;
+    int64_t best = -1;
+    for (int want = 1; want <= c.tiles && want <= 512; want++) {
+        const int run = (c.tiles + want - 1) / want, nsplit = (c.tiles + run - 1) / run;
+        const int64_t cost = (groups * nsplit + slots - 1) / slots * (run + 2) + (nsplit > 1);
+        if (best < 0 || cost < best) { best = cost; c.run = run; c.nsplit = nsplit; }
+        if (groups * nsplit >= 4 * slots) break;           // (more rounds of shorter runs gain nothing)
+    }
     return c;
 }
 
@@ -797,21 +810,18 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     p.k_bits = a->T_c ? a->k_bits : 2; p.v_bits = a->T_c ? a->v_bits : 2;
     p.tiles_c = a->T_c / kChunkTile;
     p.sm_log2 = a->sm_scale * kLog2e;
-    const uint32_t k_cap = (uint32_t)k_block_bound(64, p.k_bits), v_cap = (uint32_t)v_block_bound(64, p.v_bits);
-    p.slot = (((k_cap > v_cap ? k_cap : v_cap) + 15u) & ~15u) + 32u;       // a block at any phase, and a last word's reach
     const uint32_t rg = (uint32_t)cut.rg, m = 32u * (uint32_t)cut.nb * rg, kt = rg * 4u * 32u * kKRow;
-    p.ring = (rg + 1u) * 4u * p.slot;
+    p.ring = chunk_ring(a, cut.rg, p.slot_k, p.slot_v);
     if (p.ring + kt < 4u * rg * 32u * kVRow) p.ring = 4u * rg * 32u * kVRow - kt;      // (the end's sums take less: rg * 2 x 32 x 129 floats)
     const bool wide = chunk_wide(a), bf = a->dtype == PKV_BF16;
     const uint32_t lds = p.ring + kt + rg * (4096u + 2048u) + 8u * m * 4u + m * kQRow;
     const uint64_t groups = ((uint64_t)p.BH * p.nsplit + 7) / 8, wgs = groups * 8 * (uint64_t)p.row_tiles;
     PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x queries too large");
-    const void *kernels[2][4] = {
-        {(const void *)attn_chunk_kernel<false, 1, 1, false>, (const void *)attn_chunk_kernel<false, 1, 1, true>,
-         (const void *)attn_chunk_kernel<false, 1, 2, false>, (const void *)attn_chunk_kernel<false, 2, 2, false>},
-        {(const void *)attn_chunk_kernel<true, 1, 1, false>, (const void *)attn_chunk_kernel<true, 1, 1, true>,
-         (const void *)attn_chunk_kernel<true, 1, 2, false>, (const void *)attn_chunk_kernel<true, 2, 2, false>}};
-    const void *kernel = kernels[bf][cut.rg == 2 ? 1 + cut.nb : wide];
+#define PKV_CHUNK(bf, nb, rg) {(const void *)attn_chunk_kernel<bf, nb, rg, false>, (const void *)attn_chunk_kernel<bf, nb, rg, true>}
+    const void *kernels[2][3][2] = {{PKV_CHUNK(false, 1, 1), PKV_CHUNK(false, 1, 2), PKV_CHUNK(false, 2, 2)},
+                                    {PKV_CHUNK(true, 1, 1), PKV_CHUNK(true, 1, 2), PKV_CHUNK(true, 2, 2)}};
+#undef PKV_CHUNK
+    const void *kernel = kernels[bf][cut.rg - 1 + cut.nb - 1][wide];
     PKV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *params[] = {&p};
     PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256u * rg), params, lds, s));

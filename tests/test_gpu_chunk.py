@@ -42,10 +42,12 @@ def test_chunk_follows_the_formula(cuda, dtype, B, Hq, Hkv, n, T, W):
     co.check(got, q, K, V, **size)
 
 
-@pytest.mark.parametrize("k_bits,v_bits", [(2, 2), (3, 4), (4, 3), (5, 4), (4, 6), (6, 5), (8, 7), (7, 8)])
-def test_every_width(cuda, k_bits, v_bits):
-    """Codes that use their whole width (drawn, not quantised), with packs of every length."""
-    B, Hq, Hkv, n, T, dtype = 2, 8, 2, 17, 384, torch.float16
+@pytest.mark.parametrize("k_bits,v_bits", [(2, 2), (3, 4), (4, 3), (5, 4), (4, 6), (6, 5), (8, 7), (7, 8), (5, 5), (6, 6), (8, 8), (8, 2), (2, 8)])
+@pytest.mark.parametrize("B,Hq,Hkv,n,T", [(2, 8, 2, 17, 384), (2, 32, 8, 40, 4096), (4, 8, 8, 3, 8192)])
+def test_every_width(cuda, k_bits, v_bits, B, Hq, Hkv, n, T):
+    """Codes that use their whole width (drawn, not quantised), with packs of every length; one tile a workgroup, and runs of several
+    with many rows and with few (the staged blocks of wide codes then lie beyond 64 KiB of LDS)."""
+    dtype = torch.float16
     g = torch.Generator(device=cuda).manual_seed(k_bits * 10 + v_bits)
     sides = []
     for is_k, bits in ((True, k_bits), (False, v_bits)):
