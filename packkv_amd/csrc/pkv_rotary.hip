@@ -7,7 +7,7 @@
 // an fp32 angle is off by up to 0.06.  (The chain of library kernels rounds after the norm, the cosines and each product.)
 //
 // Bound by memory: a row is read once and written once.  Eight lanes hold a row, each 8 channels of either half (two 16-byte
-// loads), so the sum of squares takes three DPP steps and both halves of a pair are in one lane; a wavefront holds eight heads
+// loads), so the sum of squares takes three exchanges and both halves of a pair are in one lane; a wavefront holds eight heads
 // of a token.  Lane i works out frequency i once for the wavefront, and the eight lanes of a row fetch theirs from LDS.
 #include "pkv_block.hpp"
 #include "pkv_runtime.hpp"
@@ -26,8 +26,9 @@ struct RotaryParams {
     const float *inv_freq;
     int64_t pos_a, pos_b, pos_t;
     uint64_t axis[2];                    // two bits a frequency
-    uint32_t n, groups;                  // groups of all sides together
-    uint64_t units;                      // tokens x groups
+    uint32_t n, groups, pieces;          // groups of all sides together, and of wavefronts' shares of them
+    uint64_t units;                      // tokens x pieces
+    int per;                             // groups a wavefront
     float eps;
     int pos64;
 };
@@ -75,71 +76,86 @@ __device__ __forceinline__ float turn_fraction(double pos, double freq) {
     return (float)(r - rint(r));
 }
 
-// One wavefront: eight heads of one token.
+// One wavefront: `per` groups of eight heads of one token, the next group's rows on their way while one is turned.
 template <int DT, bool WIDE>
 __global__ void __launch_bounds__(256) norm_rotary_kernel(const RotaryParams p) {
     __shared__ float2 turn_s[4][64];                         // (cos, sin) by frequency, one table a wavefront
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t unit = (uint64_t)blockIdx.x * 4u + (uint32_t)wave;
     if (unit >= p.units) return;                             // (no barrier below: each wavefront is on its own)
-    const uint64_t token = unit / p.groups;
-    int g = (int)(unit - token * p.groups), which = 0;
-    while (which < 2 && g >= p.side[which].groups) g -= p.side[which++].groups;
-    const RotarySide &s = p.side[which];
+    const uint64_t token = unit / p.pieces;
+    const int first = (int)(unit - token * p.pieces) * p.per, last = min(first + p.per, (int)p.groups);
     const int64_t b = (int64_t)(token / p.n), t = (int64_t)(token - (uint64_t)b * p.n);
-    const int h = min(8 * g + (lane >> 3), s.heads - 1), c = 8 * (lane & 7);      // (idle rows repeat the last head's)
-    const bool mine = 8 * g + (lane >> 3) < s.heads;
-    const uint16_t *in = s.in + b * s.in_b + (int64_t)h * s.in_h + t * s.in_t;
-    uint16_t *out = s.out + b * s.out_b + (int64_t)h * s.out_h + t * s.out_t;
-    uint32_t lo[4], hi[4];
-    load8<WIDE>(in + c, lo);
-    load8<WIDE>(in + 64 + c, hi);
-    if (which == 2) {
-        if (mine) { store8<WIDE>(out + c, lo); store8<WIDE>(out + 64 + c, hi); }
-        return;
-    }
+    const int c = 8 * (lane & 7);
+    struct Rows {
+        uint16_t *out;
+        const uint16_t *w;
+        bool mine, turned;
+        uint32_t lo[4], hi[4];
+    };
+    auto load = [&](int g) -> Rows {
+        int which = 0;
+        while (which < 2 && g >= p.side[which].groups) g -= p.side[which++].groups;
+        const RotarySide &s = p.side[which];
+        const int h = min(8 * g + (lane >> 3), s.heads - 1); // (idle rows repeat the last head's)
+        Rows r;
+        r.mine = 8 * g + (lane >> 3) < s.heads;
+        r.turned = which < 2;
+        r.w = s.w;
+        const uint16_t *in = s.in + b * s.in_b + (int64_t)h * s.in_h + t * s.in_t;
+        r.out = s.out + b * s.out_b + (int64_t)h * s.out_h + t * s.out_t;
+        load8<WIDE>(in + c, r.lo);
+        load8<WIDE>(in + 64 + c, r.hi);
+        return r;
+    };
+    Rows next = load(first);
     const int axis = (int)(p.axis[lane >> 5] >> (2 * (lane & 31))) & 3;
     const int64_t at = axis * p.pos_a + b * p.pos_b + t * p.pos_t;
     const double pos = p.pos64 ? (double)reinterpret_cast<const int64_t *>(p.pos)[at] : (double)reinterpret_cast<const int32_t *>(p.pos)[at];
     float sn, cs;
     sincospif(2.f * turn_fraction(pos, (double)p.inv_freq[lane]), &sn, &cs);
     turn_s[wave][lane] = make_float2(cs, sn);
-    float x[8], y[8];
+    wave_lds_order();
+    float2 turn[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        x[i] = half_at<DT>(lo[i >> 1], i & 1);
-        y[i] = half_at<DT>(hi[i >> 1], i & 1);
-    }
-    if (s.w) {
-        float sum = 0.f;
+    for (int i = 0; i < 8; i++) turn[i] = turn_s[wave][c + i];
+    for (int g = first; g < last; g++) {
+        Rows r = next;
+        if (g + 1 < last) next = load(g + 1);
+        if (r.turned) {
+            float x[8], y[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) sum += x[i] * x[i] + y[i] * y[i];
-        sum += __shfl_xor(sum, 1, 64);
-        sum += __shfl_xor(sum, 2, 64);
-        sum += __shfl_xor(sum, 4, 64);
-        const float r = 1.f / sqrtf(sum * (1.f / 128.f) + p.eps);
+            for (int i = 0; i < 8; i++) {
+                x[i] = half_at<DT>(r.lo[i >> 1], i & 1);
+                y[i] = half_at<DT>(r.hi[i >> 1], i & 1);
+            }
+            if (r.w) {
+                float sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            x[i] *= r * half_at<DT>(s.w[c + i], 0);
-            y[i] *= r * half_at<DT>(s.w[64 + c + i], 0);
+                for (int i = 0; i < 8; i++) sum += x[i] * x[i] + y[i] * y[i];
+                sum += __shfl_xor(sum, 1, 64);
+                sum += __shfl_xor(sum, 2, 64);
+                sum += __shfl_xor(sum, 4, 64);
+                const float scale = 1.f / sqrtf(sum * (1.f / 128.f) + p.eps);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    x[i] *= scale * half_at<DT>(r.w[c + i], 0);
+                    y[i] *= scale * half_at<DT>(r.w[64 + c + i], 0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 a = turn[2 * i], d = turn[2 * i + 1];
+                const float x0 = x[2 * i], x1 = x[2 * i + 1], y0 = y[2 * i], y1 = y[2 * i + 1];
+                r.lo[i] = half_pair<DT>(x0 * a.x - y0 * a.y, x1 * d.x - y1 * d.y);
+                r.hi[i] = half_pair<DT>(y0 * a.x + x0 * a.y, y1 * d.x + x1 * d.y);
+            }
+        }
+        if (r.mine) {
+            store8<WIDE>(r.out + c, r.lo);
+            store8<WIDE>(r.out + 64 + c, r.hi);
         }
     }
-    wave_lds_order();
-    float a[8], d[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float2 cs2 = turn_s[wave][c + i];
-        a[i] = x[i] * cs2.x - y[i] * cs2.y;
-        d[i] = y[i] * cs2.x + x[i] * cs2.y;
-    }
-    if (!mine) return;
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        lo[i] = half_pair<DT>(a[2 * i], a[2 * i + 1]);
-        hi[i] = half_pair<DT>(d[2 * i], d[2 * i + 1]);
-    }
-    store8<WIDE>(out + c, lo);
-    store8<WIDE>(out + 64 + c, hi);
 }
 
 }  // namespace pkv
@@ -178,7 +194,14 @@ extern "C" int pkv_norm_rotary(const pkv_rotary_args *a, pkv_stream_t s_) {
     p.eps = a->eps;
     p.n = (uint32_t)a->n;
     p.groups = (uint32_t)(p.side[0].groups + p.side[1].groups + p.side[2].groups);
-    p.units = (uint64_t)a->B * (uint64_t)a->n * p.groups;
+    const uint64_t tokens = (uint64_t)a->B * (uint64_t)a->n;
+    // As many groups a wavefront as leave one round of them (32 a CU): the angles are worked out once for all, and rows are on their
+    // way meanwhile.  4 x 2048 tokens of 32 + 8 heads, one group -> two, three, five: 39.2 us -> 34.1, 33.3, 31.4 (5.35 TB/s; a
+    // large copy 5.2); 2 x 1031 of 16 + 4, which are less than a round: 8.4 -> 8.7, 9.4, 9.4.
+    const uint64_t rounds = tokens * p.groups / 8192;
+    p.per = (int)(rounds < 1 ? 1 : rounds < p.groups ? rounds : p.groups);
+    p.pieces = (p.groups + (uint32_t)p.per - 1u) / (uint32_t)p.per;
+    p.units = tokens * p.pieces;
     const uint64_t wgs = (p.units + 3) / 4;
     PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x tokens x heads too large");
     const dim3 grid((unsigned)wgs);
