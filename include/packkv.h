@@ -414,9 +414,9 @@ int pkv_dense_view(const pkv_attn_args *args, void *k_out, void *v_out, pkv_stre
  * pkv_attn_chunk: pkv_attn_decode for n queries a sequence, which are the cache's last n tokens (their keys and values are in the
  * streams and the window already): query i attends to tokens starts[b] .. T_c + T_w - n + i; with causal = 0 to all from
  * starts[b] on.  `starts` [B] int32 (NULL: zeroes) is for batches padded on the left; a query that sees no token gets zeroes, and
- * what lies in front of starts[b] may be anything.  (A NaN or an infinity among the new tokens' window rows may reach queries
- * before it.)  q and out [B, Hq, n, 128] at element strides of batch, head and token, rows 16-byte aligned; Hq any multiple of Hkv;
- * widths 2..8; streams and windows 16-byte aligned; the rest as in pkv_attn_args.  fp32 accumulation, weights in fp16.  `workspace`:
+ * what lies in front of starts[b], queries too, may be anything.  (A NaN or an infinity in a new token's key, value or parameters may
+ * reach queries before it.)  q and out [B, Hq, n, 128] at element strides of batch, head and token, rows 16-byte aligned; Hq any
+ * multiple of Hkv; widths 2..8; streams and windows 16-byte aligned; the rest as in pkv_attn_args.  fp32 accumulation, weights in fp16.  `workspace`:
  * 16-byte aligned device memory of pkv_attn_chunk_workspace(args) bytes (may be 0), used until the call's kernels are done: calls
  * that overlap need one each.  Launches kernels only.  Stands in for cache.update's dense tensors + eager attention
  * (models/llama.py:189-212) where a prompt continues a cache. */

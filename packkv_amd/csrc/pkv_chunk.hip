@@ -16,7 +16,8 @@
 // the largest scale met; the zero's sum takes the rounded weight, so that the error is 2^-11 of p |v|, not of p * scale * code.
 // p is taken against a maximum that is raised only once a score exceeds it by 2^8 (weights stay below 2^15): the factor on the
 // accumulators, and the exchange of maxima between lanes, are rare, and the reference goes into the scores' own multiply-add.
-// q in bf16 becomes fp16 times one power of two for the workgroup's rows, which loses bits only 2^-39 below their largest.
+// q in bf16 becomes fp16 times one power of two for the workgroup's rows, which loses bits only of values 2^-28 below their largest (where
+// fp16 has no normal numbers left).
 //
 // K turns through LDS (a pack holds 16 tokens of one channel, the product wants channels of one token): codes as bytes in rows of
 // 136 bytes, private to the wavefront.  V needs no turn: lane = channel, and the order of the tokens in the contraction is free as
@@ -265,9 +266,10 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     int up = 0;
     if (BF) {
         uint32_t top = 0;
-        for (int r = wave; r <= row_last - row0; r += 4 * RG) {
-            const uint32_t w = reinterpret_cast<const uint32_t *>(q_row(row0 + r))[lane];
-            top = max(top, max(w & 0x7FFFu, (w >> 16) & 0x7FFFu));
+        for (int r = wave; r <= row_last - row0; r += 4 * RG) {            // (infinities, NaN and rows that see nothing do not count)
+            if (p.causal && T - p.n + (row0 + r) / p.G < start) continue;
+            const uint32_t w = reinterpret_cast<const uint32_t *>(q_row(row0 + r))[lane], lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
+            top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));

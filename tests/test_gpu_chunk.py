@@ -92,6 +92,26 @@ def test_padding_on_the_left(cuda, dtype, n, T, W, starts):
         assert bool((got[b, :, :blind] == 0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,W", [(9, 40), (60, 61)])
+def test_queries_in_the_padding_and_broken_ones(cuda, dtype, n, W):
+    """Queries of padded places, and those of one head that are infinite or NaN, leave every other row as it was."""
+    B, Hq, Hkv, T = 2, 8, 2, 256
+    q, ke, ve, kw, vw = _case(cuda, B, Hq, Hkv, n, T, W, dtype, seed=9)
+    st = torch.tensor([T + W - n + 4, 0], dtype=torch.int32, device=cuda)
+    want = ops.attn_chunk(q, ke, ve, kw, vw, win_len=W, starts=st)
+    assert bool((want[0, :, :4] == 0).all()) and bool(want[0, :, 4:].any())
+    big = torch.finfo(dtype).max
+    q[0, 0, :4], q[0, 1, :4], q[0, 2:, :4] = float("nan"), float("inf"), big
+    assert torch.equal(ops.attn_chunk(q, ke, ve, kw, vw, win_len=W, starts=st), want)
+    q[1, 3, 2, 5], q[1, 3, 5, 7] = float("inf"), float("nan")
+    got = ops.attn_chunk(q, ke, ve, kw, vw, win_len=W, starts=st)
+    q[1, 3, 2, 5] = q[1, 3, 5, 7] = 0
+    others = torch.ones(q.shape[:3], dtype=torch.bool, device=cuda)
+    others[1, 3, 2] = others[1, 3, 5] = False
+    assert torch.equal(got[others], want[others]) and bool(got[1, 3, 5].isnan().all())
+
+
 def test_rows_behind_the_last_token_are_not_read(cuda):
     q, ke, ve, kw, vw = _case(cuda, 2, 8, 2, 6, 256, 70, torch.bfloat16)
     want = ops.attn_chunk(q, ke, ve, kw, vw, win_len=70)
