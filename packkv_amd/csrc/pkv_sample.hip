@@ -18,7 +18,7 @@ constexpr int kSampThreads = 1024, kFracBits = 43;
 constexpr double kPerUnit = 64.0;                          // bins for each halving of the weight
 // Behind 44 halvings weights are below half of 2^-43: such tokens have no mass, so they are never drawn, and where a filter ends among
 // them makes no difference.  The bins go a little further, to three a thread.
-constexpr int kNoMass = 44 * 64, kBins = 3072, kCand = 3072, kMine = kBins / kSampThreads;           // (kCand: tokens looked at one by one)
+constexpr int kNoMass = 44 * 64, kMine = 3, kBins = kMine * kSampThreads, kCand = kBins;    // (kCand: tokens looked at one by one)
 constexpr int kF32 = 2;                                    // (beside PKV_F16 and PKV_BF16)
 
 struct SampleParams {
@@ -173,7 +173,7 @@ struct RowState {
     uint32_t count[kBins];
     float slice_top[kMaxSlices];
     RowPlan plan;
-    uint32_t n_cand, arrived[3];
+    uint32_t n_cand, arrived[2];
 };
 template <class T> __device__ __forceinline__ T far_load(const T *p) { return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class T> __device__ __forceinline__ void far_store(T *p, T x) { __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
@@ -322,8 +322,8 @@ __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
     return ((uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
 }
 // The keys s.cand[0 .. n) into s.mass in ascending order.  A wavefront sorts 64 in registers; a key's place is its own in its 64 plus
-// how many are smaller in each of the others, a search of six steps: two barriers, where a sort across the workgroup has one a step
-// (512 keys: 45 of them, some 25 us).
+// how many are smaller in each of the others, a search of seven steps: two barriers, where a sort across the workgroup has one for
+// each of its steps (512 keys: 45).
 __device__ __forceinline__ void sort_candidates(SampleLds &s, uint32_t n) {
     const int lane = threadIdx.x & 63;
     const uint32_t chunks = (n + 63) / 64;
@@ -363,8 +363,8 @@ __device__ __forceinline__ void answer(const SampleParams &p, int row, uint64_t 
     if (p.logprob) p.logprob[row] = (float)((-place_of(key_logit(key), top, r) / kPerUnit - (log2((double)kept) - kFracBits)) * 0.69314718055994530942);
 }
 
-// The answer from at most kCand gathered tokens (s.cand, behind a barrier; s.mass is not looked at any more).  All tokens of a span are there, so a candidate's rank and
-// the mass in front of it are its span's plus those of the candidates of its span in front of it.
+// The answer from at most kCand gathered tokens (s.cand, behind a barrier; s.mass is not looked at any more).  All tokens of a span are
+// there, so a candidate's rank and the mass in front of it are its span's plus those of the candidates of its span in front of it.
 __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const RowPlan &plan) {
     const uint32_t n = plan.gathered;
     uint64_t key[kMine], w[kMine], front[kMine];
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_top_kernel(const SamplePar
     for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d, 64));
     if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
     for (int i = (int)(blockIdx.x * kSampThreads + threadIdx.x); i < kBins; i += (int)gridDim.x * kSampThreads) { st.mass[i] = 0; st.count[i] = 0; }
-    if (blockIdx.x == 0 && threadIdx.x < 4) (&st.n_cand)[threadIdx.x] = 0;
+    if (blockIdx.x == 0 && threadIdx.x == 0) st.n_cand = st.arrived[0] = st.arrived[1] = 0;
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 16; w++) top = fmaxf(top, tops[w]);
@@ -646,8 +646,7 @@ __device__ __forceinline__ float slices_top(const RowState &st) {
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const SampleParams p, RowState *state) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
+    __shared__ SampleLds s;
     const int row = blockIdx.y;
     RowState &st = state[row];
     const float top = slices_top(st);
@@ -677,8 +676,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const SampleParams p, RowState *state) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
+    __shared__ SampleLds s;
     const int row = blockIdx.y;
     RowState &st = state[row];
     const float top = slices_top(st);
@@ -710,8 +708,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const Sampl
 // One workgroup a row.
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleParams p) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
+    __shared__ SampleLds s;
     const int row = blockIdx.x;
     const uint4 *base;
     int phase;
@@ -752,18 +749,14 @@ static int sample_check(const pkv_sample_args *a) {
 }
 
 template <int DT> static int sample_launch(const SampleParams &p, int slices, void *workspace, hipStream_t s) {
-    const size_t lds = sizeof(SampleLds);
     if (slices == 1) {
-        PKV_HIP_CHECK(hipFuncSetAttribute((const void *)sample_rows_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        sample_rows_kernel<DT><<<dim3((unsigned)p.rows), kSampThreads, lds, s>>>(p);
+        sample_rows_kernel<DT><<<dim3((unsigned)p.rows), kSampThreads, 0, s>>>(p);
     } else {
         RowState *state = (RowState *)workspace;
         const dim3 grid((unsigned)slices, (unsigned)p.rows);
-        PKV_HIP_CHECK(hipFuncSetAttribute((const void *)slice_histogram_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
-        PKV_HIP_CHECK(hipFuncSetAttribute((const void *)slice_resolve_kernel<DT>, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
         slice_top_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
-        slice_histogram_kernel<DT><<<grid, kSampThreads, lds, s>>>(p, state);
-        slice_resolve_kernel<DT><<<grid, kSampThreads, lds, s>>>(p, state);
+        slice_histogram_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
+        slice_resolve_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
     }
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;

@@ -204,4 +204,4 @@ class ShapedDecoder:
             nxt = ops.sample(logits, row, temperature, top_k, top_p, min_p).unsqueeze(1)
             out.append(nxt)
             logits = self.forward(nxt, cache, rotary="fused")
-        return torch.cat(out, dim=1)
+        return torch.cat(out, dim=1) if out else ids.new_empty(ids.size(0), 0)

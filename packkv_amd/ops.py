@@ -1277,7 +1277,7 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         a.dtype = _dtype_code(logits)
     _require(V <= 1 << 20, "not supported: %d tokens (at most 2^20)" % V)
     _require(u.shape == (R,) and u.dtype == torch.float32 and u.get_device() == at, "u must be a float32 tensor [rows] on the logits' device")
-    for name, x, ok in (("temperature", temperature, lambda x: x >= 0), ("top_k", top_k, lambda x: x >= 0 and x == int(x) and x < 1 << 31),
+    for name, x, ok in (("temperature", temperature, lambda x: x >= 0), ("top_k", top_k, lambda x: 0 <= x < 1 << 31 and x == int(x)),
                         ("top_p", top_p, lambda x: 0 <= x <= 1), ("min_p", min_p, lambda x: 0 <= x <= 1)):
         _require(torch.is_tensor(x) or ok(x), "%s is out of range" % name)
         _row_setting(a, name, int(x) if name == "top_k" and not torch.is_tensor(x) else x, R, torch.int32 if name == "top_k" else torch.float32, at, keep)

@@ -107,6 +107,7 @@ def test_generate_samples_what_forward_says(cuda):
         assert a.get_seq_length() == b.get_seq_length()
     assert torch.equal(model.generate(ids, model.new_cache(3, 512), u[:3], temperature=0.0),
                        model.generate(ids, model.new_cache(3, 512), 0 * u[:3], top_k=1))
+    assert model.generate(ids, model.new_cache(3, 512), u[:0]).shape == (3, 0)
     with pytest.raises(RuntimeError, match="rotary"):
         model.forward(ids, a)
 

@@ -205,7 +205,7 @@ def test_refusals(cuda):
     bad("2\\^20", logits=logits[:, :1].expand(3, (1 << 20) + 1))
     for wrong in (u[:2], u.double(), u.cpu(), u[:, None]):
         bad("u must be", u=wrong)
-    for kw in (dict(temperature=-0.1), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=2.5), dict(top_k=1 << 31), dict(top_p=1.1), dict(top_p=-0.1),
+    for kw in (dict(temperature=-0.1), dict(temperature=float("nan")), dict(top_k=-1), dict(top_k=2.5), dict(top_k=float("inf")), dict(top_k=1 << 31), dict(top_p=1.1), dict(top_p=-0.1),
                dict(min_p=1.5), dict(min_p=float("nan"))):
         bad("out of range", **kw)
     bad("temperature must be", temperature=u[:2])
