@@ -398,19 +398,34 @@ __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p,
     }
     __syncthreads();
     const double limit = r.by_p ? r.top_p * (double)s.sums[0] : 0.0;
+    // The order's sums rise, so of a wavefront's candidates the largest sum of a kept one, and the smallest key that reaches the target,
+    // go on (an LDS atomic a candidate at one address, which the compiler makes a loop over the lanes, took 12 us for 140 of them).
     bool kept[kMine];
+    uint64_t most = 0;
 #pragma unroll
     for (int e = 0; e < kMine; e++) {
         kept[e] = kMine * threadIdx.x + e < n && (!plan.k_limits || rank[e] < r.top_k) && (!r.by_p || rank[e] == 0 || (double)front[e] < limit) &&
                   (!r.by_min || y[e] <= r.last);
-        if (kept[e]) atomicMax((unsigned long long *)&s.sums[1], (unsigned long long)(front[e] + w[e]));
+        if (kept[e]) most = front[e] + w[e];
+    }
+    const bool any = kMine * (threadIdx.x & ~63u) < n;     // (uniform)
+    if (any) {
+#pragma unroll
+        for (int d = 32; d; d >>= 1) most = max(most, shfl_xor64(most, d));
+        if ((threadIdx.x & 63) == 0) atomicMax((unsigned long long *)&s.sums[1], (unsigned long long)most);
     }
     __syncthreads();
     const uint64_t total = s.sums[1];
     const double target = r.u * (double)total;
+    if (any) {
+        uint64_t best = ~0ull;
 #pragma unroll
-    for (int e = 0; e < kMine; e++)
-        if (kept[e] && (double)(front[e] + w[e]) > target) atomicMin((unsigned long long *)&s.best, (unsigned long long)key[e]);
+        for (int e = kMine - 1; e >= 0; e--)
+            if (kept[e] && (double)(front[e] + w[e]) > target) best = key[e];
+#pragma unroll
+        for (int d = 32; d; d >>= 1) best = min(best, shfl_xor64(best, d));
+        if ((threadIdx.x & 63) == 0) atomicMin((unsigned long long *)&s.best, (unsigned long long)best);
+    }
     __syncthreads();
     if (threadIdx.x == 0) answer(p, row, s.best, plan.top, r, total);
 }
@@ -454,11 +469,21 @@ __device__ __forceinline__ uint64_t descend(SampleLds &s, const SampleParams &p,
         const Prefix out[2] = {{in[0].mass - m0, in[0].count - c0}, {in[1].mass - m1, in[1].count - c1}};
         const uint32_t have[2] = {c0, c1};
         // the digit in which it is reached; where rounding leaves none, the last one that holds a token
+        int top = 0, last = 0;
 #pragma unroll
         for (int e = 0; e < 2; e++) {
             if (!have[e]) continue;
-            atomicMax(&s.at[2], d + e + 1);
-            if (reached(in[e])) atomicMax(&s.at[1], kDigits - (d + e));
+            last = d + e + 1;
+            if (reached(in[e])) top = max(top, kDigits - (d + e));
+        }
+#pragma unroll
+        for (int o = 32; o; o >>= 1) {
+            top = max(top, __shfl_xor(top, o, 64));
+            last = max(last, __shfl_xor(last, o, 64));
+        }
+        if ((threadIdx.x & 63) == 0) {
+            atomicMax(&s.at[1], top);
+            atomicMax(&s.at[2], last);
         }
         __syncthreads();
         const int digit = s.at[1] ? kDigits - s.at[1] : s.at[2] - 1;
@@ -504,12 +529,23 @@ __device__ __forceinline__ void resolve_many(SampleLds &s, const SampleParams &p
             const uint4 *base;
             int phase;
             const int pieces = row_pieces<DT>(p, row, base, phase);
+            uint64_t sum = 0;
+            uint32_t here = 0;
             for_tokens<DT>(p, base, phase, 0, pieces, surely_behind(s.top, b + 1, r), [&](uint32_t, float x) {
                 const double y = place_of(x, s.top, r);
                 if (bin_of(y) != b || y > r.last) return;
-                atomicAdd((unsigned long long *)&s.sums[1], (unsigned long long)weight_of(s.halves, y, b));
-                atomicAdd(&s.n_cand, 1u);
+                sum += weight_of(s.halves, y, b);
+                here++;
             });
+#pragma unroll
+            for (int d = 32; d; d >>= 1) {
+                sum += shfl_xor64(sum, d);
+                here += (uint32_t)__shfl_xor((int)here, d, 64);
+            }
+            if ((threadIdx.x & 63) == 0) {
+                atomicAdd((unsigned long long *)&s.sums[1], (unsigned long long)sum);
+                atomicAdd(&s.n_cand, here);
+            }
             __syncthreads();
             if (s.n_cand < count) { count = s.n_cand; all = s.sums[1]; }
             __syncthreads();
@@ -595,6 +631,29 @@ __device__ __forceinline__ void gather(const SampleParams &p, const RowRule &r, 
         }
     });
 }
+// top_k = 1 (temperature 0) needs no weights: the first token with the largest logit.  ~index, 0 where the pieces hold none, in every
+// thread.
+template <int DT>
+__device__ __forceinline__ uint32_t first_largest(SampleLds &s, const SampleParams &p, const uint4 *base, int phase, int from, int to, float top) {
+    uint32_t best = 0;
+    for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float most) {
+        if (!__any(most >= top)) return;
+#pragma unroll
+        for (int e = 0; e < (DT == kF32 ? 4 : 8); e++)
+            if (x[e] == top) best = max(best, ~(uint32_t)(idx + e));
+    });
+#pragma unroll
+    for (int d = 32; d; d >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, d, 64));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) s.wave_count[threadIdx.x >> 6] = best;
+    __syncthreads();
+    for (int w = 0; w < 16; w++) best = max(best, s.wave_count[w]);
+    return best;
+}
+__device__ __forceinline__ void only_token(const SampleParams &p, int row, uint32_t best) {
+    p.token[row] = (int64_t)~best;
+    if (p.logprob) p.logprob[row] = 0.f;
+}
 __device__ __forceinline__ void fill_halves(SampleLds &s) {
     if (threadIdx.x < 64) s.halves[threadIdx.x] = exp2((double)kFracBits - ((double)threadIdx.x + 0.5) / kPerUnit);
 }
@@ -655,10 +714,16 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
         return;
     }
     const RowRule r = row_rule(p, row, top);
-    fill_halves(s);
     const uint4 *base;
     int phase, from, to;
     row_slice<DT>(p, base, phase, from, to);
+    if (r.top_k == 1) {
+        const uint32_t best = first_largest<DT>(s, p, base, phase, from, to, top);
+        if (threadIdx.x == 0 && best) atomicMax(&st.n_cand, best);
+        if (last_to_arrive(s, &st.arrived[0]) && threadIdx.x == 0) only_token(p, row, far_load(&st.n_cand));
+        return;
+    }
+    fill_halves(s);
     histogram<DT>(s, p, r, base, phase, from, to, top);
     for (int i = threadIdx.x; i < kBins; i += kSampThreads)
         if (s.count[i]) {
@@ -682,6 +747,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const Sampl
     const float top = slices_top(st);
     if (top == -INFINITY) return;
     const RowRule r = row_rule(p, row, top);
+    if (r.top_k == 1) return;
     const RowPlan plan = st.plan;
     const uint32_t n = plan.gathered;
     fill_halves(s);
@@ -719,6 +785,11 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
         return;
     }
     const RowRule r = row_rule(p, row, top);
+    if (r.top_k == 1) {
+        const uint32_t best = first_largest<DT>(s, p, base, phase, 0, pieces, top);
+        if (threadIdx.x == 0) only_token(p, row, best);
+        return;
+    }
     if (threadIdx.x == 0) { s.top = top; s.n_cand = 0; }
     fill_halves(s);
     histogram<DT>(s, p, r, base, phase, 0, pieces, top);
@@ -733,11 +804,15 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
     resolve_few(s, p, row, r, plan);
 }
 
-// Slices a row: as many as make 256 workgroups, of 4096 logits or more; one where that leaves a single one.
+// Slices a row: as many as make one round of 256 workgroups (one a CU), of 4096 logits or more.  A workgroup for the whole row (one
+// launch) where slices would take fewer than 28 k of the row's logits off it.  us, fp32, no filters, one workgroup / slices:
+// 1 x 32003 25.7 / 23.8, 64 x 32003 26.3 / 30.3, 128 x 50257 36.7 / 39.8, 128 x 65537 44.2 / 45.3, 64 x 65537 40.2 / 35.1,
+// 1 x 65537 38.8 / 23.6, 64 x 151936 80.8 / 49.9, 1 x 151936 70.8 / 23.8; 200 x 151936 95.4 / (two rounds) 124.
 static int sample_slices(const pkv_sample_args *a) {
-    int g = (256 + a->rows - 1) / a->rows;
+    int g = 256 / a->rows;
     g = g < a->vocab / 4096 ? g : a->vocab / 4096;
-    return g < 1 ? 1 : g > kMaxSlices ? kMaxSlices : g;
+    g = g < kMaxSlices ? g : kMaxSlices;
+    return g < 2 || a->vocab - a->vocab / g < 28 * 1024 ? 1 : g;
 }
 
 static int sample_check(const pkv_sample_args *a) {
