@@ -57,18 +57,18 @@ __device__ __forceinline__ double place_of(float x, float top, const RowRule &r)
     return fmax(((double)top - (double)x) * r.per_logit, 0.0);             // (inf - inf: 0)
 }
 __device__ __forceinline__ int bin_of(double y) { return (int)fmin(y, (double)(kBins - 1)); }
-// 2^-(y / 64) as a whole number of 2^-43: halves[j] = 2^(43 - (j + 1/2) / 64) for the place in the middle of bin j (of 64), the series
-// of 2^-(g / 64) around it, |g| <= 1/2, to the fifth power (the rest is below 2^-54), and as many halvings as there are 64s in the bin.
-__device__ __forceinline__ uint64_t weight_of(const double *halves, double y, int bin) {
-    const double g = y - ((double)bin + 0.5);
+// 2^-(y / 64) as a whole number of 2^-43: base[bin] = 2^(43 - bin / 64), times the series of 2^-(f / 64) for what is left of the place,
+// 0 <= f < 1, to the fifth power (the rest is below 2^-48).  Right for bins in front of kNoMass.
+__device__ __forceinline__ uint64_t weight_of(const double *base, double y, int bin) {
+    const double f = __builtin_amdgcn_fract(y);
     constexpr double c = 0.69314718055994530942 / kPerUnit;
     double e = -c * c * c * c * c / 120.0;
-    e = fma(e, g, c * c * c * c / 24.0);
-    e = fma(e, g, -c * c * c / 6.0);
-    e = fma(e, g, c * c / 2.0);
-    e = fma(e, g, -c);
-    e = fma(e, g, 1.0);
-    const double fixed = ldexp(e * halves[bin & 63], -(bin >> 6)) + 0x1p52;         // (the low bits of the sum are the rounded number)
+    e = fma(e, f, c * c * c * c / 24.0);
+    e = fma(e, f, -c * c * c / 6.0);
+    e = fma(e, f, c * c / 2.0);
+    e = fma(e, f, -c);
+    e = fma(e, f, 1.0);
+    const double fixed = fma(e, base[bin], 0x1p52);        // (the low bits of the sum are the rounded number)
     return (uint64_t)__double_as_longlong(fixed) & ((1ull << 52) - 1ull);
 }
 // Ascending order of (logit descending, index ascending); x is finite or +inf and not -0.
@@ -91,9 +91,9 @@ template <int DT> __device__ __forceinline__ int row_pieces(const SampleParams &
     return (phase + p.vocab + 16 / ES - 1) / (16 / ES);
 }
 // f(index of the first, logits, the largest) for pieces from .. to - 1, called by whole wavefronts but for lanes that ran out.
-template <int DT, class F>
+template <int DT, int U = 4, class F>
 __device__ __forceinline__ void for_pieces(const SampleParams &p, const uint4 *base, int phase, int from, int to, F f) {
-    constexpr int N = DT == kF32 ? 4 : 8, U = 4;           // four pieces in flight a thread
+    constexpr int N = DT == kF32 ? 4 : 8;                  // U pieces in flight a thread
     for (int c0 = from + (int)threadIdx.x; c0 < to; c0 += U * kSampThreads) {
         uint4 v[U];
 #pragma unroll
@@ -133,7 +133,7 @@ __device__ __forceinline__ float largest(const SampleParams &p, const uint4 *bas
 template <int DT, class F>
 __device__ __forceinline__ void for_tokens(const SampleParams &p, const uint4 *base, int phase, int from, int to, float least, F f) {
     constexpr int N = DT == kF32 ? 4 : 8;
-    for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float top) {
+    for_pieces<DT, 1>(p, base, phase, from, to, [&](int idx, const float *x, float top) {
         if (!__any(top >= least)) return;
 #pragma unroll
         for (int e = 0; e < N; e++)
@@ -187,7 +187,7 @@ struct SampleLds {
     uint32_t count[kBins];
     uint64_t wave_mass[16];
     uint32_t wave_count[16];
-    double halves[64];
+    double base[kBins];                                    // weight of a bin's first place
     float top;
     uint32_t n_cand;
     uint64_t best, sums[2];
@@ -379,7 +379,7 @@ __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p,
             key[e] = s.mass[i];
             y[e] = place_of(key_logit(key[e]), plan.top, r);
             bin[e] = bin_of(y[e]);
-            w[e] = weight_of(s.halves, y[e], bin[e]);
+            w[e] = weight_of(s.base, y[e], bin[e]);
         }
     }
     if (threadIdx.x == 0) { s.sums[0] = plan.k_mass; s.sums[1] = plan.low_mass; s.best = ~0ull; }
@@ -457,7 +457,7 @@ __device__ __forceinline__ uint64_t descend(SampleLds &s, const SampleParams &p,
             const uint64_t key = order_key(x, idx);
             if (above < 64 && (key >> above) != (prefix >> above)) return;
             const int digit = (int)((key >> shift) & ((1u << kWidth[level]) - 1u));
-            atomicAdd((unsigned long long *)&hist_mass[digit], (unsigned long long)weight_of(s.halves, y, bin));
+            atomicAdd((unsigned long long *)&hist_mass[digit], (unsigned long long)weight_of(s.base, y, bin));
             atomicAdd(&hist_count[digit], 1u);
         });
         __syncthreads();
@@ -503,7 +503,7 @@ template <int DT>
 __device__ __forceinline__ void resolve_many(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const RowPlan &plan) {
     auto weight = [&](uint64_t key) {
         const double y = place_of(key_logit(key), s.top, r);
-        return weight_of(s.halves, y, bin_of(y));
+        return weight_of(s.base, y, bin_of(y));
     };
     // sums up to and with a token, in order: what the k tokens hold, then where the kept ones end
     uint64_t all = plan.k_mass;
@@ -534,7 +534,7 @@ __device__ __forceinline__ void resolve_many(SampleLds &s, const SampleParams &p
             for_tokens<DT>(p, base, phase, 0, pieces, surely_behind(s.top, b + 1, r), [&](uint32_t, float x) {
                 const double y = place_of(x, s.top, r);
                 if (bin_of(y) != b || y > r.last) return;
-                sum += weight_of(s.halves, y, b);
+                sum += weight_of(s.base, y, b);
                 here++;
             });
 #pragma unroll
@@ -586,8 +586,9 @@ __device__ __forceinline__ void histogram(SampleLds &s, const SampleParams &p, c
             for (int e = 0; e < 4; e++) {
                 const double y = place_of(x[e0 + e], top, r);
                 b[e] = bin_of(y);
-                w[e] = weight_of(s.halves, y, b[e]);
+                w[e] = weight_of(s.base, y, b[e]);
             }
+            asm volatile("" : "+v"(w[0]), "+v"(w[1]), "+v"(w[2]), "+v"(w[3]));                     // (not one by one behind the tests below)
 #pragma unroll
             for (int e = 0; e < 4; e++)
                 if (x[e0 + e] >= least && b[e] < kNoMass) {
@@ -610,8 +611,17 @@ __device__ __forceinline__ void gather(const SampleParams &p, const RowRule &r, 
         high[i] = is ? surely_before(plan.top, plan.span[i].from, r) : -INFINITY;
         least = fminf(least, low[i]);
     }
+    const bool more = plan.span[1].from <= plan.span[1].to;                // (the first is always there, and absent ones are last)
     for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float most) {
         if (!__any(most >= least)) return;
+        bool some = false;
+#pragma unroll
+        for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) some |= x[e] >= low[0] && x[e] <= high[0];
+        if (more) {
+#pragma unroll
+            for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) some |= (x[e] >= low[1] && x[e] <= high[1]) | (x[e] >= low[2] && x[e] <= high[2]);
+        }
+        if (!some) return;
         uint32_t maybe = 0;                                // a bit a token; few lanes have one
 #pragma unroll
         for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) {
@@ -654,8 +664,11 @@ __device__ __forceinline__ void only_token(const SampleParams &p, int row, uint3
     p.token[row] = (int64_t)~best;
     if (p.logprob) p.logprob[row] = 0.f;
 }
-__device__ __forceinline__ void fill_halves(SampleLds &s) {
-    if (threadIdx.x < 64) s.halves[threadIdx.x] = exp2((double)kFracBits - ((double)threadIdx.x + 0.5) / kPerUnit);
+__device__ __forceinline__ void fill_base(SampleLds &s) {
+    static_assert(kSampThreads % 64 == 0, "a thread's bins are whole halvings apart");
+    const double first = exp2((double)kFracBits - (double)(threadIdx.x & 63) / kPerUnit);
+#pragma unroll
+    for (int i = 0; i < kMine; i++) s.base[threadIdx.x + i * kSampThreads] = ldexp(first, -(int)((threadIdx.x + i * kSampThreads) >> 6));
 }
 __device__ __forceinline__ void no_token(const SampleParams &p, int row) {
     p.token[row] = -1;
@@ -705,7 +718,8 @@ __device__ __forceinline__ float slices_top(const RowState &st) {
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const SampleParams p, RowState *state) {
-    __shared__ SampleLds s;
+    extern __shared__ __align__(16) uint8_t lds[];
+    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
     const int row = blockIdx.y;
     RowState &st = state[row];
     const float top = slices_top(st);
@@ -723,7 +737,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
         if (last_to_arrive(s, &st.arrived[0]) && threadIdx.x == 0) only_token(p, row, far_load(&st.n_cand));
         return;
     }
-    fill_halves(s);
+    fill_base(s);
     histogram<DT>(s, p, r, base, phase, from, to, top);
     for (int i = threadIdx.x; i < kBins; i += kSampThreads)
         if (s.count[i]) {
@@ -741,7 +755,8 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
 }
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const SampleParams p, RowState *state) {
-    __shared__ SampleLds s;
+    extern __shared__ __align__(16) uint8_t lds[];
+    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
     const int row = blockIdx.y;
     RowState &st = state[row];
     const float top = slices_top(st);
@@ -750,7 +765,7 @@ __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const Sampl
     if (r.top_k == 1) return;
     const RowPlan plan = st.plan;
     const uint32_t n = plan.gathered;
-    fill_halves(s);
+    fill_base(s);
     if (n > kCand) {
         if (blockIdx.x) return;
         for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = st.mass[i]; s.count[i] = st.count[i]; }
@@ -774,7 +789,8 @@ __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const Sampl
 // One workgroup a row.
 template <int DT>
 __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleParams p) {
-    __shared__ SampleLds s;
+    extern __shared__ __align__(16) uint8_t lds[];
+    SampleLds &s = *reinterpret_cast<SampleLds *>(lds);
     const int row = blockIdx.x;
     const uint4 *base;
     int phase;
@@ -791,7 +807,7 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
         return;
     }
     if (threadIdx.x == 0) { s.top = top; s.n_cand = 0; }
-    fill_halves(s);
+    fill_base(s);
     histogram<DT>(s, p, r, base, phase, 0, pieces, top);
     scan_bins(s);
     const RowPlan plan = make_plan(s, r, top);
@@ -823,15 +839,21 @@ static int sample_check(const pkv_sample_args *a) {
     return PKV_OK;
 }
 
+template <class K> static hipError_t sample_lds(K kernel) {
+    return hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(SampleLds));
+}
 template <int DT> static int sample_launch(const SampleParams &p, int slices, void *workspace, hipStream_t s) {
     if (slices == 1) {
-        sample_rows_kernel<DT><<<dim3((unsigned)p.rows), kSampThreads, 0, s>>>(p);
+        PKV_HIP_CHECK(sample_lds(sample_rows_kernel<DT>));
+        sample_rows_kernel<DT><<<dim3((unsigned)p.rows), kSampThreads, sizeof(SampleLds), s>>>(p);
     } else {
         RowState *state = (RowState *)workspace;
         const dim3 grid((unsigned)slices, (unsigned)p.rows);
+        PKV_HIP_CHECK(sample_lds(slice_histogram_kernel<DT>));
+        PKV_HIP_CHECK(sample_lds(slice_resolve_kernel<DT>));
         slice_top_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
-        slice_histogram_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
-        slice_resolve_kernel<DT><<<grid, kSampThreads, 0, s>>>(p, state);
+        slice_histogram_kernel<DT><<<grid, kSampThreads, sizeof(SampleLds), s>>>(p, state);
+        slice_resolve_kernel<DT><<<grid, kSampThreads, sizeof(SampleLds), s>>>(p, state);
     }
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;
