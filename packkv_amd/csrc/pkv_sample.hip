@@ -146,12 +146,6 @@ __device__ __forceinline__ float surely_behind(float top, int bin, const RowRule
     return fabs((double)top) < 3.0e38 && x > -3.0e38 ? (float)(x - fabs(x) * 0x1p-22) : -3.402823466e38f;
 }
 
-// A logit above which every place is in front of `bin`.
-__device__ __forceinline__ float surely_before(float top, int bin, const RowRule &r) {
-    const double x = (double)top - ((double)bin - 1.0) / r.per_logit;
-    return bin > 1 && fabs((double)top) < 3.0e38 && x > -3.0e38 ? (float)(x + fabs(x) * 0x1p-22) : INFINITY;
-}
-
 // A run of bins whose tokens are looked at one by one: what lies in front of it and in it.
 struct Span {
     int from, to;                                          // (from > to: none)
@@ -187,6 +181,7 @@ struct SampleLds {
     uint32_t count[kBins];
     uint64_t wave_mass[16];
     uint32_t wave_count[16];
+    float edge[6];
     double base[kBins];                                    // weight of a bin's first place
     float top;
     uint32_t n_cand;
@@ -599,47 +594,74 @@ __device__ __forceinline__ void histogram(SampleLds &s, const SampleParams &p, c
     });
     __syncthreads();
 }
-// Tokens of the spans, each to put(index, logit).  Two fp32 comparisons a span leave few that need their place; a span that is not there
-// lets none through.
-template <int DT, class F>
-__device__ __forceinline__ void gather(const SampleParams &p, const RowRule &r, const RowPlan &plan, const uint4 *base, int phase, int from, int to, F put) {
-    float low[3], high[3], least = INFINITY;
-#pragma unroll
-    for (int i = 0; i < 3; i++) {
-        const bool is = plan.span[i].from <= plan.span[i].to;
-        low[i] = is ? surely_behind(plan.top, plan.span[i].to + 1, r) : INFINITY;
-        high[i] = is ? surely_before(plan.top, plan.span[i].from, r) : -INFINITY;
-        least = fminf(least, low[i]);
+// The smallest logit with its place in `bin` or in front of it (the place falls with the logit, so there is one), by a wavefront: of the
+// 64 numbers around where it should be the first one that is; near 0 beside a large maximum these are too close together, and a search
+// finds it.
+__device__ __forceinline__ float least_of(float top, int bin, const RowRule &r) {
+    const auto ordered = [](float x) { const int b = (int)__float_as_uint(x); return b < 0 ? b ^ 0x7FFFFFFF : b; };
+    const auto number = [](int b) { return __uint_as_float((uint32_t)(b < 0 ? b ^ 0x7FFFFFFF : b)); };
+    const auto holds = [&](int b) { return bin_of(place_of(number(b), top, r)) <= bin; };
+    int from = ordered(-3.402823466e38f), to = ordered(top);
+    const double x = (double)top - ((double)bin + 1.0) / r.per_logit;
+    const int near = ordered((float)fmin(fmax(x, -3.0e38), 3.0e38)) - 32, mine = min(max(near + (int)(threadIdx.x & 63), from), to);
+    const uint64_t ok = __ballot(holds(mine));
+    if (ok && !(ok & 1ull)) return number(__builtin_amdgcn_readlane(mine, __ffsll((unsigned long long)ok) - 1));
+    while (from < to) {
+        const int mid = (int)(((int64_t)from + to) >> 1);
+        if (holds(mid)) to = mid;
+        else from = mid + 1;
     }
-    const bool more = plan.span[1].from <= plan.span[1].to;                // (the first is always there, and absent ones are last)
-    for_pieces<DT>(p, base, phase, from, to, [&](int idx, const float *x, float most) {
-        if (!__any(most >= least)) return;
-        bool some = false;
+    return number(to);
+}
+// Tokens of the spans: reserve(how many) -> the first's number, for a wavefront's of a piece, then put(number, key) for each.  Two fp32
+// comparisons a token and span with the spans' exact ends; a span that is not there lets none through.
+template <int DT, class R, class F>
+__device__ __forceinline__ void gather(SampleLds &s, const SampleParams &p, const RowRule &r, const RowPlan &plan, const uint4 *base, int phase, int from, int to,
+                                       R reserve, F put) {
+    constexpr int N = DT == kF32 ? 4 : 8;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    int first[3], last[3];
 #pragma unroll
-        for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) some |= x[e] >= low[0] && x[e] <= high[0];
+    for (int i = 0; i < 3; i++) { first[i] = plan.span[i].from; last[i] = plan.span[i].to; }
+    if (wave < 6) {
+        const bool above = wave >= 3;
+        const int f = wave % 3 == 0 ? first[0] : wave % 3 == 1 ? first[1] : first[2], l = wave % 3 == 0 ? last[0] : wave % 3 == 1 ? last[1] : last[2];
+        float edge = above ? NAN : INFINITY;
+        if (f <= l && !(above && f == 0)) edge = least_of(plan.top, above ? f - 1 : l, r);
+        s.edge[wave] = edge;
+    }
+    __syncthreads();
+    float low[3], above[3];                                // in a span: low <= x and not above <= x
+#pragma unroll
+    for (int i = 0; i < 3; i++) { low[i] = s.edge[i]; above[i] = s.edge[3 + i]; }
+    const float least = fminf(fminf(low[0], low[1]), low[2]);
+    const bool more = first[1] <= last[1];                // (the first is always there, and absent ones are last)
+    for_pieces<DT, 2>(p, base, phase, from, to, [&](int idx, const float *x, float most) {
+        if (!__any(most >= least)) return;
+        uint64_t in[N];
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < N; e++) in[e] = __ballot((x[e] >= low[0]) & !(x[e] >= above[0]));
         if (more) {
 #pragma unroll
-            for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) some |= (x[e] >= low[1] && x[e] <= high[1]) | (x[e] >= low[2] && x[e] <= high[2]);
+            for (int e = 0; e < N; e++) in[e] |= __ballot(((x[e] >= low[1]) & !(x[e] >= above[1])) | ((x[e] >= low[2]) & !(x[e] >= above[2])));
         }
-        if (!some) return;
-        uint32_t maybe = 0;                                // a bit a token; few lanes have one
 #pragma unroll
-        for (int e = 0; e < (DT == kF32 ? 4 : 8); e++) {
-            const bool in = (x[e] >= low[0] && x[e] <= high[0]) | (x[e] >= low[1] && x[e] <= high[1]) | (x[e] >= low[2] && x[e] <= high[2]);
-            maybe |= in ? 1u << e : 0u;
-        }
-        for (; maybe; maybe &= maybe - 1) {
-            const int e = __ffs((int)maybe) - 1;
-            float v = x[0];
+        for (int e = 0; e < N; e++) n += (uint32_t)__popcll(in[e]);
+        if (!n) return;
+        uint32_t at = reserve(n);
 #pragma unroll
-            for (int k = 1; k < (DT == kF32 ? 4 : 8); k++) v = e == k ? x[k] : v;
-            const int b = bin_of(place_of(v, plan.top, r));
-            bool in = false;
-#pragma unroll
-            for (int i = 0; i < 3; i++) in |= b >= plan.span[i].from && b <= plan.span[i].to;
-            if (in) put((uint32_t)(idx + e), v + 0.f);
+        for (int e = 0; e < N; e++) {
+            if ((in[e] >> (threadIdx.x & 63)) & 1ull) put(at + __builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0u)), order_key(x[e] + 0.f, (uint32_t)(idx + e)));
+            at += (uint32_t)__popcll(in[e]);
         }
     });
+}
+// A wavefront's share of a counter (its first lane is there).
+__device__ __forceinline__ uint32_t take(uint32_t *counter, uint32_t n) {
+    uint32_t at = 0;
+    if ((threadIdx.x & 63) == 0) at = atomicAdd(counter, n);
+    return (uint32_t)__builtin_amdgcn_readfirstlane((int)at);
 }
 // top_k = 1 (temperature 0) needs no weights: the first token with the largest logit.  ~index, 0 where the pieces hold none, in every
 // thread.
@@ -777,9 +799,8 @@ __global__ void __launch_bounds__(kSampThreads) slice_resolve_kernel(const Sampl
     const uint4 *base;
     int phase, from, to;
     row_slice<DT>(p, base, phase, from, to);
-    gather<DT>(p, r, plan, base, phase, from, to, [&](uint32_t idx, float x) {
-        far_store(&st.cand[min(atomicAdd(&st.n_cand, 1u), (uint32_t)kCand - 1u)], order_key(x, idx));
-    });
+    gather<DT>(s, p, r, plan, base, phase, from, to, [&](uint32_t n) { return take(&st.n_cand, n); },
+               [&](uint32_t at, uint64_t key) { far_store(&st.cand[min(at, (uint32_t)kCand - 1u)], key); });
     if (!last_to_arrive(s, &st.arrived[1])) return;
     for (uint32_t i = threadIdx.x; i < n; i += kSampThreads) s.cand[i] = far_load(&st.cand[i]);
     __syncthreads();
@@ -815,7 +836,8 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
         resolve_many<DT>(s, p, row, r, plan);
         return;
     }
-    gather<DT>(p, r, plan, base, phase, 0, pieces, [&](uint32_t idx, float x) { s.cand[atomicAdd(&s.n_cand, 1u)] = order_key(x, idx); });
+    gather<DT>(s, p, r, plan, base, phase, 0, pieces, [&](uint32_t n) { return take(&s.n_cand, n); },
+               [&](uint32_t at, uint64_t key) { s.cand[min(at, (uint32_t)kCand - 1u)] = key; });
     __syncthreads();
     resolve_few(s, p, row, r, plan);
 }
