@@ -316,12 +316,12 @@ __device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, flo
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
     return ((uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
 }
-// The keys s.cand[0 .. n) into s.mass in ascending order.  A wavefront sorts 64 in registers; a key's place is its own in its 64 plus
-// how many are smaller in each of the others, a search of seven steps: two barriers, where a sort across the workgroup has one for
-// each of its steps (512 keys: 45).
-__device__ __forceinline__ void sort_candidates(SampleLds &s, uint32_t n) {
+// The keys s.cand[0 .. n) in ascending order, there or in s.mass.  A wavefront sorts 64 in registers; then runs are merged in pairs, a
+// key's place being its own in its run plus how many of the other run are smaller, which a search finds: a barrier for each doubling,
+// where a sort across the workgroup has one for each of its steps (512 keys: 3 against 45).
+__device__ __forceinline__ const uint64_t *sort_candidates(SampleLds &s, uint32_t n) {
     const int lane = threadIdx.x & 63;
-    const uint32_t chunks = (n + 63) / 64;
+    const uint32_t chunks = (n + 63) / 64, all = 64 * chunks;
     for (uint32_t c = threadIdx.x >> 6; c < chunks; c += kSampThreads / 64) {
         uint64_t key = 64 * c + lane < n ? s.cand[64 * c + lane] : ~0ull;
 #pragma unroll
@@ -335,22 +335,26 @@ __device__ __forceinline__ void sort_candidates(SampleLds &s, uint32_t n) {
         s.cand[64 * c + lane] = key;
     }
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 64 * chunks; i += kSampThreads) {
-        const uint64_t key = s.cand[i];
-        if (key == ~0ull) continue;
-        uint32_t place = i & 63;
-        for (uint32_t c = 0; c < chunks; c++) {
-            if (c == i >> 6) continue;
-            const uint64_t *at = s.cand + 64 * c;
-            uint32_t less = 0;                             // 0 .. 64
-#pragma unroll
-            for (uint32_t step = 32; step; step >>= 1)
-                if (at[less + step - 1] < key) less += step;
-            place += less + (at[less] < key ? 1u : 0u);
+    uint64_t *from = s.cand, *to = s.mass;
+    for (uint32_t run = 64; run < all; run *= 2) {
+        for (uint32_t i = threadIdx.x; i < all; i += kSampThreads) {
+            const uint64_t key = from[i];
+            const uint32_t own = i & ~(run - 1u), other = own ^ run;
+            uint32_t less = 0;
+            if (other < all) {                             // (the last run may be shorter, or have no other)
+                const uint32_t len = min(run, all - other);
+                for (uint32_t step = run / 2; step; step >>= 1)
+                    if (less + step <= len && from[other + less + step - 1] < key) less += step;
+                if (less < len && from[other + less] < key) less++;
+            }
+            to[min(own, other) + (i - own) + less] = key;
         }
-        s.mass[place] = key;
+        __syncthreads();
+        uint64_t *const t = from;
+        from = to;
+        to = t;
     }
-    __syncthreads();
+    return from;
 }
 
 __device__ __forceinline__ void answer(const SampleParams &p, int row, uint64_t key, float top, const RowRule &r, uint64_t kept) {
@@ -365,13 +369,13 @@ __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p,
     uint64_t key[kMine], w[kMine], front[kMine];
     int bin[kMine];
     double y[kMine];
-    sort_candidates(s, n);
+    const uint64_t *sorted = sort_candidates(s, n);
 #pragma unroll
     for (int e = 0; e < kMine; e++) {
         const uint32_t i = kMine * threadIdx.x + e;
         key[e] = ~0ull; w[e] = 0; y[e] = 0; bin[e] = 0;
         if (i < n) {
-            key[e] = s.mass[i];
+            key[e] = sorted[i];
             y[e] = place_of(key_logit(key[e]), plan.top, r);
             bin[e] = bin_of(y[e]);
             w[e] = weight_of(s.base, y[e], bin[e]);
