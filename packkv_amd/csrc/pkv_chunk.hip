@@ -1,9 +1,9 @@
 // Attention of several new tokens over a compressed cache: query i of n sits at position T - n + i of the T tokens (streams, then
 // the 16-bit window) and attends to those from the sequence's first token up to itself.
 //
-// Rows are the (token, query head) pairs of one KV head, row = token * G + head of the group: a workgroup takes 32 NB of them and a
-// run of 128-token tiles; each of its four wavefronts takes 32 tokens of every tile for ALL of these rows and keeps a softmax state
-// and an accumulator of its own, so nothing of the softmax crosses wavefronts until the run ends.
+// Rows are the (token, query head) pairs of one KV head, row = token * G + head of the group: a workgroup takes RG groups of 32 NB of
+// them and a run of 128-token tiles; each of a group's four wavefronts takes 32 tokens of every tile for ALL of the group's rows and
+// keeps a softmax state and an accumulator of its own, so nothing of the softmax crosses wavefronts until the run ends.
 //
 // Both products are formed transposed, on 32x32x16 fp16 matrix instructions (a product's columns are the lanes, here the rows):
 //   S^T [token x row]   = K codes x q      a lane holds 16 tokens' scores of one row: maxima and sums are the lane's own but for
@@ -24,6 +24,14 @@
 // long as both operands agree, so a lane unpacks ONE pack per 32 channels straight into its operand -- tokens (k, k + 8) side by
 // side, since both halves of a pack's word take the same shifts.  Which pack is where comes from a table that the half-wavefronts
 // fill, one unit each (offset, width, minimum of its 128 packs).
+//
+// Bound by the vector instructions around the products: 32 tokens take a wavefront some 800 of them with 32 rows (of a tile: K's codes
+// to bytes 220, bytes to operands 65, V's table 100 and packs 180, scores to weights 150) and 730 with 64, which the vector units issue
+// in 67 % of the cycles.  Hence as few wavefronts as possible unpack the same block: up to 128 rows a workgroup, two groups of them
+// sharing K's bytes and V's table.  8 KV heads, 4-bit codes: 8 sequences x 4 queries of 32 heads over 16384 tokens 79 us (a copy of the
+// bytes: 22), 1024 queries over 32768 1010 us, 540 TFLOP/s (a large product reaches 1160), where 64 rows a workgroup without sharing
+// took 1430; 40 heads x 333 queries of two sequences over 4096 tokens in 5-bit codes 155 to 169 us; 3 queries over 1100 tokens 14 us,
+// 4 of them the merge.
 #include "pkv_block.hpp"
 #include "pkv_runtime.hpp"
 
