@@ -651,6 +651,7 @@ def _rotary_args(q, k, positions, inv_freq, q_norm, k_norm, eps, sections, inter
     B, Hq, n, _ = q.shape
     at, dtype = q.get_device(), q.dtype
     code = _dtype_code(q)
+    _require(Hq > 0 and k.size(1) > 0, "q and k must have heads")
     _require(k.dtype == dtype, "q and k must have one dtype")
     axes = _frequency_axes(sections, interleaved)
     A = 1 if sections is None else len(tuple(sections))

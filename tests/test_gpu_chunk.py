@@ -254,3 +254,16 @@ def test_refusals(cuda):
     bad("share elements", out=q[:, :1].expand(2, 8, 6, 128))
     bad("on q's device", k=dict(ke, scale=ke["scale"].cpu()))
     bad("bits_len", k=dict(ke, bits=9))
+
+
+def test_windows_and_queries_further_apart_than_32_bits(cuda):
+    B, Hq, Hkv, n, W, cap = 2, 4, 2, 5, 150, (1 << 22) + 70
+    q, _, _, kw, vw = _case(cuda, B, Hq, Hkv, n, 0, W, torch.float16, cap=W)
+    want = ops.attn_chunk(q, None, None, kw, vw)
+    big = [torch.empty(B, Hkv, cap, 128, dtype=torch.float16, device=cuda) for _ in range(2)]
+    for far, near in zip(big, (kw, vw)):
+        far[:, :, :W].copy_(near)
+    flat = torch.empty((1 << 31) + 8192, dtype=torch.float16, device=cuda)
+    far_q, out = (flat.as_strided(q.shape, (1 << 31, n * 128, 128, 1), at) for at in (0, 4096))
+    far_q.copy_(q)
+    assert torch.equal(ops.attn_chunk(far_q, None, None, *big, win_len=W, out=out), want) and torch.equal(out, want)

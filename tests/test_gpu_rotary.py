@@ -183,3 +183,30 @@ def test_on_a_side_stream_and_in_a_graph(cuda):
         wq, wk = ops.norm_rotary(q, k, pos, inv)
         torch.cuda.synchronize()
         assert torch.equal(out, wq) and torch.equal(kw[:, :, 5:6], wk) and torch.equal(vw[:, :, 5:6], v)
+
+
+def test_no_heads_on_one_side_are_refused(cuda):
+    q, pos, inv = torch.zeros(1, 4, 2, 128, device=cuda).half(), torch.arange(2, device=cuda), _inv(cuda)
+    win = torch.zeros(1, 4, 8, 128, device=cuda).half()
+    for a, b in ((q[:, :0], q), (q, q[:, :0])):
+        with pytest.raises(RuntimeError, match="heads"):
+            ops.norm_rotary(a, b, pos, inv)
+    with pytest.raises(RuntimeError, match="heads"):
+        ops.window_append_rotary(q[:, :0], q, q, pos, inv, win, win.clone(), 0)
+
+
+def test_rows_further_apart_than_32_bits(cuda):
+    """Inputs and a window whose second sequence and last heads start behind 2^31 elements."""
+    gen = torch.Generator(device=cuda).manual_seed(9)
+    flat = torch.empty((1 << 31) + 4096, dtype=torch.float16, device=cuda)
+    q, k = flat.as_strided((2, 2, 3, 128), (1 << 31, 384, 128, 1)), flat.as_strided((2, 2, 3, 128), (1 << 31, 384, 128, 1), 1024)
+    q.copy_(torch.randn(q.shape, generator=gen, device=cuda))
+    k.copy_(torch.randn(k.shape, generator=gen, device=cuda))
+    pos, inv = torch.arange(77, 80, device=cuda), _inv(cuda)
+    want = ops.norm_rotary(q.contiguous(), k.contiguous(), pos, inv)
+    got = ops.norm_rotary(q, k, pos, inv)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    cap = (1 << 22) + 70                                   # 2 x 2 x cap x 128 elements
+    kw, vw = (torch.empty(2, 2, cap, 128, dtype=torch.float16, device=cuda) for _ in range(2))
+    assert torch.equal(ops.window_append_rotary(q, k, q, pos, inv, kw, vw, cap - 3), want[0])
+    assert torch.equal(kw[:, :, cap - 3:], want[1]) and torch.equal(vw[:, :, cap - 3:], q)

@@ -212,3 +212,44 @@ def test_refusals(cuda):
     bad("top_k must be", top_k=u)
     bad("top_p must be", top_p=u.cpu())
     bad("out must be", out=torch.zeros(3, device=cuda))
+
+
+def test_rows_further_apart_than_32_bits(cuda):
+    flat = torch.empty((1 << 31) + 80000, dtype=torch.bfloat16, device=cuda)
+    for V in (70000, 5000):                                # in slices, and not
+        far = flat.as_strided((2, V), (1 << 31, 1), 7)
+        logits, u = _logits(cuda, 2, V, torch.bfloat16, V)
+        far.copy_(logits)
+        for kw in (dict(top_p=0.9), dict(temperature=0.0)):
+            got, want = ops.sample(far, u, want_logprob=True, **kw), ops.sample(logits, u, want_logprob=True, **kw)
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_the_most_tokens_a_row_can_have(cuda):
+    V = 1 << 20
+    u = torch.tensor([0.0, 0.5, 1 - 2.0 ** -24], device=cuda)
+    tok, lp = ops.sample(torch.zeros(3, V, device=cuda), u, want_logprob=True)
+    assert tok.tolist() == [0, V // 2, int((1 - 2.0 ** -24) * V)] and (lp + 20 * np.log(2)).abs().max().item() < 1e-6
+    _check(*_logits(cuda, 2, V, torch.float16, 21), top_p=0.8)
+
+
+def test_logits_about_zero_beside_an_edge_of_the_bins(cuda):
+    """A temperature and a maximum that put zero on the border of two bins, to 2^-29 of the maximum: numbers around it are far closer
+    together than those that differ from the maximum."""
+    f32 = np.float32
+    found = []
+    for i in range(4000):
+        t = f32(1.25) + f32(i) * f32(2.0 ** -12)
+        per = 64 * 1.4426950408889634074 / float(t)
+        top = f32(512 / per)
+        if abs(float(top) * per / 512 - 1) < 2.0 ** -29:
+            found.append((float(t), float(top)))
+    assert found
+    g = torch.Generator(device=cuda).manual_seed(22)
+    for t, top in found[:6]:
+        x = torch.randn(3, 6000, generator=g, device=cuda) * 10.0 ** (-45 * torch.rand(3, 6000, generator=g, device=cuda) ** 0.5)
+        x = torch.where(x.abs() > top, torch.zeros_like(x), x)
+        x[:, 17] = top
+        u = torch.tensor([0.3, 0.6, 0.9], device=cuda)
+        for kw in (dict(), dict(top_k=2500), dict(top_p=0.4), dict(top_p=0.41, top_k=3400)):
+            _check(x, u, temperature=t, **kw)
