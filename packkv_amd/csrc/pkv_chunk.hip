@@ -271,13 +271,26 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     }
 
     // ---- q: rows into LDS as fp16 (bf16: times 2^up), their sums ----
+    constexpr int kPieces = M * 16 / (256 * RG);           // of 16 bytes, a thread
+    u4 qw[kPieces];
+#pragma unroll
+    for (int j = 0; j < kPieces; j++) {
+        const int i = tid + 256 * RG * j;
+        qw[j] = *reinterpret_cast<const u4 *>(q_row(min(row0 + (i >> 4), p.rows - 1)) + 8 * (i & 15));
+    }
     int up = 0;
     if (BF) {
         uint32_t top = 0;
-        for (int r = wave; r <= row_last - row0; r += 4 * RG) {            // (infinities, NaN and rows that see nothing do not count)
-            if (p.causal && T - p.n + (row0 + r) / p.G < start) continue;
-            const uint32_t w = reinterpret_cast<const uint32_t *>(q_row(row0 + r))[lane], lo = w & 0x7FFFu, hi = (w >> 16) & 0x7FFFu;
-            top = max(top, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) {                // (infinities, NaN and rows that see nothing do not count)
+            const int r = min(row0 + ((tid + 256 * RG * j) >> 4), p.rows - 1);
+            uint32_t most = 0;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const uint32_t lo = qw[j][k] & 0x7FFFu, hi = (qw[j][k] >> 16) & 0x7FFFu;
+                most = max(most, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
+            }
+            if (!p.causal || T - p.n + r / p.G >= start) top = max(top, most);
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
@@ -289,14 +302,15 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
         up = top ? min(max(141 - (int)(top >> 7), -120), 120) : 0;        // the largest comes to 2^14 .. 2^15
     }
     const float up_f = __uint_as_float((uint32_t)(127 + up) << 23);
-    for (int i = tid; i < M * 16; i += 256 * RG) {
-        const int r = i >> 4, c = i & 15;
-        u4 w = *reinterpret_cast<const u4 *>(q_row(min(row0 + r, p.rows - 1)) + 8 * c);
+#pragma unroll
+    for (int j = 0; j < kPieces; j++) {
+        const int i = tid + 256 * RG * j;
+        u4 w = qw[j];
         if (BF) {
 #pragma unroll
             for (int k = 0; k < 4; k++) w[k] = pack_f16(__uint_as_float(w[k] << 16) * up_f, __uint_as_float(w[k] & 0xFFFF0000u) * up_f);
         }
-        *reinterpret_cast<u4 *>(qt + r * kQRow + 16 * c) = w;
+        *reinterpret_cast<u4 *>(qt + (i >> 4) * kQRow + 16 * (i & 15)) = w;
     }
     if (c0 < c1) put(c0);
     __syncthreads();
