@@ -159,12 +159,13 @@ __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
 }
 
 template <bool BF, int NB, int RG, bool WIDE>
-__global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(const ChunkParams p) {
+__global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chunk_kernel(const ChunkParams p) {
     constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
-    constexpr int M = 32 * NB * RG, kBufs = RG + 1, kSets = RG;
+    constexpr bool ONCE = RG == 1 && !WIDE;                // a tile's blocks are staged one at a time
+    constexpr int M = 32 * NB * RG, kKBufs = ONCE ? 1 : 2, kBufs = ONCE ? 1 : RG + 1, kSets = RG;
     constexpr bool COPY = !WIDE || RG == 2;                // blocks go to LDS without registers (what is staged lies below 64 KiB)
     extern __shared__ __align__(16) uint8_t lds[];
-    uint8_t *ring = lds;                                   // staged: two tiles' K blocks, kBufs tiles' V blocks; window and end: V rows, sums (kt as well)
+    uint8_t *ring = lds;                                   // staged: kKBufs tiles' K blocks, kBufs tiles' V blocks; window and end: V rows, sums (kt as well)
     uint8_t *kt_all = lds + p.ring;                        // [kSets][4 quarters][32 tokens][kKRow]
     uint32_t *tab_all = reinterpret_cast<uint32_t *>(kt_all + kSets * 4 * 32 * kKRow);        // [kSets][8 units][4 slots][32 lanes]
     float2 *par_all = reinterpret_cast<float2 *>(tab_all + kSets * 1024);          // [kSets][2][4][32]: (scale, zero * scale), (V scale, V zero)
@@ -220,7 +221,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>(stream), 0, (int)bytes4, 0x00020000);
     const uint32_t slot = quarter < 2 ? p.slot_k : p.slot_v;
     auto block_at = [&](int side, int j, int tile_nr) -> uint32_t {            // tile_nr: counted from the run's first
-        return side ? 4u * p.slot_k + (uint32_t)(2 * (tile_nr % kBufs) + j) * p.slot_v : (uint32_t)(2 * (tile_nr & 1) + j) * p.slot_k;
+        return side ? 2u * kKBufs * p.slot_k + (uint32_t)(2 * (tile_nr % kBufs) + j) * p.slot_v : (uint32_t)(2 * (tile_nr % kKBufs) + j) * p.slot_k;
     };
     u4 raw[COPY ? 1 : NQ];
     uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     };
     if (c0 < c1) {
         look_up(c0);
-        fetch(c0);
+        if (!ONCE || quarter < 2) fetch(c0);
         if (RG == 2 && c0 + 1 < c1) fetch(c0 + 1);
         fetch_par(c0);
     }
@@ -484,7 +485,32 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
     };
 
     // ---- compressed tiles ----
-    if (RG == 1) {
+    const auto lds_barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };      // (copies go on)
+    if (ONCE) {
+        // Few rows: three workgroups a CU cover each other's waits, with one place for K's blocks and one for V's: V's are copied while the
+        // scores are formed, the next tile's K during the products with V.  Three barriers a tile: K, V, table.
+        for (int tile = c0; tile < c1; tile++) {
+            if (tile != c0) {
+                put(tile);
+                lds_barrier();                             // (and the table's readers are done)
+            }
+            if (quarter >= 2) fetch(tile);
+            const float grow = raise_scale(write_par(tile, 0));
+            unpack_k(tile, kt_all);
+            wave_lds_order();
+            u4 w[NB][2];
+            weights_of(tile, kt_all, par_all, grow, w);
+            put(tile);
+            lds_barrier();
+            if (tile + 1 < c1) {
+                if (quarter < 2) fetch(tile + 1);
+                fetch_par(tile + 1);
+            }
+            parse_v(tile, tab_all);
+            lds_barrier();
+            add_values(tab_all, w);
+        }
+    } else if (RG == 1) {
         // Few rows: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
         for (int tile = c0; tile < c1; tile++) {
             if (tile != c0) __syncthreads();               // the tile is staged, and the table's readers are done
@@ -498,8 +524,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : 2) attn_chunk_kernel(c
             wave_lds_order();
             u4 w[NB][2];
             weights_of(tile, kt_all, par_all, grow, w);
-            if (!COPY) __syncthreads();
-            else asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");        // the table is there; copies go on
+            __syncthreads();
             add_values(tab_all, w);
             if (tile + 1 < c1) put(tile + 1);
         }
@@ -734,13 +759,14 @@ static bool chunk_wide(const pkv_chunk_args *a) { return a->T_c && (a->k_bits > 
 
 // LDS bytes of what is staged, and of a block of either side: a block at any phase, and a last word's reach.
 static uint32_t chunk_ring(const pkv_chunk_args *a, int rg, uint32_t &slot_k, uint32_t &slot_v) {
+    const bool once = rg == 1 && !chunk_wide(a);
     slot_k = (((uint32_t)k_block_bound(64, a->T_c ? a->k_bits : 2) + 15u) & ~15u) + 32u;
     slot_v = (((uint32_t)v_block_bound(64, a->T_c ? a->v_bits : 2) + 15u) & ~15u) + 32u;
-    return 4u * slot_k + 2u * (uint32_t)(rg + 1) * slot_v;
+    return once ? 2u * slot_k + 2u * slot_v : 4u * slot_k + 2u * (uint32_t)(rg + 1) * slot_v;
 }
 
-// How a call is cut: rows a workgroup (32 NB RG), and runs of tiles, so that the rounds of workgroups the device takes -- two a CU of the
-// small kind, one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
+// How a call is cut: rows a workgroup (32 NB RG), and runs of tiles, so that the rounds of workgroups the device takes -- three a CU of
+// the small kind (wide codes: two), one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
 // partials as one.
 struct ChunkCut {
     int nb, rg, row_tiles, tiles, run, nsplit;
@@ -754,7 +780,7 @@ static ChunkCut chunk_cut(const pkv_chunk_args *a) {
     const int64_t m = 32 * c.nb * c.rg;
     c.row_tiles = (int)((rows + m - 1) / m);
     c.tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
-    const int64_t groups = (int64_t)a->B * a->Hkv * c.row_tiles, slots = c.rg == 1 ? 512 : 256;
+    const int64_t groups = (int64_t)a->B * a->Hkv * c.row_tiles, slots = c.rg == 2 ? 256 : chunk_wide(a) ? 512 : 768;
     int64_t best = -1;
     for (int want = 1; want <= c.tiles && want <= 512; want++) {
         const int run = (c.tiles + want - 1) / want, nsplit = (c.tiles + run - 1) / run;
