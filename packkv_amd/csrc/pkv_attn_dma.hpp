@@ -2,7 +2,7 @@
 // travel global memory -> LDS with LDS-direct buffer loads (no registers, 16 bytes per lane,
 // fully coalesced) into one of two tile slots, one tile ahead of their use; lanes then parse their
 // packs out of LDS.  Included by pkv_attn.hip after pkv_attn_direct.hpp (shares UnitRegs,
-// meta_fields, unit_windows, pack_offsets8 and the fused DPP reductions).
+// meta_fields, unit_windows and the fused DPP reductions).
 //
 // Tile = 128 tokens of one (sequence, KV head) = 2 K blocks (64 x 128) + 2 V blocks (128 x 64);
 // wave w copies block w (0, 1: K; 2, 3: V) and quantizer-parameter array w of the tile.

@@ -145,14 +145,8 @@ __device__ __forceinline__ void unit_codes_wide(const uint8_t *blk, uint32_t uni
 // register), so one packed 16-bit shift moves two packs at a time and a byte permute gathers the
 // four codes of a token: 5 instructions per four codes instead of a 64-bit shift per code.
 template <class Sink>
-__device__ __forceinline__ void unit_codes(const uint8_t *blk, uint32_t unit_off, int t, const UnitGeom g, Sink sink) {
+__device__ __forceinline__ void packs_codes(const UnitPacks &u, Sink sink) {
     typedef unsigned short u16pair __attribute__((ext_vector_type(2)));
-    if (g.W > 4) {      // uniform
-        unit_codes_wide(blk, unit_off, t, g, sink);
-        return;
-    }
-    UnitPacks u;
-    unit_parse(blk, unit_off, t, g, u);
     uint32_t hlf[4][2];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -182,6 +176,16 @@ __device__ __forceinline__ void unit_codes(const uint8_t *blk, uint32_t unit_off
             sink(4 * q + pp, (__builtin_amdgcn_perm(x23, x01, 0x06040200u) & mq) + minq);
         }
     }
+}
+template <class Sink>
+__device__ __forceinline__ void unit_codes(const uint8_t *blk, uint32_t unit_off, int t, const UnitGeom g, Sink sink) {
+    if (g.W > 4) {      // uniform
+        unit_codes_wide(blk, unit_off, t, g, sink);
+        return;
+    }
+    UnitPacks u;
+    unit_parse(blk, unit_off, t, g, u);
+    packs_codes(u, sink);
 }
 
 // The same for a width known at compile time (2..4), for consumers that multiply: `sink(k, c01, c23)` gets the codes of

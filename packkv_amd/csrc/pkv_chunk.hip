@@ -124,6 +124,20 @@ template <bool WIDE> __device__ __forceinline__ void pack_operand(const uint8_t 
     }
 }
 
+// Widths, minima and places (bytes from the unit's start) of the lane's four packs, for codes of up to 4 bits.
+__device__ __forceinline__ void narrow_packs(const uint8_t *unit, int t, const UnitGeom g, uint32_t len[4], uint32_t mn[4], uint32_t at[4]) {
+    const uint32_t minsw = lds_meta_word(unit, t, g.W), lensw = lds_meta_word(unit + g.mins_bytes, t, g.LB);
+    uint32_t off2[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        len[i] = (lensw >> (i * g.LB)) & ((1u << g.LB) - 1u);
+        mn[i] = (minsw >> (i * g.W)) & ((1u << g.W) - 1u);
+    }
+    pack_offsets8(len[0] | (len[1] << 8) | (len[2] << 16) | (len[3] << 24), off2);        // (widths of 7, damaged, do not carry either)
+#pragma unroll
+    for (int i = 0; i < 4; i++) at[i] = (uint32_t)(g.mins_bytes + g.lens_bytes) + 2u * off2[i];
+}
+
 // Blocks of widths up to 4 travel from memory to LDS without registers, 16 bytes a lane: lane l's land at lds_addr + 16 l, lanes behind
 // the buffer's end get zeroes, lanes that are off write nothing.  lds_addr and rsrc are wave-uniform.  The compiler does not see the
 // copies: s_waitcnt vmcnt(0) stands in front of the barrier that hands them on, and the barrier between waits for LDS only.
@@ -355,11 +369,29 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     auto unpack_k = [&](int tile, uint8_t *kt) {           // 16 tokens x 128 channels; the quarter's two units make its 32 tokens
         uint8_t *dst = kt + quarter * 32 * kKRow + 16 * h * kKRow + 4 * t;
         const uint32_t blk_at = block_at(0, hw >> 2, tile - c0);
-        unit_codes(ring + blk_at, unit_start(tile, 0, blk_at), t, gk, [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; });
+        const uint32_t at = unit_start(tile, 0, blk_at);
+        const auto put_codes = [&](int k, uint32_t c4) { *reinterpret_cast<uint32_t *>(dst + k * kKRow) = c4; };
+        if (WIDE) {
+            unit_codes(ring + blk_at, at, t, gk, put_codes);
+        } else {
+            UnitPacks packs;
+            uint32_t where[4];
+            narrow_packs(ring + blk_at + at, t, gk, packs.len, packs.mn, where);
+#pragma unroll
+            for (int i = 0; i < 4; i++) packs.word[i] = lds_load64(ring, blk_at + at + where[i]);
+            packs_codes(packs, put_codes);
+        }
     };
     auto parse_v = [&](int tile, uint32_t *tab) {          // where the unit's packs are
         const uint32_t blk_at = block_at(1, hw >> 2, tile - c0), at = unit_start(tile, 1, blk_at);
         const uint8_t *blk = ring + blk_at;
+        if (!WIDE) {                                       // (damaged fields reach 2 KiB behind what is staged, at K's codes)
+            uint32_t len[4], mn[4], where[4];
+            narrow_packs(blk + at, t, gv, len, mn, where);
+#pragma unroll
+            for (int i = 0; i < 4; i++) tab[(hw * 4 + i) * 32 + t] = (blk_at + at + where[i]) | (len[i] << 17) | (mn[i] << 21);
+            return;
+        }
         const uint32_t minsw = lds_meta_word(blk + at, t, gv.W), lensw = lds_meta_word(blk + at + gv.mins_bytes, t, gv.LB);
         uint32_t len[4], off[4], payload;
 #pragma unroll

@@ -102,6 +102,23 @@ __device__ __forceinline__ void pack_offsets(const uint32_t len[4], uint32_t off
     payload = t012 + (tb >> 16);
 }
 
+// Payload offsets (in 2-byte units) of a lane's four packs from their widths `lens_b` (one per
+// byte): a single packed scan over the 32 lanes of the half-wavefront.  A slot's widths sum to at
+// most 32 * 4 = 128, so the four running sums never carry into each other.
+__device__ __forceinline__ void pack_offsets8(uint32_t lens_b, uint32_t off2[4]) {
+    const uint32_t incl = half_incl_scan(lens_b);
+    const uint32_t excl = incl - lens_b;
+    // the four slot totals of this lane's half = the running sums of its lane 31: one cross-lane read on the LDS
+    // crossbar (bit-mask swizzle within 32 lanes: lane | 31), no memory access, no scalar round trip, and the slot
+    // bases are byte-select additions
+    const uint32_t tot = (uint32_t)__builtin_amdgcn_ds_swizzle((int)incl, 0x03E0);
+    const uint32_t a0 = tot & 0xFFu, a01 = a0 + ((tot >> 8) & 0xFFu), a012 = a01 + ((tot >> 16) & 0xFFu);
+    off2[0] = excl & 0xFFu;
+    off2[1] = ((excl >> 8) & 0xFFu) + a0;
+    off2[2] = ((excl >> 16) & 0xFFu) + a01;
+    off2[3] = (excl >> 24) + a012;
+}
+
 // 64 bits starting at byte offset `off` (2-byte aligned) of an LDS byte array whose base is
 // 4-byte aligned.  gfx950 does execute DS reads at any alignment, but a misaligned 64-bit read
 // stalls the LDS pipeline (SQ_LDS_UNALIGNED_STALL), so this reads the three aligned dwords that
