@@ -6,9 +6,8 @@
 // rounded once when it is stored; the angle is formed and reduced to a fraction of a turn in fp64 pairs, since at position 10^6
 // an fp32 angle is off by up to 0.06.  (The chain of library kernels rounds after the norm, the cosines and each product.)
 //
-// Bound by memory, and by the launch where rows are few: a row is read once and written once.  4 x 2048 tokens of 32 + 8 heads 31 us in a
-// loop over four sets of tensors, 37 with caches that hold none of them (a copy of the same bytes: 33); a decode step's write, 1 to 64
-// sequences, 5.2 us.  Eight lanes hold a row, each 8 channels of either half (two 16-byte
+// Bound by memory, and by the launch where rows are few: a row is read once and written once.  4 x 2048 tokens of 32 + 8 heads, caches
+// cold, 30 us (5.6 TB/s; a large copy 5.2); a decode step's write, 1 to 64 sequences, 5.3 us.  Eight lanes hold a row, each 8 channels of either half (two 16-byte
 // loads), so the sum of squares takes three exchanges and both halves of a pair are in one lane; a wavefront holds eight heads
 // of a token.  Lane i works out frequency i once for the wavefront, and the eight lanes of a row fetch theirs from LDS.
 #include "pkv_block.hpp"
@@ -58,9 +57,12 @@ template <bool WIDE> __device__ __forceinline__ void load8(const uint16_t *p, ui
 #pragma unroll
     for (int i = 0; i < 4; i++) w[i] = (uint32_t)p[2 * i] | ((uint32_t)p[2 * i + 1] << 16);
 }
-template <bool WIDE> __device__ __forceinline__ void store8(uint16_t *p, const uint32_t w[4]) {
+template <bool WIDE, bool PAST> __device__ __forceinline__ void store8(uint16_t *p, const uint32_t w[4]) {
+    typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
     if (WIDE) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        const u32x4 v = {w[0], w[1], w[2], w[3]};
+        if (PAST) __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>(p));
+        else *reinterpret_cast<u32x4 *>(p) = v;
         return;
     }
 #pragma unroll
@@ -79,8 +81,9 @@ __device__ __forceinline__ float turn_fraction(double pos, double freq) {
 }
 
 // One wavefront: `per` groups of eight heads of one token, the next group's rows on their way while one is turned.
-template <int DT, bool WIDE>
-__global__ void __launch_bounds__(256) norm_rotary_kernel(const RotaryParams p) {
+// PAST: what is stored does not stay in the caches.
+template <int DT, bool WIDE, bool PAST>
+__global__ void __launch_bounds__(256, 8) norm_rotary_kernel(const RotaryParams p) {
     __shared__ float2 turn_s[4][64];                         // (cos, sin) by frequency, one table a wavefront
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t unit = (uint64_t)blockIdx.x * 4u + (uint32_t)wave;
@@ -154,8 +157,8 @@ __global__ void __launch_bounds__(256) norm_rotary_kernel(const RotaryParams p) 
             }
         }
         if (r.mine) {
-            store8<WIDE>(r.out + c, r.lo);
-            store8<WIDE>(r.out + 64 + c, r.hi);
+            store8<WIDE, PAST>(r.out + c, r.lo);
+            store8<WIDE, PAST>(r.out + 64 + c, r.hi);
         }
     }
 }
@@ -202,17 +205,24 @@ extern "C" int pkv_norm_rotary(const pkv_rotary_args *a, pkv_stream_t s_) {
     // large copy 5.2); 2 x 1031 of 16 + 4, which are less than a round: 8.4 -> 8.7, 9.4, 9.4.
     const uint64_t rounds = tokens * p.groups / 8192;
     p.per = (int)(rounds < 1 ? 1 : rounds < p.groups ? rounds : p.groups);
+    // Results that no L2 would hold until they are read go past it, where they push out what is still to be read otherwise: 4 x 2048
+    // tokens (84 MB of results), caches cold, 37.3 -> 29.8 us, 2 x 1031 (10.5 MB) 7.75 -> 6.52; 64 x 1 (0.8 MB) 5.3 -> 5.4.  (Loads that way
+    // too: 32.8, alone 31.4.)
+    const bool past = tokens * (uint64_t)(a->Hq + (a->v ? 2 : 1) * a->Hkv) * 256u > (4u << 20);
     p.pieces = (p.groups + (uint32_t)p.per - 1u) / (uint32_t)p.per;
     p.units = tokens * p.pieces;
     const uint64_t wgs = (p.units + 3) / 4;
     PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x tokens x heads too large");
     const dim3 grid((unsigned)wgs);
     if (off & 15u) {
-        if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, false><<<grid, 256, 0, s>>>(p);
-        else norm_rotary_kernel<PKV_BF16, false><<<grid, 256, 0, s>>>(p);
+        if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, false, false><<<grid, 256, 0, s>>>(p);
+        else norm_rotary_kernel<PKV_BF16, false, false><<<grid, 256, 0, s>>>(p);
+    } else if (past) {
+        if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, true, true><<<grid, 256, 0, s>>>(p);
+        else norm_rotary_kernel<PKV_BF16, true, true><<<grid, 256, 0, s>>>(p);
     } else {
-        if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, true><<<grid, 256, 0, s>>>(p);
-        else norm_rotary_kernel<PKV_BF16, true><<<grid, 256, 0, s>>>(p);
+        if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, true, false><<<grid, 256, 0, s>>>(p);
+        else norm_rotary_kernel<PKV_BF16, true, false><<<grid, 256, 0, s>>>(p);
     }
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;
