@@ -25,13 +25,14 @@
 // side, since both halves of a pack's word take the same shifts.  Which pack is where comes from a table that the half-wavefronts
 // fill, one unit each (offset, width, minimum of its 128 packs).
 //
-// Bound by the vector instructions around the products: 32 tokens take a wavefront some 800 of them with 32 rows (of a tile: K's codes
-// to bytes 220, bytes to operands 65, V's table 100 and packs 180, scores to weights 150) and 730 with 64, which the vector units issue
-// in 67 % of the cycles.  Hence as few wavefronts as possible unpack the same block: up to 128 rows a workgroup, two groups of them
-// sharing K's bytes and V's table.  8 KV heads, 4-bit codes: 8 sequences x 4 queries of 32 heads over 16384 tokens 79 us (a copy of the
-// bytes: 22), 1024 queries over 32768 1010 us, 540 TFLOP/s (a large product reaches 1160), where 64 rows a workgroup without sharing
-// took 1430; 40 heads x 333 queries of two sequences over 4096 tokens in 5-bit codes 155 to 169 us; 3 queries over 1100 tokens 14 us,
-// 4 of them the merge.
+// Bound by the vector instructions around the products: 32 tokens take a wavefront some 770 of them with 32 rows (of a tile: K's codes
+// to bytes 210, bytes to operands 65, V's table 80 and packs 180, scores to weights 150), 70 less with 16, 730 with 64.  Hence as few
+// wavefronts as possible unpack the same block, up to 128 rows a workgroup, two groups of them sharing K's bytes and V's table; and
+// three workgroups a CU where rows are few (vector units busy 79 % of the cycles, 67 % with two).  8 KV heads, 4-bit codes: 8 sequences
+// x 4 queries of 32 heads over 16384 tokens 68.5 us (79 with two workgroups a CU, 74 with products of 32 rows; a copy of the bytes: 22),
+// 1024 queries over 32768 1010 us, 540 TFLOP/s (a large product reaches 1160), where 64 rows a workgroup without sharing took 1430;
+// 40 heads x 333 queries of two sequences over 4096 tokens in 5-bit codes 139 to 157 us; 3 queries over 1100 tokens 13 us, 4 of them the
+// merge.
 #include "pkv_block.hpp"
 #include "pkv_runtime.hpp"
 
@@ -41,6 +42,7 @@ typedef _Float16 h2v __attribute__((ext_vector_type(2)));
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 b8 __attribute__((ext_vector_type(8)));
 typedef float f16v __attribute__((ext_vector_type(16)));
+typedef float f4v __attribute__((ext_vector_type(4)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
 
 constexpr int kChunkTile = 128;
@@ -80,6 +82,11 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
 template <bool BF> __device__ __forceinline__ f16v product(u4 a, u4 b, f16v c) {
     if (BF) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+}
+
+template <bool BF> __device__ __forceinline__ f4v product16(u4 a, u4 b, f4v c) {
+    if (BF) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
 }
 
 // Two of four codes (one a byte) as halves.
@@ -172,11 +179,12 @@ __device__ __forceinline__ float softmax_step(f16v &y, float &m) {
     return __builtin_amdgcn_exp2f(was - m);
 }
 
-template <bool BF, int NB, int RG, bool WIDE>
+template <bool BF, int NB, int RG, bool WIDE, bool R16 = false>
 __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chunk_kernel(const ChunkParams p) {
     constexpr int NQ = WIDE ? 9 : 5;                       // 1 KiB steps that hold a staged block
     constexpr bool ONCE = RG == 1 && !WIDE;                // a tile's blocks are staged one at a time
-    constexpr int M = 32 * NB * RG, kKBufs = ONCE ? 1 : 2, kBufs = ONCE ? 1 : RG + 1, kSets = RG;
+    static_assert(!R16 || (ONCE && NB == 1), "sixteen rows: one workgroup's, narrow codes");
+    constexpr int M = R16 ? 16 : 32 * NB * RG, kKBufs = ONCE ? 1 : 2, kBufs = ONCE ? 1 : RG + 1, kSets = RG;
     constexpr bool COPY = !WIDE || RG == 2;                // blocks go to LDS without registers (what is staged lies below 64 KiB)
     extern __shared__ __align__(16) uint8_t lds[];
     uint8_t *ring = lds;                                   // staged: kKBufs tiles' K blocks, kBufs tiles' V blocks; window and end: V rows, sums (kt as well)
@@ -195,6 +203,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     const int rt = (int)(seq % (uint32_t)p.row_tiles), bh = (int)(group % (uint32_t)p.BH), split = (int)(group / (uint32_t)p.BH);
     const int b = bh / p.Hkv, hkv = bh % p.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, t = lane & 31;
+    const int tr = R16 ? lane & 15 : t, g = lane >> 4;     // this lane's row of a block; sixteen rows: its quarter of what the products add up
     const int rg = wave >> 2, quarter = wave & 3;          // rows, and tokens, of this wavefront
     const int T = p.T_c + p.T_w;
     const int row0 = rt * M, row_last = min(row0 + M, p.rows) - 1, mine0 = 32 * NB * rg;
@@ -204,7 +213,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     int row[NB], pos[NB];                                  // the lane's rows, and the last token that each sees
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        row[nb] = min(row0 + mine0 + 32 * nb + t, p.rows - 1);
+        row[nb] = min(row0 + mine0 + 32 * nb + tr, p.rows - 1);
         pos[nb] = p.causal ? T - p.n + row[nb] / p.G : T - 1;
     }
     auto q_row = [&](int r) -> const uint16_t * {
@@ -331,19 +340,23 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     __syncthreads();
     float qsum[NB];
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++) {                      // half the channels each
+    for (int nb = 0; nb < NB; nb++) {                      // half the channels each (a quarter)
         float s = 0.f;
 #pragma unroll
-        for (int c = 0; c < 8; c++) {
-            const h8 v = *reinterpret_cast<const h8 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * c + 16 * h);
+        for (int c = 0; c < (R16 ? 4 : 8); c++) {
+            const h8 v = *reinterpret_cast<const h8 *>(qt + (mine0 + 32 * nb + tr) * kQRow + (R16 ? 64 * c + 16 * g : 32 * c + 16 * h));
 #pragma unroll
             for (int k = 0; k < 8; k++) s += (float)v[k];
         }
+        if (R16) s += __shfl_xor(s, 16, 64);
         qsum[nb] = s + __shfl_xor(s, 32, 64);
     }
 
     f16v acc[NB][4];
+    f4v acc16[8];
     float m[NB], l[NB], z[NB];
+#pragma unroll
+    for (int c = 0; c < 8; c++) acc16[c] = (f4v){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
         m[nb] = kLowest; l[nb] = 0.f; z[nb] = 0.f;
@@ -516,6 +529,91 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
         }
     };
 
+    // Sixteen rows (R16): the same on 16x16x32 products, which leave no columns idle.  S^T's two products are tokens 0..7 and 8..15 of
+    // either pack, so that a lane's scores of the two are the pairs (j, j + 8) of an operand: packs g / 2, tokens 4 (g % 2) + i and that + 8.
+    // V is unpacked as above, a pack a lane; its halves change places between neighbouring rows of 16 lanes, which makes of 32 channels'
+    // packs the operands of 16 and 16.
+    const int base16 = 16 * (g >> 1) + 4 * (g & 1), tok16 = 16 * ((lane & 15) >> 3) + (lane & 7);
+    auto weights_of_16 = [&](int tile, const uint8_t *kt, const float2 *par, float grow, u4 &w) {
+        const int tok0 = tile * kChunkTile + 32 * quarter;
+        kt += quarter * 32 * kKRow;
+        const float2 *par_s = par + quarter * 32 + base16, *par_w = par_s + 128;
+        f4v y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            const u4 b = *reinterpret_cast<const u4 *>(qt + tr * kQRow + 64 * s + 16 * g);
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                const uint2 c8 = *reinterpret_cast<const uint2 *>(kt + (tok16 + 8 * n) * kKRow + 32 * s + 8 * g);
+                const u4 a = {codes_f16(c8.x, 0x04010400u), codes_f16(c8.x, 0x04030402u), codes_f16(c8.y, 0x04010400u), codes_f16(c8.y, 0x04030402u)};
+                y[n] = product16<false>(a, b, y[n]);
+            }
+        }
+        const float ref = m[0] == kLowest ? 0.f : m[0];
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float2 q2 = par_s[8 * n + i];
+                y[n][i] = fmaf(y[n][i], q2.x, fmaf(q2.y, qsum[0], -ref));
+            }
+        if (tok0 + 31 > pos_first || tok0 < start) {
+            int up_to = pos[0] - (tok0 + base16), from = start - (tok0 + base16);
+            asm volatile("" : "+v"(up_to), "+v"(from));
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) y[n][i] = 8 * n + i > up_to || 8 * n + i < from ? -INFINITY : y[n][i];
+        }
+        float over = y[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) over = fmaxf(over, y[i >> 2][i & 3]);
+        if (__any(over > 8.f || m[0] == kLowest) || grow != 1.f) {
+            over = fmaxf(over, __shfl_xor(over, 16, 64));
+            over = fmaxf(over, __shfl_xor(over, 32, 64));
+            const bool none = m[0] == kLowest;
+            const float raise = over > 8.f || (none && over > -INFINITY) ? over : 0.f;
+            if (raise != 0.f || (none && over == 0.f)) m[0] = ref + raise;
+            const float alpha = none ? 1.f : __builtin_amdgcn_exp2f(-raise);
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i >> 2][i & 3] -= raise;
+            l[0] *= alpha;
+            z[0] *= alpha * grow;
+#pragma unroll
+            for (int c = 0; c < 8; c++) acc16[c] *= alpha * grow;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 pa = par_w[i], pb = par_w[i + 8];
+            const float a = __builtin_amdgcn_exp2f(y[0][i]), d = __builtin_amdgcn_exp2f(y[1][i]);
+            l[0] += a;
+            l[0] += d;
+            uint32_t f = pack_f16(a * pa.x, d * pb.x);
+            asm("" : "+v"(f));
+            const h2v f2 = __builtin_bit_cast(h2v, f);
+            z[0] = fmaf((float)f2[0], pa.y, z[0]);
+            z[0] = fmaf((float)f2[1], pb.y, z[0]);
+            w[i] = f;
+        }
+    };
+    auto add_values_16 = [&](const uint32_t *tab, const u4 &w) {
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            const uint32_t e = tab[((((c >> 1) * 4 + (c & 1) * 2 + (quarter >> 1)) * 4) + 2 * (quarter & 1) + h) * 32 + t];
+            uint32_t v[8];
+            pack_operand<false>(ring, e, v);
+            u4 lo, hi;
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const auto both = __builtin_amdgcn_permlane16_swap(v[i], v[4 + i], false, false);
+                lo[i] = both[0];
+                hi[i] = both[1];
+            }
+            acc16[2 * c] = product16<false>(lo, w, acc16[2 * c]);
+            acc16[2 * c + 1] = product16<false>(hi, w, acc16[2 * c + 1]);
+        }
+    };
+
     // ---- compressed tiles ----
     const auto lds_barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };      // (copies go on)
     if (ONCE) {
@@ -531,7 +629,8 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
             unpack_k(tile, kt_all);
             wave_lds_order();
             u4 w[NB][2];
-            weights_of(tile, kt_all, par_all, grow, w);
+            if constexpr (R16) weights_of_16(tile, kt_all, par_all, grow, w[0][0]);
+            else weights_of(tile, kt_all, par_all, grow, w);
             put(tile);
             lds_barrier();
             if (tile + 1 < c1) {
@@ -540,7 +639,8 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
             }
             parse_v(tile, tab_all);
             lds_barrier();
-            add_values(tab_all, w);
+            if constexpr (R16) add_values_16(tab_all, w[0][0]);
+            else add_values(tab_all, w);
         }
     } else if (RG == 1) {
         // Few rows: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
@@ -609,6 +709,8 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
 #pragma unroll
                     for (int r = 0; r < 16; r++) acc[nb][c][r] = acc[nb][c][r] * unit * kUp;
             }
+#pragma unroll
+            for (int c = 0; c < 8; c++) acc16[c] = acc16[c] * unit * kUp;
         }
         unit = 1.f / kUp;
         uint8_t *vt = ring + wave * 32 * kVRow;            // (into the K codes' place, where two groups of rows need it)
@@ -627,6 +729,54 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
                 uint2 *dst = reinterpret_cast<uint2 *>(vt + k * kVRow + 16 * c);
                 dst[0] = real ? a : make_uint2(0u, 0u);
                 dst[1] = real ? d : make_uint2(0u, 0u);
+            }
+            if constexpr (R16) {
+                f4v y[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+                const uint16_t *kw = late->k_win + (size_t)bh * late->win_stride * kHeadDim + 8 * g;
+                const uint16_t *qr = late->q + (int64_t)b * late->q_b + (int64_t)(hkv * late->G + row[0] % late->G) * late->q_h + (int64_t)(row[0] / late->G) * late->q_t;
+#pragma unroll
+                for (int s = 0; s < 4; s++) {
+                    const u4 x = BF ? *reinterpret_cast<const u4 *>(qr + 32 * s + 8 * g) : *reinterpret_cast<const u4 *>(qt + tr * kQRow + 64 * s + 16 * g);
+#pragma unroll
+                    for (int n = 0; n < 2; n++)
+                        y[n] = product16<BF>(*reinterpret_cast<const u4 *>(kw + (size_t)min(r0 + tok16 + 8 * n, late->T_w - 1) * kHeadDim + 32 * s), x, y[n]);
+                }
+                float most = -INFINITY;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const int tok = tok0 + base16 + 8 * (i >> 2) + (i & 3);
+                    const float x = tok > pos[0] || tok < start ? -INFINITY : y[i >> 2][i & 3] * late->sm_log2;
+                    y[i >> 2][i & 3] = x;
+                    most = fmaxf(most, x);
+                }
+                most = fmaxf(most, __shfl_xor(most, 16, 64));
+                most = fmaxf(most, __shfl_xor(most, 32, 64));
+                const float was = m[0];
+                m[0] = fmaxf(was, most);
+                const float alpha = __builtin_amdgcn_exp2f(was - m[0]);
+                l[0] *= alpha;
+                z[0] *= alpha;
+#pragma unroll
+                for (int c = 0; c < 8; c++) acc16[c] *= alpha;
+                u4 w, wl;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float a = __builtin_amdgcn_exp2f(y[0][i] - m[0]), d = __builtin_amdgcn_exp2f(y[1][i] - m[0]);
+                    l[0] += a + d;
+                    w[i] = BF ? pack_bf16(a, d) : pack_f16(a * kUp, d * kUp);
+                    wl[i] = BF ? pack_bf16(a - __uint_as_float(w[i] << 16), d - __uint_as_float(w[i] & 0xFFFF0000u)) : 0u;
+                }
+                wave_lds_order();
+#pragma unroll
+                for (int c = 0; c < 8; c++) {
+                    const uint16_t *col = reinterpret_cast<const uint16_t *>(vt + base16 * kVRow) + 16 * c + (lane & 15);
+                    u4 v;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) v[i] = (uint32_t)col[i * (kVRow / 2)] | ((uint32_t)col[(i + 8) * (kVRow / 2)] << 16);
+                    acc16[c] = product16<BF>(v, w, acc16[c]);
+                    if (BF) acc16[c] = product16<BF>(v, wl, acc16[c]);
+                }
+                continue;
             }
             f16v y[NB];
 #pragma unroll
@@ -691,20 +841,26 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     // ---- the states of a row's four wavefronts become one ----
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
+        if (R16) {
+            l[nb] += __shfl_xor(l[nb], 16, 64);
+            z[nb] += __shfl_xor(z[nb], 16, 64);
+        }
         l[nb] += __shfl_xor(l[nb], 32, 64);
         z[nb] += __shfl_xor(z[nb], 32, 64);
-        if (h == 0) st[quarter * M + mine0 + 32 * nb + t] = m[nb];
+        if (R16 ? g == 0 : h == 0) st[quarter * M + mine0 + 32 * nb + tr] = m[nb];
     }
     __syncthreads();
     float *sums = st + 4 * M;
     float top[NB];
 #pragma unroll
     for (int nb = 0; nb < NB; nb++) {
-        const float *at = st + mine0 + 32 * nb + t;
+        const float *at = st + mine0 + 32 * nb + tr;
         top[nb] = fmaxf(fmaxf(at[0], at[M]), fmaxf(at[2 * M], at[3 * M]));
         const float f = __builtin_amdgcn_exp2f(m[nb] - top[nb]);
-        if (h == 0) sums[quarter * M + mine0 + 32 * nb + t] = l[nb] * f;
+        if (R16 ? g == 0 : h == 0) sums[quarter * M + mine0 + 32 * nb + tr] = l[nb] * f;
         const float fu = f * unit;
+#pragma unroll
+        for (int c = 0; c < 8; c++) acc16[c] = (acc16[c] + z[nb]) * fu;
 #pragma unroll
         for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -717,7 +873,15 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
         float *mine = buf0 + (quarter & 1) * 32 * kSumRow + t * kSumRow + 4 * h;
 #pragma unroll
         for (int step = 0; step < 2; step++) {
-            if ((quarter >> 1) == step) {
+            if ((quarter >> 1) == step && R16) {
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        float *at = buf0 + (quarter & 1) * 32 * kSumRow + tr * kSumRow + 16 * c + 4 * g + i;
+                        *at = step ? *at + acc16[c][i] : acc16[c][i];
+                    }
+            } else if ((quarter >> 1) == step) {
 #pragma unroll
                 for (int c = 0; c < 4; c++)
 #pragma unroll
@@ -801,7 +965,7 @@ static uint32_t chunk_ring(const pkv_chunk_args *a, int rg, uint32_t &slot_k, ui
 // the small kind (wide codes: two), one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
 // partials as one.
 struct ChunkCut {
-    int nb, rg, row_tiles, tiles, run, nsplit;
+    int nb, rg, r16, row_tiles, tiles, run, nsplit;
 };
 static ChunkCut chunk_cut(const pkv_chunk_args *a) {
     ChunkCut c;
@@ -809,6 +973,7 @@ static ChunkCut chunk_cut(const pkv_chunk_args *a) {
     uint32_t slot_k, slot_v;
     c.rg = rows <= 32 || chunk_ring(a, 2, slot_k, slot_v) > 63u * 1024u ? 1 : 2;     // (copies reach 64 KiB: not widths of 6 and more on both sides)
     c.nb = c.rg == 1 || rows <= 64 ? 1 : 2;
+    c.r16 = rows <= 16 && !chunk_wide(a);                  // 1 x 4 queries of 32 + 8 heads over 131072 tokens 75 us, with 32 rows 82; over 4096 16.5 and 17.3
     const int64_t m = 32 * c.nb * c.rg;
     c.row_tiles = (int)((rows + m - 1) / m);
     c.tiles = a->T_c / kChunkTile + (a->T_w + kChunkTile - 1) / kChunkTile;
@@ -892,7 +1057,7 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     p.k_bits = a->T_c ? a->k_bits : 2; p.v_bits = a->T_c ? a->v_bits : 2;
     p.tiles_c = a->T_c / kChunkTile;
     p.sm_log2 = a->sm_scale * kLog2e;
-    const uint32_t rg = (uint32_t)cut.rg, m = 32u * (uint32_t)cut.nb * rg, kt = rg * 4u * 32u * kKRow;
+    const uint32_t rg = (uint32_t)cut.rg, m = cut.r16 ? 16u : 32u * (uint32_t)cut.nb * rg, kt = rg * 4u * 32u * kKRow;
     p.ring = chunk_ring(a, cut.rg, p.slot_k, p.slot_v);
     if (p.ring + kt < 4u * rg * 32u * kVRow) p.ring = 4u * rg * 32u * kVRow - kt;      // (the end's sums take less: rg * 2 x 32 x 129 floats)
     const bool wide = chunk_wide(a), bf = a->dtype == PKV_BF16;
@@ -904,6 +1069,7 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
                                     {PKV_CHUNK(true, 1, 1), PKV_CHUNK(true, 1, 2), PKV_CHUNK(true, 2, 2)}};
 #undef PKV_CHUNK
     const void *kernel = kernels[bf][cut.rg - 1 + cut.nb - 1][wide];
+    if (cut.r16) kernel = bf ? (const void *)attn_chunk_kernel<true, 1, 1, false, true> : (const void *)attn_chunk_kernel<false, 1, 1, false, true>;
     PKV_HIP_CHECK(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
     void *params[] = {&p};
     PKV_HIP_CHECK(hipLaunchKernel(kernel, dim3((unsigned)wgs), dim3(256u * rg), params, lds, s));

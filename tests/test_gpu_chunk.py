@@ -68,7 +68,8 @@ def test_every_width(cuda, k_bits, v_bits, B, Hq, Hkv, n, T):
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
 @pytest.mark.parametrize("n,T,W,starts", [(5, 512, 40, (0, 551, 552, 300)), (300, 256, 100, (128, 127, 256, 356)), (40, 0, 90, (89, 90, 1000, 50)),
-                                          (64, 384, 0, (-5, 383, 320, 384))])
+                                          (64, 384, 0, (-5, 383, 320, 384)), (3, 512, 40, (0, 551, 552, 300)), (4, 256, 0, (255, 256, 100, 3)),
+                                          (2, 0, 170, (169, 170, 33, 1)), (1, 256, 129, (384, 385, 256, 0)), (8, 256, 20, (270, 275, 276, 31))])
 def test_padding_on_the_left(cuda, dtype, n, T, W, starts):
     """Starts in streams and window, on and off tile borders, rows that see one token and rows that see none; what lies in the
     padding is NaN or infinite."""
@@ -93,10 +94,10 @@ def test_padding_on_the_left(cuda, dtype, n, T, W, starts):
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("n,W", [(9, 40), (60, 61)])
+@pytest.mark.parametrize("n,W", [(9, 40), (60, 61), (6, 70)])
 def test_queries_in_the_padding_and_broken_ones(cuda, dtype, n, W):
     """Queries of padded places, and those of one head that are infinite or NaN, leave every other row as it was."""
-    B, Hq, Hkv, T = 2, 8, 2, 256
+    B, Hq, Hkv, T = 2, 8, 4 if n < 9 else 2, 256
     q, ke, ve, kw, vw = _case(cuda, B, Hq, Hkv, n, T, W, dtype, seed=9)
     st = torch.tensor([T + W - n + 4, 0], dtype=torch.int32, device=cuda)
     want = ops.attn_chunk(q, ke, ve, kw, vw, win_len=W, starts=st)
@@ -267,3 +268,19 @@ def test_windows_and_queries_further_apart_than_32_bits(cuda):
     far_q, out = (flat.as_strided(q.shape, (1 << 31, n * 128, 128, 1), at) for at in (0, 4096))
     far_q.copy_(q)
     assert torch.equal(ops.attn_chunk(far_q, None, None, *big, win_len=W, out=out), want) and torch.equal(out, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("Hq,Hkv,n", [(8, 2, 4), (5, 1, 3), (8, 2, 5), (6, 6, 2), (17, 1, 1), (16, 1, 1)])
+def test_few_rows_and_scales_of_far_apart_sizes(cuda, dtype, Hq, Hkv, n):
+    """Up to and over sixteen rows a KV head, with and without the causal mask; values' scales that grow and fall over the tokens."""
+    B, T, W = 2, 1024, 50
+    q, ke, ve, kw, vw = _case(cuda, B, Hq, Hkv, n, T, W, dtype, seed=Hq + n)
+    span = 2.0 ** torch.linspace(-9, 9, T, device=cuda)
+    for order in (1, -1):
+        ve2 = dict(ve, scale=(ve["scale"].float() * (span if order > 0 else span.flip(0))).to(dtype))
+        q2 = q.clone()
+        q2[:, 0] *= 7
+        K, V, size = _values(ke, ve2, kw, vw, B, Hkv, W)
+        co.check(ops.attn_chunk(q2, ke, ve2, kw, vw, win_len=W), q2, K, V, **size)
+        co.check(ops.attn_chunk(q2, ke, ve2, kw, vw, win_len=W, causal=False, sm_scale=0.2), q2, K, V, causal=False, sm=0.2, **size)
