@@ -11,10 +11,10 @@
 // apart at 10^-13 of its mass, against 2^-24 of the uniform numbers.
 //
 // A row is read three times: its maximum, the histogram, the gathering.  Many rows are bound by the histogram's instructions and LDS
-// atomics (vector units 53 % busy, LDS 28 %), not by bytes: 256 rows of 151936 in bf16 79 us, 71 with top-k 50, 92 with top-p 0.9 (more
+// atomics (vector units 53 % busy, LDS 28 %), not by bytes: 256 rows of 151936 in bf16 80 us, 69 with top-k 50, 91 with top-p 0.9 (more
 // candidates), 88 with settings of every kind, where reading them once takes 15; held in registers between the passes the rows took 2 %
-// less, not worth a second way of reading.  Few rows are bound by the latency of what follows one another: a row of 151936 24 us in three
-// launches (3 + 13 + 9), a row of temperature 0 8.5 us.
+// less, not worth a second way of reading.  Few rows are bound by the latency of what follows one another: a row of 151936 20.5 us in three
+// launches (3 + 12 + 6), a row of temperature 0 8.5 us.
 #include "pkv_block.hpp"
 #include "pkv_runtime.hpp"
 
@@ -210,26 +210,44 @@ __device__ __forceinline__ Prefix block_scan(SampleLds &s, Prefix v) {
     __syncthreads();
     if (lane == 63) { s.wave_mass[wave] = v.mass; s.wave_count[wave] = v.count; }
     __syncthreads();
-    for (int w = 0; w < wave; w++) { v.mass += s.wave_mass[w]; v.count += s.wave_count[w]; }
+#pragma unroll 5
+    for (int w = 0; w < kSampThreads / 64 - 1; w++) {      // (five are read at once)
+        const uint64_t m = s.wave_mass[w];
+        const uint32_t c = s.wave_count[w];
+        v.mass += w < wave ? m : 0ull;
+        v.count += w < wave ? c : 0u;
+    }
     return v;
 }
-// The histogram becomes inclusive sums, and at[] is made ready for the searches.
-__device__ __forceinline__ void scan_bins(SampleLds &s) {
+// A thread's own bins' inclusive sums; [0]: what lies in front of them.
+struct MyBins { uint64_t mass[kMine + 1]; uint32_t count[kMine + 1]; };
+// The histogram, load(bin, mass, count), becomes inclusive sums in s.mass and s.count, and at[] is made ready for the searches.
+template <class F> __device__ __forceinline__ MyBins scan_bins(SampleLds &s, F load) {
     const int b = kMine * threadIdx.x;
-    uint64_t m[kMine];
-    uint32_t c[kMine];
+    MyBins r;
+    r.mass[0] = 0;
+    r.count[0] = 0;
 #pragma unroll
-    for (int i = 0; i < kMine; i++) {
-        m[i] = s.mass[b + i] + (i ? m[i - 1] : 0ull);
-        c[i] = s.count[b + i] + (i ? c[i - 1] : 0u);
-    }
-    const Prefix v = block_scan(s, Prefix{m[kMine - 1], c[kMine - 1]});
-    const uint64_t m0 = v.mass - m[kMine - 1];
-    const uint32_t c0 = v.count - c[kMine - 1];
+    for (int i = 0; i < kMine; i++) load(b + i, r.mass[i + 1], r.count[i + 1]);
 #pragma unroll
-    for (int i = 0; i < kMine; i++) { s.mass[b + i] = m0 + m[i]; s.count[b + i] = c0 + c[i]; }
+    for (int i = 0; i < kMine; i++) { r.mass[i + 1] += r.mass[i]; r.count[i + 1] += r.count[i]; }
+    const Prefix v = block_scan(s, Prefix{r.mass[kMine], r.count[kMine]});
+    const uint64_t m0 = v.mass - r.mass[kMine];
+    const uint32_t c0 = v.count - r.count[kMine];
+#pragma unroll
+    for (int i = 0; i <= kMine; i++) { r.mass[i] += m0; r.count[i] += c0; }
+#pragma unroll
+    for (int i = 0; i < kMine; i++) { s.mass[b + i] = r.mass[i + 1]; s.count[b + i] = r.count[i + 1]; }
     if (threadIdx.x < 8) s.at[threadIdx.x] = kBins;
     __syncthreads();
+    return r;
+}
+// at[slot] = the first bin whose inclusive sums satisfy the condition, out of registers; there behind the next barrier.
+template <class F> __device__ __forceinline__ void search_mine(SampleLds &s, int slot, const MyBins &mine, F holds) {
+    if (!holds(mine.mass[kMine], mine.count[kMine]) || (threadIdx.x && holds(mine.mass[0], mine.count[0]))) return;
+#pragma unroll
+    for (int i = kMine - 1; i >= 0; i--)
+        if (holds(mine.mass[i + 1], mine.count[i + 1])) s.at[slot] = kMine * threadIdx.x + i;
 }
 // at[slot] = the first bin whose inclusive sum satisfies the condition (kBins: none); there behind the next barrier.
 template <class F> __device__ __forceinline__ void search_bin(SampleLds &s, int slot, F holds) {
@@ -259,7 +277,7 @@ __device__ __forceinline__ void order_spans(Span &a, Span &b) {            // th
 }
 // Which bins the answer depends on one by one, from the scanned histogram: the one that the k-th token is in, those in which the last
 // kept token can be, those in which the draw can fall.  The same in every thread.
-__device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, float top) {
+__device__ __forceinline__ RowPlan make_plan(SampleLds &s, const MyBins &mine, const RowRule &r, float top) {
     RowPlan p;
     p.top = top;
     const uint64_t all = s.mass[kBins - 1];
@@ -268,7 +286,7 @@ __device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, flo
     p.k_limits = r.top_k && r.top_k < s.count[kBins - 1];  // (of the tokens that have mass)
     uint64_t k_low = all, k_high = all;                    // mass of the k tokens, between these
     if (p.k_limits) {
-        search_bin(s, 0, [&](int i) { return s.count[i] >= r.top_k; });
+        search_mine(s, 0, mine, [&](uint64_t, uint32_t c) { return c >= r.top_k; });
         __syncthreads();
         const int b = s.at[0];
         p.k_inside = s.count[b] != r.top_k;
@@ -280,8 +298,8 @@ __device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, flo
     int low = k_bin, high = k_bin;                         // the bins in which the last kept token can be (kBins: all are kept)
     if (r.by_p) {
         const double from = r.top_p * (double)k_low, to = r.top_p * (double)k_high;
-        search_bin(s, 1, [&](int i) { return s.count[i] && (double)s.mass[i] >= from; });
-        search_bin(s, 2, [&](int i) { return s.count[i] && (double)s.mass[i] >= to; });
+        search_mine(s, 1, mine, [&](uint64_t m, uint32_t c) { return c && (double)m >= from; });
+        search_mine(s, 2, mine, [&](uint64_t m, uint32_t c) { return c && (double)m >= to; });
         __syncthreads();
         low = min(low, s.at[1]);
         high = min(high, s.at[2]);
@@ -295,8 +313,8 @@ __device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, flo
     const bool whole = high >= kBins || (high == k_bin && !p.k_inside);    // the last bin that can hold a kept token is kept as a whole
     const uint64_t high_mass = high >= kBins ? all : whole ? mass_before(s, high) : s.mass[high];
     const double from = r.u * (double)max(p.low_mass, (1ull << kFracBits) - 1ull), to = r.u * (double)max(high_mass, 1ull << kFracBits);
-    search_bin(s, 3, [&](int i) { return (double)s.mass[i] > from; });
-    search_bin(s, 4, [&](int i) { return (double)s.mass[i] > to; });
+    search_mine(s, 3, mine, [&](uint64_t m, uint32_t) { return (double)m > from; });
+    search_mine(s, 4, mine, [&](uint64_t m, uint32_t) { return (double)m > to; });
     __syncthreads();
     p.span[0].from = k_bin; p.span[0].to = p.k_inside ? k_bin : -1;
     p.span[1].from = low; p.span[1].to = r.by_p || by_min ? min(whole ? high - 1 : high, kBins - 1) : -1;
@@ -319,8 +337,46 @@ __device__ __forceinline__ RowPlan make_plan(SampleLds &s, const RowRule &r, flo
     return p;
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d) {
-    return ((uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, d, 64);
+// The value of lane ^ J, without LDS.
+template <int J> __device__ __forceinline__ uint32_t lane_xor(uint32_t v) {
+    if (J == 1) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xF, 0xF, true);             // (quads 1 0 3 2)
+    if (J == 2) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xF, 0xF, true);             // (2 3 0 1)
+    if (J == 4) return (uint32_t)__builtin_amdgcn_update_dpp(0, __builtin_amdgcn_update_dpp(0, (int)v, 0x141, 0xF, 0xF, true), 0x1B, 0xF, 0xF, true);   // (7 - i, then 3 - i)
+    if (J == 8) return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xF, 0xF, true);            // (rows of 16 turned by 8)
+    if (J == 16) {
+        const auto both = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+        return threadIdx.x & 16 ? both[0] : both[1];
+    }
+    const auto both = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return threadIdx.x & 32 ? both[0] : both[1];
+}
+template <int J> __device__ __forceinline__ uint64_t lane_xor64(uint64_t v) {
+    return ((uint64_t)lane_xor<J>((uint32_t)(v >> 32)) << 32) | lane_xor<J>((uint32_t)v);
+}
+__device__ __forceinline__ uint64_t wave_max(uint64_t v) {
+    v = max(v, lane_xor64<1>(v));
+    v = max(v, lane_xor64<2>(v));
+    v = max(v, lane_xor64<4>(v));
+    v = max(v, lane_xor64<8>(v));
+    v = max(v, lane_xor64<16>(v));
+    return max(v, lane_xor64<32>(v));
+}
+// A wavefront's 64 keys in ascending order.
+template <int K, int J> __device__ __forceinline__ void sort_step(uint64_t &key) {
+    const int lane = threadIdx.x & 63;
+    const uint64_t other = lane_xor64<J>(key);
+    const bool low = ((lane & J) == 0) == ((lane & K) == 0);
+    key = (other < key) == low ? other : key;
+    if constexpr (J > 1) sort_step<K, J / 2>(key);
+}
+__device__ __forceinline__ uint64_t sort_wave(uint64_t key) {
+    sort_step<2, 1>(key);
+    sort_step<4, 2>(key);
+    sort_step<8, 4>(key);
+    sort_step<16, 8>(key);
+    sort_step<32, 16>(key);
+    sort_step<64, 32>(key);
+    return key;
 }
 // The keys s.cand[0 .. n) in ascending order, there or in s.mass.  A wavefront sorts 64 in registers; then runs are merged in pairs, a
 // key's place being its own in its run plus how many of the other run are smaller, which a search finds: a barrier for each doubling,
@@ -329,15 +385,7 @@ __device__ __forceinline__ const uint64_t *sort_candidates(SampleLds &s, uint32_
     const int lane = threadIdx.x & 63;
     const uint32_t chunks = (n + 63) / 64, all = 64 * chunks;
     for (uint32_t c = threadIdx.x >> 6; c < chunks; c += kSampThreads / 64) {
-        uint64_t key = 64 * c + lane < n ? s.cand[64 * c + lane] : ~0ull;
-#pragma unroll
-        for (int k = 2; k <= 64; k <<= 1)
-#pragma unroll
-            for (int j = k >> 1; j; j >>= 1) {
-                const uint64_t other = shfl_xor64(key, j);
-                const bool low = ((lane & j) == 0) == ((lane & k) == 0);
-                key = (other < key) == low ? other : key;
-            }
+        const uint64_t key = sort_wave(64 * c + lane < n ? s.cand[64 * c + lane] : ~0ull);
         s.cand[64 * c + lane] = key;
     }
     __syncthreads();
@@ -372,6 +420,33 @@ __device__ __forceinline__ void answer(const SampleParams &p, int row, uint64_t 
 // there, so a candidate's rank and the mass in front of it are its span's plus those of the candidates of its span in front of it.
 __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p, int row, const RowRule &r, const RowPlan &plan) {
     const uint32_t n = plan.gathered;
+    if (n <= 64) {                                         // one wavefront, a candidate a lane
+        if (threadIdx.x >= 64) return;
+        const int lane = threadIdx.x;
+        const bool here = (uint32_t)lane < n;
+        const uint64_t key = sort_wave(here ? s.cand[lane] : ~0ull);
+        const double y = here ? place_of(key_logit(key), plan.top, r) : 0.0;
+        const int bin = bin_of(y);
+        const uint64_t w = here ? weight_of(s.base, y, bin) : 0ull;
+        uint64_t sum = w;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint64_t m = shfl_up64(sum, d);
+            if (lane >= d) sum += m;
+        }
+        const Span &a = plan.span[0], &b = plan.span[1], &c = plan.span[2];
+        const bool in_a = a.from <= a.to && bin <= a.to, in_b = !in_a && b.from <= b.to && bin <= b.to;
+        const uint32_t rank = (uint32_t)lane + (in_a ? a.count : in_b ? b.count - a.size : c.count - a.size - b.size);
+        const uint64_t upto = sum + (in_a ? a.mass : in_b ? b.mass - a.total : c.mass - a.total - b.total), front = upto - w;
+        uint64_t k_mass = plan.k_mass;
+        if (plan.k_inside) k_mass = max(k_mass, wave_max(here && rank + 1 == r.top_k ? upto : 0ull));
+        const bool kept = here && (!plan.k_limits || rank < r.top_k) && (!r.by_p || rank == 0 || (double)front < r.top_p * (double)k_mass) &&
+                          (!r.by_min || y <= r.last);
+        const uint64_t total = max(plan.low_mass, wave_max(kept ? upto : 0ull));
+        const uint64_t hit = __ballot(kept && (double)upto > r.u * (double)total);
+        if (lane == (hit ? __ffsll((unsigned long long)hit) - 1 : 0)) answer(p, row, key, plan.top, r, total);
+        return;
+    }
     uint64_t key[kMine], w[kMine], front[kMine];
     int bin[kMine];
     double y[kMine];
@@ -415,8 +490,7 @@ __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p,
     }
     const bool any = kMine * (threadIdx.x & ~63u) < n;     // (uniform)
     if (any) {
-#pragma unroll
-        for (int d = 32; d; d >>= 1) most = max(most, shfl_xor64(most, d));
+        most = wave_max(most);
         if ((threadIdx.x & 63) == 0) atomicMax((unsigned long long *)&s.sums[1], (unsigned long long)most);
     }
     __syncthreads();
@@ -427,8 +501,7 @@ __device__ __forceinline__ void resolve_few(SampleLds &s, const SampleParams &p,
 #pragma unroll
         for (int e = kMine - 1; e >= 0; e--)
             if (kept[e] && (double)(front[e] + w[e]) > target) best = key[e];
-#pragma unroll
-        for (int d = 32; d; d >>= 1) best = min(best, shfl_xor64(best, d));
+        best = ~wave_max(~best);
         if ((threadIdx.x & 63) == 0) atomicMin((unsigned long long *)&s.best, (unsigned long long)best);
     }
     __syncthreads();
@@ -544,7 +617,7 @@ __device__ __forceinline__ void resolve_many(SampleLds &s, const SampleParams &p
             });
 #pragma unroll
             for (int d = 32; d; d >>= 1) {
-                sum += shfl_xor64(sum, d);
+                sum += ((uint64_t)(uint32_t)__shfl_xor((int)(uint32_t)(sum >> 32), d, 64) << 32) + (uint32_t)__shfl_xor((int)(uint32_t)sum, d, 64);
                 here += (uint32_t)__shfl_xor((int)here, d, 64);
             }
             if ((threadIdx.x & 63) == 0) {
@@ -777,10 +850,8 @@ __global__ void __launch_bounds__(kSampThreads) slice_histogram_kernel(const Sam
             atomicAdd(&st.count[i], s.count[i]);
         }
     if (!last_to_arrive(s, &st.arrived[0])) return;
-    for (int i = threadIdx.x; i < kBins; i += kSampThreads) { s.mass[i] = far_load(&st.mass[i]); s.count[i] = far_load(&st.count[i]); }
-    __syncthreads();
-    scan_bins(s);
-    const RowPlan plan = make_plan(s, r, top);
+    const MyBins mine = scan_bins(s, [&](int i, uint64_t &m, uint32_t &c) { m = far_load(&st.mass[i]); c = far_load(&st.count[i]); });
+    const RowPlan plan = make_plan(s, mine, r, top);
     if (threadIdx.x == 0) st.plan = plan;
     if (plan.gathered > kCand)                             // (sums from here on)
         for (int i = threadIdx.x; i < kBins; i += kSampThreads) { st.mass[i] = s.mass[i]; st.count[i] = s.count[i]; }
@@ -840,8 +911,8 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
     if (threadIdx.x == 0) { s.top = top; s.n_cand = 0; }
     fill_base(s);
     histogram<DT>(s, p, r, base, phase, 0, pieces, top);
-    scan_bins(s);
-    const RowPlan plan = make_plan(s, r, top);
+    const MyBins mine = scan_bins(s, [&](int i, uint64_t &m, uint32_t &c) { m = s.mass[i]; c = s.count[i]; });
+    const RowPlan plan = make_plan(s, mine, r, top);
     if (plan.gathered > kCand) {
         resolve_many<DT>(s, p, row, r, plan);
         return;
@@ -853,14 +924,14 @@ __global__ void __launch_bounds__(kSampThreads) sample_rows_kernel(const SampleP
 }
 
 // Slices a row: as many as make one round of 256 workgroups (one a CU), of 4096 logits or more.  A workgroup for the whole row (one
-// launch) where slices would take fewer than 28 k of the row's logits off it.  us, fp32, no filters, one workgroup / slices:
-// 1 x 32003 25.7 / 23.8, 64 x 32003 26.3 / 30.3, 128 x 50257 36.7 / 39.8, 128 x 65537 44.2 / 45.3, 64 x 65537 40.2 / 35.1,
-// 1 x 65537 38.8 / 23.6, 64 x 151936 80.8 / 49.9, 1 x 151936 70.8 / 23.8; 200 x 151936 95.4 / (two rounds) 124.
+// launch) where slices would take fewer than 44 k of the row's logits off it.  us, fp32, no filters, one workgroup / slices:
+// 1 x 32003 19.6 / 18.9, 64 x 32003 19.9 / 25.5, 64 x 50257 26.0 / 27.5, 128 x 65537 36.4 / 40.8, 128 x 100003 51.6 / 53.9,
+// 1 x 50257 23.9 / 18.4, 64 x 65537 31.0 / 29.2, 64 x 151936 69.6 / 45.8, 1 x 151936 56.5 / 19.2; 200 x 151936 83.4 / (two rounds) 111.
 static int sample_slices(const pkv_sample_args *a) {
     int g = 256 / a->rows;
     g = g < a->vocab / 4096 ? g : a->vocab / 4096;
     g = g < kMaxSlices ? g : kMaxSlices;
-    return g < 2 || a->vocab - a->vocab / g < 28 * 1024 ? 1 : g;
+    return g < 2 || a->vocab - a->vocab / g < 44 * 1024 ? 1 : g;
 }
 
 static int sample_check(const pkv_sample_args *a) {
