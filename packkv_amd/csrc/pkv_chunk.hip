@@ -145,7 +145,7 @@ __device__ __forceinline__ void narrow_packs(const uint8_t *unit, int t, const U
     for (int i = 0; i < 4; i++) at[i] = (uint32_t)(g.mins_bytes + g.lens_bytes) + 2u * off2[i];
 }
 
-// Blocks of widths up to 4 travel from memory to LDS without registers, 16 bytes a lane: lane l's land at lds_addr + 16 l, lanes behind
+// Blocks travel from memory to LDS without registers (but for wide codes where rows are few), 16 bytes a lane: lane l's land at lds_addr + 16 l, lanes behind
 // the buffer's end get zeroes, lanes that are off write nothing.  lds_addr and rsrc are wave-uniform.  The compiler does not see the
 // copies: s_waitcnt vmcnt(0) stands in front of the barrier that hands them on, and the barrier between waits for LDS only.
 #pragma clang diagnostic push
@@ -248,7 +248,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
     };
     u4 raw[COPY ? 1 : NQ];
     uint32_t raw_phase = 0, par_k = 0, par_kz = 0, par_v = 0, par_vz = 0;
-    // starts the copies of `tile`, whose entry look_up has fetched (widths above 4: into registers, for put)
+    // starts the copies of `tile`, whose entry look_up has fetched (COPY = false: into registers, for put)
     auto fetch = [&](int tile) {
         uint32_t off = next_off, size = min(next_size, cap);               // (never outside the stream, whatever block_info says)
         if ((uint64_t)off > bytes) off = (uint32_t)bytes;
@@ -643,7 +643,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
             else add_values(tab_all, w);
         }
     } else if (RG == 1) {
-        // Few rows: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
+        // Few rows and wide codes: two workgroups a CU cover each other's waits.  Two barriers a tile: staged blocks, table.
         for (int tile = c0; tile < c1; tile++) {
             if (tile != c0) __syncthreads();               // the tile is staged, and the table's readers are done
             const float grow = raise_scale(write_par(tile, 0));
