@@ -964,6 +964,8 @@ static uint32_t chunk_ring(const pkv_chunk_args *a, int rg, uint32_t &slot_k, ui
 // How a call is cut: rows a workgroup (32 NB RG), and runs of tiles, so that the rounds of workgroups the device takes -- three a CU of
 // the small kind (wide codes: two), one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
 // partials as one.
+// Rows of 33 to 64 as one workgroup of two groups against two small ones a KV head against half of a large one: 8 sequences x 10 queries of
+// 32 + 8 heads over 8192 tokens 65.7, 72.3, 81.3 us, 1 x 16 over 16384 33.3, 38.8, 39.8; sixteen rows or fewer stand at r16.
 struct ChunkCut {
     int nb, rg, r16, row_tiles, tiles, run, nsplit;
 };
