@@ -18,8 +18,9 @@
 // follow what it sees (unseen_shift; 1 to 2 % of a prompt's time, 116 us to 118 for 2048 queries on 2048 tokens).
 // p is taken against a maximum that is raised only once a score exceeds it by 2^8 (weights stay below 2^15): the factor on the
 // accumulators, and the exchange of maxima between lanes, are rare, and the reference goes into the scores' own multiply-add.
-// q in bf16 becomes fp16 times one power of two for the workgroup's rows, which loses bits only of values 2^-28 below their largest (where
-// fp16 has no normal numbers left).
+// q in bf16 becomes fp16 times one power of two for the workgroup's rows, or one of each row's own where they lie 2^8 apart or more, which
+// loses bits only of values 2^-20 below their row's largest (where fp16 has no normal numbers left; rows up to 2^100 apart).  The branch
+// for such rows costs the others up to 3 % (1024 queries over 16384 tokens 522 -> 539 us, 8 x 8 over 16384 none).
 //
 // K turns through LDS (a pack holds 16 tokens of one channel, the product wants channels of one token): codes as bytes in rows of
 // 136 bytes, private to the wavefront.  V needs no turn: lane = channel, and the order of the tokens in the contraction is free as
@@ -313,8 +314,11 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
         qw[j] = *reinterpret_cast<const u4 *>(q_row(min(row0 + (i >> 4), p.rows - 1)) + 8 * (i & 15));
     }
     int up = 0;
+    bool apart = false;                                    // rows further apart than 2^8: each has a power of two of its own on top
     if (BF) {
-        uint32_t top = 0;
+        typedef unsigned short u16pair __attribute__((ext_vector_type(2)));
+        uint32_t high[kPieces];                            // a row's largest size; 0: it sees nothing, or holds nothing finite but zeroes
+        u16pair both = {0, 0};                             // the largest of the rows', 0x7FFF - the least
 #pragma unroll
         for (int j = 0; j < kPieces; j++) {                // (infinities, NaN and rows that see nothing do not count)
             const int r = min(row0 + ((tid + 256 * RG * j) >> 4), p.rows - 1);
@@ -324,27 +328,36 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
                 const uint32_t lo = qw[j][k] & 0x7FFFu, hi = (qw[j][k] >> 16) & 0x7FFFu;
                 most = max(most, max(lo < 0x7F80u ? lo : 0u, hi < 0x7F80u ? hi : 0u));
             }
-            if (!p.causal || T - p.n + r / p.G >= start) top = max(top, most);
+            most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0xB1, 0xF, 0xF, true));   // (sixteen lanes a row: pairs,
+            most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0x4E, 0xF, 0xF, true));   // fours,
+            most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0x141, 0xF, 0xF, true));  // eights mirrored,
+            most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0x140, 0xF, 0xF, true));  // sixteens mirrored)
+            high[j] = !p.causal || T - p.n + r / p.G >= start ? most : 0u;
+            both = __builtin_elementwise_max(both, (u16pair){(unsigned short)high[j], (unsigned short)(high[j] ? 0x7FFFu - high[j] : 0u)});
         }
 #pragma unroll
-        for (int d = 32; d; d >>= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d, 64));
-        if (lane == 0) tab_all[wave] = top;
+        for (int d = 32; d >= 16; d >>= 1)
+            both = __builtin_elementwise_max(both, __builtin_bit_cast(u16pair, __shfl_xor(__builtin_bit_cast(int, both), d, 64)));
+        if (lane == 0) tab_all[wave] = __builtin_bit_cast(uint32_t, both);
         __syncthreads();
-        top = tab_all[0];
 #pragma unroll
-        for (int i = 1; i < 4 * RG; i++) top = max(top, tab_all[i]);
+        for (int i = 0; i < 4 * RG; i++) both = __builtin_elementwise_max(both, __builtin_bit_cast(u16pair, tab_all[i]));
+        const uint32_t top = both[0], least = 0x7FFFu - both[1];
         up = top ? min(max(141 - (int)(top >> 7), -120), 120) : 0;        // the largest comes to 2^14 .. 2^15
+        apart = __builtin_amdgcn_readfirstlane((int)(top >> 7) - (int)(least >> 7)) >= 8;
+#pragma unroll
+        for (int j = 0; j < kPieces; j++) {
+            const int i = tid + 256 * RG * j, own = apart && high[j] ? min((int)(top >> 7) - (int)(high[j] >> 7), 100 - max(up - 20, 0)) : 0;
+            const float up_f = __uint_as_float((uint32_t)(127 + up + own) << 23);
+#pragma unroll
+            for (int k = 0; k < 4; k++) qw[j][k] = pack_f16(__uint_as_float(qw[j][k] << 16) * up_f, __uint_as_float(qw[j][k] & 0xFFFF0000u) * up_f);
+            if ((i & 15) == 0) st[i >> 4] = __uint_as_float((uint32_t)(127 - own) << 23);      // (scores are taken times that; the place is the end's)
+        }
     }
-    const float up_f = __uint_as_float((uint32_t)(127 + up) << 23);
 #pragma unroll
     for (int j = 0; j < kPieces; j++) {
         const int i = tid + 256 * RG * j;
-        u4 w = qw[j];
-        if (BF) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) w[k] = pack_f16(__uint_as_float(w[k] << 16) * up_f, __uint_as_float(w[k] & 0xFFFF0000u) * up_f);
-        }
-        *reinterpret_cast<u4 *>(qt + (i >> 4) * kQRow + 16 * (i & 15)) = w;
+        *reinterpret_cast<u4 *>(qt + (i >> 4) * kQRow + 16 * (i & 15)) = qw[j];
     }
     if (c0 < c1) put(c0);
     __syncthreads();
@@ -360,6 +373,7 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
         }
         if (R16) s += __shfl_xor(s, 16, 64);
         qsum[nb] = s + __shfl_xor(s, 32, 64);
+        if (BF && apart) qsum[nb] *= st[mine0 + 32 * nb + tr];
     }
 
     f16v acc[NB][4];
@@ -471,6 +485,14 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
             for (int nb = 0; nb < NB; nb++)
                 y[nb] = product<false>(a, *reinterpret_cast<const u4 *>(qt + (mine0 + 32 * nb + t) * kQRow + 32 * s + 16 * h), y[nb]);
         }
+        if (BF && apart) {
+#pragma unroll
+            for (int nb = 0; nb < NB; nb++) {
+                const float down = st[mine0 + 32 * nb + t];
+#pragma unroll
+                for (int r = 0; r < 16; r++) y[nb][r] *= down;
+            }
+        }
         float ref[NB];                                     // what the scores are taken against
 #pragma unroll
         for (int nb = 0; nb < NB; nb++) ref[nb] = m[nb] == kLowest ? 0.f : m[nb];
@@ -566,6 +588,11 @@ __global__ void __launch_bounds__(256 * RG, RG == 2 ? 1 : WIDE ? 2 : 3) attn_chu
                 const u4 a = {codes_f16(c8.x, 0x04010400u), codes_f16(c8.x, 0x04030402u), codes_f16(c8.y, 0x04010400u), codes_f16(c8.y, 0x04030402u)};
                 y[n] = product16<false>(a, b, y[n]);
             }
+        }
+        if (BF && apart) {
+            const float down = st[tr];
+#pragma unroll
+            for (int i = 0; i < 8; i++) y[i >> 2][i & 3] *= down;
         }
         const float ref = m[0] == kLowest ? 0.f : m[0];
 #pragma unroll
