@@ -450,8 +450,8 @@ int pkv_attn_chunk(const pkv_chunk_args *args, void *workspace, uint64_t workspa
  * whose mass with all in front of it exceeds u times the mass kept.  Temperature 0 (or less, or NaN): the first of the order.  A
  * row in which nothing can be chosen gives token -1.  temperature, top_k, top_p, min_p: device arrays [rows], or NULL and the _all
  * numbers for every row.  token [rows] int64; logprob [rows] fp32 (NULL: none): log of the token's share of the mass kept (-inf
- * with token -1).  Weights in fp64, sums as whole numbers: the same token whatever the launch.  vocab at most 2^20.  `workspace` as
- * in pkv_attn_chunk.  No counterpart in the reference. */
+ * with token -1).  Weights in fp64, sums as whole numbers: the same token whatever the launch.  vocab at most 2^20, rows fewer than 2^22.
+ * `workspace` as in pkv_attn_chunk.  No counterpart in the reference. */
 #define PKV_F32 2
 typedef struct pkv_sample_args {
     const void *logits;

@@ -1120,7 +1120,7 @@ int pkv_attn_chunk(const pkv_chunk_args *a, void *workspace, uint64_t workspace_
     const bool wide = chunk_wide(a), bf = a->dtype == PKV_BF16;
     const uint32_t lds = p.ring + kt + rg * (4096u + 2048u) + 8u * m * 4u + m * kQRow;
     const uint64_t groups = ((uint64_t)p.BH * p.nsplit + 7) / 8, wgs = groups * 8 * (uint64_t)p.row_tiles;
-    PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x queries too large");
+    PKV_REQUIRE(wgs < (1ull << 24) / rg, PKV_ERR_UNSUPPORTED, "batch x queries too large");           // (2^32 threads)
 #define PKV_CHUNK(bf, nb, rg) {(const void *)attn_chunk_kernel<bf, nb, rg, false>, (const void *)attn_chunk_kernel<bf, nb, rg, true>}
     const void *kernels[2][3][2] = {{PKV_CHUNK(false, 1, 1), PKV_CHUNK(false, 1, 2), PKV_CHUNK(false, 2, 2)},
                                     {PKV_CHUNK(true, 1, 1), PKV_CHUNK(true, 1, 2), PKV_CHUNK(true, 2, 2)}};

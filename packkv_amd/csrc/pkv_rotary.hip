@@ -212,7 +212,7 @@ extern "C" int pkv_norm_rotary(const pkv_rotary_args *a, pkv_stream_t s_) {
     p.pieces = (p.groups + (uint32_t)p.per - 1u) / (uint32_t)p.per;
     p.units = tokens * p.pieces;
     const uint64_t wgs = (p.units + 3) / 4;
-    PKV_REQUIRE(wgs < (1ull << 31), PKV_ERR_UNSUPPORTED, "batch x tokens x heads too large");
+    PKV_REQUIRE(wgs < (1ull << 24), PKV_ERR_UNSUPPORTED, "batch x tokens x heads too large");         // (2^32 threads)
     const dim3 grid((unsigned)wgs);
     if (off & 15u) {
         if (a->dtype == PKV_F16) norm_rotary_kernel<PKV_F16, false, false><<<grid, 256, 0, s>>>(p);

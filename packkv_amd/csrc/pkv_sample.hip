@@ -938,6 +938,7 @@ static int sample_check(const pkv_sample_args *a) {
     PKV_REQUIRE(a != nullptr, PKV_ERR_INVALID, "null pointer argument");
     PKV_REQUIRE(a->dtype == PKV_F16 || a->dtype == PKV_BF16 || a->dtype == PKV_F32, PKV_ERR_UNSUPPORTED, "Unsupported data type");
     PKV_REQUIRE(a->rows > 0 && a->vocab > 0, PKV_ERR_INVALID, "sizes must be positive");
+    PKV_REQUIRE(a->rows < (1 << 22), PKV_ERR_UNSUPPORTED, "not supported: %d rows (fewer than 2^22)", a->rows);        // (2^32 threads)
     PKV_REQUIRE(a->vocab <= (1 << 20), PKV_ERR_UNSUPPORTED, "not supported: %d tokens (at most 2^20)", a->vocab);
     return PKV_OK;
 }

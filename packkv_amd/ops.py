@@ -1258,8 +1258,8 @@ def _row_setting(a, name, x, rows, dtype, at, keep):
 
 
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, want_logprob=False):
-    """A token, int64 [rows], for each row of logits [rows, vocab] (fp16, bf16 or fp32; at most 2^20 tokens) from uniform numbers u [rows]
-    float32 in [0, 1).  In this order: the top_k largest logits are kept (0: all), of them the smallest set that holds top_p of their
+    """A token, int64 [rows], for each row of logits [rows, vocab] (fp16, bf16 or fp32; at most 2^20 tokens, fewer than 2^22 rows) from uniform
+    numbers u [rows] float32 in [0, 1).  In this order: the top_k largest logits are kept (0: all), of them the smallest set that holds top_p of their
     mass (1: all), of them those at least min_p times as likely as the first (0: all); the draw goes through what is left, most likely
     first.  Equal logits are ordered by index.  temperature 0 takes the first.  Every setting is a number or a device tensor [rows]
     (float32; top_k int32; numbers are rounded to float32).  -inf and NaN are never chosen; a row with nothing else gives -1.  With
