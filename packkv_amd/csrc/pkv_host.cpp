@@ -517,8 +517,8 @@ PyObject *sample(PyObject *, PyObject *const *o, Py_ssize_t n) {
         if (t) {
             if (!row_tensor(t, at::kFloat)) Py_RETURN_NONE;
             *at_[i] = at_ptr<float>(*t);
-        } else if (!real(given[i], all[i]) || !(*all[i] >= 0.f) || (i && *all[i] > 1.f)) {
-            Py_RETURN_NONE;
+        } else if (!real(given[i], all[i]) || !(PyFloat_AS_DOUBLE(given[i]) >= 0.0) || (i && PyFloat_AS_DOUBLE(given[i]) > 1.0)) {
+            Py_RETURN_NONE;                                // (as given, not as rounded)
         }
     }
     const at::Tensor *k = tensor(o[3]);
