@@ -197,11 +197,17 @@ class ShapedDecoder:
     @torch.no_grad()
     def generate(self, ids, cache, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
         """`ids` [B, n] (a first prompt, or a later one on a cache that holds tokens), then a sampled token for each row of u
-        [steps, B], uniform numbers in [0, 1); the settings as ops.sample takes them.  Returns the generated ids [B, steps]."""
+        [steps, B], uniform numbers in [0, 1); the settings as ops.sample takes them.  Returns the generated ids [B, steps].  Logits from
+        which nothing can be chosen (all NaN or -inf) are an error at the end, with the tokens in the cache."""
         logits = self.forward(ids, cache, attention="fused" if cache.get_seq_length(0) else "dense", rotary="fused")
         out = []
         for row in u:
             nxt = ops.sample(logits, row, temperature, top_k, top_p, min_p).unsqueeze(1)
             out.append(nxt)
             logits = self.forward(nxt, cache, rotary="fused")
-        return torch.cat(out, dim=1) if out else ids.new_empty(ids.size(0), 0)
+        if not out:
+            return ids.new_empty(ids.size(0), 0)
+        out = torch.cat(out, dim=1)
+        if not torch.cuda.is_current_stream_capturing() and bool((out < 0).any()):         # (one wait, behind the last step)
+            raise RuntimeError("a row of logits in which nothing can be chosen (sequences %s)" % (out < 0).any(1).nonzero().flatten().tolist())
+        return out

@@ -1,0 +1,32 @@
+"""generate and forward: what they refuse, and that a refused call leaves the cache as it was."""
+import pytest
+import torch
+
+from packkv_amd.decoder import DecoderShape, ShapedDecoder
+
+pytestmark = pytest.mark.gpu
+
+SHAPE = dict(layers=1, hidden=256, q_heads=4, kv_heads=2, mlp=512, vocab=640)
+
+
+@pytest.fixture(scope="module")
+def model(cuda):
+    return ShapedDecoder(DecoderShape(**SHAPE), dtype=torch.float16, device=cuda, seed=3)
+
+
+def _prompt(cuda, n=140, B=2):
+    return torch.randint(1, 640, (B, n), generator=torch.Generator().manual_seed(n)).to(cuda)
+
+
+def test_rows_without_a_token_are_no_result(cuda, model):
+    """A sequence whose logits are NaN has no next token: generate says so instead of going on with another one's embedding."""
+    ids, u = _prompt(cuda), torch.rand(4, 2, generator=torch.Generator().manual_seed(1)).to(cuda)
+    model.generate(ids, model.new_cache(2, 512), u)
+    kept = model.embed[0].clone()
+    ids[1, -1] = 0
+    try:
+        model.embed[0] = float("nan")
+        with pytest.raises(RuntimeError, match="nothing can be chosen"):
+            model.generate(ids, model.new_cache(2, 512), u)
+    finally:
+        model.embed[0] = kept
