@@ -123,6 +123,8 @@ class ShapedDecoder:
         B, n = ids.shape
         pos0 = cache.get_seq_length(0)
         one_pass = rotary == "fused"
+        if not one_pass and rotary != "chain":
+            raise RuntimeError("not supported: rotary %r (\"chain\" or \"fused\")" % (rotary,))
         if one_pass:
             if positions is None:
                 positions = torch.arange(pos0, pos0 + n, device=self.device)

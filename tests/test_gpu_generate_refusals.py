@@ -30,3 +30,11 @@ def test_rows_without_a_token_are_no_result(cuda, model):
             model.generate(ids, model.new_cache(2, 512), u)
     finally:
         model.embed[0] = kept
+
+
+def test_forward_refuses_unknown_ways(cuda, model, monkeypatch):
+    cache, ids = model.new_cache(2, 512), _prompt(cuda)
+    for way in ("one", "", None, "Fused"):
+        with pytest.raises(RuntimeError, match="rotary"):
+            model.forward(ids, cache, rotary=way)
+    assert cache.get_seq_length() == 0
