@@ -130,12 +130,13 @@ class ShapedDecoder:
                 positions = torch.arange(pos0, pos0 + n, device=self.device)
         elif positions is not None or s.rope_sections is not None:
             raise RuntimeError("not supported: positions of their own need rotary=\"fused\"")
-        cos, sin = self._rotary(pos0, n, B)
+        else:
+            cos, sin = self._rotary(pos0, n, B)
+            half = s.head_dim // 2
+            sin_signed = torch.cat((-sin[..., :half], sin[..., half:]), dim=-1)
+            kw = {"cos": cos, "sin": sin}
         fused = attention == "fused" and (n == 1 or pos0 > 0)
         scaling = 1.0 / math.sqrt(s.head_dim)
-        half = s.head_dim // 2
-        sin_signed = torch.cat((-sin[..., :half], sin[..., half:]), dim=-1)
-        kw = {"cos": cos, "sin": sin}
         h = self.embed[ids].view(B * n, s.hidden)
         for li, blk in enumerate(self.blocks):
             x = _rms(h, blk["in_norm"], s.rms_eps)

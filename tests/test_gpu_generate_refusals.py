@@ -38,3 +38,15 @@ def test_forward_refuses_unknown_ways(cuda, model, monkeypatch):
         with pytest.raises(RuntimeError, match="rotary"):
             model.forward(ids, cache, rotary=way)
     assert cache.get_seq_length() == 0
+
+
+def test_one_pass_forms_no_tables(cuda, model, monkeypatch):
+    """rotary="fused" turns rows by positions; the chain's cosines and sines are not formed beside it."""
+    cache, ids = model.new_cache(2, 512), _prompt(cuda)
+    calls = []
+    tables = model._rotary
+    monkeypatch.setattr(model, "_rotary", lambda *a: calls.append(a) or tables(*a))
+    model.generate(ids, cache, torch.rand(3, 2, device=cuda))
+    assert calls == [] and cache.get_seq_length() == 143
+    model.forward(ids[:, :1], cache)
+    assert len(calls) == 1
