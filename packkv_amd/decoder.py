@@ -202,6 +202,9 @@ class ShapedDecoder:
         """`ids` [B, n] (a first prompt, or a later one on a cache that holds tokens), then a sampled token for each row of u
         [steps, B], uniform numbers in [0, 1); the settings as ops.sample takes them.  Returns the generated ids [B, steps].  Logits from
         which nothing can be chosen (all NaN or -inf) are an error at the end, with the tokens in the cache."""
+        u = list(u)
+        for row in u:                                     # (refused here, not with the prompt in the cache)
+            ops._sample_settings(row, ids.size(0), self.embed.get_device(), temperature, top_k, top_p, min_p)
         logits = self.forward(ids, cache, attention="fused" if cache.get_seq_length(0) else "dense", rotary="fused")
         out = []
         for row in u:

@@ -1257,6 +1257,20 @@ def _row_setting(a, name, x, rows, dtype, at, keep):
     setattr(a, name, x.data_ptr())
 
 
+def _sample_settings(u, rows, at, temperature, top_k, top_p, min_p):
+    """The arguments of pkv_sample that are not logits or results, checked, and the tensors that the addresses in them need alive."""
+    a, keep = _lib.SampleArgs(), []
+    _require(u.shape == (rows,) and u.dtype == torch.float32 and u.get_device() == at, "u must be a float32 tensor [rows] on the logits' device")
+    for name, x, ok in (("temperature", temperature, lambda x: x >= 0), ("top_k", top_k, lambda x: 0 <= x < 1 << 31 and x == int(x)),
+                        ("top_p", top_p, lambda x: 0 <= x <= 1), ("min_p", min_p, lambda x: 0 <= x <= 1)):
+        _require(torch.is_tensor(x) or ok(x), "%s is out of range" % name)
+        _row_setting(a, name, int(x) if name == "top_k" and not torch.is_tensor(x) else x, rows, torch.int32 if name == "top_k" else torch.float32, at, keep)
+    u = u.contiguous()
+    keep.append(u)
+    a.u = u.data_ptr()
+    return a, keep
+
+
 def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, want_logprob=False):
     """A token, int64 [rows], for each row of logits [rows, vocab] (fp16, bf16 or fp32; at most 2^20 tokens, fewer than 2^22 rows) from uniform
     numbers u [rows] float32 in [0, 1).  In this order: the top_k largest logits are kept (0: all), of them the smallest set that holds top_p of their
@@ -1270,18 +1284,10 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
         return _lib.check(served) if type(served) is int else served
     _require(logits.is_cuda and logits.dim() == 2 and logits.size(1) > 0, "logits must be a device tensor [rows, vocab]")
     R, V = logits.shape
-    at, dev, keep = logits.get_device(), logits.device, []
-    a = _lib.SampleArgs()
-    if logits.dtype == torch.float32:
-        a.dtype = _lib.F32
-    else:
-        a.dtype = _dtype_code(logits)
+    at, dev = logits.get_device(), logits.device
+    code = _lib.F32 if logits.dtype == torch.float32 else _dtype_code(logits)
     _require(V <= 1 << 20, "not supported: %d tokens (at most 2^20)" % V)
-    _require(u.shape == (R,) and u.dtype == torch.float32 and u.get_device() == at, "u must be a float32 tensor [rows] on the logits' device")
-    for name, x, ok in (("temperature", temperature, lambda x: x >= 0), ("top_k", top_k, lambda x: 0 <= x < 1 << 31 and x == int(x)),
-                        ("top_p", top_p, lambda x: 0 <= x <= 1), ("min_p", min_p, lambda x: 0 <= x <= 1)):
-        _require(torch.is_tensor(x) or ok(x), "%s is out of range" % name)
-        _row_setting(a, name, int(x) if name == "top_k" and not torch.is_tensor(x) else x, R, torch.int32 if name == "top_k" else torch.float32, at, keep)
+    a, keep = _sample_settings(u, R, at, temperature, top_k, top_p, min_p)
     if out is None:
         out = torch.empty(R, dtype=torch.int64, device=dev)
     else:
@@ -1291,9 +1297,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
     if R:
         if logits.stride(1) != 1 and V > 1:
             logits = logits.contiguous()
-        u = u.contiguous()
-        a.logits, a.u, a.token, a.logprob = logits.data_ptr(), u.data_ptr(), out.data_ptr(), logprob.data_ptr() if want_logprob else None
-        a.row_stride, a.rows, a.vocab = logits.stride(0) if R > 1 else 0, R, V
+        a.logits, a.token, a.logprob = logits.data_ptr(), out.data_ptr(), logprob.data_ptr() if want_logprob else None
+        a.dtype, a.row_stride, a.rows, a.vocab = code, logits.stride(0) if R > 1 else 0, R, V
         lib, ref = _lib.load(), ctypes.byref(a)
         with _on(dev):
             need = lib.pkv_sample_workspace(ref)

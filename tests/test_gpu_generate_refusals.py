@@ -50,3 +50,14 @@ def test_one_pass_forms_no_tables(cuda, model, monkeypatch):
     assert calls == [] and cache.get_seq_length() == 143
     model.forward(ids[:, :1], cache)
     assert len(calls) == 1
+
+
+def test_generate_refuses_before_the_prompt_is_in_the_cache(cuda, model):
+    cache, ids, u = model.new_cache(2, 512), _prompt(cuda), torch.rand(3, 2, device=cuda)
+    for kw in (dict(u=u.double()), dict(u=u.cpu()), dict(u=u[:, :1]), dict(u=u[:, None]), dict(u=u[0]), dict(temperature=-1.0), dict(top_p=1.5),
+               dict(top_k=-1), dict(min_p=torch.zeros(3, device=cuda)), dict(top_k=torch.zeros(2, device=cuda)), dict(temperature=torch.ones(2))):
+        with pytest.raises(RuntimeError):
+            model.generate(ids, cache, **{"u": u, **kw})
+        assert cache.get_seq_length() == 0, kw
+    want = model.generate(ids, cache, u, top_k=torch.full((2,), 9, dtype=torch.int32, device=cuda))
+    assert torch.equal(model.generate(ids, model.new_cache(2, 512), (row for row in u), top_k=9), want)
