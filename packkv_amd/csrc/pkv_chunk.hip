@@ -32,9 +32,9 @@
 // to bytes 210, bytes to operands 65, V's table 80 and packs 180, scores to weights 150), 70 less with 16, 730 with 64.  Hence as few
 // wavefronts as possible unpack the same block, up to 128 rows a workgroup, two groups of them sharing K's bytes and V's table; and
 // three workgroups a CU where rows are few (vector units busy 79 % of the cycles, 67 % with two).  8 KV heads, 4-bit codes: 8 sequences
-// x 4 queries of 32 heads over 16384 tokens 68.5 us (79 with two workgroups a CU, 74 with products of 32 rows; a copy of the bytes: 22),
-// 1024 queries over 32768 1010 us, 540 TFLOP/s (a large product reaches 1160), where 64 rows a workgroup without sharing took 1430;
-// 40 heads x 333 queries of two sequences over 4096 tokens in 5-bit codes 139 to 157 us; 3 queries over 1100 tokens 13 us, 4 of them the
+// x 4 queries of 32 heads over 16384 tokens 69 us (79 with two workgroups a CU, 74 with products of 32 rows; a copy of the bytes: 22),
+// 1024 queries over 32768 1015 us, 540 TFLOP/s (a large product reaches 1160), where 64 rows a workgroup without sharing took 1430;
+// 40 heads x 333 queries of two sequences over 4096 tokens in 5-bit codes 138 to 171 us, by their padding; 3 queries over 1100 tokens 13 us, 4 of them the
 // merge.
 #include "pkv_block.hpp"
 #include "pkv_runtime.hpp"
@@ -1017,10 +1017,13 @@ static uint32_t chunk_ring(const pkv_chunk_args *a, int rg, uint32_t &slot_k, ui
 }
 
 // How a call is cut: rows a workgroup (32 NB RG), and runs of tiles, so that the rounds of workgroups the device takes -- three a CU of
-// the small kind (wide codes: two), one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
+// the small kind (wide codes: two, although their LDS leaves one from 6 bits on both sides on: 87 KB, and 105 at 8), one of the large -- times the tiles of a run are fewest; a workgroup's start and end count as two tiles, the merge of
 // partials as one.
 // Rows of 33 to 64 as one workgroup of two groups against two small ones a KV head against half of a large one: 8 sequences x 10 queries of
 // 32 + 8 heads over 8192 tokens 65.7, 72.3, 81.3 us, 1 x 16 over 16384 33.3, 38.8, 39.8; sixteen rows or fewer stand at r16.
+// What is staged for two groups, 4 K blocks and 6 V blocks, does not fit with (K, V) widths (3, 8), (4, 7), (4, 8), (5, 7), (5, 8), (7, 5),
+// (8, 5) and 6 to 8 on both sides: these take 32 rows a workgroup for any prompt, 1 x 512 queries over 8192 tokens 611 us at (4, 8), 654 at
+// (6, 6), where (5, 5) takes 189.
 struct ChunkCut {
     int nb, rg, r16, row_tiles, tiles, run, nsplit;
 };
@@ -1028,7 +1031,7 @@ static ChunkCut chunk_cut(const pkv_chunk_args *a) {
     ChunkCut c;
     const int64_t rows = (int64_t)a->n * (a->Hq / a->Hkv);
     uint32_t slot_k, slot_v;
-    c.rg = rows <= 32 || chunk_ring(a, 2, slot_k, slot_v) > 63u * 1024u ? 1 : 2;     // (copies reach 64 KiB: not widths of 6 and more on both sides)
+    c.rg = rows <= 32 || chunk_ring(a, 2, slot_k, slot_v) > 63u * 1024u ? 1 : 2;     // (copies reach 64 KiB)
     c.nb = c.rg == 1 || rows <= 64 ? 1 : 2;
     c.r16 = rows <= 16 && !chunk_wide(a);                  // 1 x 4 queries of 32 + 8 heads over 131072 tokens 75 us, with 32 rows 82; over 4096 16.5 and 17.3
     const int64_t m = 32 * c.nb * c.rg;
