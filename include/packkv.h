@@ -417,7 +417,7 @@ int pkv_dense_view(const pkv_attn_args *args, void *k_out, void *v_out, pkv_stre
  * what lies in front of starts[b], queries too, may be anything.  (A NaN or an infinity in a new token's key, value or parameters may
  * reach queries before it.)  q and out [B, Hq, n, 128] at element strides of batch, head and token, rows 16-byte aligned; Hq any
  * multiple of Hkv; widths 2..8; streams and windows 16-byte aligned; the rest as in pkv_attn_args.  fp32 accumulation; weights in fp16, so off by 2^-11 of
- * p |v|, or by 2^-31 of the largest V scale that the query sees where that is more (finite scales up to 2^80 times that, of tokens behind a
+ * p |v|, or by 2^-31 of the largest V scale that the query sees, for each step of a code, where that is more (finite scales up to 2^80 times that, of tokens behind a
  * query, do not reach it).  `workspace`:
  * 16-byte aligned device memory of pkv_attn_chunk_workspace(args) bytes (may be 0), used until the call's kernels are done: calls
  * that overlap need one each.  Launches kernels only.  Stands in for cache.update's dense tensors + eager attention

@@ -13,7 +13,7 @@
 // itself, read as a half, is the code times 2^-24 and needs no subtraction, but the matrix cores add up products of subnormals
 // without normalising them, to about 18 bits.)  Scale and zero of a token are applied to what the products need of them, in fp32:  score = scale (q . code + zero sum(q)),
 // out = sum p scale code + sum p scale zero.  The weight p * scale is rounded to fp16, scaled by a power of two that follows
-// the largest scale met: by 2^-11 of it, or 2^-31 of the largest scale that the row sees, where that is more; the zero's sum takes the
+// the largest scale met: by 2^-11 of it, or 2^-31 of the largest scale that the row sees where that is more; the zero's sum takes the
 // rounded weight, so that the error is 2^-11 of p |v|, not of p * scale * code.  Where a row does not see all that was met, its weights
 // follow what it sees (unseen_shift; 1 to 2 % of a prompt's time, 116 us to 118 for 2048 queries on 2048 tokens).
 // p is taken against a maximum that is raised only once a score exceeds it by 2^8 (weights stay below 2^15): the factor on the
