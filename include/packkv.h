@@ -466,6 +466,55 @@ typedef struct pkv_sample_args {
 uint64_t pkv_sample_workspace(const pkv_sample_args *args);
 int pkv_sample(const pkv_sample_args *args, void *workspace, uint64_t workspace_bytes, pkv_stream_t s);
 
+/* ---- 8-bit floating point ---------------------------------------------------------------
+ * What lies between the attention over the cache and the next layer with weights and activations in 8 bits.  No counterpart in the
+ * reference, whose decoder keeps 16-bit weights.  The 8-bit form of a matrix [rows, width] is its codes, e4m3 (OCP, largest 448),
+ * one byte each, and an fp32 scale for each block of 1 x 128 (activations) or 128 x 128 values (weights), the last blocks ragged:
+ * scale = max(largest finite |value|, 2^-100) / 448, code = value / scale to the nearest, ties to even (through a product with
+ * 1 / scale); infinities and NaN become NaN.  Strides are in elements, scale_stride: of a row of blocks and of a block in it; widths
+ * are multiples of 16; rows of everything but scales start on 16-byte boundaries.  All of them launch kernels only.
+ *
+ * pkv_add_rms_norm: h = x + residual (NULL: x), y = h / sqrt(mean(h^2) + eps) * weight for each row, in fp32; h, rounded once, to sum
+ * (NULL where there is no residual; may be the residual's own memory), y to out in `dtype` or in its 8-bit form to codes and scale.
+ * width at most 65536, rows fewer than 2^22. */
+typedef struct pkv_norm_args {
+    const void *x, *residual, *weight;
+    void *sum, *out;
+    uint8_t *codes;
+    float *scale;
+    int64_t x_stride, residual_stride, sum_stride, out_stride, codes_stride, scale_stride[2];
+    int dtype, rows, width;
+    float eps;
+} pkv_norm_args;
+int pkv_add_rms_norm(const pkv_norm_args *args, pkv_stream_t s);
+
+/* pkv_fp8_quantize: the 8-bit form of x [rows, width] `dtype`, block 1 or 128 rows a scale.  Row r of x is row r % per_batch of its
+ * batch r / per_batch, and a row's blocks of 128 may lie apart: x_stride of batch, row and block (a plain matrix: per_batch = rows, block stride 128;
+ * [B, H, n, 128] as rows of H * 128: per_batch = n and the strides of batch, token and head).  With block 128 a plain matrix only. */
+typedef struct pkv_fp8_quantize_args {
+    const void *x;
+    uint8_t *codes;
+    float *scale;
+    int64_t x_stride[3], codes_stride, scale_stride[2];
+    int dtype, rows, width, per_batch, block;
+} pkv_fp8_quantize_args;
+int pkv_fp8_quantize(const pkv_fp8_quantize_args *args, pkv_stream_t s);
+
+/* pkv_fp8_product: out [rows, cols] = x [rows, width] times w [cols, width] transposed, both in their 8-bit form (x with a scale a row, w
+ * one for 128 rows), + bias [cols] (NULL: none), summed in fp32 and rounded once to `dtype`.  gated: w [2 cols, width], its first half gives g and
+ * its second u, out = g / (1 + exp(-g)) * u; cols a multiple of 16, no bias.  The product of the two scales of a block has to be
+ * finite.  Within each eight neighbouring products every one is cut to a multiple of 2^-13 of the largest's power of two (the matrix
+ * instruction's own sums; the codes have 4 significant bits).  width at most 2^20, rows and cols at most 2^24. */
+typedef struct pkv_fp8_product_args {
+    const uint8_t *x, *w;
+    const float *x_scale, *w_scale;
+    const void *bias;
+    void *out;
+    int64_t x_stride, w_stride, out_stride, x_scale_stride[2], w_scale_stride[2];
+    int dtype, rows, width, cols, gated;
+} pkv_fp8_product_args;
+int pkv_fp8_product(const pkv_fp8_product_args *args, pkv_stream_t s);
+
 /* pkv_stream_release: gives back the device memory the library keeps for stream `s` of the current device -- its
  * scratch buffers (attention partials, the encoders' look-back state), its tile counters and every buffer it has
  * outgrown (kept until now because a captured HIP graph might still hold its address).  It has no counterpart in the

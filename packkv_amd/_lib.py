@@ -12,7 +12,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 # PACKKV_HIP_LIB names another build of the same library (kernel development: A/B runs of two builds)
 LIB_PATH = os.environ.get("PACKKV_HIP_LIB") or os.path.join(_HERE, "libpackkv_hip.so")
 HOST_SYMBOLS = ("pkv_attn_decode", "pkv_window_append", "pkv_dense_view", "pkv_kq_mat_vec_mul", "pkv_wv_mat_vec_mul", "pkv_fused_kq",
-                "pkv_fused_wv", "pkv_norm_rotary", "pkv_attn_chunk_workspace", "pkv_attn_chunk", "pkv_sample_workspace", "pkv_sample")
+                "pkv_fused_wv", "pkv_norm_rotary", "pkv_attn_chunk_workspace", "pkv_attn_chunk", "pkv_sample_workspace", "pkv_sample",
+                "pkv_add_rms_norm", "pkv_fp8_quantize", "pkv_fp8_product")
 
 F16, BF16, F32 = 0, 1, 2
 OK, ERR_UNSUPPORTED, ERR_INVALID, ERR_HIP, ERR_CAPACITY, ERR_INTERNAL = range(6)
@@ -74,6 +75,23 @@ class SampleArgs(ctypes.Structure):
                 [(n, _i) for n in ("dtype", "rows", "vocab", "top_k_all")] + [(n, _f) for n in ("temperature_all", "top_p_all", "min_p_all")])
 
 
+class NormArgs(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("x", "residual", "weight", "sum", "out", "codes", "scale")] +
+                [(n, _i64) for n in ("x_stride", "residual_stride", "sum_stride", "out_stride", "codes_stride")] + [("scale_stride", _i64 * 2)] +
+                [(n, _i) for n in ("dtype", "rows", "width")] + [("eps", _f)])
+
+
+class Fp8QuantizeArgs(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("x", "codes", "scale")] + [("x_stride", _i64 * 3), ("codes_stride", _i64), ("scale_stride", _i64 * 2)] +
+                [(n, _i) for n in ("dtype", "rows", "width", "per_batch", "block")])
+
+
+class Fp8ProductArgs(ctypes.Structure):
+    _fields_ = ([(n, _vp) for n in ("x", "w", "x_scale", "w_scale", "bias", "out")] +
+                [(n, _i64) for n in ("x_stride", "w_stride", "out_stride")] + [("x_scale_stride", _i64 * 2), ("w_scale_stride", _i64 * 2)] +
+                [(n, _i) for n in ("dtype", "rows", "width", "cols", "gated")])
+
+
 # name -> (restype, argtypes); every symbol include/packkv.h declares
 SIGNATURES = {
     "pkv_abi_version": (_i, []),
@@ -122,6 +140,9 @@ SIGNATURES = {
     "pkv_attn_chunk": (_i, [ctypes.POINTER(ChunkArgs), _vp, _u64, _vp]),
     "pkv_sample_workspace": (_u64, [ctypes.POINTER(SampleArgs)]),
     "pkv_sample": (_i, [ctypes.POINTER(SampleArgs), _vp, _u64, _vp]),
+    "pkv_add_rms_norm": (_i, [ctypes.POINTER(NormArgs), _vp]),
+    "pkv_fp8_quantize": (_i, [ctypes.POINTER(Fp8QuantizeArgs), _vp]),
+    "pkv_fp8_product": (_i, [ctypes.POINTER(Fp8ProductArgs), _vp]),
     "pkv_stream_release": (_i, [_vp]),
 }
 

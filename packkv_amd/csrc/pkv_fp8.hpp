@@ -1,0 +1,59 @@
+// What the 8-bit operators share: 16-bit values in and out, e4m3 (OCP, largest 448) values and the scales of their blocks.
+#pragma once
+#include "pkv_common.hpp"
+
+namespace pkv {
+
+constexpr int kBlock8 = 128;                       // values of a row that share a scale
+constexpr float kTop8 = 448.f;                     // e4m3's largest
+constexpr float kLeast8 = 0x1p-100f;               // what a block's largest value counts as at least: its scale stays a normal number
+
+#ifdef __HIPCC__
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+template <int DT> __device__ __forceinline__ float wide16(uint32_t w, int i) {
+    const uint32_t h = i ? w >> 16 : w & 0xFFFFu;
+    return DT == PKV_F16 ? __half2float(__ushort_as_half((unsigned short)h)) : __uint_as_float(h << 16);
+}
+template <int DT> __device__ __forceinline__ uint32_t pair16(float a, float b) {
+    if (DT == PKV_F16) {
+        typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b});
+    }
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+}
+// The largest of the caller's 16 lanes (a DPP row), in all of them.
+__device__ __forceinline__ float row16_max(float v) {
+    auto from = [&](auto ctrl) {
+        return __uint_as_float(__builtin_amdgcn_update_dpp(0u, __float_as_uint(v), decltype(ctrl)::value, 0xF, 0xF, true));
+    };
+    v = fmaxf(v, from(std::integral_constant<int, 0xB1>{}));       // lane ^ 1
+    v = fmaxf(v, from(std::integral_constant<int, 0x4E>{}));       // lane ^ 2
+    v = fmaxf(v, from(std::integral_constant<int, 0x141>{}));      // 7 - lane of eight
+    v = fmaxf(v, from(std::integral_constant<int, 0x140>{}));      // 15 - lane
+    return v;
+}
+// |v|, and 0 for infinities and NaN, which have no part in a block's scale.
+__device__ __forceinline__ float finite_size(float v) {
+    const float a = fabsf(v);
+    return a <= 3.402823466e38f ? a : 0.f;
+}
+__device__ __forceinline__ float scale_of(float largest) { return fmaxf(largest, kLeast8) / kTop8; }
+// Eight values over their block's scale, to the nearest e4m3, ties to even.  (largest / scale may come out a rounding above 448, which
+// still rounds to 448; infinities and NaN become NaN.)
+__device__ __forceinline__ u32x2 codes8(const float y[8], float inv) {
+    u32x2 r = {0u, 0u};
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, w, true);
+        r[i] = (uint32_t)w;
+    }
+    return r;
+}
+#endif
+
+}  // namespace pkv

@@ -1,0 +1,178 @@
+// Products of matrices in their 8-bit form (pkv_fp8.hip): y[m, n] = sum over blocks b of 128 of
+//     sx[m, b] * sw[n / 128, b] * sum_{k in b} cx[m, k] * cw[n, k]        (+ bias[n]),
+// rounded once to 16 bits, and the gated feed-forward of it: rows 0 .. I-1 of w give g, rows I .. 2I-1 give u, the result is
+// g / (1 + exp(-g)) * u.
+//
+// One v_mfma_f32_16x16x128_f8f6f4 is one block's sum for 16 x 16 results: it starts from zero, and its four numbers a lane are
+// added to the fp32 sums with the two scales, one fma each.  Weights are the instruction's rows and x its columns, so a lane holds
+// four neighbouring outputs of one row of x: its scale is one number a lane, the weights' scale one a wavefront.  The order of the 128
+// within a block does not matter, so lanes load what lies well: of each 128 the 16-byte pieces g and 4 + g, g = lane / 16.
+//
+// What the instruction loses: in each group of eight neighbouring k it cuts every product towards zero to a multiple of 2^-13 of the
+// group's largest power of two, and adds groups in fp32 (measured).  Products of values with 4 significant bits, which are 2^-4 off
+// themselves, come out 2^-13 of the largest of eight off at most; sums of 128 normal products 1.3e-5.  Results are 16-bit (2^-9, 2^-12).
+#include "pkv_fp8.hpp"
+#include "pkv_runtime.hpp"
+
+namespace pkv {
+
+struct ProductParams {
+    const uint8_t *x, *w;
+    const float *x_scale, *w_scale;
+    const uint16_t *bias;
+    uint16_t *out;
+    int64_t x_row, w_row, out_row, xs_row, xs_col, ws_row, ws_col;
+    uint32_t rows, width, cols;          // of x; results a row (of w: twice as many rows where gated)
+    uint32_t blocks;                     // of 128 along the width
+};
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+__device__ __forceinline__ f32x4 block_product(i32x8 w, i32x8 x) {
+    const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
+}
+constexpr uint32_t kNowhere = 0x80000000u;             // a buffer offset behind any tile: loads give zeroes
+// Rows first .. first + count - 1 of a matrix of `rows` rows as a buffer: what lies behind its last row reads as zero.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t *base, int64_t row, uint32_t first, uint32_t rows, uint32_t count, uint32_t width) {
+    const uint32_t there = first < rows ? min(count, rows - first) : 0u;
+    const uint32_t bytes = there ? (there - 1u) * (uint32_t)row + width : 0u;
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base) + (int64_t)first * row, 0, (int)bytes, 0x00020000);
+}
+// A lane's 32 bytes of block b of its row (at byte `at`), pieces g and 4 + g of 16; zeroes behind the width.
+__device__ __forceinline__ i32x8 load_piece(__amdgpu_buffer_rsrc_t r, uint32_t at, uint32_t b, uint32_t g, uint32_t width) {
+    const uint32_t k = b * 128u + 16u * g;
+    const u32x4_t lo = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k < width ? at + k : kNowhere, 0, 0));
+    const u32x4_t hi = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k + 64u < width ? at + k + 64u : kNowhere, 0, 0));
+    return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+// Few rows of x: a workgroup has 16 RT rows of weights (of gate and of up each, where gated) and 16 MT rows of x, its wavefronts
+// take the blocks of the width in turn, straight into registers, and join their sums in LDS.
+template <int DT, int RT, int MT, int WAVES, bool GATED>
+__global__ void __launch_bounds__(64 * WAVES) product_few_kernel(const ProductParams p) {
+    constexpr int S = GATED ? 2 : 1, TILES = S * RT * MT;
+    __shared__ f32x4 part[WAVES][TILES][64];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = lane & 15u, g = lane >> 4;
+    const uint32_t tiles_n = (p.cols + 16u * RT - 1u) / (16u * RT);
+    const uint32_t tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x - tile_m * tiles_n;
+    const uint32_t n0 = tile_n * 16u * RT, m0 = tile_m * 16u * MT;
+    const uint32_t w_rows = S * p.cols;
+    __amdgpu_buffer_rsrc_t wr[S];
+    const float *ws[S][RT];
+#pragma unroll
+    for (int s = 0; s < S; s++) {
+        const uint32_t first = n0 + (uint32_t)s * p.cols;
+        wr[s] = tile_rsrc(p.w, p.w_row, first, GATED && s == 0 ? p.cols : w_rows, 16u * RT, p.width);
+#pragma unroll
+        for (int i = 0; i < RT; i++) ws[s][i] = p.w_scale + (int64_t)(min(first + 16u * i, w_rows - 1u) / 128u) * p.ws_row;
+    }
+    const __amdgpu_buffer_rsrc_t xr = tile_rsrc(p.x, p.x_row, m0, p.rows, 16u * MT, p.width);
+    const float *xs[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) xs[j] = p.x_scale + (int64_t)min(m0 + 16u * j + r, p.rows - 1u) * p.xs_row;
+    f32x4 acc[S][RT][MT];
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[s][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (uint32_t b = wave; b < p.blocks; b += WAVES) {
+        i32x8 wv[S][RT], xv[MT];
+        float xf[MT], wf[S][RT];
+#pragma unroll
+        for (int s = 0; s < S; s++)
+#pragma unroll
+            for (int i = 0; i < RT; i++) {
+                wv[s][i] = load_piece(wr[s], (16u * i + r) * (uint32_t)p.w_row, b, g, p.width);
+                wf[s][i] = ws[s][i][(int64_t)b * p.ws_col];
+            }
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            xv[j] = load_piece(xr, (16u * j + r) * (uint32_t)p.x_row, b, g, p.width);
+            xf[j] = xs[j][(int64_t)b * p.xs_col];
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++)
+#pragma unroll
+            for (int s = 0; s < S; s++)
+#pragma unroll
+                for (int i = 0; i < RT; i++) {
+                    const f32x4 d = block_product(wv[s][i], xv[j]);
+                    const float f = xf[j] * wf[s][i];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[s][i][j][e] = fmaf(d[e], f, acc[s][i][j][e]);
+                }
+    }
+#pragma unroll
+    for (int s = 0; s < S; s++)
+#pragma unroll
+        for (int i = 0; i < RT; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) part[wave][(s * RT + i) * MT + j][lane] = acc[s][i][j];
+    __syncthreads();
+    for (uint32_t t = wave; t < (uint32_t)(RT * MT); t += WAVES) {
+        f32x4 y[S];
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            y[s] = part[0][s * RT * MT + t][lane];
+#pragma unroll
+            for (int v = 1; v < WAVES; v++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[s][e] += part[v][s * RT * MT + t][lane][e];
+        }
+        const uint32_t m = m0 + 16u * (t % MT) + r, n = n0 + 16u * (t / MT) + 4u * g;
+        if (m >= p.rows || n >= p.cols) continue;
+        float z[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            z[e] = y[0][e];
+            if (GATED) z[e] = z[e] / (1.f + __expf(-z[e])) * y[S - 1][e];
+            else if (p.bias) z[e] += wide16<DT>(p.bias[min(n + e, p.cols - 1u)], 0);
+        }
+        uint16_t *out = p.out + (int64_t)m * p.out_row + n;
+        const uint32_t lo = pair16<DT>(z[0], z[1]), hi = pair16<DT>(z[2], z[3]);
+        out[0] = (uint16_t)lo;
+        if (n + 1 < p.cols) out[1] = (uint16_t)(lo >> 16);
+        if (n + 2 < p.cols) out[2] = (uint16_t)hi;
+        if (n + 3 < p.cols) out[3] = (uint16_t)(hi >> 16);
+    }
+}
+
+template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
+    constexpr int RT = GATED ? 1 : 2, MT = 2, WAVES = 8;
+    const uint64_t wgs = (uint64_t)((p.cols + 16 * RT - 1) / (16 * RT)) * ((p.rows + 16 * MT - 1) / (16 * MT));
+    PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");            // (2^32 threads)
+    product_few_kernel<DT, RT, MT, WAVES, GATED><<<dim3((unsigned)wgs), 64 * WAVES, 0, s>>>(p);
+    PKV_HIP_CHECK(hipGetLastError());
+    return PKV_OK;
+}
+
+}  // namespace pkv
+
+extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
+    using namespace pkv;
+    hipStream_t s = (hipStream_t)s_;
+    PKV_REQUIRE(a && a->x && a->w && a->x_scale && a->w_scale && a->out, PKV_ERR_INVALID, "null pointer argument");
+    PKV_REQUIRE(a->dtype == PKV_F16 || a->dtype == PKV_BF16, PKV_ERR_UNSUPPORTED, "Unsupported data type");
+    PKV_REQUIRE(a->rows > 0 && a->width > 0 && a->cols > 0, PKV_ERR_INVALID, "sizes must be positive");
+    PKV_REQUIRE(a->width % 16 == 0 && a->width <= (1 << 20), PKV_ERR_UNSUPPORTED, "not supported: width %d (multiples of 16 up to 2^20)", a->width);
+    PKV_REQUIRE(a->rows <= (1 << 24) && a->cols <= (1 << 24), PKV_ERR_UNSUPPORTED, "not supported: more than 2^24 rows or results");
+    PKV_REQUIRE(!a->gated || (a->cols % 16 == 0 && !a->bias), PKV_ERR_UNSUPPORTED, "not supported: a gated product of %d results (multiples of 16, no bias)", a->cols);
+    PKV_REQUIRE((((uintptr_t)a->x | (uintptr_t)a->w | (uintptr_t)a->x_stride | (uintptr_t)a->w_stride) % 16) == 0, PKV_ERR_INVALID,
+                "rows must start on 16-byte boundaries");
+    // (a row that overlaps the next is one that the caller repeats: stride 0)
+    PKV_REQUIRE((a->x_stride == 0 || a->x_stride >= a->width) && a->x_stride <= (1 << 20) && a->w_stride >= 0 && a->w_stride <= (1 << 20) &&
+                (a->w_stride == 0 || a->w_stride >= a->width), PKV_ERR_UNSUPPORTED, "not supported: rows of x or w more than 2^20 bytes apart, or that overlap");
+    ProductParams p;
+    p.x = a->x; p.w = a->w; p.x_scale = a->x_scale; p.w_scale = a->w_scale; p.bias = (const uint16_t *)a->bias; p.out = (uint16_t *)a->out;
+    p.x_row = a->x_stride; p.w_row = a->w_stride; p.out_row = a->out_stride;
+    p.xs_row = a->x_scale_stride[0]; p.xs_col = a->x_scale_stride[1]; p.ws_row = a->w_scale_stride[0]; p.ws_col = a->w_scale_stride[1];
+    p.rows = (uint32_t)a->rows; p.width = (uint32_t)a->width; p.cols = (uint32_t)a->cols;
+    p.blocks = (p.width + kBlock8 - 1) / kBlock8;
+    if (a->gated) return a->dtype == PKV_F16 ? launch_product<PKV_F16, true>(p, s) : launch_product<PKV_BF16, true>(p, s);
+    return a->dtype == PKV_F16 ? launch_product<PKV_F16, false>(p, s) : launch_product<PKV_BF16, false>(p, s);
+}

@@ -1,6 +1,6 @@
 // The host side of the calls that a decode loop repeats, in native code: the checks, the argument block and the result
 // tensors of ops.attn_decode, AttnPlan's step, ops.window_append, ops.dense_view, the four matrix-vector ops, and ops.norm_rotary,
-// window_append_rotary, attn_chunk and sample.
+// window_append_rotary, attn_chunk, sample, add_rms_norm, fp8_quantize, fp8_linear and fp8_gated.
 //
 // A decode step is two such calls around 12 us of GPU time, and in Python their checks and ctypes' conversions take 6 to
 // 12 us each besides the launch.  Every function here serves the usual call and gives up on any other before it has done
@@ -16,6 +16,7 @@
 #include <ATen/PythonTorchFunctionTLS.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../include/packkv.h"
@@ -35,6 +36,9 @@ struct Library {                   // libpackkv_hip.so, as _lib.py has loaded it
     decltype(&pkv_attn_chunk) attn_chunk = nullptr;
     decltype(&pkv_sample_workspace) sample_workspace = nullptr;
     decltype(&pkv_sample) sample = nullptr;
+    decltype(&pkv_add_rms_norm) add_rms_norm = nullptr;
+    decltype(&pkv_fp8_quantize) fp8_quantize = nullptr;
+    decltype(&pkv_fp8_product) fp8_product = nullptr;
 } lib;
 
 // A plain torch.Tensor (a subclass, or a mode that wants to see the calls, gets the general code).
@@ -553,15 +557,181 @@ PyObject *sample(PyObject *, PyObject *const *o, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of attn_decode, window_append, dense_view, kq, wv, fused_kq, fused_wv, norm_rotary, attn_chunk_workspace, attn_chunk,
-// sample_workspace, sample)
-PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
-    void *p[12];
-    if (n != 12) {
-        PyErr_SetString(PyExc_TypeError, "twelve addresses");
+// Rows of [..., width] that lie one behind the other from a 16-byte boundary on.
+bool rows16(const at::Tensor &x, int dev) {
+    return dense(x, dev) && x.dim() >= 1 && x.numel() > 0 && x.size(-1) % 16 == 0 && reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 == 0;
+}
+// The 8-bit form's memory for [lead, width], `rows` rows in all (ops._fp8_empty), as a dict.
+struct Eight {
+    at::Tensor codes, scale;
+};
+Eight eight_empty(at::IntArrayRef lead, int64_t rows, int64_t width, int64_t block, const at::TensorOptions &like) {
+    const int64_t down = (rows + block - 1) / block;
+    c10::SmallVector<int64_t, 6> shape(lead.begin(), lead.end()), sizes, strides;
+    shape.push_back(width);
+    if (block == 1) sizes.append(lead.begin(), lead.end());
+    else sizes.push_back(down);
+    strides.resize(sizes.size());
+    int64_t step = 1;
+    for (size_t i = sizes.size(); i-- > 0; step *= sizes[i]) strides[i] = step;
+    sizes.push_back((width + 127) / 128);
+    strides.push_back(down);
+    return Eight{at::empty(shape, like.dtype(at::kFloat8_e4m3fn)), at::empty_strided(sizes, strides, like.dtype(at::kFloat))};
+}
+PyObject *const s_codes() { static PyObject *const s = PyUnicode_InternFromString("codes"); return s; }
+PyObject *const s_scale() { static PyObject *const s = PyUnicode_InternFromString("scale"); return s; }
+PyObject *eight_dict(Eight &&e) {
+    PyObject *d = PyDict_New(), *c = THPVariable_Wrap(std::move(e.codes)), *s = THPVariable_Wrap(std::move(e.scale));
+    if (!d || !c || !s || PyDict_SetItem(d, s_codes(), c) || PyDict_SetItem(d, s_scale(), s)) Py_CLEAR(d);
+    Py_XDECREF(c);
+    Py_XDECREF(s);
+    return d;
+}
+
+// add_rms_norm(x, weight, eps, residual, fp8) -> the norm (a tensor or the 8-bit form's dict), with a residual (norm, sum); a status
+// that is not zero; or None
+PyObject *add_rms_norm(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 5 && !modes() ? tensor(o[0]) : nullptr, *w = x ? tensor(o[1]) : nullptr, *res = x ? tensor(o[3]) : nullptr;
+    const int dev = here(x);
+    if (dev < 0 || !w || !half(*x) || !rows16(*x, dev) || !rows16(*w, dev) || w->dim() != 1 || w->size(0) != x->size(-1) || w->scalar_type() != x->scalar_type() ||
+        (o[4] != Py_True && o[4] != Py_False)) Py_RETURN_NONE;
+    if (o[3] != Py_None && (!res || !rows16(*res, dev) || res->sizes() != x->sizes() || res->scalar_type() != x->scalar_type())) Py_RETURN_NONE;
+    pkv_norm_args a{};
+    const int64_t width = x->size(-1), rows = x->numel() / width;
+    if (!real(o[2], &a.eps) || width > 65536 || rows >= 1 << 22) Py_RETURN_NONE;
+    at::Tensor y, sum;
+    Eight e;
+    a.x = at_ptr<void>(*x);
+    a.weight = at_ptr<void>(*w);
+    a.x_stride = width;
+    if (res) {
+        sum = at::empty(x->sizes(), x->options());
+        a.residual = at_ptr<void>(*res);
+        a.sum = at_ptr<void>(sum);
+        a.residual_stride = a.sum_stride = width;
+    }
+    if (o[4] == Py_True) {
+        e = eight_empty(x->sizes().slice(0, x->dim() - 1), rows, width, 1, x->options());
+        a.codes = at_ptr<uint8_t>(e.codes);
+        a.scale = at_ptr<float>(e.scale);
+        a.codes_stride = width;
+        a.scale_stride[0] = 1;
+        a.scale_stride[1] = rows;
+    } else {
+        y = at::empty(x->sizes(), x->options());
+        a.out = at_ptr<void>(y);
+        a.out_stride = width;
+    }
+    a.dtype = code(*x); a.rows = (int)rows; a.width = (int)width;
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.add_rms_norm(&a, s); });
+    if (rc) return status(rc);
+    PyObject *norm = o[4] == Py_True ? eight_dict(std::move(e)) : THPVariable_Wrap(std::move(y));
+    if (!res || !norm) return norm;
+    PyObject *both = PyTuple_New(2);
+    if (!both) {
+        Py_DECREF(norm);
         return nullptr;
     }
-    for (int i = 0; i < 12; i++) {
+    PyTuple_SET_ITEM(both, 0, norm);
+    PyTuple_SET_ITEM(both, 1, THPVariable_Wrap(std::move(sum)));
+    return both;
+    END_HANDLE_TH_ERRORS
+}
+
+// fp8_quantize(x, block, heads) -> the 8-bit form's dict, a status that is not zero, or None
+PyObject *fp8_quantize(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    const at::Tensor *x = n == 3 && !modes() ? tensor(o[0]) : nullptr;
+    const int dev = here(x);
+    pkv_fp8_quantize_args a{};
+    if (dev < 0 || !half(*x) || !integer(o[1], &a.block) || (a.block != 1 && (a.block != 128 || x->dim() != 2 || o[2] == Py_True)) ||
+        (o[2] != Py_True && o[2] != Py_False)) Py_RETURN_NONE;
+    int64_t rows, width;
+    c10::SmallVector<int64_t, 6> lead;
+    if (o[2] == Py_True) {
+        if (!whole_rows(*x, dev) || x->numel() == 0) Py_RETURN_NONE;
+        int64_t st[3];
+        row_strides(*x, st);
+        if ((reinterpret_cast<uintptr_t>(x->data_ptr()) | 2u * (uint64_t)(st[0] | st[1] | st[2])) % 16) Py_RETURN_NONE;
+        lead = {x->size(0), x->size(2)};
+        rows = x->size(0) * x->size(2);
+        width = x->size(1) * 128;
+        a.x_stride[0] = st[0]; a.x_stride[1] = st[2]; a.x_stride[2] = st[1];
+        a.per_batch = x->size(2) > INT_MAX ? 0 : (int)x->size(2);
+    } else {
+        if (!rows16(*x, dev)) Py_RETURN_NONE;
+        lead.append(x->sizes().begin(), x->sizes().end() - 1);
+        width = x->size(-1);
+        rows = x->numel() / width;
+        a.x_stride[1] = width; a.x_stride[2] = 128;
+        a.per_batch = rows > INT_MAX ? 0 : (int)rows;
+    }
+    if (rows > INT_MAX || width > INT_MAX) Py_RETURN_NONE;
+    Eight e = eight_empty(lead, rows, width, a.block, x->options());
+    a.x = at_ptr<void>(*x);
+    a.codes = at_ptr<uint8_t>(e.codes);
+    a.scale = at_ptr<float>(e.scale);
+    a.codes_stride = width;
+    a.scale_stride[0] = 1;
+    a.scale_stride[1] = (rows + a.block - 1) / a.block;
+    a.dtype = code(*x); a.rows = (int)rows; a.width = (int)width;
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.fp8_quantize(&a, s); });
+    return rc ? status(rc) : eight_dict(std::move(e));
+    END_HANDLE_TH_ERRORS
+}
+
+// fp8_product(x, w, bias, dtype, gated): ops.fp8_linear, or with gated ops.fp8_gated -> the result, a status that is not zero, or None
+PyObject *fp8_product(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    if (n != 5 || modes() || !PyDict_CheckExact(o[0]) || !PyDict_CheckExact(o[1]) || !THPDtype_Check(o[3]) || (o[4] != Py_True && o[4] != Py_False)) Py_RETURN_NONE;
+    const at::Tensor *xc = tensor(PyDict_GetItem(o[0], s_codes())), *xs = tensor(PyDict_GetItem(o[0], s_scale())), *wc = tensor(PyDict_GetItem(o[1], s_codes())),
+                     *ws = tensor(PyDict_GetItem(o[1], s_scale())), *bias = tensor(o[2]);
+    const int dev = here(xc);
+    const at::ScalarType type = reinterpret_cast<THPDtype *>(o[3])->scalar_type;
+    const bool gated = o[4] == Py_True;
+    if (dev < 0 || !xs || !wc || !ws || (type != at::kHalf && type != at::kBFloat16) || !rows16(*xc, dev) || !rows16(*wc, dev) || !there(*xs, dev) || !there(*ws, dev) ||
+        xc->scalar_type() != at::kFloat8_e4m3fn || wc->scalar_type() != at::kFloat8_e4m3fn || xs->scalar_type() != at::kFloat || ws->scalar_type() != at::kFloat)
+        Py_RETURN_NONE;
+    const int64_t width = xc->size(-1), rows = xc->numel() / width, blocks = (width + 127) / 128, d = xc->dim();
+    if (wc->dim() != 2 || ws->dim() != 2 || wc->size(1) != width || xs->dim() != d || xs->size(d - 1) != blocks || ws->size(1) != blocks ||
+        ws->size(0) != (wc->size(0) + 127) / 128 || width > 1 << 20 || rows > 1 << 24 || wc->size(0) > 1 << 24 || (gated && wc->size(0) % 32)) Py_RETURN_NONE;
+    for (int64_t i = 0; i < d - 1; i++)                    // one stride for all rows of scales
+        if (xs->size(i) != xc->size(i) || (i + 1 < d - 1 && xs->stride(i) != xs->stride(i + 1) * xs->size(i + 1))) Py_RETURN_NONE;
+    const int64_t cols = gated ? wc->size(0) / 2 : wc->size(0);
+    pkv_fp8_product_args a{};
+    if (o[2] != Py_None) {
+        if (!bias || !dense(*bias, dev) || bias->dim() != 1 || bias->size(0) != cols || bias->scalar_type() != type) Py_RETURN_NONE;
+        a.bias = at_ptr<void>(*bias);
+    }
+    c10::SmallVector<int64_t, 6> shape(xc->sizes().begin(), xc->sizes().end() - 1);
+    shape.push_back(cols);
+    at::Tensor out = at::empty(shape, xc->options().dtype(type));
+    a.x = at_ptr<uint8_t>(*xc); a.w = at_ptr<uint8_t>(*wc); a.x_scale = at_ptr<float>(*xs); a.w_scale = at_ptr<float>(*ws);
+    a.out = at_ptr<void>(out);
+    a.x_stride = a.w_stride = width;
+    a.out_stride = cols;
+    a.x_scale_stride[0] = d > 1 ? xs->stride(d - 2) : 0; a.x_scale_stride[1] = xs->stride(d - 1);
+    a.w_scale_stride[0] = ws->stride(0); a.w_scale_stride[1] = ws->stride(1);
+    a.dtype = type == at::kHalf ? PKV_F16 : PKV_BF16;
+    a.rows = (int)rows; a.width = (int)width; a.cols = (int)cols; a.gated = gated;
+    const pkv_stream_t s = stream(dev);
+    const int rc = call([&] { return lib.fp8_product(&a, s); });
+    return rc ? status(rc) : THPVariable_Wrap(std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
+// bind(addresses of attn_decode, window_append, dense_view, kq, wv, fused_kq, fused_wv, norm_rotary, attn_chunk_workspace, attn_chunk,
+// sample_workspace, sample, add_rms_norm, fp8_quantize, fp8_product)
+PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
+    void *p[15];
+    if (n != 15) {
+        PyErr_SetString(PyExc_TypeError, "fifteen addresses");
+        return nullptr;
+    }
+    for (int i = 0; i < 15; i++) {
         p[i] = PyLong_AsVoidPtr(o[i]);
         if (PyErr_Occurred()) return nullptr;
     }
@@ -577,6 +747,9 @@ PyObject *bind(PyObject *, PyObject *const *o, Py_ssize_t n) {
     lib.attn_chunk = (decltype(lib.attn_chunk))p[9];
     lib.sample_workspace = (decltype(lib.sample_workspace))p[10];
     lib.sample = (decltype(lib.sample))p[11];
+    lib.add_rms_norm = (decltype(lib.add_rms_norm))p[12];
+    lib.fp8_quantize = (decltype(lib.fp8_quantize))p[13];
+    lib.fp8_product = (decltype(lib.fp8_product))p[14];
     Py_RETURN_NONE;
 }
 
@@ -592,6 +765,9 @@ PyMethodDef methods[] = {
     {"window_append_rotary", (PyCFunction)(void (*)(void))window_append_rotary, METH_FASTCALL, nullptr},
     {"attn_chunk", (PyCFunction)(void (*)(void))attn_chunk, METH_FASTCALL, nullptr},
     {"sample", (PyCFunction)(void (*)(void))sample, METH_FASTCALL, nullptr},
+    {"add_rms_norm", (PyCFunction)(void (*)(void))add_rms_norm, METH_FASTCALL, nullptr},
+    {"fp8_quantize", (PyCFunction)(void (*)(void))fp8_quantize, METH_FASTCALL, nullptr},
+    {"fp8_product", (PyCFunction)(void (*)(void))fp8_product, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

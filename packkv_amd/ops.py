@@ -23,6 +23,7 @@ __all__ = [
     "quant_params", "quantize", "dequantize", "k_quant_encode", "v_quant_encode",
     "attn_decode", "AttnPlan", "block_bound", "bits_for_rel", "repack_quant_encode", "encode_status",
     "norm_rotary", "window_append_rotary", "attn_chunk", "sample",
+    "add_rms_norm", "fp8_quantize", "fp8_linear", "fp8_gated",
 ]
 
 
@@ -1306,6 +1307,159 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
             rc = lib.pkv_sample(ref, ws.data_ptr() if need else None, need, _stream(dev))
         _lib.check(rc)
     return (out, logprob) if want_logprob else out
+
+
+# ------------------------------------------------------------------ 8-bit floating point ---------
+
+def _matrix(x):
+    """x [..., width] as the 8-bit operators read it, [rows, width]: in place where its rows lie evenly and start on 16-byte boundaries."""
+    x = x.reshape(-1, x.size(-1)) if x.numel() else x.new_empty(0, x.size(-1))
+    return x if x.stride(1) == 1 and x.data_ptr() % 16 == 0 and (x.size(0) < 2 or x.stride(0) * x.element_size() % 16 == 0) else _copy(x)
+
+
+def _row(x):
+    """Elements from a row of x [rows, width] to the next."""
+    return x.stride(0) if x.size(0) > 1 else 0
+
+
+def _fp8_empty(lead, rows, width, block, dev):
+    """The 8-bit form's memory for [*lead, width] (`rows` rows in all).  The scales of a block of columns lie together: the product reads
+    them column by column."""
+    down = -(-rows // block)
+    lead = tuple(lead)
+    shape = lead if block == 1 else (down,)
+    step = [1] * len(shape)
+    for i in range(len(shape) - 2, -1, -1):
+        step[i] = step[i + 1] * max(shape[i + 1], 1)
+    scale = torch.empty_strided((*shape, -(-width // 128)), (*step, max(down, 1)), dtype=torch.float32, device=dev)
+    return {"codes": torch.empty(*lead, width, dtype=torch.float8_e4m3fn, device=dev), "scale": scale}
+
+
+def add_rms_norm(x, weight, eps=1e-6, residual=None, fp8=False):
+    """Root-mean-square norm over the last dimension of h = x + residual, h / sqrt(mean(h^2) + eps) * weight, in fp32 and rounded once.
+    x, residual [..., width] fp16 or bf16, weight [width] of the same type; width a multiple of 16, at most 65536.  Returns the norm, of x's
+    type or with fp8=True in its 8-bit form (fp8_quantize's, a scale for each 128 of a row); with a residual (norm, h), h rounded to x's type."""
+    served = _host().add_rms_norm(x, weight, eps, residual, fp8)
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
+    _require(x.is_cuda and x.dim() >= 1 and x.size(-1) > 0, "x must be a device tensor [..., width]")
+    at, dev, width = x.get_device(), x.device, x.size(-1)
+    a = _lib.NormArgs()
+    a.dtype = _dtype_code(x)
+    _require(weight.shape == (width,) and weight.dtype == x.dtype and weight.get_device() == at, "weight must be [width] of x's dtype on its device")
+    _require(residual is None or (residual.shape == x.shape and residual.dtype == x.dtype and residual.get_device() == at),
+             "residual must match x's shape, dtype and device")
+    _require(width % 16 == 0 and width <= 65536, "not supported: width %d (multiples of 16 up to 65536)" % width)
+    lead = x.shape[:-1]
+    xm, w = _matrix(x), weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else _copy(weight)
+    rows = xm.size(0)
+    rm = _matrix(residual) if residual is not None else None
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    y = _fp8_empty(lead, rows, width, 1, dev) if fp8 else torch.empty(x.shape, dtype=x.dtype, device=dev)
+    if rows:
+        a.x, a.weight, a.x_stride = xm.data_ptr(), w.data_ptr(), _row(xm)
+        if residual is not None:
+            a.residual, a.residual_stride, a.sum, a.sum_stride = rm.data_ptr(), _row(rm), h.data_ptr(), width
+        if fp8:
+            a.codes, a.codes_stride, a.scale = y["codes"].data_ptr(), width, y["scale"].data_ptr()
+            a.scale_stride[:] = 1, rows
+        else:
+            a.out, a.out_stride = y.data_ptr(), width
+        a.rows, a.width, a.eps = rows, width, eps
+        with _on(dev):
+            rc = _lib.load().pkv_add_rms_norm(ctypes.byref(a), _stream(dev))
+        _lib.check(rc)
+    return y if residual is None else (y, h)
+
+
+def fp8_quantize(x, block=1, heads=False):
+    """The 8-bit form of x [..., width] fp16 or bf16 (width a multiple of 16): a dict of ``codes``, float8_e4m3fn of x's shape, and ``scale``,
+    float32, for each block of 1 x 128 values [..., ceil(width / 128)] (activations) or, block=128 and x [rows, width], of 128 x 128
+    [ceil(rows / 128), ceil(width / 128)] (weights).  scale = max(largest finite |value|, 2^-100) / 448; a code is value / scale to the
+    nearest; infinities and NaN become NaN.  heads=True: x [B, H, n, 128], an attention's output, as the rows [B, n, H * 128]."""
+    served = _host().fp8_quantize(x, block, heads)
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
+    _require(x.is_cuda and x.dim() >= 1 and x.size(-1) > 0, "x must be a device tensor [..., width]")
+    _require(block == 1 or (block == 128 and x.dim() == 2 and not heads), "not supported: a scale for each row's 128 values, or for 128 x 128 of a matrix [rows, width]")
+    a, dev = _lib.Fp8QuantizeArgs(), x.device
+    a.dtype = _dtype_code(x)
+    if heads:
+        _require(x.dim() == 4 and x.size(3) == 128 and x.size(1) > 0, "heads: x must be [B, H, n, 128]")
+        x = x if _rows16(x, _strides(x)) else _copy(x)
+        B, H, n, _ = x.shape
+        lead, rows, width, st = (B, n), B * n, H * 128, _strides(x)
+        a.x_stride[:], a.per_batch = (st[0], st[2], st[1]), n
+    else:
+        lead, width = x.shape[:-1], x.size(-1)
+        _require(width % 16 == 0, "not supported: width %d (multiples of 16)" % width)
+        x = _matrix(x)
+        rows = x.size(0)
+        a.x_stride[:], a.per_batch = (0, _row(x), 128), rows
+    e = _fp8_empty(lead, rows, width, block, dev)
+    if rows:
+        a.x, a.codes, a.scale, a.codes_stride = x.data_ptr(), e["codes"].data_ptr(), e["scale"].data_ptr(), width
+        a.scale_stride[:] = 1, -(-rows // block)
+        a.rows, a.width, a.block = rows, width, block
+        with _on(dev):
+            rc = _lib.load().pkv_fp8_quantize(ctypes.byref(a), _stream(dev))
+        _lib.check(rc)
+    return e
+
+
+def _fp8_product(x, w, bias, dtype, gated):
+    xc, xs, wc, ws = x["codes"], x["scale"], w["codes"], w["scale"]
+    at, dev = xc.get_device(), xc.device
+    a = _lib.Fp8ProductArgs()
+    _require(xc.is_cuda and xc.dim() >= 1 and wc.dim() == 2 and xc.size(-1) == wc.size(1) > 0, "x must be [..., width] and w [rows, width] on a device")
+    _require(xc.dtype == wc.dtype == torch.float8_e4m3fn and xs.dtype == ws.dtype == torch.float32, "codes must be float8_e4m3fn and scales float32")
+    _require(all(t.get_device() == at for t in (xs, wc, ws)), _ONE_DEVICE)
+    _require(dtype in (torch.float16, torch.bfloat16), "Unsupported data type")
+    width, n = wc.size(1), wc.size(0)
+    blocks = -(-width // 128)
+    lead = xc.shape[:-1]
+    _require(xs.shape == (*lead, blocks), "x's scales must be [..., ceil(width / 128)]")
+    _require(ws.shape == (-(-n // 128), blocks), "w's scales must be [ceil(rows / 128), ceil(width / 128)]")
+    _require(width % 16 == 0 and width <= 1 << 20, "not supported: width %d (multiples of 16 up to 2^20)" % width)
+    _require(not gated or n % 32 == 0, "not supported: %d rows of gate and up (a multiple of 16 each)" % n)
+    cols = n // 2 if gated else n
+    if bias is not None:
+        _require(bias.shape == (cols,) and bias.dtype == dtype and bias.get_device() == at, "bias must be [rows of w] of the result's dtype on x's device")
+        bias = bias if bias.stride(0) == 1 else _copy(bias)
+    xc, wc, xs = _matrix(xc), _matrix(wc), xs.reshape(-1, blocks)
+    far = lambda c: c.size(0) > 1 and not (c.stride(0) == 0 or width <= c.stride(0) <= 1 << 20)
+    xc, wc = (_copy(c) if far(c) else c for c in (xc, wc))
+    rows = xc.size(0)
+    out = torch.empty(*lead, cols, dtype=dtype, device=dev)
+    if out.numel():
+        a.x, a.w, a.x_scale, a.w_scale, a.out = (t.data_ptr() for t in (xc, wc, xs, ws, out))
+        a.bias = bias.data_ptr() if bias is not None else None
+        a.x_stride, a.w_stride, a.out_stride = _row(xc), _row(wc), cols
+        a.x_scale_stride[:], a.w_scale_stride[:] = xs.stride(), ws.stride()
+        a.dtype, a.rows, a.width, a.cols, a.gated = _lib.F16 if dtype == torch.float16 else _lib.BF16, rows, width, cols, int(gated)
+        with _on(dev):
+            rc = _lib.load().pkv_fp8_product(ctypes.byref(a), _stream(dev))
+        _lib.check(rc)
+    return out
+
+
+def fp8_linear(x, w, bias=None, dtype=torch.bfloat16):
+    """x times w transposed, [..., rows of w], of x [..., width] and w [rows, width] in their 8-bit forms (fp8_quantize with block 1 and 128, or
+    add_rms_norm's), + bias, summed in fp32 and rounded once to `dtype` (fp16 or bf16; the bias has it too).  Within each eight neighbouring
+    products every one is cut to a multiple of 2^-13 of the largest's power of two: the matrix instruction's own sums."""
+    served = _host().fp8_product(x, w, bias, dtype, False)
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
+    return _fp8_product(x, w, bias, dtype, False)
+
+
+def fp8_gated(x, w, dtype=torch.bfloat16):
+    """A gated feed-forward's inside, silu(x Wg^T) * (x Wu^T), [..., rows / 2], in one pass: w [rows, width] holds the gate's rows in front of the
+    up projection's, a multiple of 16 each; the rest as in fp8_linear."""
+    served = _host().fp8_product(x, w, None, dtype, True)
+    if served is not None:
+        return _lib.check(served) if type(served) is int else served
+    return _fp8_product(x, w, None, dtype, True)
 
 
 # ------------------------------------------------- fused decompress-attention --------
