@@ -24,6 +24,7 @@ struct ProductParams {
     int64_t x_row, w_row, out_row, xs_row, xs_col, ws_row, ws_col;
     uint32_t rows, width, cols;          // of x; results a row (of w: twice as many rows where gated)
     uint32_t blocks;                     // of 128 along the width
+    bool whole4;
 };
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -46,6 +47,27 @@ __device__ __forceinline__ i32x8 load_piece(__amdgpu_buffer_rsrc_t r, uint32_t a
     const u32x4_t lo = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k < width ? at + k : kNowhere, 0, 0));
     const u32x4_t hi = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k + 64u < width ? at + k + 64u : kNowhere, 0, 0));
     return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+}
+
+// Results n .. n + 3 of row m from the sums (of gate, y, and of up, u).
+template <int DT, bool GATED> __device__ __forceinline__ void store_four(const ProductParams &p, uint32_t m, uint32_t n, f32x4 y, f32x4 u) {
+    float z[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        z[e] = y[e];
+        if (GATED) z[e] = z[e] / (1.f + __expf(-z[e])) * u[e];
+        else if (p.bias) z[e] += wide16<DT>(p.bias[min(n + e, p.cols - 1u)], 0);
+    }
+    uint16_t *out = p.out + (int64_t)m * p.out_row + n;
+    const u32x2 v = {pair16<DT>(z[0], z[1]), pair16<DT>(z[2], z[3])};
+    if (p.whole4) {                                        // rows and their ends at multiples of four results
+        *reinterpret_cast<u32x2 *>(out) = v;
+        return;
+    }
+    out[0] = (uint16_t)v[0];
+    if (n + 1 < p.cols) out[1] = (uint16_t)(v[0] >> 16);
+    if (n + 2 < p.cols) out[2] = (uint16_t)v[1];
+    if (n + 3 < p.cols) out[3] = (uint16_t)(v[1] >> 16);
 }
 
 // Few rows of x: a workgroup has 16 RT rows of weights (of gate and of up each, where gated) and 16 MT rows of x, its wavefronts
@@ -125,24 +147,156 @@ __global__ void __launch_bounds__(64 * WAVES) product_few_kernel(const ProductPa
                 for (int e = 0; e < 4; e++) y[s][e] += part[v][s * RT * MT + t][lane][e];
         }
         const uint32_t m = m0 + 16u * (t % MT) + r, n = n0 + 16u * (t / MT) + 4u * g;
-        if (m >= p.rows || n >= p.cols) continue;
-        float z[4];
+        if (m < p.rows && n < p.cols) store_four<DT, GATED>(p, m, n, y[0], y[S - 1]);
+    }
+}
+
+// 16 bytes a lane from a buffer straight into LDS at `lds` + 16 lane (the compiler sees neither the copy nor its wait, copies_done()).  The
+// s_nop: wait states between a write of a scalar operand by the compiler and its use here.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy_piece(u32x4_t rsrc, uint32_t lds, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// This wavefront's copies have arrived and its reads of LDS are done, and so for all wavefronts of the workgroup.
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+// tile_rsrc as the four words that the instruction takes.
+__device__ __forceinline__ u32x4_t tile_words(const uint8_t *base, int64_t row, uint32_t first, uint32_t rows, uint32_t count, uint32_t width) {
+    const uint32_t there = first < rows ? min(count, rows - first) : 0u;
+    const uint64_t a = (uint64_t)(reinterpret_cast<uintptr_t>(base) + (uint64_t)((int64_t)first * row));
+    return (u32x4_t){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xFFFFu),
+                     (uint32_t)__builtin_amdgcn_readfirstlane(there ? (there - 1u) * (uint32_t)row + width : 0u), 0x00020000u};
+}
+
+// Many rows of x: a workgroup of WN x WM wavefronts has 32 HN WN rows of weights (two halves: of gate and of up, where gated) and 16 MT WM rows
+// of x.  A block of the width is 128 bytes of each row, copied to LDS one block ahead of the products; piece p of row r lies at place
+// p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
+template <int DT, int HN, int MT, int WN, int WM, bool GATED>
+__global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
+    constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM, kStage = (2 * kHalf + kX) * 128;
+    constexpr int kHalfCopies = kHalf / 8 / kWaves, kXCopies = kX / 8 / kWaves;          // of 8 rows, a wavefront
+    static_assert(kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0, "whole copies");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t r = lane & 15u, g = lane >> 4;
+    // Workgroups go to the eight XCDs in turn: each takes a run of neighbouring tiles, eight rows of tiles wide, whose rows its L2 holds.
+    constexpr uint32_t kN = GATED ? kHalf : 2 * kHalf;     // results a workgroup
+    const uint32_t tiles_n = (p.cols + kN - 1u) / kN, tiles_m = (p.rows + kX - 1u) / kX;
+    const uint32_t at = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= tiles_n * tiles_m) return;
+    const uint32_t band = at / (8u * tiles_n), in_band = at - band * 8u * tiles_n, deep = min(8u, tiles_m - 8u * band);
+    const uint32_t tile_n = __builtin_amdgcn_readfirstlane(in_band / deep), tile_m = __builtin_amdgcn_readfirstlane(8u * band + (in_band - tile_n * deep));
+    const uint32_t n0 = tile_n * kN, m0 = tile_m * kX;
+    const uint32_t w_rows = (GATED ? 2u : 1u) * p.cols;
+    const uint32_t first[2] = {n0, n0 + (GATED ? p.cols : (uint32_t)kHalf)};
+    u32x4_t wr[2];
+    wr[0] = tile_words(p.w, p.w_row, first[0], p.cols, kHalf, p.width);
+    wr[1] = tile_words(p.w, p.w_row, first[1], w_rows, kHalf, p.width);
+    const u32x4_t xr = tile_words(p.x, p.x_row, m0, p.rows, kX, p.width);
+    const uint32_t wn = wave % WN, wm = wave / WN;
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
+    const uint32_t piece = 16u * ((lane & 7u) ^ (lane >> 3));
+    const uint32_t w_off = (wave * kHalfCopies * 8u + (lane >> 3)) * (uint32_t)p.w_row + piece, x_off = (wave * kXCopies * 8u + (lane >> 3)) * (uint32_t)p.x_row + piece;
+    auto copy_block = [&](uint32_t b, uint32_t stage) {
+        const uint32_t k = 128u * b, base = lds0 + stage * kStage;
+        const bool inside = k + piece < p.width;           // (a multiple of 16)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            z[e] = y[0][e];
-            if (GATED) z[e] = z[e] / (1.f + __expf(-z[e])) * y[S - 1][e];
-            else if (p.bias) z[e] += wide16<DT>(p.bias[min(n + e, p.cols - 1u)], 0);
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < kHalfCopies; t++)
+                copy_piece(wr[h], base + (h * kHalf + (wave * kHalfCopies + t) * 8) * 128, inside ? w_off + 8u * t * (uint32_t)p.w_row + k : kNowhere);
+#pragma unroll
+        for (int t = 0; t < kXCopies; t++)
+            copy_piece(xr, base + (2 * kHalf + (wave * kXCopies + t) * 8) * 128, inside ? x_off + 8u * t * (uint32_t)p.x_row + k : kNowhere);
+    };
+    const float *xs[MT], *ws[2][HN];
+#pragma unroll
+    for (int j = 0; j < MT; j++) xs[j] = p.x_scale + (int64_t)min(m0 + 16u * (wm * MT + j) + r, p.rows - 1u) * p.xs_row;
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < HN; i++) ws[h][i] = p.w_scale + (int64_t)(min(first[h] + 16u * (wn * HN + i), w_rows - 1u) / 128u) * p.ws_row;
+    f32x4 acc[2][HN][MT];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int i = 0; i < HN; i++)
+#pragma unroll
+            for (int j = 0; j < MT; j++) acc[h][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    float xf[MT], wf[2][HN];
+    auto load_scales = [&](uint32_t b) {
+#pragma unroll
+        for (int j = 0; j < MT; j++) xf[j] = xs[j][(int64_t)b * p.xs_col];
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < HN; i++) wf[h][i] = ws[h][i][(int64_t)b * p.ws_col];
+    };
+    load_scales(0);
+    copy_block(0, 0);
+    const uint32_t read0 = r * 128u + 16u * (g ^ (r & 7u));
+    auto read_rows = [&](uint32_t stage, uint32_t row) -> i32x8 {
+        const uint8_t *q = lds + stage * kStage + row * 128u;
+        const u32x4_t lo = *reinterpret_cast<const u32x4_t *>(q + read0), hi = *reinterpret_cast<const u32x4_t *>(q + (read0 ^ 64u));
+        return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    };
+    for (uint32_t b = 0; b < p.blocks; b++) {
+        const uint32_t stage = b & 1u;
+        copies_done();
+        float xn[MT], wv[2][HN];
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            xn[j] = xf[j];
+            asm volatile("" : "+v"(xn[j]));                // (waited for here, where nothing is on its way)
         }
-        uint16_t *out = p.out + (int64_t)m * p.out_row + n;
-        const uint32_t lo = pair16<DT>(z[0], z[1]), hi = pair16<DT>(z[2], z[3]);
-        out[0] = (uint16_t)lo;
-        if (n + 1 < p.cols) out[1] = (uint16_t)(lo >> 16);
-        if (n + 2 < p.cols) out[2] = (uint16_t)hi;
-        if (n + 3 < p.cols) out[3] = (uint16_t)(hi >> 16);
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < HN; i++) wv[h][i] = wf[h][i];
+        if (b + 1 < p.blocks) {
+            load_scales(b + 1);
+            copy_block(b + 1, stage ^ 1u);
+        }
+        i32x8 xv[MT];
+#pragma unroll
+        for (int j = 0; j < MT; j++) xv[j] = read_rows(stage, 2u * kHalf + 16u * (wm * MT + j));
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int i = 0; i < HN; i++) {
+                const i32x8 wq = read_rows(stage, h * kHalf + 16u * (wn * HN + i));
+#pragma unroll
+                for (int j = 0; j < MT; j++) {
+                    const f32x4 d = block_product(wq, xv[j]);
+                    const float f = xn[j] * wv[h][i];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) acc[h][i][j][e] = fmaf(d[e], f, acc[h][i][j][e]);
+                }
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        const uint32_t m = m0 + 16u * (wm * MT + j) + r;
+        if (m >= p.rows) continue;
+#pragma unroll
+        for (int i = 0; i < HN; i++)
+#pragma unroll
+            for (int h = 0; h < (GATED ? 1 : 2); h++) {
+                const uint32_t n = first[h] + 16u * (wn * HN + i) + 4u * g;
+                if (n < p.cols) store_four<DT, GATED>(p, m, n, acc[h][i][j], acc[1][i][j]);
+            }
     }
 }
 
 template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
+    if (p.rows > 512) {
+        const uint64_t n = GATED ? 128 : 256, tiles = (p.cols + n - 1) / n * ((p.rows + 255) / 256), wgs = (tiles + 7) / 8 * 8;
+        PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");        // (2^32 threads)
+        product_many_kernel<DT, 4, 4, 2, 4, GATED><<<dim3((unsigned)wgs), 512, 0, s>>>(p);
+        PKV_HIP_CHECK(hipGetLastError());
+        return PKV_OK;
+    }
     constexpr int RT = GATED ? 1 : 2, MT = 2, WAVES = 8;
     const uint64_t wgs = (uint64_t)((p.cols + 16 * RT - 1) / (16 * RT)) * ((p.rows + 16 * MT - 1) / (16 * MT));
     PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");            // (2^32 threads)
@@ -173,6 +327,7 @@ extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
     p.xs_row = a->x_scale_stride[0]; p.xs_col = a->x_scale_stride[1]; p.ws_row = a->w_scale_stride[0]; p.ws_col = a->w_scale_stride[1];
     p.rows = (uint32_t)a->rows; p.width = (uint32_t)a->width; p.cols = (uint32_t)a->cols;
     p.blocks = (p.width + kBlock8 - 1) / kBlock8;
+    p.whole4 = (p.cols | (uint64_t)a->out_stride) % 4 == 0 && (uintptr_t)a->out % 8 == 0;
     if (a->gated) return a->dtype == PKV_F16 ? launch_product<PKV_F16, true>(p, s) : launch_product<PKV_BF16, true>(p, s);
     return a->dtype == PKV_F16 ? launch_product<PKV_F16, false>(p, s) : launch_product<PKV_BF16, false>(p, s);
 }
