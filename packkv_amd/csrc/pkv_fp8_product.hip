@@ -258,22 +258,32 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
             load_scales(b + 1);
             copy_block(b + 1, stage ^ 1u);
         }
-        i32x8 xv[MT];
+        // Unit u is 16 rows of weights with all of the wavefront's x.  Its products start while the sums of unit u - 1 are scaled and added and
+        // the codes of unit u + 1 are on their way from LDS: a product of 32 cycles, then the five instructions for an earlier one.
+        i32x8 xv[MT], wq[2];
+        f32x4 d[2][MT];
+        auto read_unit = [&](int u) { wq[u & 1] = read_rows(stage, (u / HN) * kHalf + 16u * (wn * HN + u % HN)); };
+        auto add_one = [&](int u, int j) {
+            const float f = xn[j] * wv[u / HN][u % HN];
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[u / HN][u % HN][j][e] = fmaf(d[u & 1][j][e], f, acc[u / HN][u % HN][j][e]);
+        };
+        read_unit(0);
 #pragma unroll
         for (int j = 0; j < MT; j++) xv[j] = read_rows(stage, 2u * kHalf + 16u * (wm * MT + j));
 #pragma unroll
-        for (int h = 0; h < 2; h++)
+        for (int u = 0; u < 2 * HN; u++) {
+            if (u + 1 < 2 * HN) read_unit(u + 1);
+            __builtin_amdgcn_sched_barrier(0);             // (left to itself the compiler puts each sum right behind its product, and waits)
 #pragma unroll
-            for (int i = 0; i < HN; i++) {
-                const i32x8 wq = read_rows(stage, h * kHalf + 16u * (wn * HN + i));
-#pragma unroll
-                for (int j = 0; j < MT; j++) {
-                    const f32x4 d = block_product(wq, xv[j]);
-                    const float f = xn[j] * wv[h][i];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[h][i][j][e] = fmaf(d[e], f, acc[h][i][j][e]);
-                }
+            for (int j = 0; j < MT; j++) {
+                d[u & 1][j] = block_product(wq[u & 1], xv[j]);
+                if (u) add_one(u - 1, j);
+                __builtin_amdgcn_sched_barrier(0);
             }
+        }
+#pragma unroll
+        for (int j = 0; j < MT; j++) add_one(2 * HN - 1, j);
     }
 #pragma unroll
     for (int j = 0; j < MT; j++) {
