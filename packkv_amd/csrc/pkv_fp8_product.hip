@@ -158,6 +158,9 @@ __global__ void __launch_bounds__(64 * WAVES) product_few_kernel(const ProductPa
 __device__ __forceinline__ void copy_piece(u32x4_t rsrc, uint32_t lds, uint32_t off) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
 }
+__device__ __forceinline__ void copy_word(u32x4_t rsrc, uint32_t lds, uint32_t off) {           // 4 bytes a lane, to lds + 4 lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // This wavefront's copies have arrived and its reads of LDS are done, and so for all wavefronts of the workgroup.
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
@@ -174,9 +177,11 @@ __device__ __forceinline__ u32x4_t tile_words(const uint8_t *base, int64_t row, 
 // p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
 template <int DT, int HN, int MT, int WN, int WM, bool GATED>
 __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
-    constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM, kStage = (2 * kHalf + kX) * 128;
+    constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM;
+    constexpr int kScales = (2 * kHalf + kX) * 128, kStage = kScales + 4 * kX + 256;      // codes, scales of x, of each unit of weights
+    constexpr int kScaleCopies = (kX / 64 + kWaves) / kWaves;
     constexpr int kHalfCopies = kHalf / 8 / kWaves, kXCopies = kX / 8 / kWaves;          // of 8 rows, a wavefront
-    static_assert(kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0, "whole copies");
+    static_assert(kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0 && kX % 64 == 0 && 2 * kHalf <= 16 * 64, "whole copies");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
@@ -198,9 +203,30 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds);
     const uint32_t piece = 16u * ((lane & 7u) ^ (lane >> 3));
     const uint32_t w_off = (wave * kHalfCopies * 8u + (lane >> 3)) * (uint32_t)p.w_row + piece, x_off = (wave * kXCopies * 8u + (lane >> 3)) * (uint32_t)p.x_row + piece;
+    constexpr int kUnits = 2 * HN;
+    // Scales: 64 rows of x a copy, then one of the weights', a number for each 16 rows.  A wavefront has one copy or more of either kind (a copy
+    // too many repeats the weights'): no branch in the loop, past which the compiler would move the sums.
+    uint32_t scale_off[kScaleCopies];
+    uint64_t scale_base[kScaleCopies], scale_step[kScaleCopies];
+#pragma unroll
+    for (int c = 0; c < kScaleCopies; c++) {
+        const uint32_t t = wave + (uint32_t)(c * kWaves), u = min(lane, 2u * kHalf / 16u - 1u), h = u / (kHalf / 16u);
+        scale_off[c] = t < kX / 64u ? 4u * (min(m0 + 64u * t + lane, p.rows - 1u) - m0) * (uint32_t)p.xs_row
+                                    : 4u * (min((h ? first[1] : first[0]) + 16u * (u - h * (kHalf / 16u)), w_rows - 1u) / 128u) * (uint32_t)p.ws_row;
+        scale_base[c] = t < kX / 64u ? reinterpret_cast<uintptr_t>(p.x_scale + (int64_t)m0 * p.xs_row) : reinterpret_cast<uintptr_t>(p.w_scale);
+        scale_step[c] = 4u * (uint64_t)(t < kX / 64u ? p.xs_col : p.ws_col);
+        asm("" : "+s"(scale_base[c]), "+s"(scale_step[c]));              // (in registers: not to be chosen again each time)
+    }
+    const uint32_t last = p.blocks - 1u;
     auto copy_block = [&](uint32_t b, uint32_t stage) {
         const uint32_t k = 128u * b, base = lds0 + stage * kStage;
         const bool inside = k + piece < p.width;           // (a multiple of 16)
+#pragma unroll
+        for (int c = 0; c < kScaleCopies; c++) {
+            const uint32_t t = wave + (uint32_t)(c * kWaves);
+            const uint64_t a = scale_base[c] + min(b, last) * scale_step[c];
+            copy_word((u32x4_t){(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, 0x7FFFFFFFu, 0x00020000u}, base + kScales + (t < kX / 64u ? 256u * t : 4u * kX), scale_off[c]);
+        }
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
@@ -210,13 +236,6 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
         for (int t = 0; t < kXCopies; t++)
             copy_piece(xr, base + (2 * kHalf + (wave * kXCopies + t) * 8) * 128, inside ? x_off + 8u * t * (uint32_t)p.x_row + k : kNowhere);
     };
-    const float *xs[MT], *ws[2][HN];
-#pragma unroll
-    for (int j = 0; j < MT; j++) xs[j] = p.x_scale + (int64_t)min(m0 + 16u * (wm * MT + j) + r, p.rows - 1u) * p.xs_row;
-#pragma unroll
-    for (int h = 0; h < 2; h++)
-#pragma unroll
-        for (int i = 0; i < HN; i++) ws[h][i] = p.w_scale + (int64_t)(min(first[h] + 16u * (wn * HN + i), w_rows - 1u) / 128u) * p.ws_row;
     f32x4 acc[2][HN][MT];
 #pragma unroll
     for (int h = 0; h < 2; h++)
@@ -224,67 +243,79 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
         for (int i = 0; i < HN; i++)
 #pragma unroll
             for (int j = 0; j < MT; j++) acc[h][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
-    float xf[MT], wf[2][HN];
-    auto load_scales = [&](uint32_t b) {
-#pragma unroll
-        for (int j = 0; j < MT; j++) xf[j] = xs[j][(int64_t)b * p.xs_col];
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < HN; i++) wf[h][i] = ws[h][i][(int64_t)b * p.ws_col];
-    };
-    load_scales(0);
-    copy_block(0, 0);
     const uint32_t read0 = r * 128u + 16u * (g ^ (r & 7u));
     auto read_rows = [&](uint32_t stage, uint32_t row) -> i32x8 {
         const uint8_t *q = lds + stage * kStage + row * 128u;
         const u32x4_t lo = *reinterpret_cast<const u32x4_t *>(q + read0), hi = *reinterpret_cast<const u32x4_t *>(q + (read0 ^ 64u));
         return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
     };
+    // Unit u is 16 rows of weights with all of the wavefront's x.  Its products start while the sums of the unit before are scaled and added
+    // and the codes of the next are on their way from LDS: a product of 32 cycles, then the five instructions for an earlier one.  The next
+    // block is waited for in front of the last unit, whose codes are in registers by then, and read beneath its products.
+    i32x8 xv[MT], wq[2];
+    f32x4 d[MT];
+    float xn[MT], wv[kUnits], late[MT];                    // scales of this block, of the last unit's sums
+    auto read_unit = [&](uint32_t stage, int u) { wq[u & 1] = read_rows(stage, (u / HN) * kHalf + 16u * (wn * HN + u % HN)); };
+    auto add = [&](int u, int j, f32x4 v, float f) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) acc[u / HN][u % HN][j][e] = fmaf(v[e], f, acc[u / HN][u % HN][j][e]);
+    };
+    auto read_scales = [&](uint32_t stage) {
+        const float *q = reinterpret_cast<const float *>(lds + stage * kStage + kScales);
+#pragma unroll
+        for (int j = 0; j < MT; j++) xn[j] = q[16u * (wm * MT + j) + r];
+#pragma unroll
+        for (int u = 0; u < kUnits; u++) wv[u] = q[kX + (u / HN) * (kHalf / 16) + wn * HN + u % HN];
+    };
+    copy_block(0, 0);
+    copies_done();
+    copy_block(1, 1);                                      // (behind the last block zeroes, from no memory)
+    read_scales(0);
+    read_unit(0, 0);
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+        xv[j] = read_rows(0, 2u * kHalf + 16u * (wm * MT + j));
+        d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+        late[j] = 0.f;
+    }
     for (uint32_t b = 0; b < p.blocks; b++) {
         const uint32_t stage = b & 1u;
-        copies_done();
-        float xn[MT], wv[2][HN];
 #pragma unroll
-        for (int j = 0; j < MT; j++) {
-            xn[j] = xf[j];
-            asm volatile("" : "+v"(xn[j]));                // (waited for here, where nothing is on its way)
-        }
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int i = 0; i < HN; i++) wv[h][i] = wf[h][i];
-        if (b + 1 < p.blocks) {
-            load_scales(b + 1);
-            copy_block(b + 1, stage ^ 1u);
-        }
-        // Unit u is 16 rows of weights with all of the wavefront's x.  Its products start while the sums of unit u - 1 are scaled and added and
-        // the codes of unit u + 1 are on their way from LDS: a product of 32 cycles, then the five instructions for an earlier one.
-        i32x8 xv[MT], wq[2];
-        f32x4 d[2][MT];
-        auto read_unit = [&](int u) { wq[u & 1] = read_rows(stage, (u / HN) * kHalf + 16u * (wn * HN + u % HN)); };
-        auto add_one = [&](int u, int j) {
-            const float f = xn[j] * wv[u / HN][u % HN];
-#pragma unroll
-            for (int e = 0; e < 4; e++) acc[u / HN][u % HN][j][e] = fmaf(d[u & 1][j][e], f, acc[u / HN][u % HN][j][e]);
-        };
-        read_unit(0);
-#pragma unroll
-        for (int j = 0; j < MT; j++) xv[j] = read_rows(stage, 2u * kHalf + 16u * (wm * MT + j));
-#pragma unroll
-        for (int u = 0; u < 2 * HN; u++) {
-            if (u + 1 < 2 * HN) read_unit(u + 1);
+        for (int u = 0; u < kUnits - 1; u++) {
+            read_unit(stage, u + 1);
             __builtin_amdgcn_sched_barrier(0);             // (left to itself the compiler puts each sum right behind its product, and waits)
 #pragma unroll
             for (int j = 0; j < MT; j++) {
-                d[u & 1][j] = block_product(wq[u & 1], xv[j]);
-                if (u) add_one(u - 1, j);
+                const f32x4 v = d[j];
+                d[j] = block_product(wq[u & 1], xv[j]);
+                if (u) add(u - 1, j, v, xn[j] * wv[u - 1]);
+                else add(kUnits - 1, j, v, late[j]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
+        float f[MT];
 #pragma unroll
-        for (int j = 0; j < MT; j++) add_one(2 * HN - 1, j);
+        for (int j = 0; j < MT; j++) {
+            f[j] = xn[j] * wv[kUnits - 2];
+            late[j] = xn[j] * wv[kUnits - 1];
+        }
+        copies_done();                                     // (behind the last block: what is read below is not used)
+        copy_block(b + 2u, stage);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int j = 0; j < MT; j++) {
+            const f32x4 v = d[j];
+            d[j] = block_product(wq[1], xv[j]);
+            if (j == 0) read_unit(stage ^ 1u, 0);
+            xv[j] = read_rows(stage ^ 1u, 2u * kHalf + 16u * (wm * MT + j));
+            add(kUnits - 2, j, v, f[j]);
+            if (j + 1 == MT) read_scales(stage ^ 1u);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
+    copies_done();                                         // (nothing may arrive in LDS that another workgroup has by then)
+#pragma unroll
+    for (int j = 0; j < MT; j++) add(kUnits - 1, j, d[j], late[j]);
 #pragma unroll
     for (int j = 0; j < MT; j++) {
         const uint32_t m = m0 + 16u * (wm * MT + j) + r;
@@ -328,6 +359,9 @@ extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
     PKV_REQUIRE(!a->gated || (a->cols % 16 == 0 && !a->bias), PKV_ERR_UNSUPPORTED, "not supported: a gated product of %d results (multiples of 16, no bias)", a->cols);
     PKV_REQUIRE((((uintptr_t)a->x | (uintptr_t)a->w | (uintptr_t)a->x_stride | (uintptr_t)a->w_stride) % 16) == 0, PKV_ERR_INVALID,
                 "rows must start on 16-byte boundaries");
+    PKV_REQUIRE(a->x_scale_stride[0] >= 0 && a->x_scale_stride[0] <= (1 << 20) && a->w_scale_stride[0] >= 0 && a->w_scale_stride[0] <= (1 << 20) &&
+                (uint64_t)a->w_scale_stride[0] * (uint64_t)((a->gated ? 2 : 1) * (int64_t)a->cols / kBlock8 + 1) < (1u << 29), PKV_ERR_UNSUPPORTED,
+                "not supported: scales of neighbouring rows more than 2^20 apart, or of w over 2 GiB");
     // (a row that overlaps the next is one that the caller repeats: stride 0)
     PKV_REQUIRE((a->x_stride == 0 || a->x_stride >= a->width) && a->x_stride <= (1 << 20) && a->w_stride >= 0 && a->w_stride <= (1 << 20) &&
                 (a->w_stride == 0 || a->w_stride >= a->width), PKV_ERR_UNSUPPORTED, "not supported: rows of x or w more than 2^20 bytes apart, or that overlap");
