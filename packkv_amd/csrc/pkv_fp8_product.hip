@@ -218,23 +218,22 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
         asm("" : "+s"(scale_base[c]), "+s"(scale_step[c]));              // (in registers: not to be chosen again each time)
     }
     const uint32_t last = p.blocks - 1u;
-    auto copy_block = [&](uint32_t b, uint32_t stage) {
+    // Copy q of a wavefront's kCopies of block b (behind the last block: zeroes, from no memory).
+    constexpr int kCopies = kScaleCopies + 2 * kHalfCopies + kXCopies;
+    auto copy_part = [&](uint32_t b, uint32_t stage, int q) {
         const uint32_t k = 128u * b, base = lds0 + stage * kStage;
         const bool inside = k + piece < p.width;           // (a multiple of 16)
-#pragma unroll
-        for (int c = 0; c < kScaleCopies; c++) {
-            const uint32_t t = wave + (uint32_t)(c * kWaves);
-            const uint64_t a = scale_base[c] + min(b, last) * scale_step[c];
-            copy_word((u32x4_t){(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, 0x7FFFFFFFu, 0x00020000u}, base + kScales + (t < kX / 64u ? 256u * t : 4u * kX), scale_off[c]);
-        }
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-#pragma unroll
-            for (int t = 0; t < kHalfCopies; t++)
-                copy_piece(wr[h], base + (h * kHalf + (wave * kHalfCopies + t) * 8) * 128, inside ? w_off + 8u * t * (uint32_t)p.w_row + k : kNowhere);
-#pragma unroll
-        for (int t = 0; t < kXCopies; t++)
+        if (q < kScaleCopies) {
+            const uint32_t t = wave + (uint32_t)(q * kWaves);
+            const uint64_t a = scale_base[q] + min(b, last) * scale_step[q];
+            copy_word((u32x4_t){(uint32_t)a, (uint32_t)(a >> 32) & 0xFFFFu, 0x7FFFFFFFu, 0x00020000u}, base + kScales + (t < kX / 64u ? 256u * t : 4u * kX), scale_off[q]);
+        } else if (q < kScaleCopies + 2 * kHalfCopies) {
+            const int h = (q - kScaleCopies) / kHalfCopies, t = (q - kScaleCopies) % kHalfCopies;
+            copy_piece(wr[h], base + (h * kHalf + (wave * kHalfCopies + t) * 8) * 128, inside ? w_off + 8u * t * (uint32_t)p.w_row + k : kNowhere);
+        } else {
+            const int t = q - kScaleCopies - 2 * kHalfCopies;
             copy_piece(xr, base + (2 * kHalf + (wave * kXCopies + t) * 8) * 128, inside ? x_off + 8u * t * (uint32_t)p.x_row + k : kNowhere);
+        }
     };
     f32x4 acc[2][HN][MT];
 #pragma unroll
@@ -267,9 +266,11 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
 #pragma unroll
         for (int u = 0; u < kUnits; u++) wv[u] = q[kX + (u / HN) * (kHalf / 16) + wn * HN + u % HN];
     };
-    copy_block(0, 0);
+#pragma unroll
+    for (int q = 0; q < kCopies; q++) copy_part(0, 0, q);
     copies_done();
-    copy_block(1, 1);                                      // (behind the last block zeroes, from no memory)
+#pragma unroll
+    for (int q = 0; q < MT; q++) copy_part(1, 1, q);
     read_scales(0);
     read_unit(0, 0);
 #pragma unroll
@@ -290,6 +291,7 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
                 d[j] = block_product(wq[u & 1], xv[j]);
                 if (u) add(u - 1, j, v, xn[j] * wv[u - 1]);
                 else add(kUnits - 1, j, v, late[j]);
+                if (MT * (u + 1) + j < kCopies) copy_part(b + 1u, stage ^ 1u, MT * (u + 1) + j);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -300,12 +302,12 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
             late[j] = xn[j] * wv[kUnits - 1];
         }
         copies_done();                                     // (behind the last block: what is read below is not used)
-        copy_block(b + 2u, stage);
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             const f32x4 v = d[j];
             d[j] = block_product(wq[1], xv[j]);
+            copy_part(b + 2u, stage, j);                   // (one at a time: all at once the wavefronts wait to issue them, 40 us of 190)
             if (j == 0) read_unit(stage ^ 1u, 0);
             xv[j] = read_rows(stage ^ 1u, 2u * kHalf + 16u * (wm * MT + j));
             add(kUnits - 2, j, v, f[j]);
