@@ -29,26 +29,41 @@ struct ProductParams {
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+// The weights' scales are scalar loads: nothing writes them while a kernel runs.
+typedef const __attribute__((address_space(4))) float scalar_float;
 
 __device__ __forceinline__ f32x4 block_product(i32x8 w, i32x8 x) {
     const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, zero, 0, 0, 0, 0, 0, 0);
 }
 constexpr uint32_t kNowhere = 0x80000000u;             // a buffer offset behind any tile: loads give zeroes
-// Rows first .. first + count - 1 of a matrix of `rows` rows as a buffer: what lies behind its last row reads as zero.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(const uint8_t *base, int64_t row, uint32_t first, uint32_t rows, uint32_t count, uint32_t width) {
+// Rows first .. first + count - 1 of a matrix of `rows` rows as a buffer: what lies behind its last row reads as zero.  (Scalars by force: the
+// compiler would loop over the lanes of a descriptor that it formed in vector registers.)
+__device__ __forceinline__ u32x4_t tile_words(const uint8_t *base, int64_t row, uint32_t first, uint32_t rows, uint32_t count, uint32_t width) {
     const uint32_t there = first < rows ? min(count, rows - first) : 0u;
-    const uint32_t bytes = there ? (there - 1u) * (uint32_t)row + width : 0u;
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base) + (int64_t)first * row, 0, (int)bytes, 0x00020000);
+    const uint64_t a = (uint64_t)(reinterpret_cast<uintptr_t>(base) + (uint64_t)((int64_t)first * row));
+    return (u32x4_t){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xFFFFu),
+                     (uint32_t)__builtin_amdgcn_readfirstlane(there ? (there - 1u) * (uint32_t)row + width : 0u), 0x00020000u};
 }
-// A lane's 32 bytes of block b of its row (at byte `at`), pieces g and 4 + g of 16; zeroes behind the width.
-__device__ __forceinline__ i32x8 load_piece(__amdgpu_buffer_rsrc_t r, uint32_t at, uint32_t b, uint32_t g, uint32_t width) {
-    const uint32_t k = b * 128u + 16u * g;
-    const u32x4_t lo = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k < width ? at + k : kNowhere, 0, 0));
-    const u32x4_t hi = __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, k + 64u < width ? at + k + 64u : kNowhere, 0, 0));
-    return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t tile_rsrc(u32x4_t w) {
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void *>((uint64_t)w[0] | (uint64_t)w[1] << 32), 0, (int)w[2], 0x00020000);
 }
-
+// 16 bytes a lane from a buffer straight into LDS at `lds` + 16 lane (the compiler sees neither the copy nor its wait, copies_done()).  The
+// s_nop: wait states between a write of a scalar operand by the compiler and its use here.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void copy_piece(u32x4_t rsrc, uint32_t lds, uint32_t off) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+__device__ __forceinline__ void copy_word(u32x4_t rsrc, uint32_t lds, uint32_t off) {           // 4 bytes a lane, to lds + 4 lane
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+// This wavefront's copies have arrived and its reads of LDS are done, and so for all wavefronts of the workgroup.
+template <int N> __device__ __forceinline__ void copies_but() {            // (all but the last N of the wavefront's copies)
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
+}
+__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 // Results n .. n + 3 of row m from the sums (of gate, y, and of up, u).
 template <int DT, bool GATED> __device__ __forceinline__ void store_four(const ProductParams &p, uint32_t m, uint32_t n, f32x4 y, f32x4 u) {
     float z[4];
@@ -70,119 +85,131 @@ template <int DT, bool GATED> __device__ __forceinline__ void store_four(const P
     if (n + 3 < p.cols) out[3] = (uint16_t)(v[1] >> 16);
 }
 
-// Few rows of x: a workgroup has 16 RT rows of weights (of gate and of up each, where gated) and 16 MT rows of x, its wavefronts
-// take the blocks of the width in turn, straight into registers, and join their sums in LDS.
-template <int DT, int RT, int MT, int WAVES, bool GATED>
-__global__ void __launch_bounds__(64 * WAVES) product_few_kernel(const ProductParams p) {
-    constexpr int S = GATED ? 2 : 1, TILES = S * RT * MT;
-    __shared__ f32x4 part[WAVES][TILES][64];
+// Few rows of x: a workgroup has 16 RT rows of weights (of gate and of up each, where gated) and 16 MT rows of x.  Its eight wavefronts take the
+// blocks of the width in turn, each through LDS of its own, the next block on its way while one is multiplied, without a barrier until they
+// join their sums.  (Loaded straight into registers, neighbouring lanes are on different rows, and a load takes 64 cycles for the 16 of whole
+// lines: 48 x 4096 x 6144 12.5 us, 7.9 this way.  Four wavefronts with two places each: 8.7.)
+template <int DT, int RT, int MT, bool GATED>
+__global__ void __launch_bounds__(512) product_few_kernel(const ProductParams p) {
+    constexpr int WAVES = 8, S = GATED ? 2 : 1, UNITS = S * RT, TILES = UNITS * MT;
+    constexpr int kScales = (UNITS + MT) * 2048, kStage = kScales + 256;
+    constexpr int kRing = WAVES * kStage, kPart = WAVES * TILES * 1024, kLds = kRing > kPart ? kRing : kPart;
+    static_assert(MT <= 4, "64 scales of x");
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[kLds];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
-    const uint32_t tiles_n = (p.cols + 16u * RT - 1u) / (16u * RT);
-    const uint32_t tile_m = blockIdx.x / tiles_n, tile_n = blockIdx.x - tile_m * tiles_n;
+    // Workgroups go to the eight XCDs in turn: those that share rows of weights follow each other on one.
+    const uint32_t tiles_n = (p.cols + 16u * RT - 1u) / (16u * RT), tiles_m = (p.rows + 16u * MT - 1u) / (16u * MT);
+    const uint32_t at = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
+    if (at >= tiles_n * tiles_m) return;
+    const uint32_t tile_n = __builtin_amdgcn_readfirstlane(at / tiles_m), tile_m = __builtin_amdgcn_readfirstlane(at - at / tiles_m * tiles_m);
     const uint32_t n0 = tile_n * 16u * RT, m0 = tile_m * 16u * MT;
     const uint32_t w_rows = S * p.cols;
-    __amdgpu_buffer_rsrc_t wr[S];
-    const float *ws[S][RT];
+    u32x4_t wr[S];
+    scalar_float *ws[UNITS];
 #pragma unroll
     for (int s = 0; s < S; s++) {
         const uint32_t first = n0 + (uint32_t)s * p.cols;
-        wr[s] = tile_rsrc(p.w, p.w_row, first, GATED && s == 0 ? p.cols : w_rows, 16u * RT, p.width);
+        wr[s] = tile_words(p.w, p.w_row, first, GATED && s == 0 ? p.cols : w_rows, 16u * RT, p.width);
 #pragma unroll
-        for (int i = 0; i < RT; i++) ws[s][i] = p.w_scale + (int64_t)(min(first + 16u * i, w_rows - 1u) / 128u) * p.ws_row;
+        for (int i = 0; i < RT; i++) ws[s * RT + i] = (scalar_float *)(p.w_scale + (int64_t)(min(first + 16u * i, w_rows - 1u) / 128u) * p.ws_row);
     }
-    const __amdgpu_buffer_rsrc_t xr = tile_rsrc(p.x, p.x_row, m0, p.rows, 16u * MT, p.width);
-    const float *xs[MT];
+    const u32x4_t xr = tile_words(p.x, p.x_row, m0, p.rows, 16u * MT, p.width);
+    const uint32_t lds0 = (uint32_t)reinterpret_cast<uintptr_t>(lds) + wave * kStage;
+    const uint32_t piece = 16u * ((lane & 7u) ^ (lane >> 3)), w_off = (lane >> 3) * (uint32_t)p.w_row + piece, x_off = (lane >> 3) * (uint32_t)p.x_row + piece;
+    const uint32_t scale_off = 4u * (min(m0 + lane, p.rows - 1u) - m0) * (uint32_t)p.xs_row, last = p.blocks - 1u;
+    const uint64_t scale_base = reinterpret_cast<uintptr_t>(p.x_scale + (int64_t)m0 * p.xs_row);
+    auto copy_block = [&](uint32_t b) {                    // (behind the last block zeroes, from no memory)
+        const uint32_t k = 128u * b;
+        const bool inside = k + piece < p.width;           // (a multiple of 16)
 #pragma unroll
-    for (int j = 0; j < MT; j++) xs[j] = p.x_scale + (int64_t)min(m0 + 16u * j + r, p.rows - 1u) * p.xs_row;
-    f32x4 acc[S][RT][MT];
+        for (int u = 0; u < UNITS; u++)
 #pragma unroll
-    for (int s = 0; s < S; s++)
+            for (int h = 0; h < 2; h++)
+                copy_piece(wr[u / RT], lds0 + u * 2048 + h * 1024, inside ? w_off + (16u * (u % RT) + 8u * h) * (uint32_t)p.w_row + k : kNowhere);
 #pragma unroll
-        for (int i = 0; i < RT; i++)
+        for (int j = 0; j < 2 * MT; j++) copy_piece(xr, lds0 + UNITS * 2048 + j * 1024, inside ? x_off + 8u * j * (uint32_t)p.x_row + k : kNowhere);
+        const uint64_t a = scale_base + 4u * (uint64_t)(min(b, last) * p.xs_col);
+        copy_word((u32x4_t){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xFFFFu), 0x7FFFFFFFu, 0x00020000u},
+                  lds0 + kScales, scale_off);
+    };
+    f32x4 acc[UNITS][MT];
 #pragma unroll
-            for (int j = 0; j < MT; j++) acc[s][i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int u = 0; u < UNITS; u++)
+#pragma unroll
+        for (int j = 0; j < MT; j++) acc[u][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    const uint32_t read0 = r * 128u + 16u * (g ^ (r & 7u));
+    float wf[UNITS];
+    auto load_w_scales = [&](uint32_t b) {
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) wf[u] = ws[u][(int64_t)min(b, last) * p.ws_col];
+    };
+    load_w_scales(wave);
+    copy_block(wave);
+    const uint8_t *q = lds + wave * kStage;
     for (uint32_t b = wave; b < p.blocks; b += WAVES) {
-        i32x8 wv[S][RT], xv[MT];
-        float xf[MT], wf[S][RT];
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        auto read_rows = [&](int tile) -> i32x8 {
+            const u32x4_t lo = *reinterpret_cast<const u32x4_t *>(q + tile * 2048 + read0), hi = *reinterpret_cast<const u32x4_t *>(q + tile * 2048 + (read0 ^ 64u));
+            return (i32x8){(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+        };
+        i32x8 wv[UNITS], xv[MT];
+        float xf[MT], wn[UNITS];
 #pragma unroll
-        for (int s = 0; s < S; s++)
-#pragma unroll
-            for (int i = 0; i < RT; i++) {
-                wv[s][i] = load_piece(wr[s], (16u * i + r) * (uint32_t)p.w_row, b, g, p.width);
-                wf[s][i] = ws[s][i][(int64_t)b * p.ws_col];
-            }
+        for (int u = 0; u < UNITS; u++) wv[u] = read_rows(u);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
-            xv[j] = load_piece(xr, (16u * j + r) * (uint32_t)p.x_row, b, g, p.width);
-            xf[j] = xs[j][(int64_t)b * p.xs_col];
+            xv[j] = read_rows(UNITS + j);
+            xf[j] = *reinterpret_cast<const float *>(q + kScales + 4 * (16 * j + (int)r));
         }
+#pragma unroll
+        for (int u = 0; u < UNITS; u++) wn[u] = wf[u];
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (read, before the next copies take the place)
+        load_w_scales(b + WAVES);
+        copy_block(b + WAVES);
 #pragma unroll
         for (int j = 0; j < MT; j++)
 #pragma unroll
-            for (int s = 0; s < S; s++)
+            for (int u = 0; u < UNITS; u++) {
+                const f32x4 d = block_product(wv[u], xv[j]);
+                const float f = xf[j] * wn[u];
 #pragma unroll
-                for (int i = 0; i < RT; i++) {
-                    const f32x4 d = block_product(wv[s][i], xv[j]);
-                    const float f = xf[j] * wf[s][i];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) acc[s][i][j][e] = fmaf(d[e], f, acc[s][i][j][e]);
-                }
+                for (int e = 0; e < 4; e++) acc[u][j][e] = fmaf(d[e], f, acc[u][j][e]);
+            }
     }
+    copies_done();                                         // (none may arrive where the sums lie)
+    f32x4 *part = reinterpret_cast<f32x4 *>(lds);
 #pragma unroll
-    for (int s = 0; s < S; s++)
+    for (int u = 0; u < UNITS; u++)
 #pragma unroll
-        for (int i = 0; i < RT; i++)
-#pragma unroll
-            for (int j = 0; j < MT; j++) part[wave][(s * RT + i) * MT + j][lane] = acc[s][i][j];
+        for (int j = 0; j < MT; j++) part[(wave * TILES + u * MT + j) * 64 + lane] = acc[u][j];
     __syncthreads();
     for (uint32_t t = wave; t < (uint32_t)(RT * MT); t += WAVES) {
         f32x4 y[S];
 #pragma unroll
         for (int s = 0; s < S; s++) {
-            y[s] = part[0][s * RT * MT + t][lane];
+            y[s] = part[(s * RT * MT + t) * 64 + lane];
 #pragma unroll
             for (int v = 1; v < WAVES; v++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) y[s][e] += part[v][s * RT * MT + t][lane][e];
+                for (int e = 0; e < 4; e++) y[s][e] += part[(v * TILES + s * RT * MT + t) * 64 + lane][e];
         }
         const uint32_t m = m0 + 16u * (t % MT) + r, n = n0 + 16u * (t / MT) + 4u * g;
         if (m < p.rows && n < p.cols) store_four<DT, GATED>(p, m, n, y[0], y[S - 1]);
     }
 }
 
-// 16 bytes a lane from a buffer straight into LDS at `lds` + 16 lane (the compiler sees neither the copy nor its wait, copies_done()).  The
-// s_nop: wait states between a write of a scalar operand by the compiler and its use here.
-#pragma clang diagnostic push
-#pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void copy_piece(u32x4_t rsrc, uint32_t lds, uint32_t off) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
-}
-__device__ __forceinline__ void copy_word(u32x4_t rsrc, uint32_t lds, uint32_t off) {           // 4 bytes a lane, to lds + 4 lane
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dword %1, %2, 0 offen lds" :: "s"(lds), "v"(off), "s"(rsrc) : "memory", "m0");
-}
-#pragma clang diagnostic pop
-// This wavefront's copies have arrived and its reads of LDS are done, and so for all wavefronts of the workgroup.
-__device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// tile_rsrc as the four words that the instruction takes.
-__device__ __forceinline__ u32x4_t tile_words(const uint8_t *base, int64_t row, uint32_t first, uint32_t rows, uint32_t count, uint32_t width) {
-    const uint32_t there = first < rows ? min(count, rows - first) : 0u;
-    const uint64_t a = (uint64_t)(reinterpret_cast<uintptr_t>(base) + (uint64_t)((int64_t)first * row));
-    return (u32x4_t){(uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)a), (uint32_t)__builtin_amdgcn_readfirstlane((uint32_t)(a >> 32) & 0xFFFFu),
-                     (uint32_t)__builtin_amdgcn_readfirstlane(there ? (there - 1u) * (uint32_t)row + width : 0u), 0x00020000u};
-}
-
 // Many rows of x: a workgroup of WN x WM wavefronts has 32 HN WN rows of weights (two halves: of gate and of up, where gated) and 16 MT WM rows
 // of x.  A block of the width is 128 bytes of each row, copied to LDS one block ahead of the products; piece p of row r lies at place
 // p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
-template <int DT, int HN, int MT, int WN, int WM, bool GATED>
+template <int DT, int HN, int MT, int WN, int WM, int STAGES, bool GATED>
 __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
     constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM;
     constexpr int kScales = (2 * kHalf + kX) * 128, kStage = kScales + 4 * kX + 256;      // codes, scales of x, of each unit of weights
     constexpr int kScaleCopies = (kX / 64 + kWaves) / kWaves;
     constexpr int kHalfCopies = kHalf / 8 / kWaves, kXCopies = kX / 8 / kWaves;          // of 8 rows, a wavefront
     static_assert(kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0 && kX % 64 == 0 && 2 * kHalf <= 16 * 64, "whole copies");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * kStage];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
     // Workgroups go to the eight XCDs in turn: each takes a run of neighbouring tiles, eight rows of tiles wide, whose rows its L2 holds.
@@ -220,6 +247,7 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     const uint32_t last = p.blocks - 1u;
     // Copy q of a wavefront's kCopies of block b (behind the last block: zeroes, from no memory).
     constexpr int kCopies = kScaleCopies + 2 * kHalfCopies + kXCopies;
+    static_assert(kCopies >= MT && kCopies <= MT * kUnits && (STAGES - 2) * kCopies < 64, "a place for each copy, a count of six bits");
     auto copy_part = [&](uint32_t b, uint32_t stage, int q) {
         const uint32_t k = 128u * b, base = lds0 + stage * kStage;
         const bool inside = k + piece < p.width;           // (a multiple of 16)
@@ -267,10 +295,12 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
         for (int u = 0; u < kUnits; u++) wv[u] = q[kX + (u / HN) * (kHalf / 16) + wn * HN + u % HN];
     };
 #pragma unroll
-    for (int q = 0; q < kCopies; q++) copy_part(0, 0, q);
-    copies_done();
+    for (int b = 0; b + 1 < STAGES; b++)
 #pragma unroll
-    for (int q = 0; q < MT; q++) copy_part(1, 1, q);
+        for (int q = 0; q < kCopies; q++) copy_part(b, b, q);
+    copies_but<(STAGES - 2) * kCopies>();
+#pragma unroll
+    for (int q = 0; q < MT; q++) copy_part(STAGES - 1, STAGES - 1, q);
     read_scales(0);
     read_unit(0, 0);
 #pragma unroll
@@ -279,8 +309,9 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
         d[j] = (f32x4){0.f, 0.f, 0.f, 0.f};
         late[j] = 0.f;
     }
+    uint32_t stage = 0, before = STAGES - 1;               // of this block, of the one in front of it (where the block STAGES - 1 behind it goes)
     for (uint32_t b = 0; b < p.blocks; b++) {
-        const uint32_t stage = b & 1u;
+        const uint32_t next = stage + 1 == STAGES ? 0u : stage + 1u;
 #pragma unroll
         for (int u = 0; u < kUnits - 1; u++) {
             read_unit(stage, u + 1);
@@ -291,7 +322,7 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
                 d[j] = block_product(wq[u & 1], xv[j]);
                 if (u) add(u - 1, j, v, xn[j] * wv[u - 1]);
                 else add(kUnits - 1, j, v, late[j]);
-                if (MT * (u + 1) + j < kCopies) copy_part(b + 1u, stage ^ 1u, MT * (u + 1) + j);
+                if (MT * (u + 1) + j < kCopies) copy_part(b + (STAGES - 1), before, MT * (u + 1) + j);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -301,19 +332,21 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
             f[j] = xn[j] * wv[kUnits - 2];
             late[j] = xn[j] * wv[kUnits - 1];
         }
-        copies_done();                                     // (behind the last block: what is read below is not used)
+        copies_but<(STAGES - 2) * kCopies>();              // the next block is there (behind the last one, what is read below is not used)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             const f32x4 v = d[j];
             d[j] = block_product(wq[1], xv[j]);
-            copy_part(b + 2u, stage, j);                   // (one at a time: all at once the wavefronts wait to issue them, 40 us of 190)
-            if (j == 0) read_unit(stage ^ 1u, 0);
-            xv[j] = read_rows(stage ^ 1u, 2u * kHalf + 16u * (wm * MT + j));
+            copy_part(b + STAGES, stage, j);                  // (one at a time: all at once the wavefronts wait to issue them, 40 us of 190)
+            if (j == 0) read_unit(next, 0);
+            xv[j] = read_rows(next, 2u * kHalf + 16u * (wm * MT + j));
             add(kUnits - 2, j, v, f[j]);
-            if (j + 1 == MT) read_scales(stage ^ 1u);
+            if (j + 1 == MT) read_scales(next);
             __builtin_amdgcn_sched_barrier(0);
         }
+        before = stage;
+        stage = next;
     }
     copies_done();                                         // (nothing may arrive in LDS that another workgroup has by then)
 #pragma unroll
@@ -332,20 +365,61 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     }
 }
 
-template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
-    if (p.rows > 512) {
-        const uint64_t n = GATED ? 128 : 256, tiles = (p.cols + n - 1) / n * ((p.rows + 255) / 256), wgs = (tiles + 7) / 8 * 8;
-        PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");        // (2^32 threads)
-        product_many_kernel<DT, 4, 4, 2, 4, GATED><<<dim3((unsigned)wgs), 512, 0, s>>>(p);
-        PKV_HIP_CHECK(hipGetLastError());
-        return PKV_OK;
-    }
-    constexpr int RT = GATED ? 1 : 2, MT = 2, WAVES = 8;
-    const uint64_t wgs = (uint64_t)((p.cols + 16 * RT - 1) / (16 * RT)) * ((p.rows + 16 * MT - 1) / (16 * MT));
+template <int DT, bool GATED, int RT, int MT> int launch_few(const ProductParams &p, hipStream_t s) {
+    const uint64_t tiles = (uint64_t)((p.cols + 16 * RT - 1) / (16 * RT)) * ((p.rows + 16 * MT - 1) / (16 * MT)), wgs = (tiles + 7) / 8 * 8;
     PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");            // (2^32 threads)
-    product_few_kernel<DT, RT, MT, WAVES, GATED><<<dim3((unsigned)wgs), 64 * WAVES, 0, s>>>(p);
+    product_few_kernel<DT, RT, MT, GATED><<<dim3((unsigned)wgs), 512, 0, s>>>(p);
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;
+}
+template <int DT, bool GATED, int HN, int MT, int WN, int WM, int STAGES> int launch_many(const ProductParams &p, hipStream_t s) {
+    constexpr uint64_t n = (GATED ? 16 : 32) * HN * WN, m = 16 * MT * WM;
+    const uint64_t tiles = (p.cols + n - 1) / n * ((p.rows + m - 1) / m), wgs = (tiles + 7) / 8 * 8;
+    PKV_REQUIRE(wgs * (64 * WN * WM) < (1ull << 32), PKV_ERR_UNSUPPORTED, "rows x results too large");           // (threads)
+    product_many_kernel<DT, HN, MT, WN, WM, STAGES, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
+    PKV_HIP_CHECK(hipGetLastError());
+    return PKV_OK;
+}
+// Which workgroup a product gets: the one with the shortest estimate
+//     max(bytes of w / 6.4 TB/s, rounds of 256 workgroups * (blocks of the width * us a block + us a round)),
+// both times a shape's own, fitted to 120 products of 1 to 2048 rows, 896 to 12288 wide, 1024 to 24576 rows of w (0.3 % slower in the mean than the
+// best shape of each, 26 % at most).  What that is about: 48 x 4096 x 6144, 32 x 48 results a workgroup 7.9 us, 64 x 64 10.7, 128 x 64 13.6; 512 x 4096 x 6144,
+// 64 x 64 27.4, 128 x 128 21.6; 2048 x 4096 x 6144, 128 x 128 67, 256 x 256 58; one row of 4096 x 1024, 16 x 16 3.6, 32 x 32 5.1.
+struct Shape {
+    int rt, mt;                          // tiles of 16 results: of w (of gate and up each half as many, from 128 results on), of x
+    float block_us, round_us;
+};
+constexpr Shape kShapes[] = {{1, 1, .053f, .3f},  {1, 2, .070f, .6f},  {2, 2, .102f, .8f}, {2, 3, .126f, 1.4f}, {4, 2, .133f, 1.5f}, {4, 3, .155f, 2.f},
+                             {4, 4, .185f, 2.6f}, {8, 4, .463f, 1.8f}, {8, 8, .574f, 2.4f}, {16, 16, 1.6f, 5.1f}};
+template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
+    const double stream_us = (double)p.width * p.cols * (GATED ? 2 : 1) / 6.4e6;
+    double least = 0.;
+    uint64_t rounds_of = 0;
+    int best = -1;
+    for (int i = 0; i < (int)(sizeof kShapes / sizeof kShapes[0]); i++) {
+        const Shape &h = kShapes[i];
+        const bool many = h.rt >= 8;
+        if (GATED && h.rt == 4) continue;                  // (32 tiles of sums and their codes: not in registers and LDS together)
+        const uint64_t n = 16u * h.rt / (GATED && many ? 2 : 1), m = 16u * h.mt;
+        const uint64_t rounds = ((p.cols + n - 1) / n * ((p.rows + m - 1) / m) + 255) / 256;
+        double block = h.block_us, round = h.round_us;
+        if (GATED && !many) block *= 1.3 * (2 * h.rt + h.mt) / (h.rt + h.mt);
+        if (h.rt == 8 && h.mt == 8 && rounds > 1) { block = .60; round = 1.6; }          // (two workgroups a CU)
+        const double us = (double)rounds * (p.blocks * block + round), t = us > stream_us ? us : stream_us;
+        if (best < 0 || t < least) { least = t; best = i; rounds_of = rounds; }
+    }
+    switch (best) {
+    case 0: return launch_few<DT, GATED, 1, 1>(p, s);
+    case 1: return launch_few<DT, GATED, 1, 2>(p, s);
+    case 2: return launch_few<DT, GATED, 2, 2>(p, s);
+    case 3: return launch_few<DT, GATED, 2, 3>(p, s);
+    case 4: if constexpr (!GATED) return launch_few<DT, GATED, 4, 2>(p, s);
+    case 5: if constexpr (!GATED) return launch_few<DT, GATED, 4, 3>(p, s);
+    case 6: if constexpr (!GATED) return launch_few<DT, GATED, 4, 4>(p, s);
+    case 7: return launch_many<DT, GATED, 2, 1, 2, 4, 6>(p, s);
+    case 8: return rounds_of > 1 ? launch_many<DT, GATED, 2, 2, 2, 4, 2>(p, s) : launch_many<DT, GATED, 2, 2, 2, 4, 4>(p, s);
+    default: return launch_many<DT, GATED, 4, 4, 2, 4, 2>(p, s);
+    }
 }
 
 }  // namespace pkv
