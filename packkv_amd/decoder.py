@@ -14,6 +14,8 @@ return_dense=False)`` and ``cache.attend(q, layer)``, the fused decompress-atten
 attends to the dense tensors the cache returns, as the reference does.  A later prompt, several tokens on a cache that holds
 some, attends through the fused kernel too.  ``rotary="fused"`` replaces the head norms and the rotary embedding of both
 sides by ``cache.update_rotary``, one pass that rounds once; ``generate`` decodes that way and samples.
+``ShapedDecoder(weights="fp8")`` keeps the layers' projections in 8-bit floating point and computes norms, projections and the
+feed-forward through ops.add_rms_norm, fp8_quantize, fp8_linear and fp8_gated.
 """
 import math
 
@@ -42,11 +44,16 @@ def _rms(x, w, eps):
 
 
 class ShapedDecoder:
-    """Weights ~ N(0, 0.02), norm weights 1, in `dtype` on `device`; no gradients anywhere."""
+    """Weights ~ N(0, 0.02), norm weights 1, in `dtype` on `device`; no gradients anywhere.  weights="fp8": the layers' projections
+    as e4m3 codes with a scale for each 128 x 128 (ops.fp8_quantize), half the bytes of a decode step; embedding, norms and lm_head stay
+    in `dtype`.  hidden and mlp are multiples of 16 then."""
 
-    def __init__(self, shape=None, dtype=torch.bfloat16, device="cuda", seed=0):
+    def __init__(self, shape=None, dtype=torch.bfloat16, device="cuda", seed=0, weights="same"):
         self.shape = s = shape or DecoderShape()
         self.dtype, self.device = dtype, torch.device(device)
+        if weights not in ("same", "fp8"):
+            raise RuntimeError("not supported: weights %r (\"same\" as dtype, or \"fp8\")" % (weights,))
+        self.fp8 = weights == "fp8"
         g = torch.Generator(device=self.device).manual_seed(seed)
 
         def w(*dims):
@@ -68,6 +75,9 @@ class ShapedDecoder:
             blk["q_norm"], blk["k_norm"] = one(s.head_dim), one(s.head_dim)
             blk["gate_up"] = torch.cat((w(s.mlp, s.hidden), w(s.mlp, s.hidden)), dim=0)
             blk["down"] = w(s.hidden, s.mlp)
+            if self.fp8:
+                for name in ("qkv", "o", "gate_up", "down"):
+                    blk[name] = ops.fp8_quantize(blk[name], block=128)
             self.blocks.append(blk)
         inv = 1.0 / (s.rope_theta ** (torch.arange(0, s.head_dim, 2, device=self.device, dtype=torch.float32) / s.head_dim))
         self.inv_freq = inv
@@ -137,10 +147,14 @@ class ShapedDecoder:
             kw = {"cos": cos, "sin": sin}
         fused = attention == "fused" and (n == 1 or pos0 > 0)
         scaling = 1.0 / math.sqrt(s.head_dim)
-        h = self.embed[ids].view(B * n, s.hidden)
+        h, more = self.embed[ids].view(B * n, s.hidden), None      # `more`: what the last product adds to h, where that is left to the next norm
         for li, blk in enumerate(self.blocks):
-            x = _rms(h, blk["in_norm"], s.rms_eps)
-            qkv = F.linear(x, blk["qkv"]).view(B, n, s.q_heads + 2 * s.kv_heads, s.head_dim)
+            if self.fp8:
+                x, h = self._norm(h, more, blk["in_norm"], True)
+                qkv = ops.fp8_linear(x, blk["qkv"], dtype=self.dtype)
+            else:
+                qkv = F.linear(_rms(h, blk["in_norm"], s.rms_eps), blk["qkv"])
+            qkv = qkv.view(B, n, s.q_heads + 2 * s.kv_heads, s.head_dim)
             q, k, v = qkv[:, :, :s.q_heads], qkv[:, :, s.q_heads:s.q_heads + s.kv_heads], qkv[:, :, s.q_heads + s.kv_heads:]
             if one_pass:
                 q, k, v = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
@@ -153,7 +167,7 @@ class ShapedDecoder:
                     q, k = ops.norm_rotary(q, k, *how)
                     kd, vd = cache.update(k, v, li, None, return_dense=True)
                     a = self._dense_attention(q, kd, vd, scaling)
-                h = self._rest(blk, h, a, taps, q)
+                h, more = self._rest(blk, h, a, taps, q)
                 continue
             if s.head_norm:
                 q, k = _rms(q, blk["q_norm"], s.rms_eps), _rms(k, blk["k_norm"], s.rms_eps)
@@ -166,20 +180,35 @@ class ShapedDecoder:
             else:
                 kd, vd = cache.update(k, v, li, kw, return_dense=True)
                 a = self._dense_attention(q, kd, vd, scaling)
-            h = self._rest(blk, h, a, taps, q)
-        h = h.view(B, n, s.hidden)
-        h = _rms(h[:, -1], self.final_norm, s.rms_eps)
+            h, more = self._rest(blk, h, a, taps, q)
+        h = h.view(B, n, s.hidden)[:, -1]
+        if more is not None:
+            h, _ = self._norm(h, more.view(B, n, s.hidden)[:, -1], self.final_norm, False)
+        else:
+            h = _rms(h, self.final_norm, s.rms_eps)
         return F.linear(h, self.lm_head).float()
 
+    def _norm(self, h, more, w, fp8):
+        """(norm of h + more, the sum); more None: of h."""
+        if more is None:
+            return ops.add_rms_norm(h, w, self.shape.rms_eps, fp8=fp8), h
+        return ops.add_rms_norm(more, w, self.shape.rms_eps, residual=h, fp8=fp8)
+
     def _rest(self, blk, h, a, taps, q):
-        """A layer behind its attention output a [B, Hq, n, 128]."""
+        """A layer behind its attention output a [B, Hq, n, 128]: (h, what is still to be added to it or None)."""
         s = self.shape
         if taps is not None:
             taps.append((q, a))
+        if self.fp8:
+            a = ops.fp8_quantize(a, heads=True)
+            o = ops.fp8_linear(a, blk["o"], dtype=self.dtype).view(h.shape)
+            x, h = self._norm(h, o, blk["post_norm"], True)
+            x = ops.fp8_quantize(ops.fp8_gated(x, blk["gate_up"], dtype=self.dtype))
+            return h, ops.fp8_linear(x, blk["down"], dtype=self.dtype)
         h = torch.addmm(h, a.transpose(1, 2).reshape(h.size(0), s.q_heads * s.head_dim), blk["o"].t())
         x = _rms(h, blk["post_norm"], s.rms_eps)
         gu = F.linear(x, blk["gate_up"])
-        return torch.addmm(h, F.silu(gu[:, :s.mlp]) * gu[:, s.mlp:], blk["down"].t())
+        return torch.addmm(h, F.silu(gu[:, :s.mlp]) * gu[:, s.mlp:], blk["down"].t()), None
 
     @torch.no_grad()
     def prefill(self, ids, cache):
