@@ -200,15 +200,15 @@ __global__ void __launch_bounds__(512) product_few_kernel(const ProductParams p)
 }
 
 // Many rows of x: a workgroup of WN x WM wavefronts has 32 HN WN rows of weights (two halves: of gate and of up, where gated) and 16 MT WM rows
-// of x.  A block of the width is 128 bytes of each row, copied to LDS one block ahead of the products; piece p of row r lies at place
+// of x.  EVEN: all rows of a half have one block's scale.  A block of the width is 128 bytes of each row, copied to LDS STAGES - 1 blocks ahead; piece p of row r lies at place
 // p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
-template <int DT, int HN, int MT, int WN, int WM, int STAGES, bool GATED>
+template <int DT, int HN, int MT, int WN, int WM, int STAGES, bool EVEN, bool GATED>
 __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
     constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM;
     constexpr int kScales = (2 * kHalf + kX) * 128, kStage = kScales + 4 * kX + 256;      // codes, scales of x, of each unit of weights
     constexpr int kScaleCopies = (kX / 64 + kWaves) / kWaves;
     constexpr int kHalfCopies = kHalf / 8 / kWaves, kXCopies = kX / 8 / kWaves;          // of 8 rows, a wavefront
-    static_assert(kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0 && kX % 64 == 0 && 2 * kHalf <= 16 * 64, "whole copies");
+    static_assert(128 % kHalf == 0 && kHalf % (8 * kWaves) == 0 && kX % (8 * kWaves) == 0 && kX % 64 == 0 && 2 * kHalf <= 16 * 64, "whole copies");
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
@@ -247,7 +247,12 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     const uint32_t last = p.blocks - 1u;
     // Copy q of a wavefront's kCopies of block b (behind the last block: zeroes, from no memory).
     constexpr int kCopies = kScaleCopies + 2 * kHalfCopies + kXCopies;
-    static_assert(kCopies >= MT && kCopies <= MT * kUnits && (STAGES - 2) * kCopies < 64, "a place for each copy, a count of six bits");
+    // With two stages, the copies of x and the scales start as soon as all wavefronts have theirs in registers, behind a barrier of their own in
+    // the first units, and those of the weights behind the last unit: something is always on its way.
+    constexpr bool kEarly = STAGES == 2;
+    constexpr int kWCopies = 2 * kHalfCopies, kEarlyCopies = kCopies - kWCopies;
+    static_assert(kEarly ? kWCopies <= MT && kEarlyCopies <= MT * (kUnits - 2) : kCopies >= MT && kCopies <= MT * kUnits, "a place for each copy");
+    static_assert((STAGES - 2) * kCopies < 64 && kEarlyCopies < 64, "a count of six bits");
     auto copy_part = [&](uint32_t b, uint32_t stage, int q) {
         const uint32_t k = 128u * b, base = lds0 + stage * kStage;
         const bool inside = k + piece < p.width;           // (a multiple of 16)
@@ -263,6 +268,7 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
             copy_piece(xr, base + (2 * kHalf + (wave * kXCopies + t) * 8) * 128, inside ? x_off + 8u * t * (uint32_t)p.x_row + k : kNowhere);
         }
     };
+    auto copy_early = [&](uint32_t b, uint32_t stage, int i) { copy_part(b, stage, i < kScaleCopies ? i : i + kWCopies); };
     f32x4 acc[2][HN][MT];
 #pragma unroll
     for (int h = 0; h < 2; h++)
@@ -281,7 +287,8 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     // block is waited for in front of the last unit, whose codes are in registers by then, and read beneath its products.
     i32x8 xv[MT], wq[2];
     f32x4 d[MT];
-    float xn[MT], wv[kUnits], late[MT];                    // scales of this block, of the last unit's sums
+    constexpr int kW = EVEN ? 2 : kUnits, kPerW = kUnits / kW;
+    float xn[MT], wv[kW], late[MT];                        // scales of this block, of the last unit's sums
     auto read_unit = [&](uint32_t stage, int u) { wq[u & 1] = read_rows(stage, (u / HN) * kHalf + 16u * (wn * HN + u % HN)); };
     auto add = [&](int u, int j, f32x4 v, float f) {
 #pragma unroll
@@ -292,15 +299,17 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
 #pragma unroll
         for (int j = 0; j < MT; j++) xn[j] = q[16u * (wm * MT + j) + r];
 #pragma unroll
-        for (int u = 0; u < kUnits; u++) wv[u] = q[kX + (u / HN) * (kHalf / 16) + wn * HN + u % HN];
+        for (int u = 0; u < kUnits; u += kPerW) wv[u / kPerW] = q[kX + (u / HN) * (kHalf / 16) + wn * HN + u % HN];
     };
 #pragma unroll
-    for (int b = 0; b + 1 < STAGES; b++)
+    for (int b = 0; b + (kEarly ? 0 : 1) < STAGES; b++)
 #pragma unroll
         for (int q = 0; q < kCopies; q++) copy_part(b, b, q);
-    copies_but<(STAGES - 2) * kCopies>();
+    copies_but<(kEarly ? 1 : STAGES - 2) * kCopies>();
+    if (!kEarly) {
 #pragma unroll
-    for (int q = 0; q < MT; q++) copy_part(STAGES - 1, STAGES - 1, q);
+        for (int q = 0; q < MT; q++) copy_part(STAGES - 1, STAGES - 1, q);
+    }
     read_scales(0);
     read_unit(0, 0);
 #pragma unroll
@@ -320,25 +329,29 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
             for (int j = 0; j < MT; j++) {
                 const f32x4 v = d[j];
                 d[j] = block_product(wq[u & 1], xv[j]);
-                if (u) add(u - 1, j, v, xn[j] * wv[u - 1]);
+                if (u) add(u - 1, j, v, xn[j] * wv[(u - 1) / kPerW]);
                 else add(kUnits - 1, j, v, late[j]);
-                if (MT * (u + 1) + j < kCopies) copy_part(b + (STAGES - 1), before, MT * (u + 1) + j);
+                if (kEarly ? u >= 1 && MT * (u - 1) + j < kEarlyCopies : MT * (u + 1) + j < kCopies) {
+                    if (kEarly) copy_early(b + STAGES, stage, MT * (u - 1) + j);
+                    else copy_part(b + (STAGES - 1), before, MT * (u + 1) + j);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
+            if (kEarly && u == 0) asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
         }
         float f[MT];
 #pragma unroll
         for (int j = 0; j < MT; j++) {
-            f[j] = xn[j] * wv[kUnits - 2];
-            late[j] = xn[j] * wv[kUnits - 1];
+            f[j] = xn[j] * wv[(kUnits - 2) / kPerW];
+            late[j] = xn[j] * wv[kW - 1];
         }
-        copies_but<(STAGES - 2) * kCopies>();              // the next block is there (behind the last one, what is read below is not used)
+        copies_but<kEarly ? kEarlyCopies : (STAGES - 2) * kCopies>();              // the next block is there (behind the last one, what is read below is not used)
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int j = 0; j < MT; j++) {
             const f32x4 v = d[j];
             d[j] = block_product(wq[1], xv[j]);
-            copy_part(b + STAGES, stage, j);                  // (one at a time: all at once the wavefronts wait to issue them, 40 us of 190)
+            if (kEarly ? j < kWCopies : true) copy_part(b + STAGES, stage, kEarly ? kScaleCopies + j : j);          // (one at a time, as it is sent)
             if (j == 0) read_unit(next, 0);
             xv[j] = read_rows(next, 2u * kHalf + 16u * (wm * MT + j));
             add(kUnits - 2, j, v, f[j]);
@@ -376,7 +389,9 @@ template <int DT, bool GATED, int HN, int MT, int WN, int WM, int STAGES> int la
     constexpr uint64_t n = (GATED ? 16 : 32) * HN * WN, m = 16 * MT * WM;
     const uint64_t tiles = (p.cols + n - 1) / n * ((p.rows + m - 1) / m), wgs = (tiles + 7) / 8 * 8;
     PKV_REQUIRE(wgs * (64 * WN * WM) < (1ull << 32), PKV_ERR_UNSUPPORTED, "rows x results too large");           // (threads)
-    product_many_kernel<DT, HN, MT, WN, WM, STAGES, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
+    // (a half of a tile's rows of weights may have two blocks of 128, and two scales, only where up's rows start within one)
+    if (!GATED || p.cols % (16 * HN * WN) == 0) product_many_kernel<DT, HN, MT, WN, WM, STAGES, true, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
+    else if constexpr (GATED) product_many_kernel<DT, HN, MT, WN, WM, STAGES, false, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;
 }
