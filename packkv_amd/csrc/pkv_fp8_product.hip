@@ -418,15 +418,16 @@ template <int DT, bool GATED, int HN, int MT, int WN, int WM, int STAGES> int la
 }
 // Which workgroup a product gets: the one with the shortest estimate
 //     max(bytes of w / 6.4 TB/s, rounds of 256 workgroups * (blocks of the width * us a block + us a round)),
-// both times a shape's own, fitted to 120 products of 1 to 2048 rows, 896 to 12288 wide, 1024 to 24576 rows of w (0.3 % slower in the mean than the
-// best shape of each, 26 % at most).  What that is about: 48 x 4096 x 6144, 32 x 48 results a workgroup 7.9 us, 64 x 64 10.7, 128 x 64 13.6; 512 x 4096 x 6144,
-// 64 x 64 27.4, 128 x 128 21.6; 2048 x 4096 x 6144, 128 x 128 67, 256 x 256 58; one row of 4096 x 1024, 16 x 16 3.6, 32 x 32 5.1.
+// both times a shape's own, fitted to 125 products of 1 to 4096 rows, 896 to 12288 wide, 1024 to 24576 rows of w (0.5 % slower in the mean than the
+// best shape of each, 16 % at most).  What that is about, us: 48 x 4096 x 6144, 32 x 48 results a workgroup 7.9, 64 x 64 10.7, 128 x 64 13; 512 x 4096 x 6144,
+// 64 x 64 27.4, 128 x 128 20.5; 1024 x 4096 x 6144, 128 x 128 33.8, 128 x 256 30.8; 2048 x 4096 x 6144, 128 x 128 60, 256 x 256 49; one row of 4096 x 1024,
+// 16 x 16 3.6, 32 x 32 5.1.
 struct Shape {
     int rt, mt;                          // tiles of 16 results: of w (of gate and up each half as many, from 128 results on), of x
     float block_us, round_us;
 };
-constexpr Shape kShapes[] = {{1, 1, .053f, .3f},  {1, 2, .070f, .6f},  {2, 2, .102f, .8f}, {2, 3, .126f, 1.4f}, {4, 2, .133f, 1.5f}, {4, 3, .155f, 2.f},
-                             {4, 4, .185f, 2.6f}, {8, 4, .463f, 1.8f}, {8, 8, .574f, 2.4f}, {16, 16, 1.6f, 5.1f}};
+constexpr Shape kShapes[] = {{1, 1, .048f, .3f},  {1, 2, .068f, .5f},  {2, 2, .098f, .7f},  {2, 3, .133f, 1.1f},  {4, 2, .133f, 1.5f}, {4, 3, .155f, 2.f},
+                             {4, 4, .184f, 2.5f}, {8, 4, .367f, 1.1f}, {8, 8, .525f, 1.3f}, {8, 16, .843f, 3.6f}, {16, 16, 1.46f, 5.7f}};
 template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
     const double stream_us = (double)p.width * p.cols * (GATED ? 2 : 1) / 6.4e6;
     double least = 0.;
@@ -440,7 +441,7 @@ template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStre
         const uint64_t rounds = ((p.cols + n - 1) / n * ((p.rows + m - 1) / m) + 255) / 256;
         double block = h.block_us, round = h.round_us;
         if (GATED && !many) block *= 1.3 * (2 * h.rt + h.mt) / (h.rt + h.mt);
-        if (h.rt == 8 && h.mt == 8 && rounds > 1) { block = .60; round = 1.6; }          // (two workgroups a CU)
+        if (h.rt == 8 && h.mt == 8 && rounds == 1) { block = .544; round = 2.; }         // (four stages, one workgroup a CU: below)
         const double us = (double)rounds * (p.blocks * block + round), t = us > stream_us ? us : stream_us;
         if (best < 0 || t < least) { least = t; best = i; rounds_of = rounds; }
     }
@@ -452,8 +453,11 @@ template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStre
     case 4: if constexpr (!GATED) return launch_few<DT, GATED, 4, 2>(p, s);
     case 5: if constexpr (!GATED) return launch_few<DT, GATED, 4, 3>(p, s);
     case 6: if constexpr (!GATED) return launch_few<DT, GATED, 4, 4>(p, s);
-    case 7: return launch_many<DT, GATED, 2, 1, 2, 4, 6>(p, s);
+    // Stages: as many as leave two workgroups a CU where there are that many (64 rows, three of 25 KB: 256 x 2048 x 8192 10.2 us, with six 11.2), as LDS
+    // holds where there is one (128 x 128: 512 x 2048 x 8192 with two 17.7 us, with four 14.8; 2048 x 4096 x 6144, twice as many: 67, 70).
+    case 7: return launch_many<DT, GATED, 2, 1, 2, 4, 3>(p, s);
     case 8: return rounds_of > 1 ? launch_many<DT, GATED, 2, 2, 2, 4, 2>(p, s) : launch_many<DT, GATED, 2, 2, 2, 4, 4>(p, s);
+    case 9: return launch_many<DT, GATED, 2, 4, 2, 4, 3>(p, s);
     default: return launch_many<DT, GATED, 4, 4, 2, 4, 2>(p, s);
     }
 }

@@ -10,9 +10,11 @@ pytestmark = pytest.mark.gpu
 # rows of x, width, rows of w.  (What is chosen goes by the rows and columns of tiles and the blocks of the width.)
 LINEAR = [(16, 16, 1040), (20, 144, 2064), (33, 656, 1552), (20, 656, 4112), (130, 1040, 1040), (33, 656, 6161), (513, 144, 528), (65, 656, 4112), (257, 144, 1555),
           (97, 656, 4112), (1025, 272, 528), (97, 656, 6160), (1500, 272, 530), (200, 656, 4112), (130, 2064, 6160), (513, 656, 4112), (1025, 1040, 2064),
-          (1025, 656, 4113), (700, 144, 6160), (2100, 272, 4112), (1500, 16, 6160), (2100, 656, 4111), (4097, 912, 2070)]
+          (1025, 656, 4113), (700, 144, 6160), (2100, 272, 4112), (1500, 16, 6160), (2100, 656, 4111), (4097, 912, 2070), (97, 1040, 6160), (257, 1040, 3095), (2100, 656, 6160), (3001, 400, 4111),
+          (2100, 1040, 6152)]
 GATED = [(16, 16, 1040), (20, 656, 2064), (130, 144, 528), (20, 656, 4112), (130, 656, 1040), (33, 656, 4112), (97, 144, 2064), (65, 656, 6160), (257, 272, 2064),
-         (200, 656, 4112), (130, 2064, 6160), (513, 656, 4112), (700, 272, 3088), (1025, 656, 4112), (1500, 144, 3088), (2100, 16, 2064), (2500, 912, 2080)]
+         (200, 656, 4112), (130, 2064, 6160), (513, 656, 4112), (700, 272, 3088), (1025, 656, 4112), (1500, 144, 3088), (2100, 16, 2064), (2500, 912, 2080), (3001, 400, 2064),
+         (1500, 656, 6160), (65, 656, 6144), (200, 656, 4096), (1025, 656, 4096), (513, 656, 4096), (2100, 400, 6144), (97, 144, 2048)]          # (whole blocks of 128 last)
 
 
 def _whole(rows, width, block, gen, cuda):
