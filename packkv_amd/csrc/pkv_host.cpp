@@ -713,8 +713,9 @@ PyObject *fp8_product(PyObject *, PyObject *const *o, Py_ssize_t n) {
     a.out = at_ptr<void>(out);
     a.x_stride = a.w_stride = width;
     a.out_stride = cols;
-    a.x_scale_stride[0] = d > 1 ? xs->stride(d - 2) : 0; a.x_scale_stride[1] = xs->stride(d - 1);
-    a.w_scale_stride[0] = ws->stride(0); a.w_scale_stride[1] = ws->stride(1);
+    a.x_scale_stride[0] = rows > 1 ? xs->stride(d - 2) : 0; a.x_scale_stride[1] = xs->stride(d - 1);
+    a.w_scale_stride[0] = ws->size(0) > 1 ? ws->stride(0) : 0; a.w_scale_stride[1] = ws->stride(1);
+    if (a.x_scale_stride[0] > 1 << 20 || a.w_scale_stride[0] > 1 << 20) Py_RETURN_NONE;
     a.dtype = type == at::kHalf ? PKV_F16 : PKV_BF16;
     a.rows = (int)rows; a.width = (int)width; a.cols = (int)cols; a.gated = gated;
     const pkv_stream_t s = stream(dev);

@@ -1408,6 +1408,8 @@ def fp8_quantize(x, block=1, heads=False):
 
 
 def _fp8_product(x, w, bias, dtype, gated):
+    _require(all(isinstance(e, dict) and torch.is_tensor(e.get("codes")) and torch.is_tensor(e.get("scale")) for e in (x, w)),
+             "x and w must be 8-bit forms, dicts of codes and scale (fp8_quantize, add_rms_norm)")
     xc, xs, wc, ws = x["codes"], x["scale"], w["codes"], w["scale"]
     at, dev = xc.get_device(), xc.device
     a = _lib.Fp8ProductArgs()
@@ -1427,15 +1429,15 @@ def _fp8_product(x, w, bias, dtype, gated):
         _require(bias.shape == (cols,) and bias.dtype == dtype and bias.get_device() == at, "bias must be [rows of w] of the result's dtype on x's device")
         bias = bias if bias.stride(0) == 1 else _copy(bias)
     xc, wc, xs = _matrix(xc), _matrix(wc), xs.reshape(-1, blocks)
-    far = lambda c: c.size(0) > 1 and not (c.stride(0) == 0 or width <= c.stride(0) <= 1 << 20)
-    xc, wc = (_copy(c) if far(c) else c for c in (xc, wc))
+    xc, wc = (c if _row(c) == 0 or width <= _row(c) <= 1 << 20 else _copy(c) for c in (xc, wc))
+    xs, ws = (c if _row(c) <= 1 << 20 else _copy(c) for c in (xs, ws))
     rows = xc.size(0)
     out = torch.empty(*lead, cols, dtype=dtype, device=dev)
     if out.numel():
         a.x, a.w, a.x_scale, a.w_scale, a.out = (t.data_ptr() for t in (xc, wc, xs, ws, out))
         a.bias = bias.data_ptr() if bias is not None else None
         a.x_stride, a.w_stride, a.out_stride = _row(xc), _row(wc), cols
-        a.x_scale_stride[:], a.w_scale_stride[:] = xs.stride(), ws.stride()
+        a.x_scale_stride[:], a.w_scale_stride[:] = (_row(xs), xs.stride(1)), (_row(ws), ws.stride(1))
         a.dtype, a.rows, a.width, a.cols, a.gated = _lib.F16 if dtype == torch.float16 else _lib.BF16, rows, width, cols, int(gated)
         with _on(dev):
             rc = _lib.load().pkv_fp8_product(ctypes.byref(a), _stream(dev))
