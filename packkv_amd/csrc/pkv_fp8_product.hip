@@ -215,13 +215,14 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * kStage];
     const uint32_t lane = threadIdx.x & 63u, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t r = lane & 15u, g = lane >> 4;
-    // Workgroups go to the eight XCDs in turn: each takes a run of neighbouring tiles, eight rows of tiles wide, whose rows its L2 holds.
+    // Workgroups go to the eight XCDs in turn: each takes a run of neighbouring tiles, six rows of tiles wide, which is nearly
+    // square for the 32 it has at once, and its L2 holds their rows.
     constexpr uint32_t kN = GATED ? kHalf : 2 * kHalf;     // results a workgroup
     const uint32_t tiles_n = (p.cols + kN - 1u) / kN, tiles_m = (p.rows + kX - 1u) / kX;
     const uint32_t at = (blockIdx.x & 7u) * (gridDim.x >> 3) + (blockIdx.x >> 3);
     if (at >= tiles_n * tiles_m) return;
-    const uint32_t band = at / (8u * tiles_n), in_band = at - band * 8u * tiles_n, deep = min(8u, tiles_m - 8u * band);
-    const uint32_t tile_n = __builtin_amdgcn_readfirstlane(in_band / deep), tile_m = __builtin_amdgcn_readfirstlane(8u * band + (in_band - tile_n * deep));
+    const uint32_t band = at / (6u * tiles_n), in_band = at - band * 6u * tiles_n, deep = min(6u, tiles_m - 6u * band);
+    const uint32_t tile_n = __builtin_amdgcn_readfirstlane(in_band / deep), tile_m = __builtin_amdgcn_readfirstlane(6u * band + (in_band - tile_n * deep));
     const uint32_t n0 = tile_n * kN, m0 = tile_m * kX;
     const uint32_t w_rows = (GATED ? 2u : 1u) * p.cols;
     const uint32_t first[2] = {n0, n0 + (GATED ? p.cols : (uint32_t)kHalf)};
