@@ -115,22 +115,22 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
     const uint32_t row = down * 16u + (threadIdx.x >> 4), col = (blockIdx.x - down * across) * V;
     if (row >= p.rows) return;                             // (sixteen lanes together, as the exchange below)
     const uint32_t batch = row / p.per_batch;
-    const uint16_t *x = p.x + batch * p.x_batch + (int64_t)(row - batch * p.per_batch) * p.x_row + 8u * lane;
+    const uint16_t *x = p.x + batch * p.x_batch + (int64_t)(row - batch * p.per_batch) * p.x_row;
     u32x4_t v[V];
 #pragma unroll
-    for (int i = 0; i < V; i++) {
-        v[i] = (u32x4_t){0u, 0u, 0u, 0u};
-        if ((col + i) * kBlock8 + 8u * lane < p.width) v[i] = *reinterpret_cast<const u32x4_t *>(x + (int64_t)(col + i) * p.x_col);
+    for (int i = 0; i < V; i++) {                          // (behind the width the block's first chunk again, of blocks behind it the row's)
+        const uint32_t b = col + i < p.cols ? col + i : 0u;
+        v[i] = *reinterpret_cast<const u32x4_t *>(x + (int64_t)b * p.x_col + (b * kBlock8 + 8u * lane < p.width ? 8u * lane : 0u));
     }
 #pragma unroll
     for (int i = 0; i < V; i++) {
-        float y[8], most = 0.f;
+        Largest16<DT> most;
+        float y[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            y[j] = wide16<DT>(v[i][j >> 1], j & 1);
-            most = fmaxf(most, finite_size(y[j]));
-        }
-        const float s = scale_of(row16_max(most));
+        for (int j = 0; j < 4; j++) most.take(v[i][j]);
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = wide16<DT>(v[i][j >> 1], j & 1);
+        const float s = scale_of(row16_max(most.value()));
         if ((col + i) * kBlock8 + 8u * lane < p.width) {
             *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + (col + i) * kBlock8 + 8u * lane) = codes8(y, 1.f / s);
             if (lane == 0) p.scale[(int64_t)row * p.scale_row + (int64_t)(col + i) * p.scale_col] = s;
@@ -143,19 +143,19 @@ template <int DT>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantizeParams p) {
     __shared__ float part[4];
     const uint32_t down = blockIdx.x / p.cols, col = blockIdx.x - down * p.cols;
-    const uint32_t c = col * kBlock8 + 8u * (threadIdx.x & 15u);
+    const uint32_t c = col * kBlock8 + 8u * (threadIdx.x & 15u), first = down * kBlock8 + (threadIdx.x >> 4);
     u32x4_t x[8];
-    float most = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const uint32_t row = down * kBlock8 + (uint32_t)i * 16u + (threadIdx.x >> 4);
-        x[i] = (u32x4_t){0u, 0u, 0u, 0u};
-        if (row < p.rows && c < p.width) x[i] = *reinterpret_cast<const u32x4_t *>(p.x + (int64_t)row * p.x_row + c);
+    for (int i = 0; i < 8; i++) {                          // (behind the last row that row again, behind the width the block's first chunk)
+        const uint32_t row = first + (uint32_t)i * 16u;
+        x[i] = *reinterpret_cast<const u32x4_t *>(p.x + (int64_t)(row < p.rows ? row : p.rows - 1u) * p.x_row + (c < p.width ? c : col * kBlock8));
     }
+    Largest16<DT> sizes;
 #pragma unroll
     for (int i = 0; i < 8; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) most = fmaxf(most, finite_size(wide16<DT>(x[i][j >> 1], j & 1)));
+        for (int j = 0; j < 4; j++) sizes.take(x[i][j]);
+    float most = sizes.value();
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
     if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = most;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantizePara
     if (threadIdx.x == 0) p.scale[(int64_t)down * p.scale_row + (int64_t)col * p.scale_col] = s;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const uint32_t row = down * kBlock8 + (uint32_t)i * 16u + (threadIdx.x >> 4);
+        const uint32_t row = first + (uint32_t)i * 16u;
         if (row < p.rows && c < p.width) {
             float y[8];
 #pragma unroll

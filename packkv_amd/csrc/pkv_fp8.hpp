@@ -36,6 +36,20 @@ __device__ __forceinline__ float row16_max(float v) {
     v = fmaxf(v, from(std::integral_constant<int, 0x140>{}));      // 15 - lane
     return v;
 }
+// The largest |value| of 16-bit words, two at a time as integers: magnitudes in order, moved up so that infinities and NaN come out negative
+// and have no part.  (Three instructions a word; as fp32 numbers, compared and selected one by one, ten, and fp16's conversions twice.)
+template <int DT> struct Largest16 {
+    typedef short s16x2 __attribute__((ext_vector_type(2)));
+    static constexpr short kUp = (short)(DT == PKV_F16 ? 0x8000 - 0x7C00 : 0x8000 - 0x7F80);
+    s16x2 most = {kUp, kUp};
+    __device__ __forceinline__ void take(uint32_t w) {
+        most = __builtin_elementwise_max(most, __builtin_bit_cast(s16x2, w & 0x7FFF7FFFu) + (s16x2){kUp, kUp});
+    }
+    __device__ __forceinline__ float value() const {
+        const short m = most[0] > most[1] ? most[0] : most[1];
+        return wide16<DT>((uint32_t)(uint16_t)(m - kUp), 0);
+    }
+};
 // |v|, and 0 for infinities and NaN, which have no part in a block's scale.
 __device__ __forceinline__ float finite_size(float v) {
     const float a = fabsf(v);
