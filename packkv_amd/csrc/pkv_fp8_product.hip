@@ -477,6 +477,8 @@ extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
     PKV_REQUIRE(!a->gated || (a->cols % 16 == 0 && !a->bias), PKV_ERR_UNSUPPORTED, "not supported: a gated product of %d results (multiples of 16, no bias)", a->cols);
     PKV_REQUIRE((((uintptr_t)a->x | (uintptr_t)a->w | (uintptr_t)a->x_stride | (uintptr_t)a->w_stride) % 16) == 0, PKV_ERR_INVALID,
                 "rows must start on 16-byte boundaries");
+    PKV_REQUIRE(((uintptr_t)a->x_scale | (uintptr_t)a->w_scale) % 4 == 0 && ((uintptr_t)a->bias | (uintptr_t)a->out) % 2 == 0, PKV_ERR_INVALID,
+                "scales, bias and results must lie at multiples of their size");
     PKV_REQUIRE(a->x_scale_stride[0] >= 0 && a->x_scale_stride[0] <= (1 << 20) && a->w_scale_stride[0] >= 0 && a->w_scale_stride[0] <= (1 << 20) &&
                 (uint64_t)a->w_scale_stride[0] * (uint64_t)((a->gated ? 2 : 1) * (int64_t)a->cols / kBlock8 + 1) < (1u << 29), PKV_ERR_UNSUPPORTED,
                 "not supported: scales of neighbouring rows more than 2^20 apart, or of w over 2 GiB");

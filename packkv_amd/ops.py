@@ -1311,6 +1311,8 @@ def sample(logits, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, 
 
 # ------------------------------------------------------------------ 8-bit floating point ---------
 
+_LARGE_FP8 = "rows x width too large"
+
 def _matrix(x):
     """x [..., width] as the 8-bit operators read it, [rows, width]: in place where its rows lie evenly and start on 16-byte boundaries."""
     x = x.reshape(-1, x.size(-1)) if x.numel() else x.new_empty(0, x.size(-1))
@@ -1337,7 +1339,7 @@ def _fp8_empty(lead, rows, width, block, dev):
 
 def add_rms_norm(x, weight, eps=1e-6, residual=None, fp8=False):
     """Root-mean-square norm over the last dimension of h = x + residual, h / sqrt(mean(h^2) + eps) * weight, in fp32 and rounded once.
-    x, residual [..., width] fp16 or bf16, weight [width] of the same type; width a multiple of 16, at most 65536.  Returns the norm, of x's
+    x, residual [..., width] fp16 or bf16, weight [width] of the same type; width a multiple of 16, at most 65536, fewer than 2^22 rows.  Returns the norm, of x's
     type or with fp8=True in its 8-bit form (fp8_quantize's, a scale for each 128 of a row); with a residual (norm, h), h rounded to x's type."""
     served = _host().add_rms_norm(x, weight, eps, residual, fp8)
     if served is not None:
@@ -1351,6 +1353,7 @@ def add_rms_norm(x, weight, eps=1e-6, residual=None, fp8=False):
              "residual must match x's shape, dtype and device")
     _require(width % 16 == 0 and width <= 65536, "not supported: width %d (multiples of 16 up to 65536)" % width)
     lead = x.shape[:-1]
+    _require(x.numel() < width << 22, "not supported: %d rows (fewer than 2^22)" % (x.numel() // width))
     xm, w = _matrix(x), weight if weight.stride(0) == 1 and weight.data_ptr() % 16 == 0 else _copy(weight)
     rows = xm.size(0)
     rm = _matrix(residual) if residual is not None else None
@@ -1389,13 +1392,16 @@ def fp8_quantize(x, block=1, heads=False):
         x = x if _rows16(x, _strides(x)) else _copy(x)
         B, H, n, _ = x.shape
         lead, rows, width, st = (B, n), B * n, H * 128, _strides(x)
+        _require(rows < 1 << 31, _LARGE_FP8)
         a.x_stride[:], a.per_batch = (st[0], st[2], st[1]), n
     else:
         lead, width = x.shape[:-1], x.size(-1)
         _require(width % 16 == 0, "not supported: width %d (multiples of 16)" % width)
+        _require(x.numel() < width << 31, _LARGE_FP8)
         x = _matrix(x)
         rows = x.size(0)
         a.x_stride[:], a.per_batch = (0, _row(x), 128), rows
+    _require(width < 1 << 31, _LARGE_FP8)
     e = _fp8_empty(lead, rows, width, block, dev)
     if rows:
         a.x, a.codes, a.scale, a.codes_stride = x.data_ptr(), e["codes"].data_ptr(), e["scale"].data_ptr(), width
@@ -1425,6 +1431,7 @@ def _fp8_product(x, w, bias, dtype, gated):
     _require(width % 16 == 0 and width <= 1 << 20, "not supported: width %d (multiples of 16 up to 2^20)" % width)
     _require(not gated or n % 32 == 0, "not supported: %d rows of gate and up (a multiple of 16 each)" % n)
     cols = n // 2 if gated else n
+    _require(xc.numel() <= width << 24 and n <= 1 << 24, "not supported: more than 2^24 rows or results")
     if bias is not None:
         _require(bias.shape == (cols,) and bias.dtype == dtype and bias.get_device() == at, "bias must be [rows of w] of the result's dtype on x's device")
         bias = bias if bias.stride(0) == 1 else _copy(bias)

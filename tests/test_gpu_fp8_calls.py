@@ -213,3 +213,18 @@ def test_refusals(cuda):
     for call, text in bad:
         with pytest.raises(RuntimeError, match=text):
             call()
+
+
+def test_sizes_past_an_int_are_refused(cuda):
+    """Not taken for what is left of them in 32 bits: 2^32 + 4 rows (one row, repeated) for 4, a width of 2^32 + 16 for 16."""
+    rows = (1 << 32) + 4
+    h, one = torch.zeros(1, 16, dtype=torch.float16, device=cuda), torch.ones(16, dtype=torch.float16, device=cuda)
+    e = lambda n, f: {"codes": h.to(oracle.F8).expand(n, 16), "scale": torch.ones(1, 1, device=cuda).expand(f, 1)}
+    for call, text in ((lambda: ops.add_rms_norm(h.expand(rows, 16), one), "rows"), (lambda: ops.add_rms_norm(h.expand(1 << 22, 16), one, fp8=True), "rows"),
+                       (lambda: ops.fp8_quantize(h.expand(rows, 16)), "too large"), (lambda: ops.fp8_quantize(h.expand(rows, 16), block=128), "too large"),
+                       (lambda: ops.fp8_quantize(torch.empty(1, 1, 1, 128, dtype=torch.float16, device=cuda).expand(1 << 20, 1, 1 << 12, 128), heads=True), "too large"),
+                       (lambda: ops.fp8_quantize(torch.empty((1 << 32) + 16, dtype=torch.float16, device=cuda)), "too large"),
+                       (lambda: ops.fp8_linear(e(rows, rows), e(16, 1)), "2^24"), (lambda: ops.fp8_linear(e(2, 2), e(rows, (rows + 127) // 128)), "2^24"),
+                       (lambda: ops.fp8_gated(e(2, 2), e(rows + 28, (rows + 28 + 127) // 128)), "2^24")):
+        with pytest.raises(RuntimeError, match=text.replace("^", "\\^")):
+            call()

@@ -88,3 +88,10 @@ def test_product_checks_its_arguments():
                            ({"x_stride": (1 << 20) + 16}, "UNSUPPORTED", b"2^20"), ({"rows": 1 << 24, "cols": 1 << 24}, "UNSUPPORTED", b"too large")):
         got, said = _status(call, _product, **kw)
         assert got == getattr(_lib, "ERR_" + code) and text in said, (kw, got, said)
+
+
+def test_product_checks_what_its_numbers_lie_at():
+    call = _lib.load().pkv_fp8_product
+    for f, at in (("x_scale", 4098), ("w_scale", 4097), ("bias", 4097), ("out", 4097)):
+        got, said = _status(call, _product, **{f: at})
+        assert got == _lib.ERR_INVALID and b"multiples of their size" in said, (f, got, said)
