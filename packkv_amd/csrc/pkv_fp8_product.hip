@@ -370,34 +370,40 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
 #pragma unroll
     for (int j = 0; j < MT; j++) add(kUnits - 1, j, d[j], late[j]);
     // A lane has four neighbouring results of a row.  Through LDS, each wavefront in a part of its own, the rows' pieces are put together to whole
-    // lines: stored as they are, 4096 x 4096 results take 14 us, so 7.
+    // lines: stored as they are, 4096 x 4096 results take 14 us, so 5.  Pieces that are not there go nowhere, without a branch (with one a store,
+    // 4096 x 4096 x 12288 178 us, so 167.6); a row of tiles at once where it fills lines, or all of the wavefront's (4096 x 4096 x 4096 56.7 us and 57.4;
+    // 512 x 4096 x 6144, half lines, 19.2 and 18.9).
     constexpr int kRow = 32 * HN, kPitch = kRow + 16, kLanes = kRow / 16, kRows = 64 / kLanes;       // bytes, lanes of a row, rows of a store
-    static_assert(kWaves * 16 * MT * kPitch <= STAGES * kStage, "room for the results");
-    uint8_t *own = lds + wave * (16 * MT * kPitch);
+    constexpr int kSlice = HN == 4 ? 1 : MT;               // of 16 rows
+    static_assert(kWaves * 16 * kSlice * kPitch <= STAGES * kStage, "room for the results");
+    uint8_t *own = lds + wave * (16 * kSlice * kPitch);
+    const uint32_t m_w = m0 + 16u * MT * wm, pitch = 2u * (uint32_t)p.out_row;
+    const auto out = __builtin_amdgcn_make_buffer_rsrc(p.out + (int64_t)m_w * p.out_row, 0, (int)(m_w < p.rows ? min(p.rows - m_w, 16u * MT) * pitch : 0u), 0x00020000);
 #pragma unroll
     for (int h = 0; h < (GATED ? 1 : 2); h++) {
-        const uint32_t n_h = first[h] + 16u * (wn * HN);
+        const uint32_t n_h = first[h] + 16u * (wn * HN), n_l = n_h + 8u * (lane % kLanes), off = n_l < p.cols ? lane / kLanes * pitch + 2u * n_l : kNowhere;
 #pragma unroll
-        for (int i = 0; i < HN; i++)
+        for (int j0 = 0; j0 < MT; j0 += kSlice) {
 #pragma unroll
-            for (int j = 0; j < MT; j++) {
-                const uint32_t m = m0 + 16u * (wm * MT + j) + r, n = n_h + 16u * i + 4u * g;
-                const u32x2 v = four_results<DT, GATED>(p, n, acc[h][i][j], acc[1][i][j]);
-                if (p.whole8) *reinterpret_cast<u32x2 *>(own + (16 * j + r) * kPitch + 32 * i + 8 * g) = v;
-                else if (m < p.rows && n < p.cols) store_four(p, m, n, v);
+            for (int i = 0; i < HN; i++)
+#pragma unroll
+                for (int j = j0; j < j0 + kSlice; j++) {
+                    const uint32_t m = m0 + 16u * (wm * MT + j) + r, n = n_h + 16u * i + 4u * g;
+                    const u32x2 v = four_results<DT, GATED>(p, n, acc[h][i][j], acc[1][i][j]);
+                    if (p.whole8) *reinterpret_cast<u32x2 *>(own + (16 * (j - j0) + r) * kPitch + 32 * i + 8 * g) = v;
+                    else if (m < p.rows && n < p.cols) store_four(p, m, n, v);
+                }
+            if (!p.whole8) continue;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the wavefront's own: no barrier)
+#pragma unroll
+            for (int t = 0; t < 16 * kSlice / kRows; t++) {
+                const u32x4_t v = *reinterpret_cast<const u32x4_t *>(own + ((uint32_t)(t * kRows) + lane / kLanes) * kPitch + 16u * (lane % kLanes));
+                const uint32_t to = off + (16u * j0 + (uint32_t)(t * kRows)) * pitch;
+                if (p.past) __builtin_amdgcn_raw_buffer_store_b128(v, out, to, 0, 2);
+                else __builtin_amdgcn_raw_buffer_store_b128(v, out, to, 0, 0);
             }
-        if (!p.whole8) continue;
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); // (the wavefront's own: no barrier)
-#pragma unroll
-        for (int t = 0; t < 16 * MT / kRows; t++) {
-            const uint32_t row = (uint32_t)(t * kRows) + lane / kLanes, m = m0 + 16u * (wm * MT) + row, n = n_h + 8u * (lane % kLanes);
-            const u32x4_t v = *reinterpret_cast<const u32x4_t *>(own + row * kPitch + 16u * (lane % kLanes));
-            if (m >= p.rows || n >= p.cols) continue;
-            u32x4_t *out = reinterpret_cast<u32x4_t *>(p.out + (int64_t)m * p.out_row + n);
-            if (p.past) __builtin_nontemporal_store(v, out);
-            else *out = v;
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
@@ -494,7 +500,7 @@ extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
     p.whole4 = (p.cols | (uint64_t)a->out_stride) % 4 == 0 && (uintptr_t)a->out % 8 == 0;
     // Results that no L2 would hold until they are read: 1024 x 128 x 6144 (12.6 MB) 7.5 -> 6.7 us, 4096 x 4096 x 4096 (33.5 MB) 59.5 -> 58.2.
     p.past = (uint64_t)p.rows * p.cols * 2u > (4u << 20);
-    p.whole8 = (p.cols | (uint64_t)a->out_stride) % 8 == 0 && (uintptr_t)a->out % 16 == 0;
+    p.whole8 = (p.cols | (uint64_t)a->out_stride) % 8 == 0 && (uintptr_t)a->out % 16 == 0 && a->out_stride >= 0 && a->out_stride <= (1 << 23);       // (64 rows within 2^30 bytes)
     if (a->gated) return a->dtype == PKV_F16 ? launch_product<PKV_F16, true>(p, s) : launch_product<PKV_BF16, true>(p, s);
     return a->dtype == PKV_F16 ? launch_product<PKV_F16, false>(p, s) : launch_product<PKV_BF16, false>(p, s);
 }
