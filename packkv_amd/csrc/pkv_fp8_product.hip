@@ -92,7 +92,8 @@ __device__ __forceinline__ void store_four(const ProductParams &p, uint32_t m, u
 // Few rows of x: a workgroup has 16 RT rows of weights (of gate and of up each, where gated) and 16 MT rows of x.  Its eight wavefronts take the
 // blocks of the width in turn, each through LDS of its own, the next block on its way while one is multiplied, without a barrier until they
 // join their sums.  (Loaded straight into registers, neighbouring lanes are on different rows, and a load takes 64 cycles for the 16 of whole
-// lines: 48 x 4096 x 6144 12.5 us, 7.9 this way.  Four wavefronts with two places each: 8.7.)
+// lines: 48 x 4096 x 6144 12.5 us, 7.9 this way.  Four wavefronts with two places each: 8.7.)  Bound by the weights' bytes, 1 x 12288 x 4096 9.4 us (5.4 TB/s),
+// 1 x 4096 x 2 x 12288 gated 17.3 (5.8), and by the launch and the first blocks' way from memory where those are few.
 template <int DT, int RT, int MT, bool GATED>
 __global__ void __launch_bounds__(512) product_few_kernel(const ProductParams p) {
     constexpr int WAVES = 8, S = GATED ? 2 : 1, UNITS = S * RT, TILES = UNITS * MT;
@@ -206,6 +207,10 @@ __global__ void __launch_bounds__(512) product_few_kernel(const ProductParams p)
 // Many rows of x: a workgroup of WN x WM wavefronts has 32 HN WN rows of weights (two halves: of gate and of up, where gated) and 16 MT WM rows
 // of x.  EVEN: all rows of a half have one block's scale.  A block of the width is 128 bytes of each row, copied to LDS STAGES - 1 blocks ahead; piece p of row r lies at place
 // p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
+// 256 x 256 results take 2048 cycles a block of the matrix units, as many of the copies (a CU gets 32 bytes a cycle from L2), and 2300 of
+// a SIMD's issue slots (a product takes 16 of its 32 cycles', the 160 other vector instructions 4 each); together about 2750, at 1.8 GHz: the clock
+// falls with the matrix units' load.  4096 x 12288 x 4096 161 us (2.56 PFLOP/s), gated 4096 x 4096 x 2 x 12288 337 us (2.44), 4096 x 4096 x 4096 56.7 us; nine
+// vector instructions fewer with moving descriptors instead, 166 us for 162.
 template <int DT, int HN, int MT, int WN, int WM, int STAGES, bool EVEN, bool GATED>
 __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
     constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM;
