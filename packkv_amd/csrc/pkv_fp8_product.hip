@@ -431,8 +431,8 @@ template <int DT, bool GATED, int HN, int MT, int WN, int WM, int STAGES> int la
 }
 // Which workgroup a product gets: the one with the shortest estimate
 //     max(bytes of w / 6.4 TB/s, rounds of 256 workgroups * (blocks of the width * us a block + us a round)),
-// both times a shape's own, fitted to 125 products of 1 to 4096 rows, 896 to 12288 wide, 1024 to 24576 rows of w (0.5 % slower in the mean than the
-// best shape of each, 16 % at most).  What that is about, us: 48 x 4096 x 6144, 32 x 48 results a workgroup 7.9, 64 x 64 10.7, 128 x 64 13; 512 x 4096 x 6144,
+// both times a shape's own, fitted to 125 products of 1 to 4096 rows, 896 to 12288 wide, 1024 to 24576 rows of w (0.2 % slower in the mean than the
+// best shape of each, 6 % at most).  What that is about, us: 48 x 4096 x 6144, 32 x 48 results a workgroup 7.9, 64 x 64 10.7, 128 x 64 13; 512 x 4096 x 6144,
 // 64 x 64 27.4, 128 x 128 20.5; 1024 x 4096 x 6144, 128 x 128 33.8, 128 x 256 30.8; 2048 x 4096 x 6144, 128 x 128 60, 256 x 256 49; one row of 4096 x 1024,
 // 16 x 16 3.6, 32 x 32 5.1.
 struct Shape {
@@ -440,7 +440,7 @@ struct Shape {
     float block_us, round_us;
 };
 constexpr Shape kShapes[] = {{1, 1, .048f, .3f},  {1, 2, .068f, .5f},  {2, 2, .098f, .7f},  {2, 3, .133f, 1.1f},  {4, 2, .133f, 1.5f}, {4, 3, .155f, 2.f},
-                             {4, 4, .184f, 2.5f}, {8, 4, .367f, 1.1f}, {8, 8, .525f, 1.3f}, {8, 16, .843f, 3.6f}, {16, 16, 1.46f, 5.7f}};
+                             {4, 4, .184f, 2.5f}, {8, 4, .377f, 1.1f}, {8, 8, .521f, 1.3f}, {8, 16, .855f, 3.f}, {16, 16, 1.46f, 4.3f}};
 template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStream_t s) {
     const double stream_us = (double)p.width * p.cols * (GATED ? 2 : 1) / 6.4e6;
     double least = 0.;
@@ -454,7 +454,7 @@ template <int DT, bool GATED> int launch_product(const ProductParams &p, hipStre
         const uint64_t rounds = ((p.cols + n - 1) / n * ((p.rows + m - 1) / m) + 255) / 256;
         double block = h.block_us, round = h.round_us;
         if (GATED && !many) block *= 1.3 * (2 * h.rt + h.mt) / (h.rt + h.mt);
-        if (h.rt == 8 && h.mt == 8 && rounds == 1) { block = .544; round = 2.; }         // (four stages, one workgroup a CU: below)
+        if (h.rt == 8 && h.mt == 8 && rounds == 1) { block = .54; round = 1.8; }         // (four stages, one workgroup a CU: below)
         const double us = (double)rounds * (p.blocks * block + round), t = us > stream_us ? us : stream_us;
         if (best < 0 || t < least) { least = t; best = i; rounds_of = rounds; }
     }
