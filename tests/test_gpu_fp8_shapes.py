@@ -102,3 +102,9 @@ def test_results_behind_and_beside_stay(cuda):
         assert torch.equal(room[1:-1, 8:8 + cols], want)
         room[1:-1, 8:8 + cols] = 7.0
         assert bool((room == 7.0).all())
+
+
+@pytest.mark.parametrize("rows,width,cols", [(203, 896, 4864), (260, 272, 4096), (700, 144, 4096), (1500, 656, 6144), (1300, 400, 4096)])
+def test_gated_where_up_starts_on_a_tile(cuda, rows, width, cols):
+    """All rows of a tile's half have one scale: the other half of the kernels' forms at sizes where `GATED` has the ragged one."""
+    test_gated(cuda, rows, width, cols)
