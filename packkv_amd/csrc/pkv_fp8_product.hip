@@ -498,14 +498,14 @@ extern "C" int pkv_fp8_product(const pkv_fp8_product_args *a, pkv_stream_t s_) {
                 (a->w_stride == 0 || a->w_stride >= a->width), PKV_ERR_UNSUPPORTED, "not supported: rows of x or w more than 2^20 bytes apart, or that overlap");
     ProductParams p;
     p.x = a->x; p.w = a->w; p.x_scale = a->x_scale; p.w_scale = a->w_scale; p.bias = (const uint16_t *)a->bias; p.out = (uint16_t *)a->out;
-    p.x_row = a->x_stride; p.w_row = a->w_stride; p.out_row = a->out_stride;
+    p.x_row = a->x_stride; p.w_row = a->w_stride; p.out_row = a->rows > 1 ? a->out_stride : a->cols;            // (one row's stride means nothing)
     p.xs_row = a->x_scale_stride[0]; p.xs_col = a->x_scale_stride[1]; p.ws_row = a->w_scale_stride[0]; p.ws_col = a->w_scale_stride[1];
     p.rows = (uint32_t)a->rows; p.width = (uint32_t)a->width; p.cols = (uint32_t)a->cols;
     p.blocks = (p.width + kBlock8 - 1) / kBlock8;
-    p.whole4 = (p.cols | (uint64_t)a->out_stride) % 4 == 0 && (uintptr_t)a->out % 8 == 0;
+    p.whole4 = (p.cols | (uint64_t)p.out_row) % 4 == 0 && (uintptr_t)a->out % 8 == 0;
     // Results that no L2 would hold until they are read: 1024 x 128 x 6144 (12.6 MB) 7.5 -> 6.7 us, 4096 x 4096 x 4096 (33.5 MB) 59.5 -> 58.2.
     p.past = (uint64_t)p.rows * p.cols * 2u > (4u << 20);
-    p.whole8 = (p.cols | (uint64_t)a->out_stride) % 8 == 0 && (uintptr_t)a->out % 16 == 0 && a->out_stride >= 0 && a->out_stride <= (1 << 23);       // (64 rows within 2^30 bytes)
+    p.whole8 = (p.cols | (uint64_t)p.out_row) % 8 == 0 && (uintptr_t)a->out % 16 == 0 && p.out_row >= 0 && p.out_row <= (1 << 23);       // (64 rows within 2^30 bytes)
     if (a->gated) return a->dtype == PKV_F16 ? launch_product<PKV_F16, true>(p, s) : launch_product<PKV_BF16, true>(p, s);
     return a->dtype == PKV_F16 ? launch_product<PKV_F16, false>(p, s) : launch_product<PKV_BF16, false>(p, s);
 }
