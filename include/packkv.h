@@ -472,7 +472,8 @@ int pkv_sample(const pkv_sample_args *args, void *workspace, uint64_t workspace_
  * one byte each, and an fp32 scale for each block of 1 x 128 (activations) or 128 x 128 values (weights), the last blocks ragged:
  * scale = max(largest finite |value|, 2^-100) / 448, code = value / scale to the nearest, ties to even (through a product with
  * 1 / scale); infinities and NaN become NaN.  Strides are in elements, scale_stride: of a row of blocks and of a block in it; widths
- * are multiples of 16; rows of everything but scales start on 16-byte boundaries.  All of them launch kernels only.
+ * are multiples of 16; rows of inputs, sums and codes start on 16-byte boundaries, and so do a norm's results.  Results (codes and scales
+ * among them) must not overlap.  All of them launch kernels only.
  *
  * pkv_add_rms_norm: h = x + residual (NULL: x), y = h / sqrt(mean(h^2) + eps) * weight for each row, in fp32; h, rounded once, to sum
  * (NULL where there is no residual; may be the residual's own memory), y to out in `dtype` or in its 8-bit form to codes and scale.

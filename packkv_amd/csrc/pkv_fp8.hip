@@ -209,6 +209,9 @@ extern "C" int pkv_add_rms_norm(const pkv_norm_args *a, pkv_stream_t s_) {
     const uintptr_t off = (uintptr_t)a->x | (uintptr_t)a->residual | (uintptr_t)a->weight | (uintptr_t)a->sum | (uintptr_t)a->out | (uintptr_t)a->codes |
                           (uintptr_t)(2 * (a->x_stride | a->residual_stride | a->sum_stride | a->out_stride)) | (uintptr_t)a->codes_stride;
     PKV_REQUIRE(off % 16 == 0 && (uintptr_t)a->scale % 4 == 0, PKV_ERR_INVALID, "rows must start on 16-byte boundaries");
+    const int cols = (a->width + kBlock8 - 1) / kBlock8;
+    PKV_REQUIRE((!a->sum || apart(a->rows, a->sum_stride, a->width, 1)) && apart(a->rows, a->out ? a->out_stride : a->codes_stride, a->width, 1) &&
+                (!a->scale || apart(a->rows, a->scale_stride[0], cols, a->scale_stride[1])), PKV_ERR_INVALID, "results must not overlap");
     NormParams p;
     p.x = (const uint16_t *)a->x; p.residual = (const uint16_t *)a->residual; p.weight = (const uint16_t *)a->weight;
     p.sum = (uint16_t *)a->sum; p.out = (uint16_t *)a->out; p.codes = a->codes; p.scale = a->scale;
@@ -241,6 +244,8 @@ extern "C" int pkv_fp8_quantize(const pkv_fp8_quantize_args *a, pkv_stream_t s_)
     p.cols = (p.width + kBlock8 - 1) / kBlock8;
     const uint64_t wgs = a->block == 1 ? ((uint64_t)p.rows + 15) / 16 * ((p.cols + 7) / 8) : ((uint64_t)p.rows + kBlock8 - 1) / kBlock8 * p.cols;
     PKV_REQUIRE(wgs < (1ull << 24), PKV_ERR_UNSUPPORTED, "rows x width too large");                // (2^32 threads)
+    PKV_REQUIRE(apart(a->rows, a->codes_stride, a->width, 1) && apart((a->rows - 1) / a->block + 1, a->scale_stride[0], p.cols, a->scale_stride[1]),
+                PKV_ERR_INVALID, "results must not overlap");
     const dim3 grid((unsigned)wgs);
     if (a->block == 1) {
         if (a->dtype == PKV_F16) quantize_rows_kernel<PKV_F16><<<grid, 256, 0, s>>>(p);

@@ -8,6 +8,14 @@ constexpr int kBlock8 = 128;                       // values of a row that share
 constexpr float kTop8 = 448.f;                     // e4m3's largest
 constexpr float kLeast8 = 0x1p-100f;               // what a block's largest value counts as at least: its scale stays a normal number
 
+// Whether [a, b] elements with these strides are memory of their own each: results that are not would be written in any order.
+inline bool apart(int64_t a, int64_t a_stride, int64_t b, int64_t b_stride) {
+    uint64_t x = a_stride < 0 ? 0 - (uint64_t)a_stride : (uint64_t)a_stride, y = b_stride < 0 ? 0 - (uint64_t)b_stride : (uint64_t)b_stride;
+    if (a == 1) return b == 1 || y > 0;
+    if (b == 1) return x > 0;
+    return x <= y ? x > 0 && x <= (y - 1) / (uint64_t)(a - 1) : y > 0 && y <= (x - 1) / (uint64_t)(b - 1);
+}
+
 #ifdef __HIPCC__
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));

@@ -412,9 +412,14 @@ __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const Produc
     }
 }
 
+static int check_launch(const ProductParams &p, uint64_t threads) {
+    PKV_REQUIRE(threads < (1ull << 32), PKV_ERR_UNSUPPORTED, "rows x results too large");
+    PKV_REQUIRE(apart(p.rows, p.out_row, p.cols, 1), PKV_ERR_INVALID, "results must not overlap");
+    return PKV_OK;
+}
 template <int DT, bool GATED, int RT, int MT> int launch_few(const ProductParams &p, hipStream_t s) {
     const uint64_t tiles = (uint64_t)((p.cols + 16 * RT - 1) / (16 * RT)) * ((p.rows + 16 * MT - 1) / (16 * MT)), wgs = (tiles + 7) / 8 * 8;
-    PKV_REQUIRE(wgs < (1ull << 23), PKV_ERR_UNSUPPORTED, "rows x results too large");            // (2^32 threads)
+    if (const int rc = check_launch(p, wgs * 512)) return rc;
     product_few_kernel<DT, RT, MT, GATED><<<dim3((unsigned)wgs), 512, 0, s>>>(p);
     PKV_HIP_CHECK(hipGetLastError());
     return PKV_OK;
@@ -422,7 +427,7 @@ template <int DT, bool GATED, int RT, int MT> int launch_few(const ProductParams
 template <int DT, bool GATED, int HN, int MT, int WN, int WM, int STAGES> int launch_many(const ProductParams &p, hipStream_t s) {
     constexpr uint64_t n = (GATED ? 16 : 32) * HN * WN, m = 16 * MT * WM;
     const uint64_t tiles = (p.cols + n - 1) / n * ((p.rows + m - 1) / m), wgs = (tiles + 7) / 8 * 8;
-    PKV_REQUIRE(wgs * (64 * WN * WM) < (1ull << 32), PKV_ERR_UNSUPPORTED, "rows x results too large");           // (threads)
+    if (const int rc = check_launch(p, wgs * (64 * WN * WM))) return rc;
     // (a half of a tile's rows of weights may have two blocks of 128, and two scales, only where up's rows start within one)
     if (!GATED || p.cols % (16 * HN * WN) == 0) product_many_kernel<DT, HN, MT, WN, WM, STAGES, true, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
     else if constexpr (GATED) product_many_kernel<DT, HN, MT, WN, WM, STAGES, false, GATED><<<dim3((unsigned)wgs), 64 * WN * WM, 0, s>>>(p);
