@@ -65,14 +65,15 @@ template <int N> __device__ __forceinline__ void copies_but() {            // (a
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// Results n .. n + 3 from the sums (of gate, y, and of up, u), rounded.  g / (1 + e^-g) goes through the hardware's reciprocal (off by a step of fp32 at
-// most) of a quarter of the sum, whose own stays a normal number up to the largest e^-g.
+// Results n .. n + 3 from the sums (of gate, y, and of up, u), rounded.  g / (1 + e^-g) goes through the hardware's exponential (its argument is rounded
+// once more than exp's: |g| 2^-24 of the result) and reciprocal (off by a step of fp32 at most), both far below 16 bits.  The reciprocal is that of a quarter of
+// the sum, which stays a normal number up to the largest e^-g, and meets a quarter of g: 4 g would pass fp32 from 2^126 on.
 template <int DT, bool GATED> __device__ __forceinline__ u32x2 four_results(const ProductParams &p, uint32_t n, f32x4 y, f32x4 u) {
     float z[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         z[e] = y[e];
-        if (GATED) z[e] = z[e] * __builtin_amdgcn_rcpf(fmaf(__expf(-z[e]), .25f, .25f)) * (.25f * u[e]);
+        if (GATED) z[e] = .25f * z[e] * __builtin_amdgcn_rcpf(fmaf(__expf(-z[e]), .25f, .25f)) * u[e];
         else if (p.bias) z[e] += wide16<DT>(p.bias[min(n + e, p.cols - 1u)], 0);
     }
     return (u32x2){pair16<DT>(z[0], z[1]), pair16<DT>(z[2], z[3])};
