@@ -470,8 +470,8 @@ int pkv_sample(const pkv_sample_args *args, void *workspace, uint64_t workspace_
  * What lies between the attention over the cache and the next layer with weights and activations in 8 bits.  No counterpart in the
  * reference, whose decoder keeps 16-bit weights.  The 8-bit form of a matrix [rows, width] is its codes, e4m3 (OCP, largest 448),
  * one byte each, and an fp32 scale for each block of 1 x 128 (activations) or 128 x 128 values (weights), the last blocks ragged:
- * scale = max(largest finite |value|, 2^-100) / 448, code = value / scale to the nearest, ties to even (through a product with
- * 1 / scale); infinities and NaN become NaN.  Strides are in elements, scale_stride: of a row of blocks and of a block in it; widths
+ * scale = max(largest finite |value|, 2^-100) / 448, code = the fp32 quotient value / scale to the nearest, ties to even;
+ * infinities and NaN become NaN.  Strides are in elements, scale_stride: of a row of blocks and of a block in it; widths
  * are multiples of 16; rows of inputs, sums and codes start on 16-byte boundaries, and so do a norm's results.  Results (codes and scales
  * among them) must not overlap.  All of them launch kernels only.
  *

@@ -3,7 +3,6 @@
 // The 8-bit form of a matrix y [rows, width] has one fp32 scale for each block of 1 x 128 (activations) or 128 x 128 values
 // (weights), the last blocks ragged: s = max(max |y|, 2^-100) / 448, codes e4m3(y / s).  The norm is h = x + residual,
 // n = h / sqrt(mean(h^2) + eps) * w, all in fp32 from the sum on; h is rounded once where it is stored, n once to 16 bits or 8.
-// The quotient is a product with 1 / s: a value within 2^-23 of the middle between two codes may get the other one.
 //
 // Bound by memory, and by the launch where rows are few.  A thread holds chunks of eight values (one 16-byte load of each input),
 // so sixteen lanes hold a block and its largest value takes four DPP steps.
@@ -85,7 +84,7 @@ __global__ void __launch_bounds__(T < 256 ? 256 : T) norm_kernel(const NormParam
         if (p.codes) {
             const float s = scale_of(row16_max(most));
             if (mine) {
-                *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + c) = codes8(y, 1.f / s);
+                *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + c) = codes8(y, s);
                 if ((t & 15u) == 0) p.scale[(int64_t)row * p.scale_row + (int64_t)(c / kBlock8) * p.scale_col] = s;
             }
         } else if (mine) {
@@ -132,7 +131,7 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
         for (int j = 0; j < 8; j++) y[j] = wide16<DT>(v[i][j >> 1], j & 1);
         const float s = scale_of(row16_max(most.value()));
         if ((col + i) * kBlock8 + 8u * lane < p.width) {
-            *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + (col + i) * kBlock8 + 8u * lane) = codes8(y, 1.f / s);
+            *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + (col + i) * kBlock8 + 8u * lane) = codes8(y, s);
             if (lane == 0) p.scale[(int64_t)row * p.scale_row + (int64_t)(col + i) * p.scale_col] = s;
         }
     }
@@ -161,7 +160,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantizePara
     for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d, 64));
     if ((threadIdx.x & 63u) == 0) part[threadIdx.x >> 6] = most;
     __syncthreads();
-    const float s = scale_of(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]))), inv = 1.f / s;
+    const float s = scale_of(fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3])));
     if (threadIdx.x == 0) p.scale[(int64_t)down * p.scale_row + (int64_t)col * p.scale_col] = s;
 #pragma unroll
     for (int i = 0; i < 8; i++) {
@@ -170,7 +169,7 @@ __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantizePara
             float y[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) y[j] = wide16<DT>(x[i][j >> 1], j & 1);
-            *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + c) = codes8(y, inv);
+            *reinterpret_cast<u32x2 *>(p.codes + (int64_t)row * p.codes_row + c) = codes8(y, s);
         }
     }
 }

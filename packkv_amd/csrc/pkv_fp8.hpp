@@ -64,14 +64,25 @@ __device__ __forceinline__ float finite_size(float v) {
     return a <= 3.402823466e38f ? a : 0.f;
 }
 __device__ __forceinline__ float scale_of(float largest) { return fmaxf(largest, kLeast8) / kTop8; }
-// Eight values over their block's scale, to the nearest e4m3, ties to even.  (largest / scale may come out a rounding above 448, which
-// still rounds to 448; infinities and NaN become NaN.)
-__device__ __forceinline__ u32x2 codes8(const float y[8], float inv) {
+// Eight values over their block's scale, the fp32 quotients to the nearest e4m3, ties to even.  The product with inv, the hardware's 1 / scale (off by a step,
+// a normal number for every scale), may be off by three, which loses the ties: its remainder times inv puts it right, to 2^-45 before its
+// rounding, and 16-bit values get the codes of an exact division.  (largest / scale may come out a rounding above 448, which still rounds to
+// 448; infinities and NaN become NaN.)  8192 x 4096 by rows 19.4 us, without the
+// remainder 19.3; 4848 x 912 in blocks of 128 rows 6.1 and 5.75.
+__device__ __forceinline__ float quotient(float y, float scale, float inv) {
+    const float q = y * inv;
+    return fmaf(-fmaf(q, scale, -y), inv, q);              // (in these signs -0 stays -0)
+}
+__device__ __forceinline__ u32x2 codes8(const float y[8], float scale) {
+    const float inv = __builtin_amdgcn_rcpf(scale);
     u32x2 r = {0u, 0u};
+    float q[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) q[i] = quotient(y[i], scale, inv);
 #pragma unroll
     for (int i = 0; i < 2; i++) {
-        int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i] * inv, y[4 * i + 1] * inv, 0, false);
-        w = __builtin_amdgcn_cvt_pk_fp8_f32(y[4 * i + 2] * inv, y[4 * i + 3] * inv, w, true);
+        int w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i], q[4 * i + 1], 0, false);
+        w = __builtin_amdgcn_cvt_pk_fp8_f32(q[4 * i + 2], q[4 * i + 3], w, true);
         r[i] = (uint32_t)w;
     }
     return r;

@@ -1378,8 +1378,8 @@ def add_rms_norm(x, weight, eps=1e-6, residual=None, fp8=False):
 def fp8_quantize(x, block=1, heads=False):
     """The 8-bit form of x [..., width] fp16 or bf16 (width a multiple of 16): a dict of ``codes``, float8_e4m3fn of x's shape, and ``scale``,
     float32, for each block of 1 x 128 values [..., ceil(width / 128)] (activations) or, block=128 and x [rows, width], of 128 x 128
-    [ceil(rows / 128), ceil(width / 128)] (weights).  scale = max(largest finite |value|, 2^-100) / 448; a code is value / scale to the
-    nearest; infinities and NaN become NaN.  heads=True: x [B, H, n, 128], an attention's output, as the rows [B, n, H * 128]."""
+    [ceil(rows / 128), ceil(width / 128)] (weights).  scale = max(largest finite |value|, 2^-100) / 448; a code is the fp32
+    quotient value / scale to the nearest, ties to even; infinities and NaN become NaN.  heads=True: x [B, H, n, 128], an attention's output, as the rows [B, n, H * 128]."""
     served = _host().fp8_quantize(x, block, heads)
     if served is not None:
         return _lib.check(served) if type(served) is int else served
