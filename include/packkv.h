@@ -503,9 +503,10 @@ int pkv_fp8_quantize(const pkv_fp8_quantize_args *args, pkv_stream_t s);
 
 /* pkv_fp8_product: out [rows, cols] = x [rows, width] times w [cols, width] transposed, both in their 8-bit form (x with a scale a row, w
  * one for 128 rows), + bias [cols] (NULL: none), summed in fp32 and rounded once to `dtype`.  gated: w [2 cols, width], its first half gives g and
- * its second u, out = g / (1 + exp(-g)) * u; cols a multiple of 16, no bias.  The product of the two scales of a block has to be
- * finite.  Within each eight neighbouring products every one is cut to a multiple of 2^-13 of the largest's power of two (the matrix
- * instruction's own sums; the codes have 4 significant bits).  width at most 2^20, rows and cols at most 2^24. */
+ * its second u, out = g / (1 + exp(-g)) * u; cols a multiple of 16, no bias.  The product of the two scales of a block is an
+ * fp32 number: it has to be finite, and below 2^-126 it is off by up to 2^-150, a block's sum then by 2^-125.  Within each eight neighbouring
+ * products every one is cut to a multiple of 2^-13 of the largest's power of two (the matrix instruction's own sums; the codes have 4
+ * significant bits).  width at most 2^20, rows and cols at most 2^24. */
 typedef struct pkv_fp8_product_args {
     const uint8_t *x, *w;
     const float *x_scale, *w_scale;

@@ -65,10 +65,9 @@ __device__ __forceinline__ float finite_size(float v) {
 }
 __device__ __forceinline__ float scale_of(float largest) { return fmaxf(largest, kLeast8) / kTop8; }
 // Eight values over their block's scale, the fp32 quotients to the nearest e4m3, ties to even.  The product with inv, the hardware's 1 / scale (off by a step,
-// a normal number for every scale), may be off by three, which loses the ties: its remainder times inv puts it right, to 2^-45 before its
+// a normal number for every scale), may be off by three, which loses the ties: its remainder times inv puts it right, to 2^-43 before its
 // rounding, and 16-bit values get the codes of an exact division.  (largest / scale may come out a rounding above 448, which still rounds to
-// 448; infinities and NaN become NaN.)  8192 x 4096 by rows 19.4 us, without the
-// remainder 19.3; 4848 x 912 in blocks of 128 rows 6.1 and 5.75.
+// 448; infinities and NaN become NaN.)  8192 x 4096 by rows 19.4 us, without the remainder 19.3; 4848 x 912 in blocks of 128 rows 6.1 and 5.75.
 __device__ __forceinline__ float quotient(float y, float scale, float inv) {
     const float q = y * inv;
     return fmaf(-fmaf(q, scale, -y), inv, q);              // (in these signs -0 stays -0)

@@ -4,13 +4,16 @@
 // g / (1 + exp(-g)) * u.
 //
 // One v_mfma_f32_16x16x128_f8f6f4 is one block's sum for 16 x 16 results: it starts from zero, and its four numbers a lane are
-// added to the fp32 sums with the two scales, one fma each.  Weights are the instruction's rows and x its columns, so a lane holds
-// four neighbouring outputs of one row of x: its scale is one number a lane, the weights' scale one a wavefront.  The order of the 128
-// within a block does not matter, so lanes load what lies well: of each 128 the 16-byte pieces g and 4 + g, g = lane / 16.
+// added to the fp32 sums with the two scales, one fma each.  (The scales' product is rounded to fp32: below 2^-126 by up to 2^-150, times at
+// most 128 * 448^2 in a block's sum.  Either scale by itself would cost four more instructions a product.)  Weights are the instruction's
+// rows and x its columns, so a lane holds four neighbouring outputs of one row of x: its scale is one number a lane, the weights' scale one a
+// wavefront.  The order of the 128 within a block does not matter, so lanes load what lies well: of each 128 the 16-byte pieces g and 4 + g,
+// g = lane / 16.
 //
 // What the instruction loses: in each group of eight neighbouring k it cuts every product towards zero to a multiple of 2^-13 of the
 // group's largest power of two, and adds groups in fp32 (measured).  Products of values with 4 significant bits, which are 2^-4 off
-// themselves, come out 2^-13 of the largest of eight off at most; sums of 128 normal products 1.3e-5.  Results are 16-bit (2^-9, 2^-12).
+// themselves, come out 2^-13 of the largest of eight off at most; sums of 128 normal products 1.3e-5.  Results are 16-bit (half a step is 2^-8
+// of a value in bf16, 2^-11 in fp16).
 #include "pkv_fp8.hpp"
 #include "pkv_runtime.hpp"
 
@@ -65,15 +68,16 @@ template <int N> __device__ __forceinline__ void copies_but() {            // (a
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory");
 }
 __device__ __forceinline__ void copies_done() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// Results n .. n + 3 from the sums (of gate, y, and of up, u), rounded.  g / (1 + e^-g) goes through the hardware's exponential (its argument is rounded
-// once more than exp's: |g| 2^-24 of the result) and reciprocal (off by a step of fp32 at most), both far below 16 bits.  The reciprocal is that of a quarter of
-// the sum, which stays a normal number up to the largest e^-g, and meets a quarter of g: 4 g would pass fp32 from 2^126 on.
+// Results n .. n + 3 from the sums (of gate, y, and of up, u), rounded.  g / (1 + e^-g) goes through the hardware's exponential (its argument, times
+// log2 e, is rounded: |g| 2^-23 of the result at most) and reciprocal (off by a step of fp32 at most), both far below 16 bits.  The reciprocal is that
+// of a quarter of the sum, which stays a normal number up to the largest e^-g, and meets a quarter of up first: with g it would be 4 g, past fp32 from
+// 2^126 on.  (A quarter of g instead: gated 4096 x 4096 x 2 x 12288 339 us, so 336.)
 template <int DT, bool GATED> __device__ __forceinline__ u32x2 four_results(const ProductParams &p, uint32_t n, f32x4 y, f32x4 u) {
     float z[4];
 #pragma unroll
     for (int e = 0; e < 4; e++) {
         z[e] = y[e];
-        if (GATED) z[e] = .25f * z[e] * __builtin_amdgcn_rcpf(fmaf(__expf(-z[e]), .25f, .25f)) * u[e];
+        if (GATED) z[e] = z[e] * (__builtin_amdgcn_rcpf(fmaf(__expf(-z[e]), .25f, .25f)) * (.25f * u[e]));
         else if (p.bias) z[e] += wide16<DT>(p.bias[min(n + e, p.cols - 1u)], 0);
     }
     return (u32x2){pair16<DT>(z[0], z[1]), pair16<DT>(z[2], z[3])};

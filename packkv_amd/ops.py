@@ -1455,7 +1455,8 @@ def _fp8_product(x, w, bias, dtype, gated):
 def fp8_linear(x, w, bias=None, dtype=torch.bfloat16):
     """x times w transposed, [..., rows of w], of x [..., width] and w [rows, width] in their 8-bit forms (fp8_quantize with block 1 and 128, or
     add_rms_norm's), + bias, summed in fp32 and rounded once to `dtype` (fp16 or bf16; the bias has it too).  Within each eight neighbouring
-    products every one is cut to a multiple of 2^-13 of the largest's power of two: the matrix instruction's own sums."""
+    products every one is cut to a multiple of 2^-13 of the largest's power of two: the matrix instruction's own sums.  The product of a
+    block's two scales is an fp32 number: it has to be finite, and below 2^-126 it is off by up to 2^-150 (a block's sum by 2^-125)."""
     served = _host().fp8_product(x, w, bias, dtype, False)
     if served is not None:
         return _lib.check(served) if type(served) is int else served

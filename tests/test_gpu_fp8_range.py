@@ -30,10 +30,32 @@ def test_gated_where_fp32_ends(cuda, rows, gate, up):
     gd, ud = g.double() * 2.0 ** gate, u.double() * 2.0 ** up
     want = gd * torch.sigmoid(gd) * ud
     assert bool(torch.isfinite(got[:, want.abs() < 2.0 ** 127]).all())
-    # (e^-g of fp32 is infinite from -88.7 on; a gate's quarter is a multiple of 2^-149, so off by 2^-150, four times that of the gate and
-    # less of silu, which is half of so small a gate; bf16 has eight significant bits: half a step is 2^-8 of a value)
+    # (e^-g of fp32 is infinite from -88.7 on; up's quarter is a multiple of 2^-149, off by 2^-150, and four times that comes with at most g;
+    # its product with the reciprocal is off by 2^-150 once more, times g; bf16 has eight significant bits: half a step is 2^-8 of a value)
     fine = (want.abs() < 2.0 ** 127) & (gd > -88.5)
-    tol = (oracle.half_step(torch.bfloat16) + 2 * oracle.U * (gd.abs().clamp_max(90) + 8)) * want.abs() + oracle.tiny(torch.bfloat16) + 2.0 ** -148 * ud.abs()
+    tol = (oracle.half_step(torch.bfloat16) + 2 * oracle.U * (gd.abs().clamp_max(90) + 8)) * want.abs() + oracle.tiny(torch.bfloat16) + 2.0 ** -147 * gd.abs()
     err = (got.double() - want).abs() - tol
     assert bool((err[:, fine] <= 0).all()), (err[:, fine].max().item(), gd[fine], ud[fine], got[0, fine])
     assert bool((got[:, ud == 0] == 0).all())
+
+
+@pytest.mark.parametrize("rows", [1, 40, 700])
+@pytest.mark.parametrize("xs,ws", [(-60, -60), (-60, -75), (-109, -30), (-100, -100), (60, -109), (100, -140)])
+def test_linear_of_small_scales(cuda, rows, xs, ws):
+    """The product of a block's two scales is an fp32 number: below 2^-126 a multiple of 2^-149, off by 2^-150 at most.  (Whole codes -2 .. 2 and no cut: the
+    rest is a rounding for the scales' product, one a block, and the last one.)"""
+    gen = torch.Generator().manual_seed(rows)
+    width, cols = 400, 272
+    whole = lambda *shape: torch.randint(-2, 3, shape, generator=gen).float()
+    draw = lambda blocks, e: ((1 + torch.rand(blocks, 4, generator=gen)) * 2.0 ** e).to(cuda)
+    x, w = {"codes": whole(rows, width).to(oracle.F8).to(cuda), "scale": draw(rows, xs)}, {"codes": whole(cols, width).to(oracle.F8).to(cuda), "scale": draw(3, ws)}
+    y, mass, sums = (torch.zeros(rows, cols, dtype=torch.float64) for _ in range(3))
+    for b in range(4):
+        xa, wa = (t["codes"].cpu().double()[:, 128 * b:128 * b + 128] for t in (x, w))
+        f = x["scale"].cpu().double()[:, b, None] * w["scale"].cpu().double().repeat_interleave(128, 0)[:cols, b][None]
+        d = xa @ wa.t()
+        y, mass, sums = y + d * f, mass + d.abs() * f, sums + d.abs()
+    got = ops.fp8_linear(x, w).cpu().double()
+    tol = 12 * oracle.U * mass + 2.0 ** -150 * (sums + 12)
+    err = (got - y).abs()
+    assert bool((err <= tol + oracle.half_step(torch.bfloat16) * (y.abs() + tol) + oracle.tiny(torch.bfloat16)).all())
