@@ -105,8 +105,8 @@ struct QuantizeParams {
 };
 
 // Blocks of 1 x 128, sixteen lanes each: a workgroup has 16 rows and eight blocks of each, a thread one row's, all eight loads on their way at
-// once.  (Sixteen rows, so that their scales are whole lines where those of a column lie together: 8192 x 4096 18.4 us, 5.5 TB/s, with rows
-// of 128 blocks 19.6.)
+// once.  (Sixteen rows, so that their scales are whole lines where those of a column lie together: 8192 x 4096 18.6 us, 5.4 TB/s; without the
+// remainders of codes8 18.4, and then with rows of 128 blocks 19.6.)
 template <int DT>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams p) {
     constexpr int V = 8;
@@ -137,8 +137,8 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(const QuantizeParams
     }
 }
 
-// Blocks of 128 x 128, one a workgroup: a thread holds eight rows' chunks, so x is read once.  24576 x 4096 50 us (6.0 TB/s), 4848 x 912 5.9 us: one
-// round of 304 workgroups; with 512 threads of four chunks the same.
+// Blocks of 128 x 128, one a workgroup: a thread holds eight rows' chunks, so x is read once.  24576 x 4096 54 us (5.6 TB/s; 50 without
+// the remainders of codes8), 4848 x 912 6.1 us: one round of 304 workgroups; with 512 threads of four chunks the same.
 template <int DT>
 __global__ void __launch_bounds__(256) quantize_blocks_kernel(const QuantizeParams p) {
     __shared__ float part[4];

@@ -214,8 +214,8 @@ __global__ void __launch_bounds__(512) product_few_kernel(const ProductParams p)
 // p ^ (r & 7), so that eight lanes reading one piece of eight rows touch all banks.
 // 256 x 256 results take 2048 cycles a block of the matrix units, as many of the copies (a CU gets 32 bytes a cycle from L2), and 2300 of
 // a SIMD's issue slots (a product takes 16 of its 32 cycles', the 160 other vector instructions 4 each); together about 2750, at 1.8 GHz: the clock
-// falls with the matrix units' load.  4096 x 12288 x 4096 161 us (2.56 PFLOP/s), gated 4096 x 4096 x 2 x 12288 337 us (2.44), 4096 x 4096 x 4096 56.7 us; nine
-// vector instructions fewer with moving descriptors instead, 166 us for 162.
+// falls with the matrix units' load.  4096 x 12288 x 4096 161 us (2.56 PFLOP/s; 170 on one machine), gated 4096 x 4096 x 2 x 12288 336 us (2.45; 363), 4096 x 4096 x 4096
+// 56.7 us; nine vector instructions fewer with moving descriptors instead, 166 us for 162.
 template <int DT, int HN, int MT, int WN, int WM, int STAGES, bool EVEN, bool GATED>
 __global__ void __launch_bounds__(64 * WN * WM) product_many_kernel(const ProductParams p) {
     constexpr int kWaves = WN * WM, kHalf = 16 * HN * WN, kX = 16 * MT * WM;
